@@ -474,6 +474,114 @@ ttcd_status ttcd_ttt_scan_fwd(const void* dw, const void* w_cur, float lr, void*
                               ttcd_dtype dtype, void* stream);
 
 /*
+ * A key / value cache held in 4 bits. The reference keeps bf16 keys and values
+ * (fla's attn_state, fla/models/utils.py:35-96) and has no counterpart.
+ *
+ * Blocks of 32 channels of one position and head share a scale 2^e, held as the
+ * byte e + 127: the least with no magnitude over 6 * 2^e, e in [-125, 125] for
+ * BF16 and in [-23, 13] for F16 (so every held value is a number of the type). A
+ * value is 4 bits, a sign (8) and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (codes 0 to
+ * 7), rounded to nearest, ties to the even code; what is larger, infinities among
+ * it, is held as 6 * 2^e, NaN as 0.
+ *   k_codes  (batch, kv_heads, capacity, head_dim / 2) bytes, channel 2i in the
+ *            low half of byte i and 2i + 1 in the high one
+ *   k_scales (batch, kv_heads, capacity, head_dim / 32)
+ *   v_codes  (batch, kv_heads, capacity / 4, head_dim / 8, 4, 4): the 4-byte
+ *            words of 8 channels of 4 neighbouring slots side by side
+ *   v_scales (batch, kv_heads, capacity / 4, head_dim / 32, 4)
+ *   lengths  (batch) int32: the positions that a sequence has had, up to 2^30
+ *            (entries outside [0, 2^30] are taken as the nearest bound)
+ * all contiguous, k_codes and v_codes 16-byte aligned, v_scales and lengths
+ * 4-byte aligned. Position p of a sequence is in slot p % capacity; the last
+ * `capacity` positions are held. capacity: a multiple of 32 up to 2^30; head_dim
+ * 64 or 128. A cache that is not `const` below is written; a call that writes one
+ * may not overlap in time with another on it. No call reads a slot that holds no
+ * position into a result, so a new cache needs its lengths set to 0 and no more.
+ */
+typedef struct ttcd_kv4_cache {
+  void* k_codes;
+  void* k_scales;
+  void* v_codes;
+  void* v_scales;
+  int32_t* lengths;
+  int batch, kv_heads, head_dim, capacity;
+} ttcd_kv4_cache;
+
+/*
+ * Quantise T new positions of every sequence into the cache and add them to its
+ * lengths. k, v: (batch, T, kv_heads, head_dim) of `dtype` (BF16 or F16), strides
+ * (of b, t, h, d) as in the attention calls: d-stride 1, the others non-negative
+ * multiples of 8, 16-byte aligned bases. 1 <= T <= capacity.
+ * counts: device int32[batch] or NULL: a padded batch, sequence b has the first
+ * counts[b] (clamped to [0, T]) of the T positions; the others are not read.
+ * weights: NULL, or (batch, kv_heads, capacity) fp32 that is set to 0 in the slots
+ * written (a cache whose key weights are accumulated).
+ */
+ttcd_status ttcd_kv4_append(ttcd_kv4_cache* cache, const void* k, const void* v, int T,
+                            const int64_t k_stride[4], const int64_t v_stride[4],
+                            const int32_t* counts, float* weights, ttcd_dtype dtype,
+                            void* stream);
+
+/*
+ * The last `count` positions of every sequence as values of `dtype`: k, v (batch,
+ * count, kv_heads, head_dim) contiguous, row t position lengths[b] - count + t; 0
+ * in rows before a sequence's first held position. Exact.
+ */
+ttcd_status ttcd_kv4_read(const ttcd_kv4_cache* cache, void* k, void* v, int count,
+                          ttcd_dtype dtype, void* stream);
+
+/*
+ * Attention over the cache: the queries are the last positions of their sequence
+ * (appended before this call), query t of n = counts[b] (NULL: Tq) at position
+ * lengths[b] - n + t, and see the held keys j with i - window < j <= i (window
+ * <= 0: all up to i). q, o: (batch, Tq, Hq, head_dim) of `dtype`, strides as in
+ * the attention calls above; Hq a multiple of kv_heads. lse: (batch, Hq, Tq) fp32
+ * or NULL, natural log. Rows without a key, and rows t >= counts[b], get o = 0
+ * and lse = -inf.
+ * workspace (device memory, 16-byte aligned): with at least
+ * ttcd_kv4_attn_workspace_bytes(...) the keys are swept in parts by different
+ * workgroups and added in fp32; with less, or NULL, by one each (slower, equal to
+ * rounding). 0 bytes: the call would not be split. Not read before it is written;
+ * calls that may overlap in time need one each.
+ */
+size_t ttcd_kv4_attn_workspace_bytes(const ttcd_kv4_cache* cache, int Tq, int Hq, int window);
+ttcd_status ttcd_kv4_attn_fwd(const ttcd_kv4_cache* cache, const void* q, void* o, float* lse,
+                              int Tq, int Hq, const int64_t q_stride[4],
+                              const int64_t o_stride[4], const int32_t* counts, int window,
+                              float sm_scale, ttcd_dtype dtype, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/*
+ * The attention weight of every held key, summed over the query heads of its
+ * key / value head and over the queries: weights[b, h, p % capacity] = sum_i
+ * exp(sm_scale * q_i . k_p - lse_i) over the queries i that see position p, in
+ * fp32; 0 in slots that hold nothing. lse: (batch, Hq, Tq) as ttcd_kv4_attn_fwd
+ * of the same call gives it (rows of -inf count for nothing). accumulate != 0: the
+ * sums are added to what weights holds. weights: (batch, kv_heads, capacity).
+ */
+ttcd_status ttcd_kv4_key_weights_fwd(const ttcd_kv4_cache* cache, const void* q,
+                                     const float* lse, float* weights, int Tq, int Hq,
+                                     const int64_t q_stride[4], const int32_t* counts,
+                                     int window, float sm_scale, int accumulate,
+                                     ttcd_dtype dtype, void* stream);
+
+/*
+ * The cache without the keys of least weight, per key / value head: of n held
+ * positions min(n, keep) stay, the newest `recent` of them in any case and of the
+ * older ones those of the largest weight, ties to the oldest (NaN counts as less
+ * than any number). They become positions 0, 1, .. of `out`, in their order, whose
+ * lengths are set to their number. weights: (batch, kv_heads, capacity) fp32 by
+ * slot. out: another cache of the same batch, kv_heads and head_dim and a capacity
+ * >= keep, none of its memory shared with `cache`. new_weights: (batch, kv_heads,
+ * out->capacity) fp32 or NULL: the kept keys' weights, 0 behind them. index:
+ * (batch, kv_heads, keep) int32: the position that each new one had, -1 behind the
+ * last. 1 <= keep, 0 <= recent.
+ */
+ttcd_status ttcd_kv4_evict(const ttcd_kv4_cache* cache, const float* weights, int keep,
+                           int recent, ttcd_kv4_cache* out, float* new_weights, int32_t* index,
+                           void* stream);
+
+/*
  * Host-only schedule check (no GPU work). Replays the attention kernels'
  * exact tile/phase schedule for one (b, h) slice of length T and adds, for
  * every (query i, key j) pair the kernel would fold into each output, one

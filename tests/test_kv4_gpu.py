@@ -1,0 +1,540 @@
+"""The 4-bit key / value cache on the GPU against the float64 oracle.
+
+Bounds, with u half a step of the type (bf16 2^-8, f16 2^-11) and e = 2^-24:
+* what the cache holds is determined: codes, scales and read values are equal;
+* lse: a score is a sum of D exact products and one scaling, off by at most
+  d = (D + 4) e scale max_j sum |q k_j|; the exponential's argument and the
+  logarithm are rounded at the lse's own size; the sum over n keys is in chains of
+  at most n / 8 + 64 additions;
+* o: probabilities are rounded once, u, beside what their scores are off by, and
+  the result once: u |o| + (u + 4 d + chain e) sum p |v|. f16 rounds those under
+  2^-14 to multiples of 2^-24, off by 2^-25; they are held times 2^7 against a
+  maximum that is some key's own, so sum p >= 1 and n keys add n 2^-32 max |v|;
+* key weights: sums of exp(score - lse), off by the scores' and the lse's share.
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import ttcd_amd
+from oracle import kv4_ref
+from ttcd_amd import KV4Cache, kv4_append, kv4_attn, kv4_evict, kv4_key_weights, kv4_read
+
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+U = {BF: 2.0 ** -8, HF: 2.0 ** -11}
+E = 2.0 ** -24
+
+
+def _rand(seed, *shape, dtype=BF, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(dtype)
+
+
+def _pair(B, H, D, C, dtype, lengths=(), seed=0, weights=False):
+    """A cache whose slots all start as garbage (NaN scales), and its oracle, with
+    lengths[b] positions appended."""
+    c = KV4Cache(B, H, D, C, dtype, weights=weights)
+    for t in (c.k_codes, c.k_scales, c.v_codes, c.v_scales):
+        t.fill_(255)
+    r = kv4_ref.Ref(B, H, D, C, dtype)
+    left = list(lengths)
+    i = 0
+    while any(left):
+        step = [min(n, C) for n in left]
+        T = max(step)
+        k, v = (_rand(seed + 7 * i + j, B, T, H, D, dtype=dtype, scale=1 + 2 * j) for j in (0, 1))
+        n = torch.tensor(step, dtype=torch.int32)
+        kv4_append(c, k.cuda(), v.cuda(), counts=n.cuda())
+        r.append(k, v, n)
+        left = [a - b for a, b in zip(left, step)]
+        i += 1
+    return c, r
+
+
+def _score_error(r, q):
+    """d of the bounds: over all queries and positions of the call, per sequence."""
+    out = []
+    for b in range(r.B):
+        k = r.rows[b][0].abs()
+        if not len(k):
+            out.append(0.0)
+            continue
+        k = k.repeat_interleave(q.shape[2] // r.H, 1)
+        s = torch.einsum("thd,lhd->htl", q[b].double().cpu().abs().nan_to_num(0), k).max().item()
+        out.append((r.D + 4) * E * s * r.D ** -0.5)
+    return torch.tensor(out)
+
+
+def _check_attn(r, q, o, lse, window, counts):
+    want, wl, mag = r.attn(q, window, counts)
+    chain = (max(r.length(b) for b in range(r.B)) / 8 + 64) * E
+    d = _score_error(r, q)[:, None, None]
+    u = U[r.dtype]
+    assert o.shape == q.shape and o.dtype == r.dtype
+    limit = u * want.abs() + (u + 4 * d[..., None] + chain) * mag
+    if r.dtype == HF:
+        limit += torch.tensor([len(v) * 2.0 ** -32 * v.abs().max() if len(v) else 0.0
+                               for _, v in r.rows])[:, None, None, None]
+    bad = ((o.double().cpu() - want).abs() - limit).max().item()
+    assert bad <= 0, bad
+    empty = wl == -math.inf
+    assert torch.equal(lse.cpu() == -math.inf, empty)
+    ll = 2 * d + chain + 8 * E * (1 + wl.masked_fill(empty, 0).abs())
+    assert ((lse.double().cpu() - wl).masked_fill(empty, 0).abs() <= ll).all()
+
+
+# ------------------------------------------------------------ append and read
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [1, 2, 4, 5, 33, 64])
+def test_append_holds_what_the_format_says(gpu, dtype, D, T):
+    B, H, C = 3, 2, 64
+    c, r = _pair(B, H, D, C, dtype, (0, 63, 129), seed=T)
+    before = [t.cpu().clone() for t in (c.k_codes, c.k_scales, c.v_codes, c.v_scales)]
+    k, v = _rand(1, B, T, H, D, dtype=dtype), _rand(2, B, T, H, D, dtype=dtype, scale=40.0)
+    kv4_append(c, k.cuda(), v.cuda())
+    r.append(k, v)
+    assert c.lengths.tolist() == [T, 63 + T, 129 + T]
+    for x, y in zip(kv4_read(c, C), r.read(C)):
+        assert torch.equal(x.cpu(), y)
+    # the new slots' bytes as the layout says, every other slot as it was
+    for b, old in enumerate((0, 63, 129)):
+        slots = (old + torch.arange(T)) % C
+        kk, vv = (torch.zeros(1, H, C, D, dtype=dtype) for _ in range(2))
+        kk[0, :, slots] = k[b].transpose(0, 1)
+        vv[0, :, slots] = v[b].transpose(0, 1)
+        want = kv4_ref.codes_of(kk, vv)
+        for got, w, was, is_v in zip((c.k_codes, c.k_scales, c.v_codes, c.v_scales), want, before,
+                                     (0, 0, 1, 1)):
+            exp = was[b].clone()
+            if is_v:
+                exp[:, slots // 4, :, slots % 4] = w[0][:, slots // 4, :, slots % 4]
+            else:
+                exp[:, slots] = w[0][:, slots]
+            assert torch.equal(got[b].cpu(), exp)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_append_of_any_value(gpu, dtype):
+    """Ties, zeros of both signs, subnormals, the largest values, infinities, NaN."""
+    g = torch.Generator().manual_seed(3)
+    bits = torch.randint(-2 ** 15, 2 ** 15, (1, 64, 4, 128), generator=g, dtype=torch.int16)
+    k = bits.view(dtype)
+    v = (torch.randint(-26, 27, (1, 64, 4, 128), generator=g) / 4).to(dtype)
+    for i, x in enumerate((0.0, -0.0, math.inf, -math.inf, math.nan, torch.finfo(dtype).max,
+                           torch.finfo(dtype).tiny, torch.finfo(dtype).smallest_normal / 4)):
+        v[0, 2 * i, :, :] = 0
+        v[0, 2 * i, :, 5::9] = x
+        v[0, 2 * i + 1, :, 7] = x
+    c, r = _pair(1, 4, 128, 64, dtype)
+    kv4_append(c, k.cuda(), v.cuda())
+    r.append(k, v)
+    for x, y in zip(kv4_read(c, 64), r.read(64)):
+        assert torch.isfinite(x).all() and torch.equal(x.cpu(), y)
+
+
+@pytest.mark.parametrize("counts", [(0, 9, 30), (30, 1, 0), (0, 0, 0), (-5, 2, 99)])
+def test_padded_batch(gpu, counts):
+    c, r = _pair(3, 2, 64, 64, BF, (50, 3, 64), weights=True)
+    c.weights.fill_(2.0)
+    k, v = _rand(4, 3, 30, 2, 64), _rand(5, 3, 30, 2, 64)
+    n = torch.tensor(counts, dtype=torch.int32)
+    m = n.clamp(0, 30)
+    for b in range(3):  # what is not appended is not looked at
+        k[b, m[b]:] = math.nan
+    kv4_append(c, k.cuda(), v.cuda(), counts=n.cuda())
+    r.append(k, v, m)
+    assert c.lengths.tolist() == [r.length(b) for b in range(3)]
+    for x, y in zip(kv4_read(c, 100), r.read(100)):
+        assert torch.equal(x.cpu(), y)
+    new = torch.zeros(3, 64, dtype=torch.bool)
+    for b, old in enumerate((50, 3, 64)):
+        new[b, (old + torch.arange(int(m[b]))) % 64] = True
+    assert torch.equal(c.weights.cpu(), torch.where(new, 0.0, 2.0)[:, None].expand(3, 2, 64))
+
+
+def test_views_of_a_fused_projection(gpu):
+    """k and v as slices of one (B, T, Hq + 2 Hkv, D) output, a transposed layout, a
+    broadcast row, and rows off 16-byte alignment (copied)."""
+    B, T, H, D = 2, 37, 2, 128
+    qkv = _rand(6, B, T, 8, D).cuda()
+    _, k, v = qkv.split((4, H, H), 2)
+    kt = _rand(7, B, H, T, D).cuda().transpose(1, 2)
+    odd = _rand(8, B * T * H * D + 3).cuda()[3:].view(B, T, H, D)
+    row = _rand(9, B, 1, H, D).cuda().expand(B, T, H, D)
+    for a, b in ((k, v), (kt, v), (odd, kt), (row, odd)):
+        c, r = _pair(B, H, D, 64, BF, (5, 0))
+        kv4_append(c, a, b)
+        r.append(a, b)
+        for x, y in zip(kv4_read(c, 64), r.read(64)):
+            assert torch.equal(x.cpu(), y)
+
+
+@pytest.mark.parametrize("T", [300, 2048])
+def test_large_append(gpu, T):
+    """More rows than one workgroup writes, over the ring's end."""
+    c, r = _pair(2, 3, 128, 2048, HF, (2040, 1111))
+    k, v = _rand(1, 2, T, 3, 128, dtype=HF), _rand(2, 2, T, 3, 128, dtype=HF)
+    n = torch.tensor([T, T - 3], dtype=torch.int32)
+    kv4_append(c, k.cuda(), v.cuda(), counts=n.cuda())
+    r.append(k, v, n)
+    assert c.lengths.tolist() == [r.length(0), r.length(1)]
+    for x, y in zip(kv4_read(c, 2048), r.read(2048)):
+        assert torch.equal(x.cpu(), y)
+
+
+@pytest.mark.parametrize("count", [0, 1, 3, 64, 65, 200])
+def test_read_counts(gpu, count):
+    c, r = _pair(3, 1, 64, 64, HF, (0, 2, 99))
+    for x, y in zip(kv4_read(c, count), r.read(count)):
+        assert torch.equal(x.cpu(), y)
+
+
+# ------------------------------------------------------------------ attention
+
+ATTN = [
+    # B, T, Hq, H, D, C, lengths, window, counts, dtype
+    (1, 1, 4, 2, 64, 64, (1,), None, None, BF),
+    (1, 1, 4, 2, 64, 64, (0,), None, None, BF),                  # nothing held
+    (2, 1, 16, 8, 128, 96, (33, 96), None, None, BF),
+    (1, 1, 15, 5, 64, 512, (2000,), None, None, HF),             # wrapped ring, odd group
+    (3, 1, 8, 1, 128, 256, (31, 32, 700), 32, None, HF),
+    (1, 1, 20, 1, 64, 128, (128,), 1, None, BF),                 # two row tiles, window 1
+    (2, 5, 6, 2, 64, 64, (64, 150), 20, None, BF),
+    (2, 7, 16, 8, 128, 160, (7, 200), None, (7, 3), HF),
+    (3, 9, 4, 4, 128, 64, (40, 9, 500), 8, (0, 9, 4), BF),
+    (1, 33, 8, 2, 64, 192, (33,), None, None, BF),               # a prompt of its own
+    (1, 64, 4, 4, 128, 96, (97,), 64, None, HF),                 # queries lose their oldest keys
+    (2, 130, 6, 2, 128, 320, (130, 1000), 100, (130, 77), BF),
+    (1, 200, 12, 2, 64, 256, (256,), None, None, HF),
+    (1, 100, 2, 2, 64, 64, (50,), None, None, BF),               # more queries than positions
+    (1, 3, 48, 1, 128, 4096, (4000,), None, None, BF),           # split over keys
+    (4, 1, 9, 3, 64, 8192, (8192, 100, 5000, 20000), 3000, None, HF),
+    (1, 2, 4, 2, 128, 32768, (40000,), None, None, BF),
+]
+
+
+@pytest.mark.parametrize("B,T,Hq,H,D,C,lengths,window,counts,dtype", ATTN)
+def test_attention_matches_64_bits(gpu, B, T, Hq, H, D, C, lengths, window, counts, dtype):
+    c, r = _pair(B, H, D, C, dtype, lengths, seed=T + D)
+    q = _rand(11, B, T, Hq, D, dtype=dtype, scale=1.5)
+    n = None if counts is None else torch.tensor(counts, dtype=torch.int32)
+    if n is not None:
+        for b in range(B):
+            q[b, n[b]:] = math.nan  # padding does not matter
+    o, lse = kv4_attn(q.cuda(), c, window, counts=None if n is None else n.cuda(),
+                      return_lse=True)
+    _check_attn(r, q, o, lse, window, n)
+    whole, wl = kv4_attn(q.cuda(), c, window, counts=None if n is None else n.cuda(),
+                         return_lse=True, split_keys=False)
+    _check_attn(r, q, whole, wl, window, n)
+    assert torch.equal(kv4_attn(q.cuda(), c, window, counts=None if n is None else n.cuda()), o)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_scores_that_grow_along_the_keys(gpu, dtype):
+    """Running maxima that move at every tile, by more and less than the lazy limit,
+    and one key far above all."""
+    B, H, D, C = 1, 2, 64, 1024
+    c, r = _pair(B, H, D, C, dtype)
+    k = _rand(1, B, C, H, D, dtype=dtype) * torch.linspace(0.1, 6, C)[:, None, None]
+    k[0, 777] *= 4
+    k, v = k.to(dtype), _rand(2, B, C, H, D, dtype=dtype)
+    kv4_append(c, k.cuda(), v.cuda())
+    r.append(k, v)
+    q = _rand(3, B, 3, 4, D, dtype=dtype, scale=3.0)
+    for split in (False, True):
+        o, lse = kv4_attn(q.cuda(), c, return_lse=True, split_keys=split)
+        _check_attn(r, q, o, lse, None, None)
+
+
+def test_nan_queries_stay_in_their_row(gpu):
+    c, r = _pair(1, 2, 64, 4096, BF, (4096,))
+    q = _rand(3, 1, 4, 4, 64)
+    good = kv4_attn(q.cuda(), c)
+    q[0, 1, 2, 5] = math.nan
+    for split in (True, False):
+        o, lse = kv4_attn(q.cuda(), c, return_lse=True, split_keys=split)
+        assert torch.isnan(o[0, 1, 2]).all() and torch.isnan(lse[0, 2, 1])
+        o[0, 1, 2] = good[0, 1, 2]
+        assert torch.isfinite(o).all()
+        assert (o - good).abs().max() < 0.02
+
+
+def test_strided_queries(gpu):
+    c, r = _pair(2, 2, 128, 64, BF, (64, 20))
+    wide = _rand(3, 2, 5, 12, 128).cuda()
+    for q in (wide[:, :, 2:6], wide.transpose(1, 2)[:, :5].transpose(1, 2)[:, :, :4],
+              wide[:, :, ::3], wide[:, 1:2].expand(2, 5, 12, 128)):
+        o, lse = kv4_attn(q, c, return_lse=True)
+        _check_attn(r, q, o, lse, None, None)
+        w = kv4_key_weights(q, c, lse)
+        assert torch.equal(w, kv4_key_weights(q.contiguous(), c, lse))
+
+
+def test_lengths_out_of_range_read_nothing_wrong(gpu):
+    """Entries that no append leaves: every slot is still in range and rows without a
+    position are empty."""
+    c, _ = _pair(3, 1, 64, 64, BF, (64, 64, 64))
+    c.lengths.copy_(torch.tensor([-7, 2 ** 31 - 1, 3], dtype=torch.int32))
+    q = _rand(1, 3, 8, 2, 64).cuda()
+    o, lse = kv4_attn(q, c, return_lse=True)
+    assert (o[0] == 0).all() and (lse[0] == -math.inf).all()
+    assert torch.isfinite(o).all()
+    assert (lse[2, :, :5] == -math.inf).all() and torch.isfinite(lse[2, :, 5:]).all()
+    kv4_key_weights(q, c, lse)
+    kv4_evict(c, torch.rand(3, 1, 64, device=gpu), 32)
+    for x in kv4_read(c, 10):
+        assert (x[0] == 0).all()
+
+
+# ---------------------------------------------------------------- key weights
+
+@pytest.mark.parametrize("B,T,Hq,H,D,C,lengths,window,counts,dtype", ATTN)
+def test_key_weights_match_64_bits(gpu, B, T, Hq, H, D, C, lengths, window, counts, dtype):
+    c, r = _pair(B, H, D, C, dtype, lengths, seed=T + D)
+    q = _rand(11, B, T, Hq, D, dtype=dtype, scale=1.5)
+    n = None if counts is None else torch.tensor(counts, dtype=torch.int32)
+    nc = None if n is None else n.cuda()
+    if n is not None:
+        for b in range(B):
+            q[b, n[b]:] = math.nan
+    _, lse = kv4_attn(q.cuda(), c, window, counts=nc, return_lse=True)
+    w = kv4_key_weights(q.cuda(), c, lse, window, counts=nc)
+    want = r.key_weights(q, lse, window, n)
+    rows = T * (Hq // H)
+    top = 0 if not torch.isfinite(lse).any() else lse[torch.isfinite(lse)].abs().max().item()
+    d = _score_error(r, q)[:, None, None] + 8 * E * (1 + 2 * top) + (rows / 16 + 16) * E
+    assert w.shape == (B, H, C)
+    assert ((w.double().cpu() - want).abs() <= 2 * d * want + 1e-30).all()
+    # accumulated, and every weight is some row's: their sum is the number of rows
+    twice = kv4_key_weights(q.cuda(), c, lse, window, counts=nc, out=w.clone(), accumulate=True)
+    assert torch.equal(twice, 2 * w)
+    seen = torch.isfinite(lse).view(B, H, -1).sum(-1).double().cpu()
+    assert ((w.double().sum(-1).cpu() - seen).abs() <= 1e-3 * seen).all()
+
+
+# ------------------------------------------------------------------- eviction
+
+def _evict_case(c, r, w, keep, recent, out=None):
+    new, index, nw = kv4_evict(c, w, keep, recent, out=out)
+    wi, ww = r.evict(w.cpu(), keep, recent)
+    assert torch.equal(index.cpu(), wi)
+    assert torch.equal(torch.nan_to_num(nw[..., :keep].cpu(), nan=9.0),
+                       torch.nan_to_num(ww, nan=9.0))
+    assert (nw[..., keep:] == 0).all()
+    rn = r.take(wi, new.capacity)
+    assert new.lengths.tolist() == [rn.length(b) for b in range(r.B)]
+    for x, y in zip(kv4_read(new, keep), rn.read(keep)):
+        assert torch.equal(x.cpu(), y)
+    return new, rn
+
+
+@pytest.mark.parametrize("keep,recent", [(1, 0), (1, 5), (20, 0), (20, 7), (20, 20), (64, 3),
+                                         (63, 0), (50, 100)])
+@pytest.mark.parametrize("kind", ["random", "ties", "signs"])
+def test_evict_keeps_the_heaviest(gpu, keep, recent, kind):
+    c, r = _pair(4, 2, 64, 64, BF, (0, 13, 64, 150))
+    g = torch.Generator().manual_seed(keep + recent)
+    w = torch.rand(4, 2, 64, generator=g)
+    if kind == "ties":
+        w = (w * 4).floor()
+    elif kind == "signs":
+        w = (w - 0.5) * 1e-3
+        w[..., ::7] = -0.0
+        w[..., 3::7] = 0.0
+        w[..., 5::11] = math.nan
+        w[..., 6::11] = math.inf
+        w[..., 8::11] = -math.inf
+    _evict_case(c, r, w.cuda(), keep, recent)
+
+
+@pytest.mark.parametrize("C,lengths,keep,recent,dtype", [
+    (4096, (4096, 9001), 1500, 100, HF), (8192, (8000, 5), 4095, 0, BF),
+    (2048, (1025, 2048), 1024, 1024, BF)])
+def test_evict_of_long_caches(gpu, C, lengths, keep, recent, dtype):
+    c, r = _pair(2, 2, 128, C, dtype, lengths)
+    g = torch.Generator().manual_seed(C)
+    for w in (torch.rand(2, 2, C, generator=g).log().square(),
+              torch.randint(0, 3, (2, 2, C), generator=g).float(), torch.ones(2, 2, C)):
+        _evict_case(c, r, w.cuda(), keep, recent)
+
+
+def test_evict_into_another_cache(gpu):
+    c, r = _pair(2, 2, 64, 64, BF, (64, 10))
+    out = KV4Cache(2, 2, 64, 32, weights=True)
+    w = torch.rand(2, 2, 64, device=gpu)
+    new, _ = _evict_case(c, r, w, 32, 4, out)
+    assert new is out
+    with pytest.raises(ValueError):
+        kv4_evict(c, w, 33, out=out)
+    with pytest.raises(ValueError):
+        kv4_evict(c, w, 8, out=c)
+    with pytest.raises(ValueError):
+        kv4_evict(c, None, 8)
+    with pytest.raises(ValueError):
+        kv4_evict(c, w, 8, out=KV4Cache(2, 2, 64, 32, HF))
+
+
+# ------------------------------------------------------------------- together
+
+@pytest.mark.parametrize("dtype,D,Hq,H", [(BF, 128, 4, 2), (HF, 64, 9, 3)])
+def test_prefill_decode_evict_and_on(gpu, dtype, D, Hq, H):
+    """A prompt in chunks, tokens one by one, a cut by accumulated weight, more tokens:
+    every output against the oracle's own cache."""
+    B, C = 2, 160
+    c, r = _pair(B, H, D, C, dtype, weights=True)
+    acc = torch.zeros(B, H, C, dtype=torch.float64)
+
+    def step(T, seed):
+        k, v = _rand(seed, B, T, H, D, dtype=dtype), _rand(seed + 1, B, T, H, D, dtype=dtype)
+        q = _rand(seed + 2, B, T, Hq, D, dtype=dtype, scale=2.0)
+        kv4_append(c, k.cuda(), v.cuda())
+        r.append(k, v)
+        o, lse = kv4_attn(q.cuda(), c, return_lse=True)
+        _check_attn(r, q, o, lse, None, None)
+        kv4_key_weights(q.cuda(), c, lse, out=c.weights, accumulate=True)
+        acc.add_(r.key_weights(q, lse))
+
+    for i, T in enumerate((60, 37, 1, 1, 1, 20, 1)):
+        step(T, 10 * i)
+    assert torch.allclose(c.weights.double().cpu(), acc, rtol=1e-3, atol=1e-6)
+    index, _ = r.evict(c.weights.cpu(), 48, 16)
+    new, got, w = kv4_evict(c, None, 48, 16)
+    assert torch.equal(got.cpu(), index) and new.weights is w
+    r, c = r.take(index, C), new
+    acc = w.double().cpu()
+    for i, T in enumerate((1, 1, 30, 1)):
+        step(T, 1000 + 10 * i)
+    assert torch.allclose(c.weights.double().cpu(), acc, rtol=1e-3, atol=1e-6)
+
+
+def test_another_stream(gpu):
+    c, r = _pair(1, 2, 64, 256, BF, (200,))
+    k, v, q = (_rand(i, 1, 9, h, 64).cuda() for i, h in ((1, 2), (2, 2), (3, 4)))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        kv4_append(c, k, v)
+        o, lse = kv4_attn(q, c, return_lse=True)
+        w = kv4_key_weights(q, c, lse)
+        new, index, _ = kv4_evict(c, w, 100)
+        got = kv4_read(new, 100)
+    torch.cuda.current_stream().wait_stream(s)
+    r.append(k, v)
+    _check_attn(r, q, o, lse, None, None)
+    wi, _ = r.evict(w.cpu(), 100, 0)
+    assert torch.equal(index.cpu(), wi)
+    for x, y in zip(got, r.take(wi, 256).read(100)):
+        assert torch.equal(x.cpu(), y)
+
+
+def test_a_captured_step_decodes_on(gpu):
+    """One decode step in a graph (append, attention split over keys, key weights):
+    each replay is the next position, over the ring's end, with eager work between."""
+    B, H, Hq, D, C = 2, 2, 8, 64, 2048
+    c, r = _pair(B, H, D, C, BF, (2040, 300), weights=True)
+    k, v, q = (torch.zeros(B, 1, h, D, dtype=BF, device=gpu) for h in (H, H, Hq))
+
+    def step():
+        kv4_append(c, k, v)
+        o, lse = kv4_attn(q, c, return_lse=True)
+        kv4_key_weights(q, c, lse, out=c.weights, accumulate=True)
+        return o, lse
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        kept = [t.clone() for t in (c.k_codes, c.k_scales, c.v_codes, c.v_scales, c.lengths)]
+        step()
+        for t, x in zip((c.k_codes, c.k_scales, c.v_codes, c.v_scales, c.lengths), kept):
+            t.copy_(x)
+        c.weights.zero_()
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o, lse = step()
+    acc = torch.zeros(B, H, C, dtype=torch.float64)
+    for i in range(12):
+        kn, vn = _rand(40 + i, B, 1, H, D), _rand(80 + i, B, 1, H, D)
+        qn = _rand(120 + i, B, 1, Hq, D, scale=2.0)
+        k.copy_(kn)
+        v.copy_(vn)
+        q.copy_(qn)
+        g.replay()
+        r.append(kn, vn)
+        _check_attn(r, qn, o, lse, None, None)
+        new = torch.stack([torch.arange(C) == (r.length(b) - 1) % C for b in range(B)])[:, None]
+        acc = acc.masked_fill(new, 0) + r.key_weights(qn, lse)
+        eager = kv4_attn(q, c)
+        assert torch.equal(eager, o)
+        torch.cuda.synchronize()
+    assert torch.allclose(c.weights.double().cpu(), acc, rtol=1e-3, atol=1e-6)
+
+
+def test_offsets_past_32_bits(gpu):
+    """Codes of more than 4 GiB: the last sequence's rows lie behind them."""
+    B, H, D, C = 66, 8, 128, 131072
+    c = KV4Cache(B, H, D, C)
+    assert c.k_codes.numel() > 2 ** 32
+    r = kv4_ref.Ref(1, H, D, C)
+    n = torch.zeros(B, dtype=torch.int32, device=gpu)
+    n[-1] = 40
+    k, v = _rand(1, 1, 40, H, D), _rand(2, 1, 40, H, D)
+    wide = [x.cuda().expand(B, 40, H, D) for x in (k, v)]
+    c.lengths[-1] = C - 17  # over the ring's end
+    kv4_append(c, *wide, counts=n)
+    r.append(k, v)
+    for x, y in zip(kv4_read(c, 40), r.read(40)):
+        assert torch.equal(x[-1:].cpu(), y)
+    q = _rand(3, 1, 2, 16, D)
+    o, lse = kv4_attn(q.cuda().expand(B, 2, 16, D).contiguous(), c, 30, return_lse=True)
+    _check_attn(r, q, o[-1:], lse[-1:], 30, None)
+    w = kv4_key_weights(q.cuda().expand(B, 2, 16, D).contiguous(), c, lse, 30)
+    want = r.key_weights(q, lse[-1:], 30)[0]
+    at = (C - 17 + torch.arange(40)) % C
+    assert torch.allclose(w[-1][:, at.cuda()].double().cpu(), want[:, :40], rtol=1e-4, atol=1e-9)
+    new, index, _ = kv4_evict(c, w, 20, 4, out=KV4Cache(B, H, D, 32))
+    assert new.lengths.tolist()[-1] == 20 and int(index[-1].max()) == C + 22
+
+
+def test_refusals(gpu):
+    c = KV4Cache(2, 2, 64, 64)
+    x = _rand(1, 2, 4, 2, 64).cuda()
+    q = _rand(1, 2, 4, 4, 64).cuda()
+    lse = torch.zeros(2, 4, 4, device=gpu)
+    n = torch.zeros(2, dtype=torch.int32, device=gpu)
+    bad = [lambda: kv4_append(c, x[:1], x[:1]), lambda: kv4_append(c, x, x[:, :3]),
+           lambda: kv4_append(c, x.half(), x.half()), lambda: kv4_append(c, q, q),
+           lambda: kv4_append(c, x.cpu(), x.cpu()), lambda: kv4_append(c, x[0], x[0]),
+           lambda: kv4_append(c, x, x, counts=n.long()), lambda: kv4_append(c, x, x, counts=n[:1]),
+           lambda: kv4_append(c, *[x[:, :1].expand(2, 65, 2, 64)] * 2),
+           lambda: kv4_attn(q[..., :32], c), lambda: kv4_attn(q[:, :, :3], c),
+           lambda: kv4_attn(q, c, 0), lambda: kv4_attn(q, c, counts=n.cpu()),
+           lambda: kv4_key_weights(q, c, lse[:, :, :3]), lambda: kv4_key_weights(q, c, lse.double()),
+           lambda: kv4_key_weights(q, c, lse, accumulate=True),
+           lambda: kv4_key_weights(q, c, lse, out=torch.zeros(2, 2, 32, device=gpu)),
+           lambda: kv4_read(c, -1), lambda: kv4_evict(c, torch.zeros(2, 2, 32, device=gpu), 4),
+           lambda: kv4_evict(c, torch.zeros(2, 2, 64, device=gpu), 0),
+           lambda: kv4_evict(c, torch.zeros(2, 2, 64, device=gpu), 4, -1),
+           lambda: KV4Cache.from_parts(c.k_codes, c.k_scales, c.v_codes, c.v_codes, c.lengths),
+           lambda: KV4Cache.from_parts(c.k_codes[:, :, ::2], c.k_scales, c.v_codes, c.v_scales,
+                                       c.lengths)]
+    for f in bad:
+        with pytest.raises(ValueError):
+            f()
+    with pytest.raises(RuntimeError, match="forward-only"):
+        kv4_attn(q.clone().requires_grad_(), c)
+    assert kv4_attn(q[:, :0], c).shape == (2, 0, 4, 64)
+    kv4_append(c, x[:, :0], x[:, :0])
+    assert (kv4_key_weights(q[:, :0], c, lse[:, :, :0]) == 0).all()
+    assert c.lengths.tolist() == [0, 0]
+    c.lengths.fill_(5)
+    c.reset()
+    assert c.lengths.tolist() == [0, 0]

@@ -58,6 +58,12 @@ EXPORTS = (
     "ttcd_ttt_proj_beta_t_fwd",
     "ttcd_ttt_beta_fwd",
     "ttcd_ttt_scan_fwd",
+    "ttcd_kv4_append",
+    "ttcd_kv4_read",
+    "ttcd_kv4_attn_workspace_bytes",
+    "ttcd_kv4_attn_fwd",
+    "ttcd_kv4_key_weights_fwd",
+    "ttcd_kv4_evict",
     "ttcd_attn_schedule_coverage",
     "ttcd_attn_block_coverage",
 )
@@ -68,6 +74,16 @@ _vp = ctypes.c_void_p
 _fp = ctypes.c_void_p  # float* passed as a raw address
 _i64x4 = ctypes.POINTER(ctypes.c_int64)
 _i64x3 = ctypes.POINTER(ctypes.c_int64)
+
+
+class KV4CacheStruct(ctypes.Structure):
+    """ttcd_kv4_cache of include/ttcd.h."""
+    _fields_ = [("k_codes", _vp), ("k_scales", _vp), ("v_codes", _vp), ("v_scales", _vp),
+                ("lengths", _vp), ("batch", _i32), ("kv_heads", _i32), ("head_dim", _i32),
+                ("capacity", _i32)]
+
+
+_kv4 = ctypes.POINTER(KV4CacheStruct)
 
 _SIGS = {
     "ttcd_status_string": (ctypes.c_char_p, [_i32]),
@@ -157,6 +173,15 @@ _SIGS = {
     "ttcd_ttt_beta_fwd": (_i32, [_vp, _i64, _vp, _vp, _i32, _i32, _i32, _i32, _vp]),
     "ttcd_ttt_scan_fwd": (_i32, [
         _vp, _vp, ctypes.c_float, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "ttcd_kv4_append": (_i32, [_kv4, _vp, _vp, _i32, _i64x4, _i64x4, _vp, _fp, _i32, _vp]),
+    "ttcd_kv4_read": (_i32, [_kv4, _vp, _vp, _i32, _i32, _vp]),
+    "ttcd_kv4_attn_workspace_bytes": (ctypes.c_size_t, [_kv4, _i32, _i32, _i32]),
+    "ttcd_kv4_attn_fwd": (_i32, [
+        _kv4, _vp, _vp, _fp, _i32, _i32, _i64x4, _i64x4, _vp, _i32, ctypes.c_float, _i32, _vp,
+        ctypes.c_size_t, _vp]),
+    "ttcd_kv4_key_weights_fwd": (_i32, [
+        _kv4, _vp, _fp, _fp, _i32, _i32, _i64x4, _vp, _i32, ctypes.c_float, _i32, _i32, _vp]),
+    "ttcd_kv4_evict": (_i32, [_kv4, _fp, _i32, _i32, _kv4, _fp, _vp, _vp]),
     "ttcd_attn_schedule_coverage": (_i32, [
         _i32, _i32, _i32, _i32, _i32, _vp, _vp]),
     "ttcd_attn_block_coverage": (_i32, [_i32, _i32, _i32, _i32, _vp, _vp]),

@@ -1135,6 +1135,264 @@ ttcd_status ttcd_ttt_scan_fwd(const void* dw, const void* w_cur, float lr, void*
                   "ttt scan launch");
 }
 
+// ---------------------------------------------------------------------------
+// The 4-bit key / value cache.
+namespace {
+
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+ttcd_status check_kv4(const ttcd_kv4_cache* c) {
+  if (!c || !c->k_codes || !c->k_scales || !c->v_codes || !c->v_scales || !c->lengths)
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "null cache pointer");
+  if (c->batch < 1 || c->kv_heads < 1)
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "need batch, kv_heads >= 1 (got %d, %d)", c->batch,
+                c->kv_heads);
+  if (c->head_dim != 64 && c->head_dim != 128)
+    return fail(TTCD_ERR_UNSUPPORTED, "head_dim %d not supported (64 or 128)", c->head_dim);
+  if (c->capacity < 32 || c->capacity % 32 != 0 || c->capacity > ttcd::kKv4MaxLength)
+    return fail(TTCD_ERR_INVALID_ARGUMENT,
+                "capacity must be a multiple of 32 in 32 .. 2^30 (got %d)", c->capacity);
+  if (!aligned16(c->k_codes) || !aligned16(c->v_codes) || !aligned4(c->v_scales) ||
+      !aligned4(c->lengths))
+    return fail(TTCD_ERR_UNSUPPORTED,
+                "codes must be 16-byte aligned, v_scales and lengths 4-byte aligned");
+  if ((int64_t)c->batch * c->kv_heads > 65535)
+    return fail(TTCD_ERR_UNSUPPORTED, "batch * kv_heads above 65535 (grid y)");
+  return TTCD_OK;
+}
+
+ttcd::Kv4Cache kv4(const ttcd_kv4_cache* c) {
+  return {static_cast<uint8_t*>(c->k_codes), static_cast<uint8_t*>(c->k_scales),
+          static_cast<uint8_t*>(c->v_codes), static_cast<uint8_t*>(c->v_scales),
+          c->lengths, c->batch, c->kv_heads, c->head_dim, c->capacity};
+}
+
+ttcd_status check_kv4_dtype(ttcd_dtype dtype) {
+  if (dtype != TTCD_DTYPE_BF16 && dtype != TTCD_DTYPE_F16)
+    return fail(TTCD_ERR_UNSUPPORTED, "dtype must be bf16 or f16");
+  return TTCD_OK;
+}
+
+ttcd_status check_kv4_strides(const void* p, const int64_t* s) {
+  if (!p) return fail(TTCD_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (!s) return fail(TTCD_ERR_INVALID_ARGUMENT, "null stride array");
+  if (s[3] != 1) return fail(TTCD_ERR_INVALID_ARGUMENT, "head_dim must be contiguous (d-stride 1)");
+  for (int i = 0; i < 3; ++i)
+    if (s[i] % 8 != 0 || s[i] < 0)
+      return fail(TTCD_ERR_UNSUPPORTED,
+                  "strides must be non-negative multiples of 8 elements (16-byte rows)");
+  if (!aligned16(p))
+    return fail(TTCD_ERR_UNSUPPORTED, "tensor base pointers must be 16-byte aligned");
+  return TTCD_OK;
+}
+
+ttcd_status check_kv4_rows(const ttcd_kv4_cache* c, int Tq, int Hq) {
+  if (Tq < 1 || Hq < 1)
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "need Tq, Hq >= 1 (got %d, %d)", Tq, Hq);
+  if (Hq % c->kv_heads != 0)
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "Hq (%d) must be a multiple of kv_heads (%d)", Hq,
+                c->kv_heads);
+  // a workgroup a row of the sum over the parts
+  if ((int64_t)c->batch * Hq * Tq > 0x7fffffffLL - 1024)
+    return fail(TTCD_ERR_UNSUPPORTED, "grid too large");
+  return TTCD_OK;
+}
+
+int kv4_window(int window) {
+  return window <= 0 ? 0 : (window < ttcd::kKv4MaxLength ? window : ttcd::kKv4MaxLength);
+}
+
+struct Kv4Plan {
+  int row_tiles, nrb, parts;
+};
+
+// Workgroups over rows and keys. The lengths are on the GPU: parts go by the most
+// keys that a row block can see, and each takes its share of what there is.
+Kv4Plan kv4_plan(const ttcd_kv4_cache* c, int Tq, int Hq, int window) {
+  const int G = Hq / c->kv_heads;
+  const int64_t rows = (int64_t)Tq * G;
+  Kv4Plan p;
+  p.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  const int rb = 16 * p.row_tiles;
+  p.nrb = (int)((rows + rb - 1) / rb);
+  int64_t keys = c->capacity;
+  if (window > 0) {
+    const int64_t span = (int64_t)window + (rb + G - 1) / G;
+    keys = span < keys ? span : keys;
+  }
+  const int64_t tiles = keys / 32 + 1, groups = (int64_t)c->batch * c->kv_heads * p.nrb;
+  int64_t parts = (1024 + groups - 1) / groups;
+  if (parts > tiles / 8) parts = tiles / 8;
+  p.parts = parts < 1 ? 1 : (int)parts;
+  return p;
+}
+
+size_t kv4_part_bytes(const ttcd_kv4_cache* c, int Tq, int Hq) {
+  return (size_t)c->batch * Tq * Hq * (c->head_dim + 2) * sizeof(float);
+}
+
+}  // namespace
+
+ttcd_status ttcd_kv4_append(ttcd_kv4_cache* cache, const void* k, const void* v, int T,
+                            const int64_t k_stride[4], const int64_t v_stride[4],
+                            const int32_t* counts, float* weights, ttcd_dtype dtype,
+                            void* stream) {
+  ttcd_status st = check_kv4(cache);
+  if (st == TTCD_OK) st = check_kv4_dtype(dtype);
+  if (st == TTCD_OK) st = check_kv4_strides(k, k_stride);
+  if (st == TTCD_OK) st = check_kv4_strides(v, v_stride);
+  if (st != TTCD_OK) return st;
+  if (T < 1 || T > cache->capacity)
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "need 1 <= T <= capacity (got T=%d, capacity %d)", T,
+                cache->capacity);
+  ttcd::Kv4AppendArgs a = {};
+  a.c = kv4(cache);
+  a.k = k;
+  a.v = v;
+  a.k_sb = k_stride[0];
+  a.k_st = k_stride[1];
+  a.k_sh = k_stride[2];
+  a.v_sb = v_stride[0];
+  a.v_st = v_stride[1];
+  a.v_sh = v_stride[2];
+  a.counts = counts;
+  a.weights = weights;
+  a.T = T;
+  return from_hip(ttcd::launch_kv4_append(a, elem(dtype), static_cast<hipStream_t>(stream)),
+                  "kv4 append launch");
+}
+
+ttcd_status ttcd_kv4_read(const ttcd_kv4_cache* cache, void* k, void* v, int count,
+                          ttcd_dtype dtype, void* stream) {
+  ttcd_status st = check_kv4(cache);
+  if (st == TTCD_OK) st = check_kv4_dtype(dtype);
+  if (st != TTCD_OK) return st;
+  if (!k || !v) return fail(TTCD_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (!aligned16(k) || !aligned16(v))
+    return fail(TTCD_ERR_UNSUPPORTED, "tensor base pointers must be 16-byte aligned");
+  if (count < 1) return fail(TTCD_ERR_INVALID_ARGUMENT, "need count >= 1 (got %d)", count);
+  const int64_t blocks = ((int64_t)(count + 3LL) / 4 + 1) * cache->kv_heads * (cache->head_dim / 8);
+  if (blocks / 256 >= 0x7fffffffLL) return fail(TTCD_ERR_UNSUPPORTED, "grid too large");
+  ttcd::Kv4ReadArgs a = {kv4(cache), k, v, count};
+  return from_hip(ttcd::launch_kv4_read(a, elem(dtype), static_cast<hipStream_t>(stream)),
+                  "kv4 read launch");
+}
+
+size_t ttcd_kv4_attn_workspace_bytes(const ttcd_kv4_cache* cache, int Tq, int Hq, int window) {
+  if (!cache || cache->batch < 1 || cache->kv_heads < 1 || Tq < 1 || Hq < cache->kv_heads ||
+      Hq % cache->kv_heads != 0 || (cache->head_dim != 64 && cache->head_dim != 128) ||
+      cache->capacity < 32)
+    return 0;
+  const Kv4Plan p = kv4_plan(cache, Tq, Hq, kv4_window(window));
+  return p.parts > 1 ? p.parts * kv4_part_bytes(cache, Tq, Hq) : 0;
+}
+
+ttcd_status ttcd_kv4_attn_fwd(const ttcd_kv4_cache* cache, const void* q, void* o, float* lse,
+                              int Tq, int Hq, const int64_t q_stride[4],
+                              const int64_t o_stride[4], const int32_t* counts, int window,
+                              float sm_scale, ttcd_dtype dtype, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  ttcd_status st = check_kv4(cache);
+  if (st == TTCD_OK) st = check_kv4_dtype(dtype);
+  if (st == TTCD_OK) st = check_kv4_strides(q, q_stride);
+  if (st == TTCD_OK) st = check_kv4_strides(o, o_stride);
+  if (st == TTCD_OK) st = check_kv4_rows(cache, Tq, Hq);
+  if (st != TTCD_OK) return st;
+  if (!(sm_scale > 0.f) || !isfinite(sm_scale))
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "sm_scale must be finite and > 0");
+  ttcd::Kv4AttnArgs a = {};
+  a.c = kv4(cache);
+  a.q = q;
+  a.o = o;
+  a.lse = lse;
+  a.counts = counts;
+  a.q_sb = q_stride[0];
+  a.q_st = q_stride[1];
+  a.q_sh = q_stride[2];
+  a.o_sb = o_stride[0];
+  a.o_st = o_stride[1];
+  a.o_sh = o_stride[2];
+  a.Tq = Tq;
+  a.G = Hq / cache->kv_heads;
+  a.window = kv4_window(window);
+  a.c_log2 = sm_scale * 1.4426950408889634f;
+  const Kv4Plan p = kv4_plan(cache, Tq, Hq, a.window);
+  a.row_tiles = p.row_tiles;
+  a.nrb = p.nrb;
+  a.parts = 1;
+  const size_t part = kv4_part_bytes(cache, Tq, Hq);
+  if (p.parts > 1 && workspace && aligned16(workspace) && workspace_bytes >= p.parts * part) {
+    a.parts = p.parts;
+    a.part = static_cast<float*>(workspace);
+    a.part_ml = a.part + p.parts * (part / sizeof(float) / (cache->head_dim + 2)) * cache->head_dim;
+  }
+  return from_hip(ttcd::launch_kv4_attn(a, elem(dtype), static_cast<hipStream_t>(stream)),
+                  "kv4 attention launch");
+}
+
+ttcd_status ttcd_kv4_key_weights_fwd(const ttcd_kv4_cache* cache, const void* q,
+                                     const float* lse, float* weights, int Tq, int Hq,
+                                     const int64_t q_stride[4], const int32_t* counts,
+                                     int window, float sm_scale, int accumulate,
+                                     ttcd_dtype dtype, void* stream) {
+  ttcd_status st = check_kv4(cache);
+  if (st == TTCD_OK) st = check_kv4_dtype(dtype);
+  if (st == TTCD_OK) st = check_kv4_strides(q, q_stride);
+  if (st == TTCD_OK) st = check_kv4_rows(cache, Tq, Hq);
+  if (st != TTCD_OK) return st;
+  if (!lse || !weights) return fail(TTCD_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (!(sm_scale > 0.f) || !isfinite(sm_scale))
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "sm_scale must be finite and > 0");
+  if ((int64_t)cache->batch * cache->kv_heads * (cache->capacity / 32) > 0x7fffffffLL)
+    return fail(TTCD_ERR_UNSUPPORTED, "grid too large");
+  ttcd::Kv4WeightsArgs a = {};
+  a.c = kv4(cache);
+  a.q = q;
+  a.lse = lse;
+  a.weights = weights;
+  a.counts = counts;
+  a.q_sb = q_stride[0];
+  a.q_st = q_stride[1];
+  a.q_sh = q_stride[2];
+  a.Tq = Tq;
+  a.G = Hq / cache->kv_heads;
+  a.window = kv4_window(window);
+  a.c_log2 = sm_scale * 1.4426950408889634f;
+  a.accumulate = accumulate != 0;
+  return from_hip(ttcd::launch_kv4_weights(a, elem(dtype), static_cast<hipStream_t>(stream)),
+                  "kv4 key weights launch");
+}
+
+ttcd_status ttcd_kv4_evict(const ttcd_kv4_cache* cache, const float* weights, int keep,
+                           int recent, ttcd_kv4_cache* out, float* new_weights, int32_t* index,
+                           void* stream) {
+  ttcd_status st = check_kv4(cache);
+  if (st == TTCD_OK) st = check_kv4(out);
+  if (st != TTCD_OK) return st;
+  if (!weights || !index) return fail(TTCD_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (out->batch != cache->batch || out->kv_heads != cache->kv_heads ||
+      out->head_dim != cache->head_dim)
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "out must have the cache's batch, kv_heads and head_dim");
+  if (keep < 1 || keep > out->capacity || recent < 0)
+    return fail(TTCD_ERR_INVALID_ARGUMENT,
+                "need 1 <= keep <= out's capacity and recent >= 0 (got %d, %d, %d)", keep,
+                out->capacity, recent);
+  if (out->k_codes == cache->k_codes || out->k_scales == cache->k_scales ||
+      out->v_codes == cache->v_codes || out->v_scales == cache->v_scales ||
+      out->lengths == cache->lengths || new_weights == weights)
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "out must not share memory with the cache");
+  ttcd::Kv4EvictArgs a = {};
+  a.c = kv4(cache);
+  a.out = kv4(out);
+  a.weights = weights;
+  a.new_weights = new_weights;
+  a.index = index;
+  a.keep = keep;
+  a.recent = recent;
+  return from_hip(ttcd::launch_kv4_evict(a, static_cast<hipStream_t>(stream)),
+                  "kv4 eviction launch");
+}
+
 ttcd_status ttcd_attn_schedule_coverage(int T, int dual, int window_s, int window_t,
                                         int gqa_group, int32_t* counts_near,
                                         int32_t* counts_far) {

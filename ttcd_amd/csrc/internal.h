@@ -1,6 +1,6 @@
 // internal.h - launcher interface between the C ABI (api.hip) and the
 // gfx950 kernels (attn.hip, conv.hip, merge.hip, prologue.hip, epilogue.hip,
-// ttt.hip, linear.hip).
+// ttt.hip, linear.hip, kv4.hip).
 // Not part of the ABI.
 #pragma once
 
@@ -188,5 +188,78 @@ struct CombineArgs {
   int64_t sb, st, sh;     // strides of o and o_near
 };
 hipError_t launch_attn_combine(const CombineArgs& a, Elem dtype, hipStream_t stream);
+
+// The 4-bit key / value cache (kv4.hip; its format is told there).
+constexpr int kKv4MaxLength = 1 << 30;  // positions of a sequence
+
+struct Kv4Cache {
+  uint8_t* kc;  // (B, H, C, D / 2)
+  uint8_t* ks;  // (B, H, C, D / 32)
+  uint8_t* vc;  // (B, H, C / 4, D / 8, 4, 4)
+  uint8_t* vs;  // (B, H, C / 4, D / 32, 4)
+  int32_t* len; // (B) positions that a sequence has had
+  int B, H, D, C;
+};
+
+struct Kv4AppendArgs {
+  Kv4Cache c;
+  const void* k;  // (B, T, H, D), d-stride 1
+  const void* v;
+  int64_t k_sb, k_st, k_sh;
+  int64_t v_sb, v_st, v_sh;
+  const int32_t* counts;  // new positions of each sequence, or null: T
+  float* weights;         // (B, H, C), or null: 0 in the slots that are written
+  int T;
+};
+hipError_t launch_kv4_append(const Kv4AppendArgs& a, Elem dtype, hipStream_t stream);
+
+struct Kv4ReadArgs {
+  Kv4Cache c;
+  void* k;  // (B, count, H, D) contiguous
+  void* v;
+  int count;
+};
+hipError_t launch_kv4_read(const Kv4ReadArgs& a, Elem dtype, hipStream_t stream);
+
+struct Kv4AttnArgs {
+  Kv4Cache c;
+  const void* q;  // (B, Tq, H * G, D)
+  void* o;
+  float* lse;     // (B, H * G, Tq), or null
+  const int32_t* counts;
+  int64_t q_sb, q_st, q_sh;
+  int64_t o_sb, o_st, o_sh;
+  int Tq, G;
+  int window;     // <= 0: none
+  float c_log2;   // sm_scale * log2(e)
+  int row_tiles;  // tiles of 16 rows (position, head of the group) a workgroup
+  int nrb;        // workgroups over the rows of a key / value head
+  int parts;      // workgroups over the keys
+  float* part;    // parts > 1: (parts, B, H, Tq * G, D) sums and (.., 2) maximum, sum
+  float* part_ml;
+};
+hipError_t launch_kv4_attn(const Kv4AttnArgs& a, Elem dtype, hipStream_t stream);
+
+struct Kv4WeightsArgs {
+  Kv4Cache c;
+  const void* q;
+  const float* lse;
+  float* weights;  // (B, H, C)
+  const int32_t* counts;
+  int64_t q_sb, q_st, q_sh;
+  int Tq, G, window;
+  float c_log2;
+  bool accumulate;
+};
+hipError_t launch_kv4_weights(const Kv4WeightsArgs& a, Elem dtype, hipStream_t stream);
+
+struct Kv4EvictArgs {
+  Kv4Cache c, out;
+  const float* weights;  // (B, H, C)
+  float* new_weights;    // (B, H, out.C), or null
+  int32_t* index;        // (B, H, keep)
+  int keep, recent;
+};
+hipError_t launch_kv4_evict(const Kv4EvictArgs& a, hipStream_t stream);
 
 }  // namespace ttcd

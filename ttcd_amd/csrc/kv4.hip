@@ -1,0 +1,977 @@
+// kv4.hip - a key / value cache held in 4 bits: quantising new rows into it,
+// reading them back, attention over it, the attention weight of its keys and
+// the eviction of those with the least, on gfx950.
+//
+// Format. Blocks of 32 channels of one position share a power of two 2^e
+// (byte e + 127); a value is a sign and one of 0, .5, 1, 1.5, 2, 3, 4, 6
+// (e2m1), rounded to nearest even. e is the least with no value over 6 2^e, so
+// nothing but an infinity is clipped: the largest value of a block weighs most
+// in a dot product. Scales are powers of two because every held value is then
+// exact in bf16 and f16 (the range of e sees to that, below): gfx950 converts
+// pairs of codes to either in one instruction, products with q are exact in an
+// MFMA, and no code depends on how a division rounds.
+//
+// Position p is in slot p % C, C a multiple of 32, so 32 positions from a
+// multiple of 32 on are 32 slots in a row, wherever the ring has wrapped. A
+// key is the A operand of K q^T as it lies: lane (m, quarter) of a 16-key tile
+// reads a quarter of row m. A value has to be read by channel over 8 keys, so
+// words of 8 channels of 4 neighbouring slots lie side by side: lane r reads
+// the words of channels 8 r .. of 4 keys in 16 bytes, and a transposed pair of
+// conversions is one permute.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "internal.h"
+
+namespace ttcd {
+namespace {
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr float kLn2 = 0.693147180559945309f;
+constexpr float kLog2e = 1.44269504088896341f;
+
+// The exponents of a scale keep 0.5 2^e .. 6 2^e normal numbers of bf16, and
+// numbers (normal or not) of f16.
+template <typename T>
+struct Fmt;
+template <>
+struct Fmt<__bf16> {
+  typedef bf16x2 v2;
+  typedef bf16x8 v8;
+  static constexpr int kLoExp = -125, kHiExp = 125;
+  static constexpr float kBias = 0.f;
+  template <int J>
+  static __device__ __forceinline__ uint32_t cvt(uint32_t w, float s) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, J));
+  }
+  template <int J>
+  static __device__ __forceinline__ uint32_t pack(uint32_t old, uint32_t pair, float s) {
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(old, __builtin_bit_cast(bf16x2, pair), s, J);
+  }
+  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float lo(uint32_t p) { return __uint_as_float(p << 16); }
+  static __device__ __forceinline__ float hi(uint32_t p) {
+    return __uint_as_float(p & 0xffff0000u);
+  }
+};
+template <>
+struct Fmt<_Float16> {
+  typedef f16x2 v2;
+  typedef f16x8 v8;
+  static constexpr int kLoExp = -23, kHiExp = 13;
+  static constexpr float kBias = 7.f;
+  template <int J>
+  static __device__ __forceinline__ uint32_t cvt(uint32_t w, float s) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, J));
+  }
+  template <int J>
+  static __device__ __forceinline__ uint32_t pack(uint32_t old, uint32_t pair, float s) {
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(old, __builtin_bit_cast(f16x2, pair), s, J);
+  }
+  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float lo(uint32_t p) {
+    return static_cast<float>(__builtin_bit_cast(f16x2, p)[0]);
+  }
+  static __device__ __forceinline__ float hi(uint32_t p) {
+    return static_cast<float>(__builtin_bit_cast(f16x2, p)[1]);
+  }
+};
+
+__device__ __forceinline__ float scale_of(uint32_t byte) {
+  return __uint_as_float(byte << 23);
+}
+
+// 8 codes as 8 values, channel 0 in the low half of the first register.
+template <typename T>
+__device__ __forceinline__ u32x4 values8(uint32_t w, float s) {
+  return u32x4{Fmt<T>::template cvt<0>(w, s), Fmt<T>::template cvt<1>(w, s),
+               Fmt<T>::template cvt<2>(w, s), Fmt<T>::template cvt<3>(w, s)};
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pair_of(float a, float b) {
+  typename Fmt<T>::v2 v;
+  v[0] = static_cast<T>(a);
+  v[1] = static_cast<T>(b);
+  return __builtin_bit_cast(uint32_t, v);
+}
+
+// Positions of a sequence, as its lengths entry says (a malformed one is
+// brought into range: no access depends on its value).
+__device__ __forceinline__ int length_of(const int32_t* lengths, int b) {
+  const int n = lengths[b];
+  return n < 0 ? 0 : (n > kKv4MaxLength ? kKv4MaxLength : n);
+}
+
+__device__ __forceinline__ int count_of(const int32_t* counts, int b, int T) {
+  if (counts == nullptr) return T;
+  const int n = counts[b];
+  return n < 0 ? 0 : (n > T ? T : n);
+}
+
+// ---------------------------------------------------------------------------
+// Append. 4 slots in a row (a word group of the values) of one head are D / 2
+// threads, each with 8 channels of one of them: 16 bytes in, 4 out. Threads go
+// by channel first for the keys and by slot first for the values, as either
+// lies in the cache, so a wavefront's stores are whole lines. The 4 threads of
+// a block find its largest magnitude by two shuffles.
+template <typename T, int D, bool V>
+__device__ __forceinline__ void append_word(const Kv4AppendArgs& a, int b, int h, int len,
+                                            int n_new, int group, int i) {
+  constexpr int R = D / 8;
+  const int e = V ? i & 3 : i / R, r = V ? i >> 2 : i % R;
+  const int p = ((len >> 2) + group) * 4 + e;
+  const int t = p - len;
+  const bool on = t >= 0 && t < n_new;
+  u32x4 x = {0u, 0u, 0u, 0u};
+  if (on) {
+    const T* src = static_cast<const T*>(V ? a.v : a.k) + b * (V ? a.v_sb : a.k_sb) +
+                   t * (V ? a.v_st : a.k_st) + h * (V ? a.v_sh : a.k_sh) + r * 8;
+    x = *reinterpret_cast<const u32x4*>(src);
+  }
+  // NaN counts as 0: the format holds none
+  float top = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float lo = Fmt<T>::lo(x[j]), hi = Fmt<T>::hi(x[j]);
+    if (!(lo == lo)) x[j] &= 0xffff0000u;
+    if (!(hi == hi)) x[j] &= 0x0000ffffu;
+    top = fmaxf(top, fmaxf(fabsf(lo), fabsf(hi)));  // fmaxf passes NaN over
+  }
+  // the threads of the block are 1 and 2 (keys), 4 and 8 (values) lanes away
+  top = fmaxf(top, __shfl_xor(top, V ? 4 : 1));
+  top = fmaxf(top, __shfl_xor(top, V ? 8 : 2));
+  // top = 1.f 2^E <= 1.5 2^(e + 2)
+  const uint32_t bits = __float_as_uint(top);
+  int exp = (int)(bits >> 23) - 127 - ((bits & 0x7fffffu) <= 0x400000u ? 2 : 1);
+  exp = min(max(exp, Fmt<T>::kLoExp), Fmt<T>::kHiExp);
+  const float s = scale_of((uint32_t)(exp + 127));
+  uint32_t w = Fmt<T>::template pack<0>(0u, x[0], s);
+  w = Fmt<T>::template pack<1>(w, x[1], s);
+  w = Fmt<T>::template pack<2>(w, x[2], s);
+  w = Fmt<T>::template pack<3>(w, x[3], s);
+  if (!on) return;
+  const int slot = p % a.c.C;
+  const int64_t row = ((int64_t)b * a.c.H + h) * a.c.C + slot;
+  if constexpr (V) {
+    const int64_t g = row >> 2;
+    *reinterpret_cast<uint32_t*>(a.c.vc + ((g * R + r) * 4 + e) * 4) = w;
+    if ((r & 3) == 0) a.c.vs[(g * (D / 32) + (r >> 2)) * 4 + e] = (uint8_t)(exp + 127);
+  } else {
+    *reinterpret_cast<uint32_t*>(a.c.kc + (row * R + r) * 4) = w;
+    if ((r & 3) == 0) a.c.ks[row * (D / 32) + (r >> 2)] = (uint8_t)(exp + 127);
+    if (a.weights != nullptr && r == 0) a.weights[row] = 0.f;
+  }
+}
+
+// SMALL: one workgroup writes all of a sequence's rows and then its length;
+// else the lengths are another launch's.
+template <typename T, int D, bool SMALL>
+__global__ __launch_bounds__(SMALL ? 1024 : 256) void append_kernel(Kv4AppendArgs a) {
+  constexpr int PER = D / 2;  // threads per group of 4 slots
+  const int b = SMALL ? blockIdx.x : blockIdx.y;
+  const int len = length_of(a.c.len, b), n_new = count_of(a.counts, b, a.T);
+  const int groups = ((len + n_new + 3) >> 2) - (len >> 2);
+  if constexpr (SMALL) {
+    const int items = groups * a.c.H * PER;
+    for (int i = threadIdx.x; i < items; i += 1024) {
+      const int g = i / PER;
+      append_word<T, D, false>(a, b, g % a.c.H, len, n_new, g / a.c.H, i % PER);
+      append_word<T, D, true>(a, b, g % a.c.H, len, n_new, g / a.c.H, i % PER);
+    }
+    __syncthreads();  // every thread has read the length
+    if (threadIdx.x == 0) a.c.len[b] = len + n_new;
+  } else {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int g = (int)(i / PER);
+    if (g >= groups * a.c.H) return;
+    append_word<T, D, false>(a, b, g / groups, len, n_new, g % groups, (int)(i % PER));
+    append_word<T, D, true>(a, b, g / groups, len, n_new, g % groups, (int)(i % PER));
+  }
+}
+
+__global__ void advance_kernel(Kv4AppendArgs a) {
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b < a.c.B) a.c.len[b] = length_of(a.c.len, b) + count_of(a.counts, b, a.T);
+}
+
+template <typename T, int D>
+hipError_t launch_append(const Kv4AppendArgs& a, hipStream_t st) {
+  const int64_t items = ((int64_t)(a.T + 3) / 4 + 1) * a.c.H * (D / 2);
+  if (items <= 8 * 1024) {
+    hipLaunchKernelGGL((append_kernel<T, D, true>), dim3(a.c.B), dim3(1024), 0, st, a);
+    return hipGetLastError();
+  }
+  hipLaunchKernelGGL((append_kernel<T, D, false>), dim3((unsigned)((items + 255) / 256), a.c.B),
+                     dim3(256), 0, st, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(advance_kernel, dim3((a.c.B + 255) / 256), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// Read back the last `count` positions. A thread takes 8 channels of the 4
+// slots of a group: 16 bytes of value codes in one load, 4 rows of 16 bytes out
+// for keys and for values each.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void read_kernel(Kv4ReadArgs a) {
+  constexpr int R = D / 8, BL = D / 32;
+  const int b = blockIdx.y;
+  const int len = length_of(a.c.len, b);
+  const int p0 = len - a.count;  // may be below 0
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int r = (int)(i % R), h = (int)(i / R % a.c.H);
+  const int64_t gi = i / ((int64_t)R * a.c.H);
+  const int p = (int)((int64_t)(p0 >> 2) + gi) * 4;  // floor: aligned below 0 too
+  if (p >= len) return;
+  const int first = len > a.c.C ? len - a.c.C : 0;
+  const bool any = p + 3 >= first;  // then p >= 0: first is one of the 4 at the least
+  u32x4 vw = {0u, 0u, 0u, 0u};
+  uint32_t vsw = 0u, kw[4], ksb[4];
+  if (any) {
+    const int64_t row = ((int64_t)b * a.c.H + h) * a.c.C + p % a.c.C, g = row >> 2;
+    vw = *reinterpret_cast<const u32x4*>(a.c.vc + (g * R + r) * 16);
+    vsw = *reinterpret_cast<const uint32_t*>(a.c.vs + (g * BL + (r >> 2)) * 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      kw[e] = *reinterpret_cast<const uint32_t*>(a.c.kc + ((row + e) * R + r) * 4);
+      ksb[e] = a.c.ks[(row + e) * BL + (r >> 2)];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int t = p + e - p0;
+    if (t < 0 || t >= a.count) continue;
+    const int64_t at = ((((int64_t)b * a.count + t) * a.c.H + h) * R + r) * 8;
+    u32x4 k = {0u, 0u, 0u, 0u}, v = k;
+    if (any && p + e >= first) {
+      k = values8<T>(kw[e], scale_of(ksb[e]));
+      v = values8<T>(vw[e], scale_of((vsw >> (8 * e)) & 255u));
+    }
+    *reinterpret_cast<u32x4*>(static_cast<T*>(a.k) + at) = k;
+    *reinterpret_cast<u32x4*>(static_cast<T*>(a.v) + at) = v;
+  }
+}
+
+template <typename T, int D>
+hipError_t launch_read(const Kv4ReadArgs& a, hipStream_t st) {
+  const int64_t items = ((int64_t)(a.count + 3) / 4 + 1) * a.c.H * (D / 8);
+  hipLaunchKernelGGL((read_kernel<T, D>), dim3((unsigned)((items + 255) / 256), a.c.B), dim3(256),
+                     0, st, a);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// Attention. The rows of a key / value head are its group's query heads times
+// the new positions; a wavefront holds NT tiles of 16 of them and sweeps tiles
+// of 32 keys: S^T = K Q^T (16x16x32: keys x rows), online softmax over the
+// registers, O^T = V^T P^T with P as it lies after the first product (the keys
+// of a lane's quarter are the 8 that the second product wants from it, in the
+// order in which it then reads V). The 4 wavefronts of a workgroup take every
+// fourth tile of its part of the keys and are added through LDS; the parts of a
+// row are added by a second launch.
+//
+// The reference maximum of a row moves only where a score exceeds it by more
+// than 8 (log2): up to then probabilities stay under 2^8, and the four
+// quarters of a row need not agree on a maximum at every tile. P is rounded to
+// the inputs' type for the product, as the prefill kernels round it; sums and
+// statistics are fp32. In f16 the reference is 7 lower (probabilities up to
+// 2^15), so that small ones keep 7 bits more above f16's least step.
+template <int D>
+struct KvTile {
+  u32x4 v[2];
+  uint32_t vs[2];
+  u32x4 k[2];  // D = 64: the first two words
+  uint32_t ks[2];
+};
+
+template <typename T, int D, int NT>
+struct RowState {
+  f32x4 o[NT][D / 16];
+  float m[NT], l[NT];
+};
+
+// 8 keys' values of channels (2 j, 2 j + 1) of the words w0, w1 as the two A
+// operands of those channels.
+template <typename T, int J>
+__device__ __forceinline__ void transpose_pair(const uint32_t (&w)[8], const float (&s)[8],
+                                               u32x4* even, u32x4* odd) {
+  uint32_t c[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c[e] = Fmt<T>::template cvt<J>(w[e], s[e]);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    (*even)[e] = __builtin_amdgcn_perm(c[2 * e + 1], c[2 * e], 0x05040100u);
+    (*odd)[e] = __builtin_amdgcn_perm(c[2 * e + 1], c[2 * e], 0x07060302u);
+  }
+}
+
+template <typename T, int D, int NT>
+__device__ __forceinline__ void fold_tile(RowState<T, D, NT>& st, const KvTile<D>& kv,
+                                          const u32x4 (&q)[NT][D / 32], float c, int p0, bool masked,
+                                          const int (&lo)[NT], const int (&hi)[NT], int len,
+                                          int lane) {
+  constexpr int STEPS = D / 32, NM = D / 16;
+  const int quarter = lane >> 4;
+  f32x4 s[NT][2];
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const float sc = scale_of(kv.ks[g]);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) s[nt][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const u32x4 kf = values8<T>(kv.k[g][i], sc);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[nt][g] = Fmt<T>::mfma(kf, q[nt][i], s[nt][g]);
+    }
+  }
+  uint32_t vs0 = kv.vs[0], vs1 = kv.vs[1];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) s[nt][g] *= c;
+  }
+  if (masked) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int p = p0 + 16 * g + 4 * quarter + e;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          if (p < lo[nt] || p > hi[nt]) s[nt][g][e] = -INFINITY;
+        // past the sequence's end a slot holds anything: make it finite
+        if (p >= len) {
+          if (g == 0)
+            vs0 &= ~(255u << (8 * e));
+          else
+            vs1 &= ~(255u << (8 * e));
+        }
+      }
+  }
+  u32x4 pf[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = fmaxf(top, s[nt][g][e]);
+    if (__any(top > st.m[nt] + 8.0f)) {
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float m = fmaxf(st.m[nt], top);
+      const float f = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.m[nt] - m);
+      st.m[nt] = m;
+      st.l[nt] *= f;
+#pragma unroll
+      for (int i = 0; i < NM; ++i) st.o[nt][i] *= f;
+    }
+    const float ref = st.m[nt] == -INFINITY ? 0.f : st.m[nt] - Fmt<T>::kBias;
+    float pr[8];
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        pr[4 * g + e] = __builtin_amdgcn_exp2f(s[nt][g][e] - ref);
+        st.l[nt] += pr[4 * g + e];
+      }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) pf[nt][e] = pair_of<T>(pr[2 * e], pr[2 * e + 1]);
+  }
+  uint32_t w[8];
+  float sc[8];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    w[e] = kv.v[0][e];
+    w[4 + e] = kv.v[1][e];
+    sc[e] = scale_of((vs0 >> (8 * e)) & 255u);
+    sc[4 + e] = scale_of((vs1 >> (8 * e)) & 255u);
+  }
+  if constexpr (D == 64) {  // the lane's 4 channels of the word
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] >>= (lane & 1) * 16;
+  }
+  auto product = [&](int i, u32x4 even, u32x4 odd) __attribute__((always_inline)) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      st.o[nt][2 * i] = Fmt<T>::mfma(even, pf[nt], st.o[nt][2 * i]);
+      st.o[nt][2 * i + 1] = Fmt<T>::mfma(odd, pf[nt], st.o[nt][2 * i + 1]);
+    }
+  };
+  u32x4 even, odd;
+  transpose_pair<T, 0>(w, sc, &even, &odd);
+  product(0, even, odd);
+  transpose_pair<T, 1>(w, sc, &even, &odd);
+  product(1, even, odd);
+  if constexpr (D == 128) {
+    transpose_pair<T, 2>(w, sc, &even, &odd);
+    product(2, even, odd);
+    transpose_pair<T, 3>(w, sc, &even, &odd);
+    product(3, even, odd);
+  }
+}
+
+// The keys [lo, hi] that a row sees; none of a row that the sequence lacks.
+struct RowRange {
+  int lo, hi;
+};
+__device__ __forceinline__ RowRange row_range(int t, int n_new, int len, int C, int W) {
+  if (t >= n_new) return {1, 0};
+  const int pos = len - n_new + t;
+  int lo = max(0, len - C);
+  if (W > 0) lo = max(lo, pos - W + 1);
+  return {lo, pos};
+}
+
+template <typename T, int D, int NT>
+__global__ __launch_bounds__(256) void kv4_rows_kernel(Kv4AttnArgs a) {
+  constexpr int STEPS = D / 32, NM = D / 16, RB = 16 * NT, R = D / 8;
+  __shared__ float so[4][16][D + 4];
+  __shared__ float sml[4][RB][2];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int quarter = lane >> 4, n = lane & 15;
+  const int part = blockIdx.x % a.parts;
+  const int rest = blockIdx.x / a.parts;
+  const int rb = rest % a.nrb, bh = rest / a.nrb;
+  const int b = bh / a.c.H, h = bh % a.c.H;
+  const int len = length_of(a.c.len, b), n_new = count_of(a.counts, b, a.Tq);
+  const int row0 = rb * RB, C = a.c.C;
+
+  u32x4 q[NT][STEPS];
+  int lo[NT], hi[NT];
+  RowState<T, D, NT> st;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int row = row0 + 16 * nt + n, t = min(row / a.G, a.Tq - 1);
+    const T* src = static_cast<const T*>(a.q) + b * a.q_sb + t * a.q_st +
+                   (int64_t)(h * a.G + row % a.G) * a.q_sh + quarter * (D / 4);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) q[nt][i] = *reinterpret_cast<const u32x4*>(src + 8 * i);
+    const RowRange rr = row_range(row / a.G, n_new, len, C, a.window);
+    lo[nt] = rr.lo;
+    hi[nt] = rr.hi;
+    st.m[nt] = -INFINITY;
+    st.l[nt] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NM; ++i) st.o[nt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  // the block's keys, and those that all its rows see
+  const int t_lo = row0 / a.G, t_hi = min((row0 + RB - 1) / a.G, n_new - 1);
+  if (t_lo <= t_hi) {
+    const RowRange first = row_range(t_lo, n_new, len, C, a.window);
+    const RowRange last = row_range(t_hi, n_new, len, C, a.window);
+    if (first.lo <= last.hi) {
+      const int tile_lo = first.lo >> 5, tiles = (last.hi >> 5) - tile_lo + 1;
+      const int per = (tiles + a.parts - 1) / a.parts;
+      const int t0 = tile_lo + part * per, t1 = min(t0 + per, tile_lo + tiles);
+      const uint8_t* kc = a.c.kc + ((int64_t)bh * C + n) * (D / 2) + quarter * (D / 8);
+      const uint8_t* ks = a.c.ks + ((int64_t)bh * C + n) * (D / 32) + quarter * (D / 4) / 32;
+      const int word = D == 128 ? n : n >> 1;
+      const uint8_t* vc = a.c.vc + (((int64_t)bh * (C / 4) + quarter) * R + word) * 16;
+      const uint8_t* vs = a.c.vs + (((int64_t)bh * (C / 4) + quarter) * (D / 32) + word / 4) * 4;
+      auto load = [&](KvTile<D>& kv, int slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const uint8_t* src = kc + (int64_t)(slot + 16 * g) * (D / 2);
+          if constexpr (D == 128) {
+            kv.k[g] = *reinterpret_cast<const u32x4*>(src);
+          } else {
+            const u32x2 half = *reinterpret_cast<const u32x2*>(src);
+            kv.k[g][0] = half[0];
+            kv.k[g][1] = half[1];
+          }
+          kv.ks[g] = ks[(int64_t)(slot + 16 * g) * (D / 32)];
+          kv.v[g] = *reinterpret_cast<const u32x4*>(vc + (int64_t)(slot + 16 * g) * (D / 2));
+          kv.vs[g] = *reinterpret_cast<const uint32_t*>(vs + (int64_t)(slot + 16 * g) * (D / 32));
+        }
+      };
+      const int step = 128 % C;
+      int tile = t0 + wave;
+      int slot = (int)(((int64_t)tile * 32) % C);
+      KvTile<D> kv, next;
+      if (tile < t1) load(kv, slot);
+      for (; tile < t1; tile += 4) {
+        if (tile + 4 < t1) {
+          slot += step;
+          if (slot >= C) slot -= C;
+          load(next, slot);
+        }
+        const bool masked = tile * 32 < last.lo || tile * 32 + 31 > first.hi;
+        fold_tile<T, D, NT>(st, kv, q, a.c_log2, tile * 32, masked, lo, hi, len, lane);
+        kv = next;
+      }
+    }
+  }
+  // add the wavefronts
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    float l = st.l[nt];
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    // a row that the sequence lacks saw the tiles that nobody's mask cuts
+    const bool none = lo[nt] > hi[nt];
+    if (quarter == 0) {
+      sml[wave][16 * nt + n][0] = none ? -INFINITY : st.m[nt] - Fmt<T>::kBias;
+      sml[wave][16 * nt + n][1] = none ? 0.f : l;
+    }
+  }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    if (nt > 0) __syncthreads();  // the tile before is read
+    // accumulator element e of product i: channel NM (4 quarter + e) + i
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int i = 0; i < NM; ++i)
+        so[wave][n][NM * (4 * quarter + e) + i] = st.o[nt][i][e];
+    __syncthreads();
+    constexpr int PER = D / 16;  // channels a thread
+    const int r = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * PER;
+    const int row = row0 + 16 * nt + r;
+    if (row < a.Tq * a.G) {
+      float m = -INFINITY, l = 0.f, o[PER];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) m = fmaxf(m, sml[w][16 * nt + r][0]);
+      const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) o[i] = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = __builtin_amdgcn_exp2f(sml[w][16 * nt + r][0] - ref);
+        l = fmaf(sml[w][16 * nt + r][1], f, l);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) o[i] = fmaf(so[w][r][d0 + i], f, o[i]);
+      }
+      if (a.parts > 1) {
+        const int64_t at = ((int64_t)part * a.c.B * a.c.H + bh) * ((int64_t)a.Tq * a.G) + row;
+        if ((threadIdx.x & 15) == 0) {
+          a.part_ml[2 * at] = m;
+          a.part_ml[2 * at + 1] = l;
+        }
+        if (l != 0.f) {  // an empty part is not read
+#pragma unroll
+          for (int i = 0; i < PER; i += 4)
+            *reinterpret_cast<f32x4*>(a.part + at * D + d0 + i) =
+                f32x4{o[i], o[i + 1], o[i + 2], o[i + 3]};
+        }
+      } else {
+        const int t = row / a.G, head = h * a.G + row % a.G;
+        const float inv = 1.f / l;
+        T* dst = static_cast<T*>(a.o) + b * a.o_sb + t * a.o_st + head * a.o_sh + d0;
+        uint32_t w[PER / 2];
+#pragma unroll
+        for (int i = 0; i < PER / 2; ++i)
+          w[i] = l == 0.f ? 0u : pair_of<T>(o[2 * i] * inv, o[2 * i + 1] * inv);
+        if constexpr (PER == 8)
+          *reinterpret_cast<u32x4*>(dst) = u32x4{w[0], w[1], w[2], w[3]};
+        else
+          *reinterpret_cast<u32x2*>(dst) = u32x2{w[0], w[1]};
+        if (a.lse != nullptr && (threadIdx.x & 15) == 0)
+          a.lse[((int64_t)b * a.G * a.c.H + head) * a.Tq + t] =
+              l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+      }
+    }
+  }
+}
+
+// The parts of a row: D / 4 threads with 4 channels each in every one of the
+// 256 / (D / 4) groups that share the parts between them.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4AttnArgs a) {
+  constexpr int TH = D / 4, GR = 256 / TH;
+  __shared__ f32x4 so[GR][TH];
+  __shared__ float sl[GR];
+  const int rows = a.Tq * a.G;
+  const int64_t id = blockIdx.x, all = (int64_t)a.c.B * a.c.H * rows;
+  const int bh = (int)(id / rows), row = (int)(id % rows);
+  const int b = bh / a.c.H, h = bh % a.c.H;
+  const int d4 = threadIdx.x % TH, g = threadIdx.x / TH;
+  float m = -INFINITY;
+  for (int p = 0; p < a.parts; ++p) m = fmaxf(m, a.part_ml[2 * (p * all + id)]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+  for (int p = g; p < a.parts; p += GR) {
+    const int64_t at = p * all + id;
+    const float lp = a.part_ml[2 * at + 1];
+    if (lp == 0.f) continue;
+    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - ref);
+    l = fmaf(lp, f, l);
+    const f32x4 v = *reinterpret_cast<const f32x4*>(a.part + at * D + 4 * d4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(v[e], f, o[e]);
+  }
+  so[g][d4] = o;
+  if (d4 == 0) sl[g] = l;
+  __syncthreads();
+  if (g != 0) return;
+  for (int i = 1; i < GR; ++i) {
+    l += sl[i];
+    o += so[i][d4];
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int t = row / a.G, head = h * a.G + row % a.G;
+  T* dst = static_cast<T*>(a.o) + b * a.o_sb + t * a.o_st + head * a.o_sh + 4 * d4;
+  *reinterpret_cast<u32x2*>(dst) =
+      u32x2{pair_of<T>(o[0] * inv, o[1] * inv), pair_of<T>(o[2] * inv, o[3] * inv)};
+  if (a.lse != nullptr && d4 == 0)
+    a.lse[((int64_t)b * a.G * a.c.H + head) * a.Tq + t] =
+        l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+template <typename T, int D, int NT>
+hipError_t launch_rows(const Kv4AttnArgs& a, hipStream_t st) {
+  const int64_t grid = (int64_t)a.parts * a.nrb * a.c.B * a.c.H;
+  hipLaunchKernelGGL((kv4_rows_kernel<T, D, NT>), dim3((unsigned)grid), dim3(256), 0, st, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.parts == 1) return e;
+  const int64_t rows = (int64_t)a.c.B * a.c.H * a.G * a.Tq;
+  hipLaunchKernelGGL((kv4_combine_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+template <typename T, int D>
+hipError_t launch_attn_typed(const Kv4AttnArgs& a, hipStream_t st) {
+  if (a.row_tiles == 1) return launch_rows<T, D, 1>(a, st);
+  if (a.row_tiles == 2) return launch_rows<T, D, 2>(a, st);
+  return launch_rows<T, D, 4>(a, st);
+}
+
+// ---------------------------------------------------------------------------
+// Key weights: w_j = sum over the rows of exp(s_ij - lse_i). A wavefront holds
+// NK tiles of 16 keys and sweeps the rows 16 at a time; its lanes add up their
+// 4 keys of each tile, and the 16 rows of a lane's column at the end, so no sum
+// depends on the order of anything else. Every slot is written (added to): 0 in
+// those that hold nothing.
+template <typename T, int D, int NK>
+__global__ __launch_bounds__(256) void kv4_weights_kernel(Kv4WeightsArgs a) {
+  constexpr int STEPS = D / 32;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int quarter = lane >> 4, n = lane & 15;
+  const int C = a.c.C;
+  const int per_bh = (C + 64 * NK - 1) / (64 * NK);  // workgroups
+  const int bh = blockIdx.x / per_bh, b = bh / a.c.H, h = bh % a.c.H;
+  const int slot0 = ((blockIdx.x % per_bh) * 4 + wave) * 16 * NK;
+  if (slot0 >= C) return;
+  const int len = length_of(a.c.len, b), n_new = count_of(a.counts, b, a.Tq);
+
+  // positions of the lane's keys: the newest in its slot, -1 if there is none
+  u32x4 k[NK][STEPS];
+  int pos[NK][4], least = 0x7fffffff, most = -1;
+  float w[NK][4];
+#pragma unroll
+  for (int i = 0; i < NK; ++i) {
+    const int s = min(slot0 + 16 * i, C - 16);  // past the last slot: unused
+    const int64_t row = (int64_t)bh * C + s + n;
+    const uint8_t* src = a.c.kc + row * (D / 2) + quarter * (D / 8);
+    const float sc = scale_of(a.c.ks[row * (D / 32) + quarter * (D / 4) / 32]);
+    if constexpr (D == 128) {
+      const u32x4 words = *reinterpret_cast<const u32x4*>(src);
+#pragma unroll
+      for (int j = 0; j < STEPS; ++j) k[i][j] = values8<T>(words[j], sc);
+    } else {
+      const u32x2 words = *reinterpret_cast<const u32x2*>(src);
+#pragma unroll
+      for (int j = 0; j < STEPS; ++j) k[i][j] = values8<T>(words[j], sc);
+    }
+    // of slot x: len - 1 - (len - 1 - x) mod C, from the tile's first slot on
+    const int back = len > 0 ? (int)(((int64_t)len - 1 - s) % C) : 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int x = 4 * quarter + e;
+      int p = len - 1 - (back < 0 ? back + C : back) + x;
+      if (p >= len) p -= C;
+      if (len == 0 || p < 0 || slot0 + 16 * i >= C) p = -1;
+      pos[i][e] = p;
+      w[i][e] = 0.f;
+      if (p >= 0) least = min(least, p);
+      most = max(most, p);
+    }
+  }
+#pragma unroll
+  for (int d = 16; d < 64; d *= 2) {
+    least = min(least, __shfl_xor(least, d));
+    most = max(most, __shfl_xor(most, d));
+  }
+  least = __builtin_amdgcn_readfirstlane(least);
+  most = __builtin_amdgcn_readfirstlane(most);
+  // rows that can see one of them: pos >= least, pos - W < most
+  int64_t t0 = 0, t1 = 0;
+  if (most >= 0) {
+    const int64_t base = (int64_t)len - n_new;
+    t1 = n_new;
+    if (a.window > 0) t1 = min(t1, most + a.window - base);
+    t1 = max(t1, (int64_t)0);
+    t0 = min(max((int64_t)least - base, (int64_t)0), t1);
+  }
+  const int row_end = (int)t1 * a.G;  // at most Tq G
+  for (int row0 = (int)t0 * a.G; row0 < row_end; row0 += 16) {
+    const int row = row0 + n, t = min(row, row_end - 1) / a.G;
+    const int head = h * a.G + min(row, row_end - 1) % a.G;
+    const T* src = static_cast<const T*>(a.q) + b * a.q_sb + t * a.q_st + (int64_t)head * a.q_sh +
+                   quarter * (D / 4);
+    u32x4 q[STEPS];
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) q[i] = *reinterpret_cast<const u32x4*>(src + 8 * i);
+    const float lse = a.lse[((int64_t)b * a.G * a.c.H + head) * a.Tq + t] * kLog2e;
+    const RowRange rr = row_range(t, n_new, len, C, a.window);
+    const bool on = row < row_end && lse != -INFINITY;
+    const int lo = on ? rr.lo : 1, hi = on ? rr.hi : 0;
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < STEPS; ++j) s = Fmt<T>::mfma(k[i][j], q[j], s);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[e], a.c_log2, -lse));
+        w[i][e] += pos[i][e] >= lo && pos[i][e] <= hi ? x : 0.f;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NK; ++i) {
+    if (slot0 + 16 * i >= C) break;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float x = w[i][e];
+      x += __shfl_xor(x, 1);
+      x += __shfl_xor(x, 2);
+      x += __shfl_xor(x, 4);
+      x += __shfl_xor(x, 8);
+      if (n == 0) {
+        float* dst = a.weights + (int64_t)bh * C + slot0 + 16 * i + 4 * quarter + e;
+        *dst = a.accumulate ? *dst + x : x;
+      }
+    }
+  }
+}
+
+template <typename T, int D>
+hipError_t launch_weights_typed(const Kv4WeightsArgs& a, hipStream_t st) {
+  constexpr int NK = 2;
+  const int64_t grid = (int64_t)((a.c.C + 64 * NK - 1) / (64 * NK)) * a.c.B * a.c.H;
+  hipLaunchKernelGGL((kv4_weights_kernel<T, D, NK>), dim3((unsigned)grid), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// Eviction. One workgroup per head finds the weight of the last key to keep by
+// its digits, most significant first (11, 11 and 10 bits), and writes the
+// positions that stay, in order. Wavefronts own runs of keys, so a key's place
+// is the count of kept ones before it: in the wavefront by ballot, over the
+// wavefronts by one sum.
+constexpr int kSelThreads = 1024;
+
+// Weights in the order of unsigned numbers, NaN before all of them; -0 is 0.
+__device__ __forceinline__ uint32_t order_of(float w) {
+  if (!(w == w)) return 0u;
+  const uint32_t u = __float_as_uint(w + 0.f);
+  return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+}
+
+__global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(Kv4EvictArgs a) {
+  constexpr int WAVES = kSelThreads / 64;
+  __shared__ uint32_t hist[2048];
+  __shared__ uint32_t wsum[WAVES];
+  __shared__ uint32_t found[2];
+  __shared__ int above[WAVES], equal[WAVES];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int bh = blockIdx.x, b = bh / a.c.H, C = a.c.C;
+  const int len = length_of(a.c.len, b);
+  const int n = min(len, C), first = len - n;
+  const int kept = min(n, a.keep), must = min(a.recent, kept);
+  const int cand = n - must;      // the older keys, of which
+  const uint32_t want = kept - must;  // so many stay
+  const float* wt = a.weights + (int64_t)bh * C;
+  const int slot0 = first % C;
+  auto slot_of = [&](int j) {
+    const int s = slot0 + j;
+    return s >= C ? s - C : s;
+  };
+  uint32_t prefix = 0, need = want;  // of the keys with this prefix, so many stay
+  if (want > 0 && (int)want < cand) {
+    int shift = 21, bits = 11;
+    for (int pass = 0; pass < 3; ++pass) {
+      for (int i = tid; i < 2048; i += kSelThreads) hist[i] = 0;
+      __syncthreads();
+      const uint32_t mask = pass == 0 ? 0u : 0xffffffffu << (shift + bits);
+      for (int j = tid; j < cand; j += kSelThreads) {
+        const uint32_t u = order_of(wt[slot_of(j)]);
+        if ((u & mask) == prefix) atomicAdd(&hist[(u >> shift) & ((1u << bits) - 1)], 1u);
+      }
+      __syncthreads();
+      // bins from the top: thread t has bins 2047 - 2 t and the one below
+      const uint32_t hi = hist[2047 - 2 * tid], lo = hist[2046 - 2 * tid];
+      uint32_t sum = hi + lo;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const uint32_t o = __shfl_up(sum, d);
+        if (lane >= d) sum += o;
+      }
+      if (lane == 63) wsum[wave] = sum;
+      __syncthreads();
+      for (int w = 0; w < wave; ++w) sum += wsum[w];
+      const uint32_t before = sum - hi - lo;
+      if (before < need && need <= before + hi) {
+        found[0] = 2047 - 2 * tid;
+        found[1] = need - before;
+      } else if (before + hi < need && need <= sum) {
+        found[0] = 2046 - 2 * tid;
+        found[1] = need - before - hi;
+      }
+      __syncthreads();
+      prefix |= found[0] << shift;
+      need = found[1];
+      bits = pass == 1 ? 10 : 11;
+      shift -= bits;
+      __syncthreads();
+    }
+  } else {
+    need = want == 0 ? 0 : 0xffffffffu;  // none, or every one of the older keys
+    prefix = want == 0 ? 0xffffffffu : 0u;
+  }
+  // a run of keys for each wavefront; need of those equal to prefix stay
+  const int run = (n + WAVES - 1) / WAVES;
+  const int j0 = wave * run, j1 = min(j0 + run, n);
+  int up = 0, eq = 0;
+  for (int j = j0 + lane; j - lane < j1; j += 64) {
+    const bool in = j < j1;
+    const bool is_new = in && j >= cand;
+    const uint32_t u = in && !is_new ? order_of(wt[slot_of(j)]) : 0u;
+    up += __popcll(__ballot(is_new || (in && u > prefix)));
+    eq += __popcll(__ballot(in && !is_new && u == prefix));
+  }
+  if (lane == 0) {
+    above[wave] = up;
+    equal[wave] = eq;
+  }
+  __syncthreads();
+  uint32_t eq_at = 0;
+  int at = 0;
+  for (int w = 0; w < wave; ++w) {
+    const uint32_t left = need > eq_at ? need - eq_at : 0u;
+    at += above[w] + (int)min((uint32_t)equal[w], left);
+    eq_at += equal[w];
+  }
+  const uint64_t below = (1ull << lane) - 1;
+  int32_t* index = a.index + (int64_t)bh * a.keep;
+  for (int j = j0 + lane; j - lane < j1; j += 64) {
+    const bool in = j < j1;
+    const bool is_new = in && j >= cand;
+    const uint32_t u = in && !is_new ? order_of(wt[slot_of(j)]) : 0u;
+    const bool is_eq = in && !is_new && u == prefix;
+    const uint64_t eqs = __ballot(is_eq);
+    const bool stays = is_new || (in && !is_new && u > prefix) ||
+                       (is_eq && eq_at + __popcll(eqs & below) < need);
+    const uint64_t all = __ballot(stays);
+    if (stays) index[at + __popcll(all & below)] = first + j;
+    at += __popcll(all);
+    eq_at += __popcll(eqs);
+  }
+  for (int j = kept + tid; j < a.keep; j += kSelThreads) index[j] = -1;
+  if (tid == 0 && bh % a.c.H == 0) a.out.len[b] = kept;
+}
+
+// The kept rows, 4 new slots a group: a thread takes 8 channels of the 4.
+template <int D>
+__global__ __launch_bounds__(256) void kv4_gather_kernel(Kv4EvictArgs a) {
+  constexpr int R = D / 8, BL = D / 32;
+  const int bh = blockIdx.y, C = a.c.C, CN = a.out.C;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int r = (int)(i % R), g = (int)(i / R);
+  if (4 * g >= CN) return;
+  const int32_t* index = a.index + (int64_t)bh * a.keep;
+  const int64_t row_n = (int64_t)bh * CN + 4 * g, gn = row_n >> 2;
+  u32x4 vw = {0u, 0u, 0u, 0u};
+  uint32_t vsw = 0u;
+  bool any = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int j = 4 * g + e;
+    const int p = j < a.keep ? index[j] : -1;
+    if (a.new_weights != nullptr && r == 0)
+      a.new_weights[row_n + e] =
+          p >= 0 ? a.weights[(int64_t)bh * C + p % C] : 0.f;
+    if (p < 0) continue;
+    any = true;
+    const int64_t row = (int64_t)bh * C + p % C, go = row >> 2;
+    const int eo = (int)(row & 3);
+    vw[e] = *reinterpret_cast<const uint32_t*>(a.c.vc + ((go * R + r) * 4 + eo) * 4);
+    *reinterpret_cast<uint32_t*>(a.out.kc + ((row_n + e) * R + r) * 4) =
+        *reinterpret_cast<const uint32_t*>(a.c.kc + (row * R + r) * 4);
+    if ((r & 3) == 0) {
+      a.out.ks[(row_n + e) * BL + (r >> 2)] = a.c.ks[row * BL + (r >> 2)];
+      vsw |= (uint32_t)a.c.vs[(go * BL + (r >> 2)) * 4 + eo] << (8 * e);
+    }
+  }
+  if (!any) return;
+  *reinterpret_cast<u32x4*>(a.out.vc + (gn * R + r) * 16) = vw;
+  if ((r & 3) == 0) *reinterpret_cast<uint32_t*>(a.out.vs + (gn * BL + (r >> 2)) * 4) = vsw;
+}
+
+}  // namespace
+
+hipError_t launch_kv4_append(const Kv4AppendArgs& a, Elem dtype, hipStream_t st) {
+  if (dtype == Elem::BF16)
+    return a.c.D == 128 ? launch_append<__bf16, 128>(a, st) : launch_append<__bf16, 64>(a, st);
+  return a.c.D == 128 ? launch_append<_Float16, 128>(a, st) : launch_append<_Float16, 64>(a, st);
+}
+
+hipError_t launch_kv4_read(const Kv4ReadArgs& a, Elem dtype, hipStream_t st) {
+  if (dtype == Elem::BF16)
+    return a.c.D == 128 ? launch_read<__bf16, 128>(a, st) : launch_read<__bf16, 64>(a, st);
+  return a.c.D == 128 ? launch_read<_Float16, 128>(a, st) : launch_read<_Float16, 64>(a, st);
+}
+
+hipError_t launch_kv4_attn(const Kv4AttnArgs& a, Elem dtype, hipStream_t st) {
+  if (dtype == Elem::BF16)
+    return a.c.D == 128 ? launch_attn_typed<__bf16, 128>(a, st)
+                        : launch_attn_typed<__bf16, 64>(a, st);
+  return a.c.D == 128 ? launch_attn_typed<_Float16, 128>(a, st)
+                      : launch_attn_typed<_Float16, 64>(a, st);
+}
+
+hipError_t launch_kv4_weights(const Kv4WeightsArgs& a, Elem dtype, hipStream_t st) {
+  if (dtype == Elem::BF16)
+    return a.c.D == 128 ? launch_weights_typed<__bf16, 128>(a, st)
+                        : launch_weights_typed<__bf16, 64>(a, st);
+  return a.c.D == 128 ? launch_weights_typed<_Float16, 128>(a, st)
+                      : launch_weights_typed<_Float16, 64>(a, st);
+}
+
+hipError_t launch_kv4_evict(const Kv4EvictArgs& a, hipStream_t st) {
+  const int heads = a.c.B * a.c.H;
+  hipLaunchKernelGGL(kv4_select_kernel, dim3(heads), dim3(kSelThreads), 0, st, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const int64_t items = (int64_t)(a.out.C / 4) * (a.c.D / 8);
+  const dim3 grid((unsigned)((items + 255) / 256), heads);
+  if (a.c.D == 128)
+    hipLaunchKernelGGL((kv4_gather_kernel<128>), grid, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((kv4_gather_kernel<64>), grid, dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+}  // namespace ttcd
