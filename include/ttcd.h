@@ -557,7 +557,8 @@ ttcd_status ttcd_kv4_attn_fwd(const ttcd_kv4_cache* cache, const void* q, void* 
  * exp(sm_scale * q_i . k_p - lse_i) over the queries i that see position p, in
  * fp32; 0 in slots that hold nothing. lse: (batch, Hq, Tq) as ttcd_kv4_attn_fwd
  * of the same call gives it (rows of -inf count for nothing). accumulate != 0: the
- * sums are added to what weights holds. weights: (batch, kv_heads, capacity).
+ * sums are added to what weights holds. weights: (batch, kv_heads, capacity), 16-byte
+ * aligned.
  */
 ttcd_status ttcd_kv4_key_weights_fwd(const ttcd_kv4_cache* cache, const void* q,
                                      const float* lse, float* weights, int Tq, int Hq,

@@ -97,7 +97,7 @@ def test_bad_arguments():
     assert _attn(qs=odd) == _attn(os=odd) == _attn(o=P + 8) == _attn(dt=2) == UNSUP
     assert _attn(Tq=1 << 29) == UNSUP
     assert _weights(lse=None) == _weights(w=None) == _weights(Tq=0) == _weights(Hq=5) == INV
-    assert _weights(qs=odd) == _weights(dt=7) == UNSUP
+    assert _weights(qs=odd) == _weights(dt=7) == _weights(w=P + 4) == UNSUP
     assert _read(k=None) == _read(count=0) == INV
     assert _read(v=P + 8) == _read(dt=2) == UNSUP
     assert _evict(w=None) == _evict(index=None) == _evict(keep=0) == _evict(keep=65) == INV

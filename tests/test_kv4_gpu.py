@@ -357,7 +357,8 @@ def test_evict_keeps_the_heaviest(gpu, keep, recent, kind):
 
 @pytest.mark.parametrize("C,lengths,keep,recent,dtype", [
     (4096, (4096, 9001), 1500, 100, HF), (8192, (8000, 5), 4095, 0, BF),
-    (2048, (1025, 2048), 1024, 1024, BF)])
+    (2048, (1025, 2048), 1024, 1024, BF), (40960, (40960, 123), 9999, 77, BF),
+    (65568, (70000, 65000), 32768, 1, BF)])
 def test_evict_of_long_caches(gpu, C, lengths, keep, recent, dtype):
     c, r = _pair(2, 2, 128, C, dtype, lengths)
     g = torch.Generator().manual_seed(C)

@@ -237,8 +237,8 @@ def strides3(strides) -> ctypes.Array:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def stream(t: torch.Tensor) -> int:
-    """The handle of torch's current stream on t's device."""
+def stream(t) -> int:
+    """The handle of torch's current stream on t's device (a tensor, or what has one)."""
     if _raw_stream is not None:
         return _raw_stream(t.device.index)
     return torch.cuda.current_stream(t.device).cuda_stream

@@ -1212,7 +1212,7 @@ Kv4Plan kv4_plan(const ttcd_kv4_cache* c, int Tq, int Hq, int window) {
   const int G = Hq / c->kv_heads;
   const int64_t rows = (int64_t)Tq * G;
   Kv4Plan p;
-  p.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  p.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 8;
   const int rb = 16 * p.row_tiles;
   p.nrb = (int)((rows + rb - 1) / rb);
   int64_t keys = c->capacity;
@@ -1221,9 +1221,9 @@ Kv4Plan kv4_plan(const ttcd_kv4_cache* c, int Tq, int Hq, int window) {
     keys = span < keys ? span : keys;
   }
   const int64_t tiles = keys / 32 + 1, groups = (int64_t)c->batch * c->kv_heads * p.nrb;
-  int64_t parts = (1024 + groups - 1) / groups;
+  int64_t parts = tiles <= 32 ? 1 : ((p.row_tiles < 8 ? 1024 : 512) + groups - 1) / groups;
   if (parts > tiles / 8) parts = tiles / 8;
-  p.parts = parts < 1 ? 1 : (int)parts;
+  p.parts = parts < 1 ? 1 : parts < ttcd::kKv4MaxParts ? (int)parts : ttcd::kKv4MaxParts;
   return p;
 }
 
@@ -1343,8 +1343,8 @@ ttcd_status ttcd_kv4_key_weights_fwd(const ttcd_kv4_cache* cache, const void* q,
   if (!lse || !weights) return fail(TTCD_ERR_INVALID_ARGUMENT, "null tensor pointer");
   if (!(sm_scale > 0.f) || !isfinite(sm_scale))
     return fail(TTCD_ERR_INVALID_ARGUMENT, "sm_scale must be finite and > 0");
-  if ((int64_t)cache->batch * cache->kv_heads * (cache->capacity / 32) > 0x7fffffffLL)
-    return fail(TTCD_ERR_UNSUPPORTED, "grid too large");
+  if (!aligned16(weights))
+    return fail(TTCD_ERR_UNSUPPORTED, "weights must be 16-byte aligned");
   ttcd::Kv4WeightsArgs a = {};
   a.c = kv4(cache);
   a.q = q;

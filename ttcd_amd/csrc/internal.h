@@ -191,6 +191,7 @@ hipError_t launch_attn_combine(const CombineArgs& a, Elem dtype, hipStream_t str
 
 // The 4-bit key / value cache (kv4.hip; its format is told there).
 constexpr int kKv4MaxLength = 1 << 30;  // positions of a sequence
+constexpr int kKv4MaxParts = 128;       // workgroups over the keys of a row
 
 struct Kv4Cache {
   uint8_t* kc;  // (B, H, C, D / 2)
@@ -232,7 +233,7 @@ struct Kv4AttnArgs {
   int Tq, G;
   int window;     // <= 0: none
   float c_log2;   // sm_scale * log2(e)
-  int row_tiles;  // tiles of 16 rows (position, head of the group) a workgroup
+  int row_tiles;  // tiles of 16 rows (position, head of the group) a workgroup: 1, 2 or 8
   int nrb;        // workgroups over the rows of a key / value head
   int parts;      // workgroups over the keys
   float* part;    // parts > 1: (parts, B, H, Tq * G, D) sums and (.., 2) maximum, sum

@@ -35,6 +35,11 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
+template <bool V>
+struct Bool {
+  static constexpr bool value = V;
+};
+
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kLog2e = 1.44269504088896341f;
 
@@ -125,24 +130,12 @@ __device__ __forceinline__ int count_of(const int32_t* counts, int b, int T) {
 
 // ---------------------------------------------------------------------------
 // Append. 4 slots in a row (a word group of the values) of one head are D / 2
-// threads, each with 8 channels of one of them: 16 bytes in, 4 out. Threads go
-// by channel first for the keys and by slot first for the values, as either
-// lies in the cache, so a wavefront's stores are whole lines. The 4 threads of
-// a block find its largest magnitude by two shuffles.
-template <typename T, int D, bool V>
-__device__ __forceinline__ void append_word(const Kv4AppendArgs& a, int b, int h, int len,
-                                            int n_new, int group, int i) {
-  constexpr int R = D / 8;
-  const int e = V ? i & 3 : i / R, r = V ? i >> 2 : i % R;
-  const int p = ((len >> 2) + group) * 4 + e;
-  const int t = p - len;
-  const bool on = t >= 0 && t < n_new;
-  u32x4 x = {0u, 0u, 0u, 0u};
-  if (on) {
-    const T* src = static_cast<const T*>(V ? a.v : a.k) + b * (V ? a.v_sb : a.k_sb) +
-                   t * (V ? a.v_st : a.k_st) + h * (V ? a.v_sh : a.k_sh) + r * 8;
-    x = *reinterpret_cast<const u32x4*>(src);
-  }
+// threads, each with 8 channels of one of them: 16 bytes in, 4 out, of a key and
+// of a value. Threads go by channel first for the keys and by slot first for the
+// values, as either lies in the cache, so a wavefront's stores are whole lines.
+// The 4 threads of a block find its largest magnitude by two shuffles.
+template <typename T>
+__device__ __forceinline__ uint32_t quantise8(u32x4 x, int d1, int d2, uint32_t* scale) {
   // NaN counts as 0: the format holds none
   float top = 0.f;
 #pragma unroll
@@ -152,29 +145,48 @@ __device__ __forceinline__ void append_word(const Kv4AppendArgs& a, int b, int h
     if (!(hi == hi)) x[j] &= 0x0000ffffu;
     top = fmaxf(top, fmaxf(fabsf(lo), fabsf(hi)));  // fmaxf passes NaN over
   }
-  // the threads of the block are 1 and 2 (keys), 4 and 8 (values) lanes away
-  top = fmaxf(top, __shfl_xor(top, V ? 4 : 1));
-  top = fmaxf(top, __shfl_xor(top, V ? 8 : 2));
+  top = fmaxf(top, __shfl_xor(top, d1));
+  top = fmaxf(top, __shfl_xor(top, d2));
   // top = 1.f 2^E <= 1.5 2^(e + 2)
   const uint32_t bits = __float_as_uint(top);
   int exp = (int)(bits >> 23) - 127 - ((bits & 0x7fffffu) <= 0x400000u ? 2 : 1);
   exp = min(max(exp, Fmt<T>::kLoExp), Fmt<T>::kHiExp);
-  const float s = scale_of((uint32_t)(exp + 127));
+  *scale = (uint32_t)(exp + 127);
+  const float s = scale_of(*scale);
   uint32_t w = Fmt<T>::template pack<0>(0u, x[0], s);
   w = Fmt<T>::template pack<1>(w, x[1], s);
   w = Fmt<T>::template pack<2>(w, x[2], s);
-  w = Fmt<T>::template pack<3>(w, x[3], s);
-  if (!on) return;
-  const int slot = p % a.c.C;
-  const int64_t row = ((int64_t)b * a.c.H + h) * a.c.C + slot;
-  if constexpr (V) {
+  return Fmt<T>::template pack<3>(w, x[3], s);
+}
+
+// Thread i of D / 2 of the group-th group of slots from the sequence's end on.
+template <typename T, int D>
+__device__ __forceinline__ void append_words(const Kv4AppendArgs& a, int b, int h, int len,
+                                             int n_new, int group, int i) {
+  constexpr int R = D / 8;
+  const int ek = i / R, rk = i % R, ev = i & 3, rv = i >> 2;
+  const int p = ((len >> 2) + group) * 4;
+  const int tk = p + ek - len, tv = p + ev - len;
+  const bool on_k = tk >= 0 && tk < n_new, on_v = tv >= 0 && tv < n_new;
+  u32x4 xk = {0u, 0u, 0u, 0u}, xv = xk;
+  if (on_k)
+    xk = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.k) + b * a.k_sb + tk * a.k_st +
+                                         h * a.k_sh + rk * 8);
+  if (on_v)
+    xv = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.v) + b * a.v_sb + tv * a.v_st +
+                                         h * a.v_sh + rv * 8);
+  uint32_t sk, sv;
+  const uint32_t wk = quantise8<T>(xk, 1, 2, &sk), wv = quantise8<T>(xv, 4, 8, &sv);
+  const int64_t row = ((int64_t)b * a.c.H + h) * a.c.C + (uint32_t)p % (uint32_t)a.c.C;
+  if (on_k) {
+    *reinterpret_cast<uint32_t*>(a.c.kc + ((row + ek) * R + rk) * 4) = wk;
+    if ((rk & 3) == 0) a.c.ks[(row + ek) * (D / 32) + (rk >> 2)] = (uint8_t)sk;
+    if (a.weights != nullptr && rk == 0) a.weights[row + ek] = 0.f;
+  }
+  if (on_v) {
     const int64_t g = row >> 2;
-    *reinterpret_cast<uint32_t*>(a.c.vc + ((g * R + r) * 4 + e) * 4) = w;
-    if ((r & 3) == 0) a.c.vs[(g * (D / 32) + (r >> 2)) * 4 + e] = (uint8_t)(exp + 127);
-  } else {
-    *reinterpret_cast<uint32_t*>(a.c.kc + (row * R + r) * 4) = w;
-    if ((r & 3) == 0) a.c.ks[row * (D / 32) + (r >> 2)] = (uint8_t)(exp + 127);
-    if (a.weights != nullptr && r == 0) a.weights[row] = 0.f;
+    *reinterpret_cast<uint32_t*>(a.c.vc + ((g * R + rv) * 4 + ev) * 4) = wv;
+    if ((rv & 3) == 0) a.c.vs[(g * (D / 32) + (rv >> 2)) * 4 + ev] = (uint8_t)sv;
   }
 }
 
@@ -190,17 +202,14 @@ __global__ __launch_bounds__(SMALL ? 1024 : 256) void append_kernel(Kv4AppendArg
     const int items = groups * a.c.H * PER;
     for (int i = threadIdx.x; i < items; i += 1024) {
       const int g = i / PER;
-      append_word<T, D, false>(a, b, g % a.c.H, len, n_new, g / a.c.H, i % PER);
-      append_word<T, D, true>(a, b, g % a.c.H, len, n_new, g / a.c.H, i % PER);
+      append_words<T, D>(a, b, g % a.c.H, len, n_new, g / a.c.H, i % PER);
     }
     __syncthreads();  // every thread has read the length
     if (threadIdx.x == 0) a.c.len[b] = len + n_new;
   } else {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int g = (int)(i / PER);
-    if (g >= groups * a.c.H) return;
-    append_word<T, D, false>(a, b, g / groups, len, n_new, g % groups, (int)(i % PER));
-    append_word<T, D, true>(a, b, g / groups, len, n_new, g % groups, (int)(i % PER));
+    const int g = (int)(((int64_t)blockIdx.x * 256 + threadIdx.x) / PER);
+    if (g < groups * a.c.H)
+      append_words<T, D>(a, b, g % a.c.H, len, n_new, g / a.c.H, threadIdx.x % PER);
   }
 }
 
@@ -592,41 +601,342 @@ __global__ __launch_bounds__(256) void kv4_rows_kernel(Kv4AttnArgs a) {
   }
 }
 
-// The parts of a row: D / 4 threads with 4 channels each in every one of the
-// 256 / (D / 4) groups that share the parts between them.
+// ---------------------------------------------------------------------------
+// Attention of many rows. A workgroup's 4 wavefronts hold 32 rows each and sweep
+// the same tiles of 64 keys; a tile is converted once, a quarter of it by
+// each wavefront, into LDS, where K and V lie as the operands of 32x32x16 MFMAs
+// (every read and write is 16 bytes a lane and 512 in a row). S^T = K Q^T, then
+// O^T = V^T P^T with P as it lies after the first product.
+//
+// One turn folds tile t: the scores of t + 1 are issued against the exponentials
+// of t, then the second product of t against the conversion of K(t + 2) and
+// V(t + 1) from codes that were loaded a turn before. Two stages of each in LDS
+// and one barrier a turn.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <typename T>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c);
+template <>
+__device__ __forceinline__ f32x16 mfma32<__bf16>(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x16 mfma32<_Float16>(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+constexpr int kBlockKeys = 64;
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
+  constexpr int KS = D / 16;  // steps of 16 channels
+  constexpr int MB = D / 32;  // blocks of 32 channels
+  constexpr int W = D / 8;    // words of 8 channels
+  constexpr int TILE = kBlockKeys * D * 2;  // bytes of a converted K or V tile
+  constexpr int RB = 128;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * TILE];  // K, K, V, V
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, n = lane & 31;
+  const int part = blockIdx.x % a.parts;
+  const int rest = blockIdx.x / a.parts;
+  const int rb = rest % a.nrb, bh = rest / a.nrb;
+  const int b = bh / a.c.H, h = bh - b * a.c.H;
+  const int len = length_of(a.c.len, b), n_new = count_of(a.counts, b, a.Tq);
+  const int row0 = rb * RB, C = a.c.C;
+
+  const int row = row0 + wave * 32 + n, t = min(row / a.G, a.Tq - 1), head = h * a.G + row % a.G;
+  u32x4 q[KS];
+  {
+    const T* src = static_cast<const T*>(a.q) + b * a.q_sb + t * a.q_st + (int64_t)head * a.q_sh +
+                   half * 8;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) q[i] = *reinterpret_cast<const u32x4*>(src + 16 * i);
+  }
+  const RowRange rr = row_range(row / a.G, n_new, len, C, a.window);
+  float m = -INFINITY, l = 0.f;
+  f32x16 o[MB];
+#pragma unroll
+  for (int i = 0; i < MB; ++i) o[i] = f32x16{};
+  // tiles [t0, t1) of 64 keys that the workgroup folds
+  int t0 = 0, t1 = 0;
+  const int t_lo = row0 / a.G, t_hi = min((row0 + RB - 1) / a.G, n_new - 1);
+  if (t_lo <= t_hi) {
+    const RowRange first = row_range(t_lo, n_new, len, C, a.window);
+    const RowRange last = row_range(t_hi, n_new, len, C, a.window);
+    if (first.lo <= last.hi) {
+      const int tile_lo = first.lo / kBlockKeys, tiles = last.hi / kBlockKeys - tile_lo + 1;
+      const int per = (tiles + a.parts - 1) / a.parts;
+      t0 = tile_lo + part * per;
+      t1 = min(t0 + per, tile_lo + tiles);
+    }
+  }
+  // the keys that all rows of this wavefront see
+  int in_lo = 0, in_hi = -1;
+  {
+    const int w0 = (row0 + wave * 32) / a.G;
+    const int w1 = min((row0 + wave * 32 + 31) / a.G, n_new - 1);
+    if (w0 <= w1) {
+      in_lo = row_range(w1, n_new, len, C, a.window).lo;
+      in_hi = row_range(w0, n_new, len, C, a.window).hi;
+    }
+  }
+
+  // Conversion. Keys: lane (key 16 wave + lane % 16, quarter of its channels).
+  // Values: the 16 keys of step `wave`, lane = channels (w, k) of its half's 8.
+  const int kq = lane >> 4, km = wave * 16 + (lane & 15);
+  const int vw = n % W, vk = n / W;
+  struct Codes {
+    u32x4 c[2];
+    uint32_t s[2];
+  };
+  Codes kc, vc;
+  // the slot of a tile's 16 keys of this wavefront: its halves may lie apart where
+  // the ring ends, a multiple of 32 slots from anything
+  auto slot_of = [&](int tile) __attribute__((always_inline)) {
+    return (int)((uint32_t)(tile * kBlockKeys + wave * 16) % (uint32_t)C);
+  };
+  auto load_k = [&](int tile) __attribute__((always_inline)) {
+    const int64_t row = (int64_t)bh * C + slot_of(tile) + (lane & 15);
+    const uint8_t* src = a.c.kc + row * (D / 2) + kq * (D / 8);
+    if constexpr (D == 128) {
+      kc.c[0] = *reinterpret_cast<const u32x4*>(src);
+    } else {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(src);
+      kc.c[0][0] = x[0];
+      kc.c[0][1] = x[1];
+    }
+    kc.s[0] = a.c.ks[row * (D / 32) + kq * (D / 4) / 32];
+  };
+  auto load_v = [&](int tile) __attribute__((always_inline)) {
+    const int64_t g = (((int64_t)bh * C + slot_of(tile)) >> 2) + half;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      vc.c[i] = *reinterpret_cast<const u32x4*>(a.c.vc + ((g + 2 * i) * W + vw) * 16);
+      vc.s[i] = *reinterpret_cast<const uint32_t*>(a.c.vs + ((g + 2 * i) * (D / 32) + vw / 4) * 4);
+    }
+  };
+  auto store_k = [&](int tile) __attribute__((always_inline)) {
+    char* dst = smem + (tile & 1) * TILE + (km >> 5) * (32 * D * 2) + (km & 31) * 16;
+    const float s = scale_of(kc.s[0]);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {  // chunk c of 8 channels: step c / 2, half c % 2
+      const int c = kq * (D / 32) + i;
+      *reinterpret_cast<u32x4*>(dst + c * 512) = values8<T>(kc.c[0][i], s);
+    }
+  };
+  auto store_v = [&](int tile) __attribute__((always_inline)) {
+    char* dst = smem + (2 + (tile & 1)) * TILE + wave * (16 * D * 2) + lane * 16;
+    uint32_t w[8];
+    float s[8];
+    // a slot past the sequence's end holds anything: make it finite
+    const int past = len - (tile * kBlockKeys + wave * 16 + 4 * half);  // keys of the lane before it
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      w[e] = vc.c[0][e] >> (vk * 4 * MB);
+      w[4 + e] = vc.c[1][e] >> (vk * 4 * MB);
+      s[e] = e < past ? scale_of((vc.s[0] >> (8 * e)) & 255u) : 0.f;
+      s[4 + e] = 8 + e < past ? scale_of((vc.s[1] >> (8 * e)) & 255u) : 0.f;
+    }
+    u32x4 even, odd;
+    transpose_pair<T, 0>(w, s, &even, &odd);
+    *reinterpret_cast<u32x4*>(dst) = even;
+    *reinterpret_cast<u32x4*>(dst + 1024) = odd;
+    if constexpr (MB == 4) {
+      transpose_pair<T, 1>(w, s, &even, &odd);
+      *reinterpret_cast<u32x4*>(dst + 2048) = even;
+      *reinterpret_cast<u32x4*>(dst + 3072) = odd;
+    }
+  };
+
+  f32x16 sa[2], sb[2];
+  auto scores = [&](f32x16 (&s)[2], int tile) __attribute__((always_inline)) {
+    const char* src = smem + (tile & 1) * TILE + lane * 16;
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        const u32x4 kf = *reinterpret_cast<const u32x4*>(src + kb * (32 * D * 2) + i * 1024);
+        s[kb] = mfma32<T>(kf, q[i], i == 0 ? f32x16{} : s[kb]);
+      }
+  };
+  // masks tile's scores and moves the reference where they exceed it by 2^8
+  auto settle = [&](f32x16 (&s)[2], int tile) __attribute__((always_inline)) {
+    const int p0 = tile * kBlockKeys;
+    if (p0 < in_lo || p0 + kBlockKeys - 1 > in_hi) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int p = p0 + 32 * kb + 8 * (e >> 2) + 4 * half + (e & 3);
+          if (p < rr.lo || p > rr.hi) s[kb][e] = -INFINITY;
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) top = fmaxf(top, s[0][e]);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) top = fmaxf(top, s[1][e]);
+    top *= a.c_log2;
+    if (__any(top > m + 8.0f)) {
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float mn = fmaxf(m, top);
+      const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < MB; ++i) o[i] *= f;
+    }
+  };
+  auto turn = [&](f32x16 (&s)[2], f32x16 (&next)[2], int tile) __attribute__((always_inline)) {
+    if (tile + 1 < t1) scores(next, tile + 1);
+    u32x4 p[4];
+    const float ref = m == -INFINITY ? 0.f : m - Fmt<T>::kBias;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x0 =
+            __builtin_amdgcn_exp2f(fmaf(s[j >> 1][8 * (j & 1) + 2 * e], a.c_log2, -ref));
+        const float x1 =
+            __builtin_amdgcn_exp2f(fmaf(s[j >> 1][8 * (j & 1) + 2 * e + 1], a.c_log2, -ref));
+        l += x0 + x1;
+        p[j][e] = pair_of<T>(x0, x1);
+      }
+    const char* src = smem + (2 + (tile & 1)) * TILE + lane * 16;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        const u32x4 vf = *reinterpret_cast<const u32x4*>(src + j * (16 * D * 2) + i * 1024);
+        o[i] = mfma32<T>(vf, p[j], o[i]);
+      }
+    if (tile + 2 < t1) store_k(tile + 2);
+    if (tile + 1 < t1) {
+      store_v(tile + 1);
+      settle(next, tile + 1);
+    }
+    if (tile + 3 < t1) load_k(tile + 3);
+    if (tile + 2 < t1) load_v(tile + 2);
+    __syncthreads();
+  };
+  if (t0 < t1) {
+    load_k(t0);
+    load_v(t0);
+    store_k(t0);
+    store_v(t0);
+    if (t0 + 1 < t1) {
+      load_k(t0 + 1);
+      load_v(t0 + 1);
+      store_k(t0 + 1);
+    }
+    if (t0 + 2 < t1) load_k(t0 + 2);
+    __syncthreads();
+    scores(sa, t0);
+    settle(sa, t0);
+    for (int tile = t0; tile < t1; tile += 2) {
+      turn(sa, sb, tile);
+      if (tile + 1 < t1) turn(sb, sa, tile + 1);
+    }
+  }
+
+  // Accumulator element e of block i: row rho = 8 (e / 4) + 4 half + e % 4, that is
+  // channel 8 (rho % W) + MB (rho / W) + i: 8 in a row a word.
+  if (row >= a.Tq * a.G) return;
+  const bool none = rr.lo > rr.hi;  // saw the tiles that nobody's mask cuts
+  l = none ? 0.f : l + __shfl_xor(l, 32);
+  m = none ? -INFINITY : m - Fmt<T>::kBias;
+  const int64_t at = ((int64_t)part * a.c.B * a.c.H + bh) * ((int64_t)a.Tq * a.G) + row;
+  if (half == 0) {
+    if (a.parts > 1) {
+      a.part_ml[2 * at] = m;
+      a.part_ml[2 * at + 1] = l;
+    } else if (a.lse != nullptr) {
+      a.lse[((int64_t)b * a.G * a.c.H + head) * a.Tq + t] =
+          l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+    }
+  }
+  const float inv = 1.f / l;
+#pragma unroll
+  for (int wi = 0; wi < W / 2; ++wi) {  // the lane's words: those with bit 2 as its half
+    const int w = 8 * (wi >> 2) + 4 * half + (wi & 3);
+    float x[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      // rho = w + W (c / MB): element 4 (rho / 8) + wi % 4
+      const int e = 4 * ((8 * (wi >> 2) + W * (c / MB)) >> 3) + (wi & 3);
+      x[c] = o[c % MB][e];
+    }
+    if (a.parts > 1) {
+      if (l != 0.f) {  // an empty part is not read
+        float* dst = a.part + at * D + 8 * w;
+        *reinterpret_cast<f32x4*>(dst) = f32x4{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<f32x4*>(dst + 4) = f32x4{x[4], x[5], x[6], x[7]};
+      }
+    } else {
+      u32x4 y;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        y[c] = l == 0.f ? 0u : pair_of<T>(x[2 * c] * inv, x[2 * c + 1] * inv);
+      *reinterpret_cast<u32x4*>(static_cast<T*>(a.o) + b * a.o_sb + t * a.o_st + head * a.o_sh +
+                                8 * w) = y;
+    }
+  }
+}
+
+// The parts of a row, at most 128: every wavefront finds their weights (2 parts a
+// lane); D / 4 threads with 4 channels each in every one of the 256 / (D / 4)
+// groups share the sums between them.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4AttnArgs a) {
   constexpr int TH = D / 4, GR = 256 / TH;
   __shared__ f32x4 so[GR][TH];
-  __shared__ float sl[GR];
   const int rows = a.Tq * a.G;
   const int64_t id = blockIdx.x, all = (int64_t)a.c.B * a.c.H * rows;
-  const int bh = (int)(id / rows), row = (int)(id % rows);
-  const int b = bh / a.c.H, h = bh % a.c.H;
-  const int d4 = threadIdx.x % TH, g = threadIdx.x / TH;
-  float m = -INFINITY;
-  for (int p = 0; p < a.parts; ++p) m = fmaxf(m, a.part_ml[2 * (p * all + id)]);
-  const float ref = m == -INFINITY ? 0.f : m;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
-  for (int p = g; p < a.parts; p += GR) {
-    const int64_t at = p * all + id;
-    const float lp = a.part_ml[2 * at + 1];
-    if (lp == 0.f) continue;
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - ref);
-    l = fmaf(lp, f, l);
-    const f32x4 v = *reinterpret_cast<const f32x4*>(a.part + at * D + 4 * d4);
+  const int bh = blockIdx.x / rows, row = blockIdx.x - bh * rows;
+  const int b = bh / a.c.H, h = bh - b * a.c.H;
+  const int d4 = threadIdx.x % TH, g = threadIdx.x / TH, lane = threadIdx.x & 63;
+  float mp[2], lp[2], f[2];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = fmaf(v[e], f, o[e]);
+  for (int i = 0; i < 2; ++i) {
+    const int p = lane + 64 * i;
+    const float* ml = a.part_ml + 2 * (p * all + id);
+    mp[i] = p < a.parts ? ml[0] : -INFINITY;
+    lp[i] = p < a.parts ? ml[1] : 0.f;
+  }
+  float m = fmaxf(mp[0], mp[1]);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    f[i] = __builtin_amdgcn_exp2f(mp[i] - ref);
+    l = lp[i] == 0.f ? l : fmaf(lp[i], f[i], l);
+    // an empty part's sums are not read
+    if (lp[i] == 0.f) f[i] = -1.f;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) l += __shfl_xor(l, d);
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  const float* src = a.part + id * D + 4 * d4;
+#pragma unroll 4
+  for (int p0 = 0; p0 < a.parts; p0 += GR) {
+    const int p = p0 + g;
+    const float w = p < 64 ? __shfl(f[0], p & 63) : __shfl(f[1], p & 63);
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (p < a.parts && !(w < 0.f)) v = *reinterpret_cast<const f32x4*>(src + p * all * D);
+    if (p < a.parts && !(w < 0.f))
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(v[e], w, o[e]);
   }
   so[g][d4] = o;
-  if (d4 == 0) sl[g] = l;
   __syncthreads();
   if (g != 0) return;
-  for (int i = 1; i < GR; ++i) {
-    l += sl[i];
-    o += so[i][d4];
-  }
+#pragma unroll
+  for (int i = 1; i < GR; ++i) o += so[i][d4];
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int t = row / a.G, head = h * a.G + row % a.G;
   T* dst = static_cast<T*>(a.o) + b * a.o_sb + t * a.o_st + head * a.o_sh + 4 * d4;
@@ -637,22 +947,20 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4AttnArgs a) {
         l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-template <typename T, int D, int NT>
-hipError_t launch_rows(const Kv4AttnArgs& a, hipStream_t st) {
-  const int64_t grid = (int64_t)a.parts * a.nrb * a.c.B * a.c.H;
-  hipLaunchKernelGGL((kv4_rows_kernel<T, D, NT>), dim3((unsigned)grid), dim3(256), 0, st, a);
+template <typename T, int D>
+hipError_t launch_attn_typed(const Kv4AttnArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)a.parts * a.nrb * a.c.B * a.c.H));
+  if (a.row_tiles == 1)
+    hipLaunchKernelGGL((kv4_rows_kernel<T, D, 1>), grid, dim3(256), 0, st, a);
+  else if (a.row_tiles == 2)
+    hipLaunchKernelGGL((kv4_rows_kernel<T, D, 2>), grid, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((kv4_block_kernel<T, D>), grid, dim3(256), 0, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.parts == 1) return e;
   const int64_t rows = (int64_t)a.c.B * a.c.H * a.G * a.Tq;
   hipLaunchKernelGGL((kv4_combine_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, st, a);
   return hipGetLastError();
-}
-
-template <typename T, int D>
-hipError_t launch_attn_typed(const Kv4AttnArgs& a, hipStream_t st) {
-  if (a.row_tiles == 1) return launch_rows<T, D, 1>(a, st);
-  if (a.row_tiles == 2) return launch_rows<T, D, 2>(a, st);
-  return launch_rows<T, D, 4>(a, st);
 }
 
 // ---------------------------------------------------------------------------
@@ -668,85 +976,135 @@ __global__ __launch_bounds__(256) void kv4_weights_kernel(Kv4WeightsArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int quarter = lane >> 4, n = lane & 15;
   const int C = a.c.C;
-  const int per_bh = (C + 64 * NK - 1) / (64 * NK);  // workgroups
-  const int bh = blockIdx.x / per_bh, b = bh / a.c.H, h = bh % a.c.H;
-  const int slot0 = ((blockIdx.x % per_bh) * 4 + wave) * 16 * NK;
+  const int bh = blockIdx.y, b = bh / a.c.H, h = bh - b * a.c.H;
+  const int slot0 = (blockIdx.x * 4 + wave) * 16 * NK;
   if (slot0 >= C) return;
   const int len = length_of(a.c.len, b), n_new = count_of(a.counts, b, a.Tq);
+  float* dst = a.weights + (int64_t)bh * C + slot0 + 4 * quarter;
 
-  // positions of the lane's keys: the newest in its slot, -1 if there is none
-  u32x4 k[NK][STEPS];
-  int pos[NK][4], least = 0x7fffffff, most = -1;
-  float w[NK][4];
-#pragma unroll
-  for (int i = 0; i < NK; ++i) {
-    const int s = min(slot0 + 16 * i, C - 16);  // past the last slot: unused
-    const int64_t row = (int64_t)bh * C + s + n;
-    const uint8_t* src = a.c.kc + row * (D / 2) + quarter * (D / 8);
-    const float sc = scale_of(a.c.ks[row * (D / 32) + quarter * (D / 4) / 32]);
-    if constexpr (D == 128) {
-      const u32x4 words = *reinterpret_cast<const u32x4*>(src);
-#pragma unroll
-      for (int j = 0; j < STEPS; ++j) k[i][j] = values8<T>(words[j], sc);
-    } else {
-      const u32x2 words = *reinterpret_cast<const u32x2*>(src);
-#pragma unroll
-      for (int j = 0; j < STEPS; ++j) k[i][j] = values8<T>(words[j], sc);
-    }
-    // of slot x: len - 1 - (len - 1 - x) mod C, from the tile's first slot on
-    const int back = len > 0 ? (int)(((int64_t)len - 1 - s) % C) : 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int x = 4 * quarter + e;
-      int p = len - 1 - (back < 0 ? back + C : back) + x;
-      if (p >= len) p -= C;
-      if (len == 0 || p < 0 || slot0 + 16 * i >= C) p = -1;
-      pos[i][e] = p;
-      w[i][e] = 0.f;
-      if (p >= 0) least = min(least, p);
-      most = max(most, p);
-    }
+  // The positions of the wavefront's slots: the newest there, len - 1 - (len - 1 -
+  // slot) mod C, in a row from p0 on but for a step back by C after len - 1, and
+  // negative where there is none.
+  const int p0 = len - 1 - (int)((uint32_t)(len - 1 - slot0 + C) % (uint32_t)C);
+  const int slots = min(16 * NK, C - slot0);
+  const int wrap = min(slots, len - p0);  // slots from wrap on hold p - C
+  // the least and most position held, of p0 .. p0 + wrap - 1 and the rest - C
+  int least, most;
+  if (p0 + wrap - 1 >= 0) {
+    most = p0 + wrap - 1;
+    least = wrap < slots && p0 + slots - 1 - C >= 0 ? max(0, p0 + wrap - C) : max(0, p0);
+  } else {
+    most = -1;
+    least = 0;
   }
-#pragma unroll
-  for (int d = 16; d < 64; d *= 2) {
-    least = min(least, __shfl_xor(least, d));
-    most = max(most, __shfl_xor(most, d));
-  }
-  least = __builtin_amdgcn_readfirstlane(least);
-  most = __builtin_amdgcn_readfirstlane(most);
   // rows that can see one of them: pos >= least, pos - W < most
+  const int base = len - n_new;
   int64_t t0 = 0, t1 = 0;
   if (most >= 0) {
-    const int64_t base = (int64_t)len - n_new;
     t1 = n_new;
-    if (a.window > 0) t1 = min(t1, most + a.window - base);
+    if (a.window > 0) t1 = min(t1, (int64_t)most + a.window - base);
     t1 = max(t1, (int64_t)0);
     t0 = min(max((int64_t)least - base, (int64_t)0), t1);
   }
   const int row_end = (int)t1 * a.G;  // at most Tq G
-  for (int row0 = (int)t0 * a.G; row0 < row_end; row0 += 16) {
-    const int row = row0 + n, t = min(row, row_end - 1) / a.G;
-    const int head = h * a.G + min(row, row_end - 1) % a.G;
-    const T* src = static_cast<const T*>(a.q) + b * a.q_sb + t * a.q_st + (int64_t)head * a.q_sh +
-                   quarter * (D / 4);
+  int row0 = (int)t0 * a.G;
+  // the lane's next row (t, g), those of the tile's first and last: no division a tile
+  const int dt = 16 / a.G, dg = 16 % a.G;
+  int t_n = (row0 + n) / a.G, g_n = (row0 + n) % a.G;
+  u32x4 qn[STEPS];
+  float lse_n = 0.f;
+  auto fetch = [&](int row) __attribute__((always_inline)) {
+    const bool in = row < row_end;  // past the end: the last row, which does not count
+    const int t = in ? t_n : (int)t1 - 1, head = h * a.G + (in ? g_n : a.G - 1);
+    const T* src = static_cast<const T*>(a.q) + b * a.q_sb + t * a.q_st +
+                   (int64_t)head * a.q_sh + quarter * (D / 4);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) qn[i] = *reinterpret_cast<const u32x4*>(src + 8 * i);
+    lse_n = a.lse[((int64_t)b * a.G * a.c.H + head) * a.Tq + t] * kLog2e;
+    // such a row, or one that sees nothing: every exponential is 0
+    if (!in || lse_n == -INFINITY) lse_n = INFINITY;
+  };
+  if (row0 >= row_end) {  // no row sees any of them
+    if (!a.accumulate)
+      for (int i = lane; i < slots; i += 64) a.weights[(int64_t)bh * C + slot0 + i] = 0.f;
+    return;
+  }
+  u32x4 kw[NK];
+  uint32_t kb[NK];
+#pragma unroll
+  for (int i = 0; i < NK; ++i) {
+    const int64_t row = (int64_t)bh * C + min(slot0 + 16 * i, C - 16) + n;  // past C: unused
+    const uint8_t* src = a.c.kc + row * (D / 2) + quarter * (D / 8);
+    if constexpr (D == 128) {
+      kw[i] = *reinterpret_cast<const u32x4*>(src);
+    } else {
+      const u32x2 half = *reinterpret_cast<const u32x2*>(src);
+      kw[i][0] = half[0];
+      kw[i][1] = half[1];
+    }
+    kb[i] = a.c.ks[row * (D / 32) + quarter * (D / 4) / 32];
+  }
+  fetch(row0 + n);
+  int pos[NK][4];
+  float w[NK][4];
+  u32x4 k[NK][STEPS];
+#pragma unroll
+  for (int i = 0; i < NK; ++i) {
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j) k[i][j] = values8<T>(kw[i][j], scale_of(kb[i]));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int x = 16 * i + 4 * quarter + e;
+      pos[i][e] = x < wrap ? p0 + x : x < slots ? p0 + x - C : -1;
+      w[i][e] = 0.f;
+    }
+  }
+  const bool whole = p0 >= 0 && wrap == 16 * NK;  // every slot holds p0 + x
+  int t_lo = (int)t0, g_lo = 0;  // of row0
+  for (; row0 < row_end; row0 += 16) {
     u32x4 q[STEPS];
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) q[i] = *reinterpret_cast<const u32x4*>(src + 8 * i);
-    const float lse = a.lse[((int64_t)b * a.G * a.c.H + head) * a.Tq + t] * kLog2e;
-    const RowRange rr = row_range(t, n_new, len, C, a.window);
-    const bool on = row < row_end && lse != -INFINITY;
-    const int lo = on ? rr.lo : 1, hi = on ? rr.hi : 0;
-#pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      f32x4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < STEPS; ++j) s = Fmt<T>::mfma(k[i][j], q[j], s);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = __builtin_amdgcn_exp2f(fmaf(s[e], a.c_log2, -lse));
-        w[i][e] += pos[i][e] >= lo && pos[i][e] <= hi ? x : 0.f;
-      }
+    for (int i = 0; i < STEPS; ++i) q[i] = qn[i];
+    const float lse = lse_n;
+    const int t = t_n;
+    t_n += dt;
+    g_n += dg;
+    if (g_n >= a.G) {
+      g_n -= a.G;
+      ++t_n;
     }
+    // every row of the 16 sees every slot
+    const int t_hi = min(t_lo + (g_lo + 15 >= a.G ? dt + 1 : 0), (int)t1 - 1);  // or more
+    const bool full = whole && p0 >= row_range(t_hi, n_new, len, C, a.window).lo &&
+                      p0 + 16 * NK - 1 <= row_range(t_lo, n_new, len, C, a.window).hi;
+    t_lo += dt;
+    g_lo += dg;
+    if (g_lo >= a.G) {
+      g_lo -= a.G;
+      ++t_lo;
+    }
+    if (row0 + 16 < row_end) fetch(row0 + 16 + n);
+    auto add = [&](auto masked) __attribute__((always_inline)) {
+      const RowRange rr = row_range(t, n_new, len, C, a.window);
+#pragma unroll
+      for (int i = 0; i < NK; ++i) {
+        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j) s = Fmt<T>::mfma(k[i][j], q[j], s);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(s[e], a.c_log2, -lse));
+          if constexpr (decltype(masked)::value)
+            w[i][e] += pos[i][e] >= rr.lo && pos[i][e] <= rr.hi ? x : 0.f;
+          else
+            w[i][e] += x;
+        }
+      }
+    };
+    if (full)
+      add(Bool<false>());
+    else
+      add(Bool<true>());
   }
 #pragma unroll
   for (int i = 0; i < NK; ++i) {
@@ -758,19 +1116,22 @@ __global__ __launch_bounds__(256) void kv4_weights_kernel(Kv4WeightsArgs a) {
       x += __shfl_xor(x, 2);
       x += __shfl_xor(x, 4);
       x += __shfl_xor(x, 8);
-      if (n == 0) {
-        float* dst = a.weights + (int64_t)bh * C + slot0 + 16 * i + 4 * quarter + e;
-        *dst = a.accumulate ? *dst + x : x;
-      }
+      w[i][e] = x;
+    }
+    if (n == 0) {
+      f32x4* at = reinterpret_cast<f32x4*>(dst + 16 * i);
+      f32x4 x = {w[i][0], w[i][1], w[i][2], w[i][3]};
+      if (a.accumulate) x += *at;
+      *at = x;
     }
   }
 }
 
 template <typename T, int D>
 hipError_t launch_weights_typed(const Kv4WeightsArgs& a, hipStream_t st) {
-  constexpr int NK = 2;
-  const int64_t grid = (int64_t)((a.c.C + 64 * NK - 1) / (64 * NK)) * a.c.B * a.c.H;
-  hipLaunchKernelGGL((kv4_weights_kernel<T, D, NK>), dim3((unsigned)grid), dim3(256), 0, st, a);
+  constexpr int NK = 4;
+  const dim3 grid((a.c.C + 64 * NK - 1) / (64 * NK), a.c.B * a.c.H);
+  hipLaunchKernelGGL((kv4_weights_kernel<T, D, NK>), grid, dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
@@ -779,16 +1140,19 @@ hipError_t launch_weights_typed(const Kv4WeightsArgs& a, hipStream_t st) {
 // its digits, most significant first (11, 11 and 10 bits), and writes the
 // positions that stay, in order. Wavefronts own runs of keys, so a key's place
 // is the count of kept ones before it: in the wavefront by ballot, over the
-// wavefronts by one sum.
+// wavefronts by one sum. A capacity of up to 64 keys a thread is read once, into
+// registers (REGS of them); a longer one at every pass (REGS = 0).
 constexpr int kSelThreads = 1024;
 
-// Weights in the order of unsigned numbers, NaN before all of them; -0 is 0.
+// Weights in the order of unsigned numbers between 0 and 2^32 - 1, NaN before all
+// of them; -0 is 0.
 __device__ __forceinline__ uint32_t order_of(float w) {
-  if (!(w == w)) return 0u;
+  if (!(w == w)) return 1u;
   const uint32_t u = __float_as_uint(w + 0.f);
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
+template <int REGS>
 __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(Kv4EvictArgs a) {
   constexpr int WAVES = kSelThreads / 64;
   __shared__ uint32_t hist[2048];
@@ -801,14 +1165,33 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(Kv4EvictArgs a)
   const int len = length_of(a.c.len, b);
   const int n = min(len, C), first = len - n;
   const int kept = min(n, a.keep), must = min(a.recent, kept);
-  const int cand = n - must;      // the older keys, of which
+  const int cand = n - must;          // the older keys, of which
   const uint32_t want = kept - must;  // so many stay
   const float* wt = a.weights + (int64_t)bh * C;
-  const int slot0 = first % C;
-  auto slot_of = [&](int j) {
+  const int slot0 = (int)((uint32_t)first % (uint32_t)C);
+  const int run = (n + WAVES * 64 - 1) / (WAVES * 64) * 64;  // keys of a wavefront
+  const int j0 = wave * run + lane;
+  // of the j-th oldest: an older key's weight, the most for a new one, 0 for none
+  auto weight = [&](int j) __attribute__((always_inline)) {
     const int s = slot0 + j;
-    return s >= C ? s - C : s;
+    return j < cand ? order_of(wt[s >= C ? s - C : s]) : j < n ? 0xffffffffu : 0u;
   };
+  uint32_t u[REGS > 0 ? REGS : 1];
+  if constexpr (REGS > 0) {
+#pragma unroll
+    for (int i = 0; i < REGS; ++i)
+      if (i * 64 < run) u[i] = weight(j0 + i * 64);
+  }
+  auto each = [&](auto f) __attribute__((always_inline)) {
+    if constexpr (REGS > 0) {
+#pragma unroll
+      for (int i = 0; i < REGS; ++i)
+        if (i * 64 < run) f(j0 + i * 64, u[i]);
+    } else {
+      for (int i = 0; i < run; i += 64) f(j0 + i, weight(j0 + i));
+    }
+  };
+
   uint32_t prefix = 0, need = want;  // of the keys with this prefix, so many stay
   if (want > 0 && (int)want < cand) {
     int shift = 21, bits = 11;
@@ -816,10 +1199,10 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(Kv4EvictArgs a)
       for (int i = tid; i < 2048; i += kSelThreads) hist[i] = 0;
       __syncthreads();
       const uint32_t mask = pass == 0 ? 0u : 0xffffffffu << (shift + bits);
-      for (int j = tid; j < cand; j += kSelThreads) {
-        const uint32_t u = order_of(wt[slot_of(j)]);
-        if ((u & mask) == prefix) atomicAdd(&hist[(u >> shift) & ((1u << bits) - 1)], 1u);
-      }
+      each([&](int j, uint32_t x) __attribute__((always_inline)) {
+        if (x - 1 < 0xfffffffeu && (x & mask) == prefix)  // an older key's
+          atomicAdd(&hist[(x >> shift) & ((1u << bits) - 1)], 1u);
+      });
       __syncthreads();
       // bins from the top: thread t has bins 2047 - 2 t and the one below
       const uint32_t hi = hist[2047 - 2 * tid], lo = hist[2046 - 2 * tid];
@@ -847,20 +1230,20 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(Kv4EvictArgs a)
       shift -= bits;
       __syncthreads();
     }
-  } else {
-    need = want == 0 ? 0 : 0xffffffffu;  // none, or every one of the older keys
-    prefix = want == 0 ? 0xffffffffu : 0u;
+  } else {  // all of the older keys, or none
+    need = 0;
+    prefix = want == 0 ? 0xfffffffeu : 0u;
   }
-  // a run of keys for each wavefront; need of those equal to prefix stay
-  const int run = (n + WAVES - 1) / WAVES;
-  const int j0 = wave * run, j1 = min(j0 + run, n);
+  // need of the keys equal to prefix stay, the oldest, and all above it
   int up = 0, eq = 0;
-  for (int j = j0 + lane; j - lane < j1; j += 64) {
-    const bool in = j < j1;
-    const bool is_new = in && j >= cand;
-    const uint32_t u = in && !is_new ? order_of(wt[slot_of(j)]) : 0u;
-    up += __popcll(__ballot(is_new || (in && u > prefix)));
-    eq += __popcll(__ballot(in && !is_new && u == prefix));
+  each([&](int j, uint32_t x) __attribute__((always_inline)) {
+    up += x > prefix;
+    eq += x == prefix;
+  });
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    up += __shfl_xor(up, d);
+    eq += __shfl_xor(eq, d);
   }
   if (lane == 0) {
     above[wave] = up;
@@ -876,58 +1259,65 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(Kv4EvictArgs a)
   }
   const uint64_t below = (1ull << lane) - 1;
   int32_t* index = a.index + (int64_t)bh * a.keep;
-  for (int j = j0 + lane; j - lane < j1; j += 64) {
-    const bool in = j < j1;
-    const bool is_new = in && j >= cand;
-    const uint32_t u = in && !is_new ? order_of(wt[slot_of(j)]) : 0u;
-    const bool is_eq = in && !is_new && u == prefix;
-    const uint64_t eqs = __ballot(is_eq);
-    const bool stays = is_new || (in && !is_new && u > prefix) ||
-                       (is_eq && eq_at + __popcll(eqs & below) < need);
+  each([&](int j, uint32_t x) __attribute__((always_inline)) {
+    bool stays = x > prefix;
+    const uint64_t eqs = __ballot(x == prefix);
+    if (eqs != 0 && need > 0) {
+      stays = stays || (x == prefix && eq_at + __popcll(eqs & below) < need);
+      eq_at += __popcll(eqs);
+    }
     const uint64_t all = __ballot(stays);
     if (stays) index[at + __popcll(all & below)] = first + j;
     at += __popcll(all);
-    eq_at += __popcll(eqs);
-  }
+  });
   for (int j = kept + tid; j < a.keep; j += kSelThreads) index[j] = -1;
   if (tid == 0 && bh % a.c.H == 0) a.out.len[b] = kept;
 }
 
-// The kept rows, 4 new slots a group: a thread takes 8 channels of the 4.
+// The kept rows, 4 new slots to D / 8 threads: a thread takes 32 channels of one
+// of the keys, 8 channels of the 4 values.
 template <int D>
 __global__ __launch_bounds__(256) void kv4_gather_kernel(Kv4EvictArgs a) {
   constexpr int R = D / 8, BL = D / 32;
   const int bh = blockIdx.y, C = a.c.C, CN = a.out.C;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int r = (int)(i % R), g = (int)(i / R);
+  const int g = (int)(((int64_t)blockIdx.x * 256 + threadIdx.x) / R), r = threadIdx.x % R;
   if (4 * g >= CN) return;
   const int32_t* index = a.index + (int64_t)bh * a.keep;
-  const int64_t row_n = (int64_t)bh * CN + 4 * g, gn = row_n >> 2;
-  u32x4 vw = {0u, 0u, 0u, 0u};
-  uint32_t vsw = 0u;
-  bool any = false;
+  const int64_t base = (int64_t)bh * C, row_n = (int64_t)bh * CN + 4 * g, gn = row_n >> 2;
+  int slot[4];  // -1: none
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const int j = 4 * g + e;
-    const int p = j < a.keep ? index[j] : -1;
-    if (a.new_weights != nullptr && r == 0)
-      a.new_weights[row_n + e] =
-          p >= 0 ? a.weights[(int64_t)bh * C + p % C] : 0.f;
-    if (p < 0) continue;
-    any = true;
-    const int64_t row = (int64_t)bh * C + p % C, go = row >> 2;
-    const int eo = (int)(row & 3);
-    vw[e] = *reinterpret_cast<const uint32_t*>(a.c.vc + ((go * R + r) * 4 + eo) * 4);
-    *reinterpret_cast<uint32_t*>(a.out.kc + ((row_n + e) * R + r) * 4) =
-        *reinterpret_cast<const uint32_t*>(a.c.kc + (row * R + r) * 4);
-    if ((r & 3) == 0) {
-      a.out.ks[(row_n + e) * BL + (r >> 2)] = a.c.ks[row * BL + (r >> 2)];
-      vsw |= (uint32_t)a.c.vs[(go * BL + (r >> 2)) * 4 + eo] << (8 * e);
-    }
+    const int j = 4 * g + e, p = j < a.keep ? index[j] : -1;
+    slot[e] = p < 0 ? -1 : (int)((uint32_t)p % (uint32_t)C);
   }
-  if (!any) return;
+  const int ek = r / BL, ck = r % BL;
+  const int sk = ek == 0 ? slot[0] : ek == 1 ? slot[1] : ek == 2 ? slot[2] : slot[3];
+  u32x4 kw = {0u, 0u, 0u, 0u}, vw = kw;
+  uint8_t ks = 0;
+  if (sk >= 0) {
+    kw = *reinterpret_cast<const u32x4*>(a.c.kc + ((base + sk) * BL + ck) * 16);
+    ks = a.c.ks[(base + sk) * BL + ck];
+  }
+  uint32_t vsw = 0u;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (slot[e] < 0) continue;
+    const int64_t go = (base + slot[e]) >> 2;
+    const int eo = slot[e] & 3;
+    vw[e] = *reinterpret_cast<const uint32_t*>(a.c.vc + ((go * R + r) * 4 + eo) * 4);
+    if (r < BL) vsw |= (uint32_t)a.c.vs[(go * BL + r) * 4 + eo] << (8 * e);
+  }
+  if (a.new_weights != nullptr && r < 4) {
+    const int s = r == 0 ? slot[0] : r == 1 ? slot[1] : r == 2 ? slot[2] : slot[3];
+    a.new_weights[row_n + r] = s >= 0 ? a.weights[base + s] : 0.f;
+  }
+  if (slot[0] < 0) return;  // kept ones come first
+  if (sk >= 0) {
+    *reinterpret_cast<u32x4*>(a.out.kc + ((row_n + ek) * BL + ck) * 16) = kw;
+    a.out.ks[(row_n + ek) * BL + ck] = ks;
+  }
   *reinterpret_cast<u32x4*>(a.out.vc + (gn * R + r) * 16) = vw;
-  if ((r & 3) == 0) *reinterpret_cast<uint32_t*>(a.out.vs + (gn * BL + (r >> 2)) * 4) = vsw;
+  if (r < BL) *reinterpret_cast<uint32_t*>(a.out.vs + (gn * BL + r) * 4) = vsw;
 }
 
 }  // namespace
@@ -962,7 +1352,15 @@ hipError_t launch_kv4_weights(const Kv4WeightsArgs& a, Elem dtype, hipStream_t s
 
 hipError_t launch_kv4_evict(const Kv4EvictArgs& a, hipStream_t st) {
   const int heads = a.c.B * a.c.H;
-  hipLaunchKernelGGL(kv4_select_kernel, dim3(heads), dim3(kSelThreads), 0, st, a);
+  const int per = (a.c.C + kSelThreads - 1) / kSelThreads;
+  if (per <= 8)
+    hipLaunchKernelGGL((kv4_select_kernel<8>), dim3(heads), dim3(kSelThreads), 0, st, a);
+  else if (per <= 32)
+    hipLaunchKernelGGL((kv4_select_kernel<32>), dim3(heads), dim3(kSelThreads), 0, st, a);
+  else if (per <= 64)
+    hipLaunchKernelGGL((kv4_select_kernel<64>), dim3(heads), dim3(kSelThreads), 0, st, a);
+  else
+    hipLaunchKernelGGL((kv4_select_kernel<0>), dim3(heads), dim3(kSelThreads), 0, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int64_t items = (int64_t)(a.out.C / 4) * (a.c.D / 8);

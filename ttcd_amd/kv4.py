@@ -56,14 +56,31 @@ class KV4Cache:
             raise ValueError(f"KV4Cache: head_dim must be 64 or 128, got {D}")
         if C < BLOCK or C % BLOCK:
             raise ValueError(f"KV4Cache: capacity must be a multiple of {BLOCK}, got {C}")
+        if dtype not in _DT:
+            raise ValueError(f"KV4Cache: dtype {dtype} not supported (bfloat16 or float16)")
+        self._alloc(B, H, D, C, dtype, device)
+        self.lengths.zero_()
+        self.weights = (torch.zeros(B, H, C, dtype=torch.float32, device=self.device)
+                        if weights else None)
 
-        def byte(*shape):
-            return torch.empty(B, H, *shape, dtype=torch.uint8, device=device)
+    def _alloc(self, B, H, D, C, dtype, device) -> None:
+        """The parts in one allocation, the lengths not set."""
+        n = B * H * C
+        codes, scales = n * D // 2, n * D // BLOCK  # multiples of 512 and 32
+        blob = torch.empty(2 * (codes + scales) + 4 * B, dtype=torch.uint8, device=device)
+        if not blob.is_cuda:
+            raise ValueError("KV4Cache: device must be a GPU (HIP) device")
+        p = blob.data_ptr()
+        self._blob, self._parts = blob, None
+        self._bind(p, p + 2 * codes, p + codes, p + 2 * codes + scales,
+                   p + 2 * (codes + scales), B, H, D, C, dtype, blob.device)
+        self.weights = None
 
-        self._set(byte(C, D // 2), byte(C, D // BLOCK), byte(C // 4, D // 8, 4, 4),
-                  byte(C // 4, D // BLOCK, 4),
-                  torch.zeros(B, dtype=torch.int32, device=device), dtype,
-                  torch.zeros(B, H, C, dtype=torch.float32, device=device) if weights else None)
+    def _bind(self, kc, ks, vc, vs, lengths, B, H, D, C, dtype, device) -> None:
+        self.batch, self.kv_heads, self.head_dim, self.capacity = B, H, D, C
+        self.dtype, self.device = dtype, device
+        self._c = _lib.KV4CacheStruct(kc, ks, vc, vs, lengths, B, H, D, C)
+        self._ref = ctypes.byref(self._c)
 
     @classmethod
     def from_parts(cls, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
@@ -71,44 +88,67 @@ class KV4Cache:
                    dtype: torch.dtype = torch.bfloat16,
                    weights: torch.Tensor | None = None) -> "KV4Cache":
         """The cache that these tensors are (shared, not copied)."""
-        self = cls.__new__(cls)
-        self._set(k_codes, k_scales, v_codes, v_scales, lengths, dtype, weights)
-        return self
-
-    def _set(self, k_codes, k_scales, v_codes, v_scales, lengths, dtype, weights) -> None:
-        if dtype not in _DT:
-            raise ValueError(f"KV4Cache: dtype {dtype} not supported (bfloat16 or float16)")
         if not isinstance(k_codes, torch.Tensor) or k_codes.dim() != 4:
             raise ValueError("KV4Cache: k_codes must be (B, H, C, D / 2)")
         B, H, C, half = k_codes.shape
         D = 2 * half
-        if D not in (64, 128) or C < BLOCK or C % BLOCK:
+        if dtype not in _DT:
+            raise ValueError(f"KV4Cache: dtype {dtype} not supported (bfloat16 or float16)")
+        if D not in (64, 128) or C < BLOCK or C % BLOCK or B < 1 or H < 1:
             raise ValueError(f"KV4Cache: head_dim must be 64 or 128 and capacity a multiple of "
-                             f"{BLOCK}, got {D}, {C}")
-        dev = k_codes.device
-        for name, t, shape, dt in (
-                ("k_codes", k_codes, (B, H, C, half), torch.uint8),
-                ("k_scales", k_scales, (B, H, C, D // BLOCK), torch.uint8),
-                ("v_codes", v_codes, (B, H, C // 4, D // 8, 4, 4), torch.uint8),
-                ("v_scales", v_scales, (B, H, C // 4, D // BLOCK, 4), torch.uint8),
-                ("lengths", lengths, (B,), torch.int32),
-                ("weights", weights, (B, H, C), torch.float32)):
-            if t is None and name == "weights":
+                             f"{BLOCK}, got {tuple(k_codes.shape)}")
+        dev, u8 = k_codes.device, torch.uint8
+        for t, shape, dt in ((k_codes, (B, H, C, half), u8), (k_scales, (B, H, C, D // 32), u8),
+                             (v_codes, (B, H, C // 4, D // 8, 4, 4), u8),
+                             (v_scales, (B, H, C // 4, D // 32, 4), u8),
+                             (lengths, (B,), torch.int32),
+                             (weights, (B, H, C), torch.float32)):
+            if t is None and t is weights:
                 continue
-            if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != dt:
-                raise ValueError(f"KV4Cache: {name} must be {shape} {dt}")
-            if t.device != dev or not t.is_cuda:
-                raise ValueError(f"KV4Cache: {name} must be on one GPU (HIP) device with the rest")
-            if not t.is_contiguous():
-                raise ValueError(f"KV4Cache: {name} must be contiguous")
-        self.k_codes, self.k_scales = k_codes, k_scales
-        self.v_codes, self.v_scales = v_codes, v_scales
-        self.lengths, self.weights, self.dtype, self.device = lengths, weights, dtype, dev
-        self.batch, self.kv_heads, self.head_dim, self.capacity = B, H, D, C
-        self._c = _lib.KV4CacheStruct(
-            k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
-            lengths.data_ptr(), B, H, D, C)
-        self._ref = ctypes.byref(self._c)
+            if (not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != dt
+                    or t.device != dev or not t.is_contiguous()):
+                raise ValueError(f"KV4Cache: expected contiguous {shape} {dt} on {dev}")
+        if not k_codes.is_cuda:
+            raise ValueError("KV4Cache: the parts must be on a GPU (HIP) device")
+        self = cls.__new__(cls)
+        self._blob = None
+        self._parts = (k_codes, k_scales, v_codes, v_scales, lengths)
+        self.weights = weights
+        self._bind(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
+                   v_scales.data_ptr(), lengths.data_ptr(), B, H, D, C, dtype, dev)
+        return self
+
+    def _part(self, i: int) -> torch.Tensor:
+        if self._parts is None:
+            B, H, D, C = self.batch, self.kv_heads, self.head_dim, self.capacity
+            shapes = ((B, H, C, D // 2), (B, H, C // 4, D // 8, 4, 4), (B, H, C, D // BLOCK),
+                      (B, H, C // 4, D // BLOCK, 4))
+            sizes = [B * H * C * D // n for n in (2, 2, BLOCK, BLOCK)]
+            kc, vc, ks, vs, n = self._blob.split(sizes + [4 * B])
+            kc, vc, ks, vs = (t.view(s) for t, s in zip((kc, vc, ks, vs), shapes))
+            self._parts = (kc, ks, vc, vs, n.view(torch.int32))
+        return self._parts[i]
+
+    @property
+    def k_codes(self) -> torch.Tensor:
+        return self._part(0)
+
+    @property
+    def k_scales(self) -> torch.Tensor:
+        return self._part(1)
+
+    @property
+    def v_codes(self) -> torch.Tensor:
+        return self._part(2)
+
+    @property
+    def v_scales(self) -> torch.Tensor:
+        return self._part(3)
+
+    @property
+    def lengths(self) -> torch.Tensor:
+        """Positions that each sequence has had, int32 (batch,)."""
+        return self._part(4)
 
     def reset(self) -> None:
         """Forget every position."""
@@ -168,10 +208,10 @@ def _window(window) -> int:
 def _call(cache: KV4Cache, fn, *args) -> None:
     """fn(*args, stream) with the cache's device current: the launches go to it."""
     if torch.cuda.current_device() == cache.device.index:
-        _lib.check(fn(*args, _lib.stream(cache.lengths)))
+        _lib.check(fn(*args, _lib.stream(cache)))
     else:
         with torch.cuda.device(cache.device):
-            _lib.check(fn(*args, _lib.stream(cache.lengths)))
+            _lib.check(fn(*args, _lib.stream(cache)))
 
 
 def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, *,
@@ -263,8 +303,9 @@ def kv4_key_weights(q: torch.Tensor, cache: KV4Cache, lse: torch.Tensor,
             raise ValueError("kv4_key_weights: accumulate needs out")
         out = torch.empty(shape, dtype=torch.float32, device=q.device)
     elif (out.shape != shape or out.dtype != torch.float32 or out.device != q.device
-          or not out.is_contiguous()):
-        raise ValueError(f"kv4_key_weights: out must be contiguous fp32 {shape} on q's device")
+          or not out.is_contiguous() or out.data_ptr() % 16):
+        raise ValueError(f"kv4_key_weights: out must be contiguous fp32 {shape} on q's device, "
+                         "16-byte aligned")
     if T == 0:
         return out if accumulate else out.zero_()
     q, lse = _ready(q), lse.contiguous()
@@ -294,7 +335,8 @@ def kv4_evict(cache: KV4Cache, weights: torch.Tensor | None, keep: int, recent: 
             or weights.dtype != torch.float32 or weights.device != cache.device):
         raise ValueError(f"kv4_evict: weights must be fp32 ({B}, {H}, {C}) on the cache's device")
     if out is None:
-        out = KV4Cache(B, H, cache.head_dim, C, cache.dtype, cache.device)
+        out = KV4Cache.__new__(KV4Cache)
+        out._alloc(B, H, cache.head_dim, C, cache.dtype, cache.device)  # the call sets its lengths
     elif (not isinstance(out, KV4Cache) or out.dtype != cache.dtype
           or out.device != cache.device):
         raise ValueError("kv4_evict: out must be a KV4Cache of the cache's dtype and device")
