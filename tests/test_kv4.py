@@ -136,3 +136,23 @@ def test_python_refusals_on_the_cpu():
                  lambda: ttcd_amd.kv4_key_weights(x, None, x)):
         with pytest.raises(ValueError, match="KV4Cache"):
             call()
+
+
+def test_model_cache_arguments():
+    from ttcd_amd import IPTTCDv9Cache
+    for bad in (dict(bits=8), dict(bits=4), dict(bits=4, capacity=0), dict(capacity=64),
+                dict(keep=4), dict(bits=4, capacity=64, keep=65),
+                dict(bits=4, capacity=64, keep=0), dict(bits=4, capacity=64, recent=-1)):
+        with pytest.raises(ValueError):
+            IPTTCDv9Cache(**bad)
+    c = IPTTCDv9Cache(bits=4, capacity=70)
+    assert c.capacity == 96
+    c.reserve(96, None)
+    with pytest.raises(ValueError, match="positions"):
+        c.reserve(97, None)
+    c.held = 500  # a window's ring has wrapped
+    c.reserve(33, 64)
+    with pytest.raises(ValueError, match="positions"):
+        c.reserve(34, 64)
+    with pytest.raises(NotImplementedError):
+        IPTTCDv9Cache(bits=4, capacity=64, keep=8).reserve(1, 32)

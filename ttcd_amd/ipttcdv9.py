@@ -69,6 +69,13 @@ the chunk's tokens at layer 0, so layers 1.. read a rotary offset one chunk
 too far (fla/models/utils.py:326-327, 349-352); here every layer uses the
 tokens seen before the chunk.
 
+IPTTCDv9Cache(bits=4, capacity=..) holds the keys and values in 4 bits
+(ttcd_amd.kv4): every layer's attention reads them from there, the chunk's own
+among them, so a row sees the same keys however its prompt is cut; decoding is
+forward() with one token a call. With keep=.. a full-causal model's layers drop
+the keys of least accumulated attention weight after a call that leaves more
+than that. The reference has neither.
+
 Not covered (raise NotImplementedError): qkv_bias, non-causal TTT conv,
 ttt_weight_renorm, Muon, normalised TTT features or proj-diff,
 ttt_output_use_teacher_conv, l2 softmax, a cache together with a padding
@@ -83,6 +90,7 @@ import torch.nn.functional as F
 
 from . import attn as _attn
 from . import epilogue as _epi
+from . import kv4 as _kv4
 from . import prologue as _pro
 from . import ttt as _ttt
 from .linear import project
@@ -315,9 +323,12 @@ class IPTTCDv9Prefill:
             return "stock"
         return "fused" if self.fuse_extra else "patched"
 
-    def _teacher_attention(self, q, k, v, ctx: "_Prefill"):
+    def _teacher_attention(self, q, k, v, ctx: "_Prefill", held=None):
         """The teacher window within each row's unpadded tokens / each packed
-        sequence (fla Attention's varlen path) or over whole rows."""
+        sequence (fla Attention's varlen path) or over whole rows; over a 4-bit
+        cache's keys where the layer has one."""
+        if held is not None:
+            return ctx.cache.attend(q, held, self.window_t)
         if ctx.cu_seqlens is None:
             return _attn.window_attn(q, k, v, self.window_t)
         B, T, Hq, D = q.shape
@@ -359,9 +370,12 @@ class IPTTCDv9Prefill:
         act = torch.sigmoid(g) if c["gate_fn"] == "sigmoid" else F.silu(g)
         return on * act
 
-    def _ttt_attention(self, q, k, v):
+    def _ttt_attention(self, q, k, v, ctx: "_Prefill", held):
         """Teacher and student outputs of a TTT layer; k / v may be longer than q
         (a cached prefill: the queries are the last positions)."""
+        if held is not None:
+            return (ctx.cache.attend(q, held, self.window_t),
+                    _kv4.kv4_attn(q, held, self.window_s))
         if self.attn_kernel == "triton":
             return _attn.fused_dual_window_attn(q, k, v, self.window_t, self.window_s)
         if self.attn_kernel == "fa3_lse":
@@ -386,22 +400,27 @@ class IPTTCDv9Prefill:
             x, residual = _epi.add_rmsnorm(y_prev, h, w[p + "attn_norm.weight"], eps)
         xa = x  # attn_norm output: the gate's input
         q, k, v = self._qkv(i, x, ctx)
+        held = None  # a 4-bit cache of this layer, this chunk in it
         if ctx.cache is not None:
-            # the cached keys of earlier chunks, then this chunk's (Tk >= T)
-            k, v = ctx.cache.extend(i, k, v, None if self.window_t < 0 else self.window_t)
+            if ctx.cache.bits == 4:
+                held = ctx.cache.append(i, k, v)
+            else:
+                # the cached keys of earlier chunks, then this chunk's (Tk >= T)
+                k, v = ctx.cache.extend(i, k, v, None if self.window_t < 0 else self.window_t)
         o_w = w[p + "attn.o_proj.weight"]
         gated = c["use_output_gate"]
         if i in self.ttt and T >= c["ttt_chunk"]:
             norm = _NormView(w[p + "mlp_norm.weight"], eps)
             proj = _LinearView(o_w)
             if ctx.fast:
-                o_t, o_s = self._ttt_attention(q, k, v)
+                o_t, o_s = self._ttt_attention(q, k, v, ctx, held)
             else:
                 # the reference's fallback (modeling_ipttcdv9.py:794-850): the
                 # teacher through the (unpad-aware) attention, the student a
                 # windowed call on the whole rows
-                o_t = self._teacher_attention(q, k, v, ctx)
-                o_s = _attn.window_attn(q, k, v, self.window_s)
+                o_t = self._teacher_attention(q, k, v, ctx, held)
+                o_s = (_attn.window_attn(q, k, v, self.window_s) if held is None
+                       else _kv4.kv4_attn(q, held, self.window_s))
             if gated:
                 o_t, o_s = self._gate(i, xa, o_t), self._gate(i, xa, o_s)
             if self.fuse_extra and ctx.fast:
@@ -416,7 +435,7 @@ class IPTTCDv9Prefill:
                              conv="kernel" if self.conv_kernel else "stock",
                              scan="kernel" if self.fuse_extra else "torch")
         else:
-            o = self._teacher_attention(q, k, v, ctx)
+            o = self._teacher_attention(q, k, v, ctx, held)
             a = project(self._gate(i, xa, o), o_w)
             x, residual = _epi.rmsnorm(a, w[p + "mlp_norm.weight"], eps, residual=residual)
             y = _ttt.swiglu_mlp(x, self.gu_w[i], w[p + "mlp.down_proj.weight"])
@@ -437,6 +456,7 @@ class IPTTCDv9Prefill:
                 raise NotImplementedError("a cached prefill with a padding mask or packed "
                                           "sequences")
             cache.check(B, self.Hkv, self.D, self.dtype, self.dev)
+            cache.reserve(T, None if self.window_t < 0 else self.window_t)
             ctx.cache, ctx.offset = cache, cache.seen
             attention_mask = None
         if attention_mask is not None:
@@ -491,7 +511,7 @@ class IPTTCDv9Prefill:
         for i in range(self.cfg["num_hidden_layers"]):
             h, y = self.layer(i, h, y, ctx)
         if cache is not None:
-            cache.seen += T
+            cache.advance(T)
         if logits_to_keep > 0:  # only the kept rows of the last block's output
             h, y = h[:, -logits_to_keep:], y[:, -logits_to_keep:]
         keep = h + y
@@ -522,11 +542,34 @@ class IPTTCDv9Cache:
     values of the last `window_size` tokens already prefilled (all of them
     when the model attends full-causally), fla's window-trimmed attn_state
     (fla/models/utils.py:35-96), and the count of tokens seen. Pass the same
-    object to every IPTTCDv9Prefill.forward of one prompt."""
+    object to every IPTTCDv9Prefill.forward of one prompt.
 
-    def __init__(self):
+    bits=4 holds them in 4 bits (ttcd_amd.kv4), `capacity` positions a layer,
+    allocated once: a window needs window_size + T - 1 of them for calls of T
+    tokens (or as many as the prompt has), full-causal attention room for every
+    token that is kept. keep: after a call that leaves more, each layer's kv heads
+    keep that many keys, the newest `recent` and those with the largest sum of
+    attention weights so far (full-causal models only)."""
+
+    def __init__(self, bits: int = 16, capacity: int | None = None, keep: int | None = None,
+                 recent: int = 0):
+        if bits not in (16, 4):
+            raise ValueError(f"IPTTCDv9Cache: bits must be 16 or 4, got {bits}")
+        if bits == 4 and (capacity is None or capacity < 1):
+            raise ValueError("IPTTCDv9Cache: a 4-bit cache needs its capacity")
+        if bits == 16 and (capacity is not None or keep is not None):
+            raise ValueError("IPTTCDv9Cache: capacity and keep are those of a 4-bit cache")
+        if keep is not None and not 1 <= keep <= capacity:
+            raise ValueError(f"IPTTCDv9Cache: keep must be in 1..{capacity}, got {keep}")
+        if recent < 0:
+            raise ValueError(f"IPTTCDv9Cache: recent must be >= 0, got {recent}")
+        self.bits, self.keep, self.recent = bits, keep, int(recent)
+        self.capacity = None if capacity is None else -(-int(capacity) // 32) * 32
         self.seen = 0
+        self.held = 0  # positions in a 4-bit layer's cache (more have wrapped off a window's)
         self.kv: dict[int, tuple[torch.Tensor, torch.Tensor]] = {}
+        self.kv4: dict[int, _kv4.KV4Cache] = {}
+        self._spare: _kv4.KV4Cache | None = None
         self._shape = None
 
     def check(self, B: int, Hkv: int, D: int, dtype, device) -> None:
@@ -535,6 +578,57 @@ class IPTTCDv9Cache:
             raise ValueError(f"cache holds (B, Hkv, D, dtype, device) = {self._shape}, "
                              f"this prefill needs {shape}")
         self._shape = shape
+
+    def reserve(self, T: int, window: int | None) -> None:
+        """Refuse T more tokens that a 4-bit cache has no room for."""
+        if self.bits != 4:
+            return
+        if self.keep is not None and window is not None:
+            raise NotImplementedError("dropping keys of a windowed model: the window counts "
+                                      "positions, and those of the kept keys are not in a row")
+        need = self.held + T
+        if window is not None:
+            need = min(need, window + T - 1)
+        if max(need, T) > self.capacity:
+            raise ValueError(f"IPTTCDv9Cache: {T} more tokens need {max(need, T)} positions of "
+                             f"{self.capacity}")
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> "_kv4.KV4Cache":
+        """The layer's 4-bit cache with this chunk's keys and values added."""
+        held = self.kv4.get(layer)
+        if held is None:
+            held = self.kv4[layer] = self._new()
+        _kv4.kv4_append(held, k, v)
+        return held
+
+    def _new(self) -> "_kv4.KV4Cache":
+        B, Hkv, D, dtype, device = self._shape
+        return _kv4.KV4Cache(B, Hkv, D, self.capacity, dtype, device,
+                             weights=self.keep is not None)
+
+    def attend(self, q: torch.Tensor, held: "_kv4.KV4Cache", window: int) -> torch.Tensor:
+        """Attention over the layer's cache; its keys' weights are summed up if some
+        are to be dropped."""
+        if self.keep is None:
+            return _kv4.kv4_attn(q, held, window)
+        o, lse = _kv4.kv4_attn(q, held, window, return_lse=True)
+        _kv4.kv4_key_weights(q, held, lse, window, out=held.weights, accumulate=True)
+        return o
+
+    def advance(self, T: int) -> None:
+        """T tokens have gone through every layer."""
+        self.seen += T
+        if self.bits != 4:
+            return
+        self.held += T
+        if self.keep is None or self.held <= self.keep:
+            return
+        if self._spare is None:
+            self._spare = self._new()
+        for i, old in self.kv4.items():
+            self.kv4[i], _, _ = _kv4.kv4_evict(old, None, self.keep, self.recent, out=self._spare)
+            self._spare = old
+        self.held = self.keep
 
     def extend(self, layer: int, k: torch.Tensor, v: torch.Tensor, keep: int | None):
         """Keys / values for layer's attention: the cached ones, then k / v of
