@@ -1202,6 +1202,15 @@ int kv4_window(int window) {
   return window <= 0 ? 0 : (window < ttcd::kKv4MaxLength ? window : ttcd::kKv4MaxLength);
 }
 
+#ifndef KV4_T1
+#define KV4_T1 1024
+#endif
+#ifndef KV4_T8
+#define KV4_T8 512
+#endif
+#ifndef KV4_MINT
+#define KV4_MINT 8
+#endif
 struct Kv4Plan {
   int row_tiles, nrb, parts;
 };
@@ -1221,8 +1230,8 @@ Kv4Plan kv4_plan(const ttcd_kv4_cache* c, int Tq, int Hq, int window) {
     keys = span < keys ? span : keys;
   }
   const int64_t tiles = keys / 32 + 1, groups = (int64_t)c->batch * c->kv_heads * p.nrb;
-  int64_t parts = tiles <= 32 ? 1 : ((p.row_tiles < 8 ? 1024 : 512) + groups - 1) / groups;
-  if (parts > tiles / 8) parts = tiles / 8;
+  int64_t parts = tiles <= 32 ? 1 : (p.row_tiles < 8 ? (KV4_T1 + groups - 1) : KV4_T8) / groups;
+  if (parts > tiles / KV4_MINT) parts = tiles / KV4_MINT;
   p.parts = parts < 1 ? 1 : parts < ttcd::kKv4MaxParts ? (int)parts : ttcd::kKv4MaxParts;
   return p;
 }

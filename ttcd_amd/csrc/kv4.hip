@@ -100,6 +100,28 @@ __device__ __forceinline__ float scale_of(uint32_t byte) {
   return __uint_as_float(byte << 23);
 }
 
+// scale_of byte J of w, in one instruction.
+template <int J>
+__device__ __forceinline__ float scale_byte(uint32_t w, uint32_t shift23) {
+  uint32_t r;
+  if constexpr (J == 0)
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_0" : "=v"(r) : "v"(shift23), "v"(w));
+  else if constexpr (J == 1)
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_1" : "=v"(r) : "v"(shift23), "v"(w));
+  else if constexpr (J == 2)
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_2" : "=v"(r) : "v"(shift23), "v"(w));
+  else
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_3" : "=v"(r) : "v"(shift23), "v"(w));
+  return __uint_as_float(r);
+}
+__device__ __forceinline__ void scales4(uint32_t w, float* s) {
+  const uint32_t shift = 23;
+  s[0] = scale_byte<0>(w, shift);
+  s[1] = scale_byte<1>(w, shift);
+  s[2] = scale_byte<2>(w, shift);
+  s[3] = scale_byte<3>(w, shift);
+}
+
 // 8 codes as 8 values, channel 0 in the low half of the first register.
 template <typename T>
 __device__ __forceinline__ u32x4 values8(uint32_t w, float s) {
@@ -301,6 +323,11 @@ hipError_t launch_read(const Kv4ReadArgs& a, hipStream_t st) {
 // the inputs' type for the product, as the prefill kernels round it; sums and
 // statistics are fp32. In f16 the reference is 7 lower (probabilities up to
 // 2^15), so that small ones keep 7 bits more above f16's least step.
+#ifndef KV4_WAVES
+#define KV4_WAVES 8
+#endif
+constexpr int kRowWaves = KV4_WAVES;
+
 template <int D>
 struct KvTile {
   u32x4 v[2];
@@ -342,20 +369,14 @@ __device__ __forceinline__ void fold_tile(RowState<T, D, NT>& st, const KvTile<D
   for (int g = 0; g < 2; ++g) {
     const float sc = scale_of(kv.ks[g]);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) s[nt][g] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
     for (int i = 0; i < STEPS; ++i) {
       const u32x4 kf = values8<T>(kv.k[g][i], sc);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[nt][g] = Fmt<T>::mfma(kf, q[nt][i], s[nt][g]);
+      for (int nt = 0; nt < NT; ++nt)
+        s[nt][g] = Fmt<T>::mfma(kf, q[nt][i], i == 0 ? f32x4{} : s[nt][g]);
     }
   }
   uint32_t vs0 = kv.vs[0], vs1 = kv.vs[1];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int g = 0; g < 2; ++g) s[nt][g] *= c;
-  }
   if (masked) {
 #pragma unroll
     for (int g = 0; g < 2; ++g)
@@ -382,6 +403,7 @@ __device__ __forceinline__ void fold_tile(RowState<T, D, NT>& st, const KvTile<D
     for (int g = 0; g < 2; ++g)
 #pragma unroll
       for (int e = 0; e < 4; ++e) top = fmaxf(top, s[nt][g][e]);
+    top *= c;
     if (__any(top > st.m[nt] + 8.0f)) {
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
@@ -398,7 +420,7 @@ __device__ __forceinline__ void fold_tile(RowState<T, D, NT>& st, const KvTile<D
     for (int g = 0; g < 2; ++g)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        pr[4 * g + e] = __builtin_amdgcn_exp2f(s[nt][g][e] - ref);
+        pr[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(s[nt][g][e], c, -ref));
         st.l[nt] += pr[4 * g + e];
       }
 #pragma unroll
@@ -410,9 +432,9 @@ __device__ __forceinline__ void fold_tile(RowState<T, D, NT>& st, const KvTile<D
   for (int e = 0; e < 4; ++e) {
     w[e] = kv.v[0][e];
     w[4 + e] = kv.v[1][e];
-    sc[e] = scale_of((vs0 >> (8 * e)) & 255u);
-    sc[4 + e] = scale_of((vs1 >> (8 * e)) & 255u);
   }
+  scales4(vs0, sc);
+  scales4(vs1, sc + 4);
   if constexpr (D == 64) {  // the lane's 4 channels of the word
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] >>= (lane & 1) * 16;
@@ -450,10 +472,10 @@ __device__ __forceinline__ RowRange row_range(int t, int n_new, int len, int C, 
 }
 
 template <typename T, int D, int NT>
-__global__ __launch_bounds__(256) void kv4_rows_kernel(Kv4AttnArgs a) {
+__global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Kv4AttnArgs a) {
   constexpr int STEPS = D / 32, NM = D / 16, RB = 16 * NT, R = D / 8;
-  __shared__ float so[4][16][D + 4];
-  __shared__ float sml[4][RB][2];
+  __shared__ float so[kRowWaves][16][D + 4];
+  __shared__ float sml[kRowWaves][RB][2];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int quarter = lane >> 4, n = lane & 15;
@@ -491,41 +513,56 @@ __global__ __launch_bounds__(256) void kv4_rows_kernel(Kv4AttnArgs a) {
       const int tile_lo = first.lo >> 5, tiles = (last.hi >> 5) - tile_lo + 1;
       const int per = (tiles + a.parts - 1) / a.parts;
       const int t0 = tile_lo + part * per, t1 = min(t0 + per, tile_lo + tiles);
-      const uint8_t* kc = a.c.kc + ((int64_t)bh * C + n) * (D / 2) + quarter * (D / 8);
-      const uint8_t* ks = a.c.ks + ((int64_t)bh * C + n) * (D / 32) + quarter * (D / 4) / 32;
+      // a lane's place in 16 keys' rows; the rest of an address is the wavefront's
       const int word = D == 128 ? n : n >> 1;
-      const uint8_t* vc = a.c.vc + (((int64_t)bh * (C / 4) + quarter) * R + word) * 16;
-      const uint8_t* vs = a.c.vs + (((int64_t)bh * (C / 4) + quarter) * (D / 32) + word / 4) * 4;
+      const uint32_t k_at = n * (D / 2) + quarter * (D / 8), ks_at = n * (D / 32) + quarter * (D / 4) / 32;
+      const uint32_t v_at = (quarter * R + word) * 16, vs_at = (quarter * (D / 32) + word / 4) * 4;
+      const int64_t row = (int64_t)bh * C;
+      const uint8_t* const kc = a.c.kc + row * (D / 2);
+      const uint8_t* const ks = a.c.ks + row * (D / 32);
+      const uint8_t* const vc = a.c.vc + row * (D / 2);
+      const uint8_t* const vs = a.c.vs + row * (D / 32);
       auto load = [&](KvTile<D>& kv, int slot) __attribute__((always_inline)) {
+        const uint8_t* const k0 = kc + (int64_t)slot * (D / 2);
+        const uint8_t* const s0 = ks + (int64_t)slot * (D / 32);
+        const uint8_t* const v0 = vc + (int64_t)slot * (D / 2);
+        const uint8_t* const t0 = vs + (int64_t)slot * (D / 32);
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          const uint8_t* src = kc + (int64_t)(slot + 16 * g) * (D / 2);
           if constexpr (D == 128) {
-            kv.k[g] = *reinterpret_cast<const u32x4*>(src);
+            kv.k[g] = *reinterpret_cast<const u32x4*>(k0 + (k_at + 16 * g * (D / 2)));
           } else {
-            const u32x2 half = *reinterpret_cast<const u32x2*>(src);
+            const u32x2 half = *reinterpret_cast<const u32x2*>(k0 + (k_at + 16 * g * (D / 2)));
             kv.k[g][0] = half[0];
             kv.k[g][1] = half[1];
           }
-          kv.ks[g] = ks[(int64_t)(slot + 16 * g) * (D / 32)];
-          kv.v[g] = *reinterpret_cast<const u32x4*>(vc + (int64_t)(slot + 16 * g) * (D / 2));
-          kv.vs[g] = *reinterpret_cast<const uint32_t*>(vs + (int64_t)(slot + 16 * g) * (D / 32));
+          kv.ks[g] = s0[ks_at + 16 * g * (D / 32)];
+          kv.v[g] = *reinterpret_cast<const u32x4*>(v0 + (v_at + 16 * g * (D / 2)));
+          kv.vs[g] = *reinterpret_cast<const uint32_t*>(t0 + (vs_at + 16 * g * (D / 32)));
         }
       };
-      const int step = 128 % C;
+      const int step = kRowWaves * 32 % C;
       int tile = t0 + wave;
-      int slot = (int)(((int64_t)tile * 32) % C);
-      KvTile<D> kv, next;
-      if (tile < t1) load(kv, slot);
-      for (; tile < t1; tile += 4) {
-        if (tile + 4 < t1) {
-          slot += step;
-          if (slot >= C) slot -= C;
-          load(next, slot);
-        }
+      int slot = (int)((uint32_t)(tile * 32) % (uint32_t)C);
+      auto fold = [&](const KvTile<D>& kv) __attribute__((always_inline)) {
         const bool masked = tile * 32 < last.lo || tile * 32 + 31 > first.hi;
         fold_tile<T, D, NT>(st, kv, q, a.c_log2, tile * 32, masked, lo, hi, len, lane);
-        kv = next;
+        tile += kRowWaves;
+      };
+      auto next = [&](KvTile<D>& kv) __attribute__((always_inline)) {
+        if (tile + kRowWaves >= t1) return;
+        slot += step;
+        if (slot >= C) slot -= C;
+        load(kv, slot);
+      };
+      KvTile<D> kv[2];
+      if (tile < t1) load(kv[0], slot);
+      while (tile < t1) {
+        next(kv[1]);
+        fold(kv[0]);
+        if (tile >= t1) break;
+        next(kv[0]);
+        fold(kv[1]);
       }
     }
   }
@@ -552,18 +589,19 @@ __global__ __launch_bounds__(256) void kv4_rows_kernel(Kv4AttnArgs a) {
       for (int i = 0; i < NM; ++i)
         so[wave][n][NM * (4 * quarter + e) + i] = st.o[nt][i][e];
     __syncthreads();
-    constexpr int PER = D / 16;  // channels a thread
-    const int r = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * PER;
+    constexpr int PER = D * 16 / (64 * kRowWaves);  // channels a thread
+    constexpr int TPR = D / PER;                    // threads a row
+    const int r = threadIdx.x / TPR, d0 = (threadIdx.x % TPR) * PER;
     const int row = row0 + 16 * nt + r;
     if (row < a.Tq * a.G) {
       float m = -INFINITY, l = 0.f, o[PER];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) m = fmaxf(m, sml[w][16 * nt + r][0]);
+      for (int w = 0; w < kRowWaves; ++w) m = fmaxf(m, sml[w][16 * nt + r][0]);
       const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int i = 0; i < PER; ++i) o[i] = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < kRowWaves; ++w) {
         const float f = __builtin_amdgcn_exp2f(sml[w][16 * nt + r][0] - ref);
         l = fmaf(sml[w][16 * nt + r][1], f, l);
 #pragma unroll
@@ -571,15 +609,13 @@ __global__ __launch_bounds__(256) void kv4_rows_kernel(Kv4AttnArgs a) {
       }
       if (a.parts > 1) {
         const int64_t at = ((int64_t)part * a.c.B * a.c.H + bh) * ((int64_t)a.Tq * a.G) + row;
-        if ((threadIdx.x & 15) == 0) {
+        if (threadIdx.x % TPR == 0) {
           a.part_ml[2 * at] = m;
           a.part_ml[2 * at + 1] = l;
         }
         if (l != 0.f) {  // an empty part is not read
 #pragma unroll
-          for (int i = 0; i < PER; i += 4)
-            *reinterpret_cast<f32x4*>(a.part + at * D + d0 + i) =
-                f32x4{o[i], o[i + 1], o[i + 2], o[i + 3]};
+          for (int i = 0; i < PER; ++i) a.part[at * D + d0 + i] = o[i];
         }
       } else {
         const int t = row / a.G, head = h * a.G + row % a.G;
@@ -591,9 +627,11 @@ __global__ __launch_bounds__(256) void kv4_rows_kernel(Kv4AttnArgs a) {
           w[i] = l == 0.f ? 0u : pair_of<T>(o[2 * i] * inv, o[2 * i + 1] * inv);
         if constexpr (PER == 8)
           *reinterpret_cast<u32x4*>(dst) = u32x4{w[0], w[1], w[2], w[3]};
-        else
+        else if constexpr (PER == 4)
           *reinterpret_cast<u32x2*>(dst) = u32x2{w[0], w[1]};
-        if (a.lse != nullptr && (threadIdx.x & 15) == 0)
+        else
+          *reinterpret_cast<uint32_t*>(dst) = w[0];
+        if (a.lse != nullptr && threadIdx.x % TPR == 0)
           a.lse[((int64_t)b * a.G * a.c.H + head) * a.Tq + t] =
               l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
       }
@@ -737,8 +775,15 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
     for (int e = 0; e < 4; ++e) {
       w[e] = vc.c[0][e] >> (vk * 4 * MB);
       w[4 + e] = vc.c[1][e] >> (vk * 4 * MB);
-      s[e] = e < past ? scale_of((vc.s[0] >> (8 * e)) & 255u) : 0.f;
-      s[4 + e] = 8 + e < past ? scale_of((vc.s[1] >> (8 * e)) & 255u) : 0.f;
+    }
+    scales4(vc.s[0], s);
+    scales4(vc.s[1], s + 4);
+    if (tile * kBlockKeys + kBlockKeys > len) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[e] = e < past ? s[e] : 0.f;
+        s[4 + e] = 8 + e < past ? s[4 + e] : 0.f;
+      }
     }
     u32x4 even, odd;
     transpose_pair<T, 0>(w, s, &even, &odd);
@@ -951,9 +996,9 @@ template <typename T, int D>
 hipError_t launch_attn_typed(const Kv4AttnArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)a.parts * a.nrb * a.c.B * a.c.H));
   if (a.row_tiles == 1)
-    hipLaunchKernelGGL((kv4_rows_kernel<T, D, 1>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((kv4_rows_kernel<T, D, 1>), grid, dim3(64 * kRowWaves), 0, st, a);
   else if (a.row_tiles == 2)
-    hipLaunchKernelGGL((kv4_rows_kernel<T, D, 2>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((kv4_rows_kernel<T, D, 2>), grid, dim3(64 * kRowWaves), 0, st, a);
   else
     hipLaunchKernelGGL((kv4_block_kernel<T, D>), grid, dim3(256), 0, st, a);
   hipError_t e = hipGetLastError();
@@ -964,174 +1009,341 @@ hipError_t launch_attn_typed(const Kv4AttnArgs& a, hipStream_t st) {
 }
 
 // ---------------------------------------------------------------------------
-// Key weights: w_j = sum over the rows of exp(s_ij - lse_i). A wavefront holds
-// NK tiles of 16 keys and sweeps the rows 16 at a time; its lanes add up their
-// 4 keys of each tile, and the 16 rows of a lane's column at the end, so no sum
-// depends on the order of anything else. Every slot is written (added to): 0 in
-// those that hold nothing.
-template <typename T, int D, int NK>
-__global__ __launch_bounds__(256) void kv4_weights_kernel(Kv4WeightsArgs a) {
-  constexpr int STEPS = D / 32;
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int quarter = lane >> 4, n = lane & 15;
-  const int C = a.c.C;
-  const int bh = blockIdx.y, b = bh / a.c.H, h = bh - b * a.c.H;
-  const int slot0 = (blockIdx.x * 4 + wave) * 16 * NK;
-  if (slot0 >= C) return;
-  const int len = length_of(a.c.len, b), n_new = count_of(a.counts, b, a.Tq);
-  float* dst = a.weights + (int64_t)bh * C + slot0 + 4 * quarter;
+// Key weights: w_j = sum over the rows of exp(s_ij - lse_i). A lane adds up its
+// 4 keys of each 16 over the rows of its column, and the 16 columns at the end, so
+// no sum depends on the order of anything else. Every slot is written (added to): 0
+// in those that hold nothing.
 
-  // The positions of the wavefront's slots: the newest there, len - 1 - (len - 1 -
-  // slot) mod C, in a row from p0 on but for a step back by C after len - 1, and
-  // negative where there is none.
-  const int p0 = len - 1 - (int)((uint32_t)(len - 1 - slot0 + C) % (uint32_t)C);
-  const int slots = min(16 * NK, C - slot0);
-  const int wrap = min(slots, len - p0);  // slots from wrap on hold p - C
-  // the least and most position held, of p0 .. p0 + wrap - 1 and the rest - C
-  int least, most;
-  if (p0 + wrap - 1 >= 0) {
-    most = p0 + wrap - 1;
-    least = wrap < slots && p0 + slots - 1 - C >= 0 ? max(0, p0 + wrap - C) : max(0, p0);
-  } else {
-    most = -1;
-    least = 0;
-  }
-  // rows that can see one of them: pos >= least, pos - W < most
-  const int base = len - n_new;
-  int64_t t0 = 0, t1 = 0;
-  if (most >= 0) {
-    t1 = n_new;
-    if (a.window > 0) t1 = min(t1, (int64_t)most + a.window - base);
-    t1 = max(t1, (int64_t)0);
-    t0 = min(max((int64_t)least - base, (int64_t)0), t1);
-  }
-  const int row_end = (int)t1 * a.G;  // at most Tq G
-  int row0 = (int)t0 * a.G;
-  // the lane's next row (t, g), those of the tile's first and last: no division a tile
-  const int dt = 16 / a.G, dg = 16 % a.G;
-  int t_n = (row0 + n) / a.G, g_n = (row0 + n) % a.G;
-  u32x4 qn[STEPS];
-  float lse_n = 0.f;
-  auto fetch = [&](int row) __attribute__((always_inline)) {
-    const bool in = row < row_end;  // past the end: the last row, which does not count
-    const int t = in ? t_n : (int)t1 - 1, head = h * a.G + (in ? g_n : a.G - 1);
-    const T* src = static_cast<const T*>(a.q) + b * a.q_sb + t * a.q_st +
-                   (int64_t)head * a.q_sh + quarter * (D / 4);
-#pragma unroll
-    for (int i = 0; i < STEPS; ++i) qn[i] = *reinterpret_cast<const u32x4*>(src + 8 * i);
-    lse_n = a.lse[((int64_t)b * a.G * a.c.H + head) * a.Tq + t] * kLog2e;
-    // such a row, or one that sees nothing: every exponential is 0
-    if (!in || lse_n == -INFINITY) lse_n = INFINITY;
-  };
-  if (row0 >= row_end) {  // no row sees any of them
-    if (!a.accumulate)
-      for (int i = lane; i < slots; i += 64) a.weights[(int64_t)bh * C + slot0 + i] = 0.f;
-    return;
-  }
-  u32x4 kw[NK];
-  uint32_t kb[NK];
+// The positions in `slots` slots from slot0 on: the newest there, len - 1 - (len - 1 -
+// slot) mod C, in a row from p0 on but for a step back by C at the wrap-th, and
+// negative where there is none. most: the newest of them, least: no later than any.
+struct Held {
+  int p0, slots, wrap, least, most;
+};
+__device__ __forceinline__ Held held_at(int slot0, int group, int len, int C) {
+  Held x;
+  x.p0 = len - 1 - (int)((uint32_t)(len - 1 - slot0 + C) % (uint32_t)C);
+  x.slots = min(group, C - slot0);
+  x.wrap = min(x.slots, len - x.p0);
+  x.most = x.p0 + x.wrap - 1 >= 0 ? x.p0 + x.wrap - 1 : -1;
+  x.least = x.wrap < x.slots && x.p0 + x.slots - 1 - C >= 0 ? max(0, x.p0 + x.wrap - C)
+                                                           : max(0, x.p0);
+  return x;
+}
+
+// Codes of 16 NK keys from slot0 on, those past the last slot of a head unused.
+template <int D, int NK>
+struct KeyCodes {
+  u32x4 w[NK];  // D = 64: the first two words
+  uint32_t s[NK];
+};
+template <int D, int NK>
+__device__ __forceinline__ void load_keys(KeyCodes<D, NK>& x, const Kv4Cache& c, int bh, int slot0,
+                                          int lane) {
+  const int quarter = lane >> 4, n = lane & 15;
+  const uint32_t at = n * (D / 2) + quarter * (D / 8), s_at = n * (D / 32) + quarter * (D / 4) / 32;
 #pragma unroll
   for (int i = 0; i < NK; ++i) {
-    const int64_t row = (int64_t)bh * C + min(slot0 + 16 * i, C - 16) + n;  // past C: unused
-    const uint8_t* src = a.c.kc + row * (D / 2) + quarter * (D / 8);
+    const int64_t row = (int64_t)bh * c.C + min(slot0 + 16 * i, c.C - 16);
+    const uint8_t* src = c.kc + row * (D / 2);
     if constexpr (D == 128) {
-      kw[i] = *reinterpret_cast<const u32x4*>(src);
+      x.w[i] = *reinterpret_cast<const u32x4*>(src + at);
     } else {
-      const u32x2 half = *reinterpret_cast<const u32x2*>(src);
-      kw[i][0] = half[0];
-      kw[i][1] = half[1];
+      const u32x2 half = *reinterpret_cast<const u32x2*>(src + at);
+      x.w[i][0] = half[0];
+      x.w[i][1] = half[1];
     }
-    kb[i] = a.c.ks[row * (D / 32) + quarter * (D / 4) / 32];
+    x.s[i] = (c.ks + row * (D / 32))[s_at];
   }
-  fetch(row0 + n);
-  int pos[NK][4];
-  float w[NK][4];
-  u32x4 k[NK][STEPS];
+}
+
+// The sum over a row of 16 lanes, in every one of them.
+template <int CTRL>
+__device__ __forceinline__ float add_ror(float x) {
+  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float row_sum(float x) {
+  x = add_ror<0x121>(x);  // row_ror:1
+  x = add_ror<0x122>(x);
+  x = add_ror<0x124>(x);
+  return add_ror<0x128>(x);
+}
+
+template <int NK>
+__device__ __forceinline__ void store_weights(const Kv4WeightsArgs& a, float (&w)[NK][4], int bh,
+                                              int slot0, int lane) {
 #pragma unroll
   for (int i = 0; i < NK; ++i) {
+    if (slot0 + 16 * i >= a.c.C) break;
+    f32x4 x;
 #pragma unroll
-    for (int j = 0; j < STEPS; ++j) k[i][j] = values8<T>(kw[i][j], scale_of(kb[i]));
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int x = 16 * i + 4 * quarter + e;
-      pos[i][e] = x < wrap ? p0 + x : x < slots ? p0 + x - C : -1;
-      w[i][e] = 0.f;
-    }
-  }
-  const bool whole = p0 >= 0 && wrap == 16 * NK;  // every slot holds p0 + x
-  int t_lo = (int)t0, g_lo = 0;  // of row0
-  for (; row0 < row_end; row0 += 16) {
-    u32x4 q[STEPS];
-#pragma unroll
-    for (int i = 0; i < STEPS; ++i) q[i] = qn[i];
-    const float lse = lse_n;
-    const int t = t_n;
-    t_n += dt;
-    g_n += dg;
-    if (g_n >= a.G) {
-      g_n -= a.G;
-      ++t_n;
-    }
-    // every row of the 16 sees every slot
-    const int t_hi = min(t_lo + (g_lo + 15 >= a.G ? dt + 1 : 0), (int)t1 - 1);  // or more
-    const bool full = whole && p0 >= row_range(t_hi, n_new, len, C, a.window).lo &&
-                      p0 + 16 * NK - 1 <= row_range(t_lo, n_new, len, C, a.window).hi;
-    t_lo += dt;
-    g_lo += dg;
-    if (g_lo >= a.G) {
-      g_lo -= a.G;
-      ++t_lo;
-    }
-    if (row0 + 16 < row_end) fetch(row0 + 16 + n);
-    auto add = [&](auto masked) __attribute__((always_inline)) {
-      const RowRange rr = row_range(t, n_new, len, C, a.window);
-#pragma unroll
-      for (int i = 0; i < NK; ++i) {
-        f32x4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < STEPS; ++j) s = Fmt<T>::mfma(k[i][j], q[j], s);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = __builtin_amdgcn_exp2f(fmaf(s[e], a.c_log2, -lse));
-          if constexpr (decltype(masked)::value)
-            w[i][e] += pos[i][e] >= rr.lo && pos[i][e] <= rr.hi ? x : 0.f;
-          else
-            w[i][e] += x;
-        }
-      }
-    };
-    if (full)
-      add(Bool<false>());
-    else
-      add(Bool<true>());
-  }
-#pragma unroll
-  for (int i = 0; i < NK; ++i) {
-    if (slot0 + 16 * i >= C) break;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float x = w[i][e];
-      x += __shfl_xor(x, 1);
-      x += __shfl_xor(x, 2);
-      x += __shfl_xor(x, 4);
-      x += __shfl_xor(x, 8);
-      w[i][e] = x;
-    }
-    if (n == 0) {
-      f32x4* at = reinterpret_cast<f32x4*>(dst + 16 * i);
-      f32x4 x = {w[i][0], w[i][1], w[i][2], w[i][3]};
+    for (int e = 0; e < 4; ++e) x[e] = row_sum(w[i][e]);
+    if ((lane & 15) == 0) {
+      f32x4* at = reinterpret_cast<f32x4*>(a.weights + (int64_t)bh * a.c.C + slot0 + 16 * i +
+                                           4 * (lane >> 4));
       if (a.accumulate) x += *at;
       *at = x;
     }
   }
 }
 
+// Up to 16 rows (a token's, or a few tokens'): they stay in registers and the keys
+// stream by, the next ones loaded ahead.
+template <typename T, int D>
+__global__ __launch_bounds__(256, 4) void kv4_weights_rows_kernel(Kv4WeightsArgs a) {
+  constexpr int STEPS = D / 32, NK = 4, GROUP = 16 * NK;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int quarter = lane >> 4, n = lane & 15;
+  const int C = a.c.C;
+  const int bh = blockIdx.y, b = bh / a.c.H, h = bh - b * a.c.H;
+  const int t = min(n / a.G, a.Tq - 1), head = h * a.G + n % a.G;
+  u32x4 q[STEPS];
+  {
+    const T* src = static_cast<const T*>(a.q) + b * a.q_sb + t * a.q_st + (int64_t)head * a.q_sh +
+                   quarter * (D / 4);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) q[i] = *reinterpret_cast<const u32x4*>(src + 8 * i);
+  }
+  float lse = a.lse[((int64_t)b * a.G * a.c.H + head) * a.Tq + t] * kLog2e;
+  const int len = length_of(a.c.len, b), n_new = count_of(a.counts, b, a.Tq);
+  const RowRange rr = row_range(n / a.G, n_new, len, C, a.window);
+  // a row that does not count, or sees nothing: every exponential is 0, whatever it holds
+  if (rr.lo > rr.hi || lse == -INFINITY) {
+    lse = INFINITY;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) q[i] = u32x4{0u, 0u, 0u, 0u};
+  }
+  // what all, and any, of the rows see
+  const int rows = min(16, n_new * a.G);
+  const RowRange first = row_range(0, n_new, len, C, a.window);
+  const RowRange last = row_range((rows - 1) / a.G, n_new, len, C, a.window);
+  const int stride = gridDim.x * 4 * GROUP;
+  int slot0 = (blockIdx.x * 4 + wave) * GROUP;
+  if (slot0 >= C) return;
+  Held at = held_at(slot0, GROUP, len, C);
+  auto seen = [&](const Held& x) { return rows > 0 && x.most >= first.lo && x.least <= last.hi; };
+  KeyCodes<D, NK> x = {}, next = {};
+  if (seen(at)) load_keys<D, NK>(x, a.c, bh, slot0, lane);
+  for (;;) {
+    const int slot_n = slot0 + stride;
+    const bool more = stride < C - slot0;
+    const Held at_n = more ? held_at(slot_n, GROUP, len, C) : at;
+    if (more && seen(at_n)) load_keys<D, NK>(next, a.c, bh, slot_n, lane);
+    if (seen(at)) {
+      const bool full = at.p0 >= last.lo && at.wrap == GROUP && at.p0 + GROUP - 1 <= first.hi;
+      float w[NK][4];
+#pragma unroll
+      for (int i = 0; i < NK; ++i) {
+        f32x4 s;
+        const float sc = scale_of(x.s[i]);
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j)
+          s = Fmt<T>::mfma(values8<T>(x.w[i][j], sc), q[j], j == 0 ? f32x4{} : s);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[i][e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.c_log2, -lse));
+      }
+      if (!full) {
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int y = 16 * i + 4 * quarter + e;
+            const int p = y < at.wrap ? at.p0 + y : y < at.slots ? at.p0 + y - C : -1;
+            if (p < rr.lo || p > rr.hi) w[i][e] = 0.f;
+          }
+      }
+      store_weights<NK>(a, w, bh, slot0, lane);
+    } else if (!a.accumulate && lane < at.slots) {
+      a.weights[(int64_t)bh * C + slot0 + lane] = 0.f;
+    }
+    if (!more) return;
+    slot0 = slot_n;
+    at = at_n;
+    x = next;
+  }
+}
+
+// Many rows: a wavefront holds 64 keys and sweeps the rows; 64 rows at a time go
+// through LDS, for the workgroup's 4 wavefronts, the next ones loaded a turn ahead
+// (each wavefront loading 16 rows for itself, a turn ahead too, waited for them: 66
+// us for 512 queries on 16384 keys, 16/8 heads of 128, against KKK). Rows of 2 D
+// bytes, chunk c of 16 at c ^ (row % 16), so that 16 rows' reads spread over the banks.
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void kv4_weights_kernel(Kv4WeightsArgs a) {
+  constexpr int STEPS = D / 32, NK = 4, GROUP = 16 * NK, ROWS = 64;
+  constexpr int CH = D / 8;            // chunks of a row
+  constexpr int PASS = ROWS * CH / 256;  // a thread loads one chunk of so many rows
+  constexpr int PROWS = ROWS / PASS;
+  __shared__ __attribute__((aligned(16))) char sq[2][ROWS * D * 2];
+  __shared__ float sl[2][ROWS];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int quarter = lane >> 4, n = lane & 15;
+  const int C = a.c.C;
+  const int bh = blockIdx.y, b = bh / a.c.H, h = bh - b * a.c.H;
+  const int slot_wg = blockIdx.x * 4 * GROUP, slot0 = slot_wg + wave * GROUP;
+  const int len = length_of(a.c.len, b), n_new = count_of(a.counts, b, a.Tq);
+  // rows that can see one of the workgroup's keys: pos >= least, pos - W < most
+  const Held all = held_at(slot_wg, 4 * GROUP, len, C);
+  const int base = len - n_new;
+  int64_t t0 = 0, t1 = 0;
+  if (all.most >= 0) {
+    t1 = n_new;
+    if (a.window > 0) t1 = min(t1, (int64_t)all.most + a.window - base);
+    t1 = max(t1, (int64_t)0);
+    t0 = min(max((int64_t)all.least - base, (int64_t)0), t1);
+  }
+  const int row_end = (int)t1 * a.G;  // at most Tq G
+  int row0 = (int)t0 * a.G;
+  const bool own = slot0 < C;  // a wavefront without slots loads rows for the others
+  const Held at = held_at(own ? slot0 : 0, GROUP, len, C);
+
+  uint32_t kw[NK][STEPS], ks[NK];
+#pragma unroll
+  for (int i = 0; i < NK; ++i) {
+    const int64_t row = (int64_t)bh * C + min(slot0 + 16 * i, C - 16) + n;  // past C: unused
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j)
+      kw[i][j] = *reinterpret_cast<const uint32_t*>(a.c.kc + row * (D / 2) + (4 * j + quarter) * 4);
+    ks[i] = 0;
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j) ks[i] |= (uint32_t)a.c.ks[row * STEPS + j] << (8 * j);
+  }
+  // The thread's rows: where they lie, moved on by 64 a turn without a division; past
+  // the end they stay where they are, and do not count.
+  const int dt = ROWS / a.G, dg = ROWS % a.G;
+  const int64_t q_step = dt * a.q_st + dg * a.q_sh, q_wrap = a.q_st - a.G * a.q_sh;
+  int row_l[PASS], g_l[PASS];
+  const T* q_l[PASS];
+  u32x4 qn[PASS];
+#pragma unroll
+  for (int i = 0; i < PASS; ++i) {
+    row_l[i] = row0 + i * PROWS + tid / CH;
+    const int row = max(min(row_l[i], row_end - 1), 0), t = row / a.G;
+    g_l[i] = row - t * a.G;
+    q_l[i] = static_cast<const T*>(a.q) + b * a.q_sb + t * a.q_st +
+             (int64_t)(h * a.G + g_l[i]) * a.q_sh + tid % CH * 8;
+  }
+  float lse_n = 0.f;  // of row row0 + tid, threads 0 .. 63
+  auto fetch = [&](int row0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PASS; ++i) qn[i] = *reinterpret_cast<const u32x4*>(q_l[i]);
+    if (wave == 0) {
+      const int row = min(row0 + lane, row_end - 1), t = row / a.G;
+      lse_n = a.lse[((int64_t)bh * a.G + row - t * a.G) * a.Tq + t] * kLog2e;
+      // a row that is not there, or sees nothing: every exponential is 0
+      if (row0 + lane >= row_end || lse_n == -INFINITY) lse_n = INFINITY;
+    }
+  };
+  auto put = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PASS; ++i) {
+      const int row = i * PROWS + tid / CH;
+      *reinterpret_cast<u32x4*>(sq[buf] + row * (D * 2) + (((tid % CH) ^ row) & (CH - 1)) * 16) =
+          qn[i];
+    }
+    if (wave == 0) sl[buf][lane] = lse_n;
+  };
+  auto move_on = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PASS; ++i) {
+      row_l[i] += ROWS;
+      if (row_l[i] < row_end) {
+        const bool wrap = g_l[i] + dg >= a.G;
+        g_l[i] += wrap ? dg - a.G : dg;
+        q_l[i] += wrap ? q_step + q_wrap : q_step;
+      }
+    }
+  };
+  float w[NK][4];
+  u32x4 k[NK][STEPS];
+#pragma unroll
+  for (int i = 0; i < NK; ++i) {
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j)
+      k[i][j] = values8<T>(kw[i][j], scale_of((ks[i] >> (8 * j)) & 255u));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[i][e] = 0.f;
+  }
+  const bool whole = at.p0 >= 0 && at.wrap == GROUP;  // every slot holds p0 + its number
+  if (row0 < row_end) {
+    fetch(row0);
+    put(0);
+    move_on();
+  }
+  int buf = 0;
+  for (; row0 < row_end; row0 += ROWS, buf ^= 1) {
+    __syncthreads();  // this turn's rows are written, the last turn's read
+    const bool more = row0 + ROWS < row_end;
+    if (more) fetch(row0 + ROWS);
+    // what all of the 64 rows see
+    const int t_lo = row0 / a.G, t_hi = (min(row0 + ROWS, row_end) - 1) / a.G;
+    const bool full = whole && at.p0 >= row_range(t_hi, n_new, len, C, a.window).lo &&
+                      at.p0 + GROUP - 1 <= row_range(t_lo, n_new, len, C, a.window).hi;
+    // the scores of 16 rows are issued against the exponentials of the 16 before
+    auto scores = [&](f32x4 (&s)[NK], int r) __attribute__((always_inline)) {
+      const int row = 16 * r + n;
+      u32x4 q[STEPS];
+#pragma unroll
+      for (int j = 0; j < STEPS; ++j)
+        q[j] = *reinterpret_cast<const u32x4*>(sq[buf] + row * (D * 2) +
+                                               (((4 * j + quarter) ^ row) & (CH - 1)) * 16);
+#pragma unroll
+      for (int j = 0; j < STEPS; ++j)
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+          s[i] = Fmt<T>::mfma(k[i][j], q[j], j == 0 ? f32x4{} : s[i]);
+    };
+    auto add = [&](auto masked) __attribute__((always_inline)) {
+      f32x4 s[2][NK];
+      scores(s[0], 0);
+#pragma unroll
+      for (int r = 0; r < ROWS / 16; ++r) {
+        if (r + 1 < ROWS / 16) scores(s[(r + 1) & 1], r + 1);
+        const float lse = sl[buf][16 * r + n];
+        RowRange rr = {0, 0};
+        if constexpr (decltype(masked)::value)
+          rr = row_range((row0 + 16 * r + n) / a.G, n_new, len, C, a.window);
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[r & 1][i][e], a.c_log2, -lse));
+            if constexpr (decltype(masked)::value) {
+              const int y = 16 * i + 4 * quarter + e;
+              const int p = y < at.wrap ? at.p0 + y : y < at.slots ? at.p0 + y - C : -1;
+              w[i][e] += p >= rr.lo && p <= rr.hi ? x : 0.f;
+            } else {
+              w[i][e] += x;
+            }
+          }
+      }
+    };
+    if (full)
+      add(Bool<false>());
+    else
+      add(Bool<true>());
+    if (more) {
+      put(buf ^ 1);
+      move_on();
+    }
+  }
+  if (own) store_weights<NK>(a, w, bh, slot0, lane);
+}
+
 template <typename T, int D>
 hipError_t launch_weights_typed(const Kv4WeightsArgs& a, hipStream_t st) {
   constexpr int NK = 4;
-  const dim3 grid((a.c.C + 64 * NK - 1) / (64 * NK), a.c.B * a.c.H);
-  hipLaunchKernelGGL((kv4_weights_kernel<T, D, NK>), grid, dim3(256), 0, st, a);
+  const int groups = (a.c.C + 64 * NK - 1) / (64 * NK), heads = a.c.B * a.c.H;  // of 4 wavefronts
+  if ((int64_t)a.Tq * a.G <= 16) {
+    const int64_t each = ((int64_t)groups * heads + 1023) / 1024;  // groups a workgroup
+    const dim3 grid((unsigned)((groups + each - 1) / each), heads);
+    hipLaunchKernelGGL((kv4_weights_rows_kernel<T, D>), grid, dim3(256), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((kv4_weights_kernel<T, D>), dim3(groups, heads), dim3(256), 0, st, a);
+  }
   return hipGetLastError();
 }
 
