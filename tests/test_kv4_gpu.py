@@ -278,6 +278,21 @@ def test_strided_queries(gpu):
         assert torch.equal(w, kv4_key_weights(q.contiguous(), c, lse))
 
 
+def test_contiguous_with_odd_strides_of_one(gpu):
+    """Dimensions of 1 may have any stride, and rows may start off 16 bytes."""
+    c, r = _pair(1, 1, 64, 64, BF, (33,))
+    flat = _rand(5, 4 * 64 + 9).cuda()
+    for off in (0, 3):
+        x = flat[off:].as_strided((1, 1, 1, 64), (77, 5, 3, 1))
+        q = flat[off:].as_strided((1, 1, 4, 64), (13, 7, 64, 1))
+        assert x.is_contiguous() and q.is_contiguous()
+        kv4_append(c, x, x)
+        r.append(x, x)
+        o, lse = kv4_attn(q, c, return_lse=True)
+        _check_attn(r, q, o, lse, None, None)
+        kv4_key_weights(q, c, lse)
+
+
 def test_lengths_out_of_range_read_nothing_wrong(gpu):
     """Entries that no append leaves: every slot is still in range and rows without a
     position are empty."""

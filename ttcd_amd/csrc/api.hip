@@ -8,6 +8,7 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <algorithm>
 #include <mutex>
 
 #include "internal.h"
@@ -1202,14 +1203,8 @@ int kv4_window(int window) {
   return window <= 0 ? 0 : (window < ttcd::kKv4MaxLength ? window : ttcd::kKv4MaxLength);
 }
 
-#ifndef KV4_T1
-#define KV4_T1 1024
-#endif
-#ifndef KV4_T8
-#define KV4_T8 512
-#endif
-#ifndef KV4_MINT
-#define KV4_MINT 8
+#ifndef KV4_UNSPLIT
+#define KV4_UNSPLIT 40
 #endif
 struct Kv4Plan {
   int row_tiles, nrb, parts;
@@ -1230,9 +1225,13 @@ Kv4Plan kv4_plan(const ttcd_kv4_cache* c, int Tq, int Hq, int window) {
     keys = span < keys ? span : keys;
   }
   const int64_t tiles = keys / 32 + 1, groups = (int64_t)c->batch * c->kv_heads * p.nrb;
-  int64_t parts = tiles <= 32 ? 1 : (p.row_tiles < 8 ? (KV4_T1 + groups - 1) : KV4_T8) / groups;
-  if (parts > tiles / KV4_MINT) parts = tiles / KV4_MINT;
-  p.parts = parts < 1 ? 1 : parts < ttcd::kKv4MaxParts ? (int)parts : ttcd::kKv4MaxParts;
+  int64_t parts = 1;
+  if (p.row_tiles < 8) {
+    if (tiles > KV4_UNSPLIT) parts = std::min((1024 + groups - 1) / groups, tiles / 16);
+  } else if (tiles > 32) {
+    parts = std::min(512 / groups, tiles / 8);
+  }
+  p.parts = (int)std::min(std::max(parts, (int64_t)1), (int64_t)ttcd::kKv4MaxParts);
   return p;
 }
 

@@ -191,7 +191,7 @@ hipError_t launch_attn_combine(const CombineArgs& a, Elem dtype, hipStream_t str
 
 // The 4-bit key / value cache (kv4.hip; its format is told there).
 constexpr int kKv4MaxLength = 1 << 30;  // positions of a sequence
-constexpr int kKv4MaxParts = 128;       // workgroups over the keys of a row
+constexpr int kKv4MaxParts = 64;        // workgroups over the keys of a row
 
 struct Kv4Cache {
   uint8_t* kc;  // (B, H, C, D / 2)

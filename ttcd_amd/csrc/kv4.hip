@@ -323,10 +323,7 @@ hipError_t launch_read(const Kv4ReadArgs& a, hipStream_t st) {
 // the inputs' type for the product, as the prefill kernels round it; sums and
 // statistics are fp32. In f16 the reference is 7 lower (probabilities up to
 // 2^15), so that small ones keep 7 bits more above f16's least step.
-#ifndef KV4_WAVES
-#define KV4_WAVES 8
-#endif
-constexpr int kRowWaves = KV4_WAVES;
+constexpr int kRowWaves = 8;
 
 template <int D>
 struct KvTile {
@@ -835,8 +832,11 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
       for (int i = 0; i < MB; ++i) o[i] *= f;
     }
   };
-  auto turn = [&](f32x16 (&s)[2], f32x16 (&next)[2], int tile) __attribute__((always_inline)) {
-    if (tile + 1 < t1) scores(next, tile + 1);
+  // Tiles past the last are read and written as the last: memory that is there, and
+  // stages that nothing reads any more.
+  auto turn = [&](f32x16 (&s)[2], f32x16 (&next)[2], int tile, auto more) __attribute__((always_inline)) {
+    constexpr bool kMore = decltype(more)::value;
+    if constexpr (kMore) scores(next, tile + 1);
     u32x4 p[4];
     const float ref = m == -INFINITY ? 0.f : m - Fmt<T>::kBias;
 #pragma unroll
@@ -858,32 +858,37 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
         const u32x4 vf = *reinterpret_cast<const u32x4*>(src + j * (16 * D * 2) + i * 1024);
         o[i] = mfma32<T>(vf, p[j], o[i]);
       }
-    if (tile + 2 < t1) store_k(tile + 2);
-    if (tile + 1 < t1) {
+    if constexpr (kMore) {
+      store_k(tile + 2);
       store_v(tile + 1);
+      load_k(min(tile + 3, t1 - 1));
+      load_v(min(tile + 2, t1 - 1));
       settle(next, tile + 1);
+      __syncthreads();
     }
-    if (tile + 3 < t1) load_k(tile + 3);
-    if (tile + 2 < t1) load_v(tile + 2);
-    __syncthreads();
   };
   if (t0 < t1) {
     load_k(t0);
     load_v(t0);
     store_k(t0);
     store_v(t0);
-    if (t0 + 1 < t1) {
-      load_k(t0 + 1);
-      load_v(t0 + 1);
-      store_k(t0 + 1);
-    }
-    if (t0 + 2 < t1) load_k(t0 + 2);
+    load_k(min(t0 + 1, t1 - 1));
+    load_v(min(t0 + 1, t1 - 1));
+    store_k(t0 + 1);
+    load_k(min(t0 + 2, t1 - 1));
     __syncthreads();
     scores(sa, t0);
     settle(sa, t0);
-    for (int tile = t0; tile < t1; tile += 2) {
-      turn(sa, sb, tile);
-      if (tile + 1 < t1) turn(sb, sa, tile + 1);
+    int tile = t0;
+    for (; tile + 2 < t1; tile += 2) {
+      turn(sa, sb, tile, Bool<true>());
+      turn(sb, sa, tile + 1, Bool<true>());
+    }
+    if (tile + 1 < t1) {
+      turn(sa, sb, tile, Bool<true>());
+      turn(sb, sa, tile + 1, Bool<false>());
+    } else {
+      turn(sa, sb, tile, Bool<false>());
     }
   }
 
@@ -931,9 +936,10 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
   }
 }
 
-// The parts of a row, at most 128: every wavefront finds their weights (2 parts a
-// lane); D / 4 threads with 4 channels each in every one of the 256 / (D / 4)
-// groups share the sums between them.
+// The parts of a row, at most 64: every wavefront finds their weights, a part a
+// lane; D / 4 threads with 4 channels each in every one of the 256 / (D / 4) groups
+// share the sums between them. (One thread after the other over the parts took 29
+// us for 103 of them.)
 template <typename T, int D>
 __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4AttnArgs a) {
   constexpr int TH = D / 4, GR = 256 / TH;
@@ -943,26 +949,19 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4AttnArgs a) {
   const int bh = blockIdx.x / rows, row = blockIdx.x - bh * rows;
   const int b = bh / a.c.H, h = bh - b * a.c.H;
   const int d4 = threadIdx.x % TH, g = threadIdx.x / TH, lane = threadIdx.x & 63;
-  float mp[2], lp[2], f[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int p = lane + 64 * i;
-    const float* ml = a.part_ml + 2 * (p * all + id);
-    mp[i] = p < a.parts ? ml[0] : -INFINITY;
-    lp[i] = p < a.parts ? ml[1] : 0.f;
+  float m = -INFINITY, l = 0.f;
+  if (lane < a.parts) {
+    const float* ml = a.part_ml + 2 * (lane * all + id);
+    m = ml[0];
+    l = ml[1];
   }
-  float m = fmaxf(mp[0], mp[1]);
+  float top = m;
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
-  const float ref = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    f[i] = __builtin_amdgcn_exp2f(mp[i] - ref);
-    l = lp[i] == 0.f ? l : fmaf(lp[i], f[i], l);
-    // an empty part's sums are not read
-    if (lp[i] == 0.f) f[i] = -1.f;
-  }
+  for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+  float f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
+  const bool empty = l == 0.f;  // such a part's sums are not there
+  l = empty ? 0.f : l * f;
+  f = empty ? -1.f : f;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) l += __shfl_xor(l, d);
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -970,12 +969,12 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4AttnArgs a) {
 #pragma unroll 4
   for (int p0 = 0; p0 < a.parts; p0 += GR) {
     const int p = p0 + g;
-    const float w = p < 64 ? __shfl(f[0], p & 63) : __shfl(f[1], p & 63);
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (p < a.parts && !(w < 0.f)) v = *reinterpret_cast<const f32x4*>(src + p * all * D);
-    if (p < a.parts && !(w < 0.f))
+    const float w = __shfl(f, p & 63);
+    if (p < a.parts && !(w < 0.f)) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(src + p * all * D);
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = fmaf(v[e], w, o[e]);
+    }
   }
   so[g][d4] = o;
   __syncthreads();
@@ -989,7 +988,7 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4AttnArgs a) {
       u32x2{pair_of<T>(o[0] * inv, o[1] * inv), pair_of<T>(o[2] * inv, o[3] * inv)};
   if (a.lse != nullptr && d4 == 0)
     a.lse[((int64_t)b * a.G * a.c.H + head) * a.Tq + t] =
-        l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+        l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 template <typename T, int D>
@@ -1369,7 +1368,7 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(Kv4EvictArgs a)
   constexpr int WAVES = kSelThreads / 64;
   __shared__ uint32_t hist[2048];
   __shared__ uint32_t wsum[WAVES];
-  __shared__ uint32_t found[2];
+  __shared__ uint32_t found[3];  // digit, how many of its keys stay, and how many there are
   __shared__ int above[WAVES], equal[WAVES];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1426,18 +1425,28 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(Kv4EvictArgs a)
       }
       if (lane == 63) wsum[wave] = sum;
       __syncthreads();
-      for (int w = 0; w < wave; ++w) sum += wsum[w];
+      uint32_t others = lane < wave ? wsum[lane] : 0u;  // wave < 16
+#pragma unroll
+      for (int d = 1; d < WAVES; d *= 2) others += __shfl_xor(others, d);
+      sum += __builtin_amdgcn_readfirstlane(others);
       const uint32_t before = sum - hi - lo;
       if (before < need && need <= before + hi) {
         found[0] = 2047 - 2 * tid;
         found[1] = need - before;
+        found[2] = hi;
       } else if (before + hi < need && need <= sum) {
         found[0] = 2046 - 2 * tid;
         found[1] = need - before - hi;
+        found[2] = lo;
       }
       __syncthreads();
       prefix |= found[0] << shift;
       need = found[1];
+      if (need == found[2]) {  // all of the digit's keys: what is above the number before it
+        prefix -= 1;           // (it is not 0: then every older key would stay)
+        need = 0;
+        break;
+      }
       bits = pass == 1 ? 10 : 11;
       shift -= bits;
       __syncthreads();
@@ -1462,20 +1471,22 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(Kv4EvictArgs a)
     equal[wave] = eq;
   }
   __syncthreads();
-  uint32_t eq_at = 0;
-  int at = 0;
-  for (int w = 0; w < wave; ++w) {
-    const uint32_t left = need > eq_at ? need - eq_at : 0u;
-    at += above[w] + (int)min((uint32_t)equal[w], left);
-    eq_at += equal[w];
+  // keys before this wavefront's run, of lanes 0 .. 15 one run each
+  int eq_at = lane < wave ? equal[lane] : 0, at = lane < wave ? above[lane] : 0;
+#pragma unroll
+  for (int d = 1; d < WAVES; d *= 2) {
+    eq_at += __shfl_xor(eq_at, d);
+    at += __shfl_xor(at, d);
   }
+  eq_at = __builtin_amdgcn_readfirstlane(eq_at);
+  at = __builtin_amdgcn_readfirstlane(at) + min(eq_at, (int)need);
   const uint64_t below = (1ull << lane) - 1;
   int32_t* index = a.index + (int64_t)bh * a.keep;
   each([&](int j, uint32_t x) __attribute__((always_inline)) {
     bool stays = x > prefix;
     const uint64_t eqs = __ballot(x == prefix);
     if (eqs != 0 && need > 0) {
-      stays = stays || (x == prefix && eq_at + __popcll(eqs & below) < need);
+      stays = stays || (x == prefix && eq_at + __popcll(eqs & below) < (int)need);
       eq_at += __popcll(eqs);
     }
     const uint64_t all = __ballot(stays);

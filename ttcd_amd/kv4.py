@@ -29,6 +29,7 @@ the others on it.
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 
 import torch
 
@@ -98,21 +99,23 @@ class KV4Cache:
             raise ValueError(f"KV4Cache: head_dim must be 64 or 128 and capacity a multiple of "
                              f"{BLOCK}, got {tuple(k_codes.shape)}")
         dev, u8 = k_codes.device, torch.uint8
-        for t, shape, dt in ((k_codes, (B, H, C, half), u8), (k_scales, (B, H, C, D // 32), u8),
-                             (v_codes, (B, H, C // 4, D // 8, 4, 4), u8),
-                             (v_scales, (B, H, C // 4, D // 32, 4), u8),
-                             (lengths, (B,), torch.int32),
-                             (weights, (B, H, C), torch.float32)):
-            if t is None and t is weights:
-                continue
-            if (not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != dt
-                    or t.device != dev or not t.is_contiguous()):
-                raise ValueError(f"KV4Cache: expected contiguous {shape} {dt} on {dev}")
-        if not k_codes.is_cuda:
+        if (k_scales.shape != (B, H, C, D // 32) or v_codes.shape != (B, H, C // 4, D // 8, 4, 4)
+                or v_scales.shape != (B, H, C // 4, D // 32, 4) or lengths.shape != (B,)
+                or k_codes.dtype != u8 or k_scales.dtype != u8 or v_codes.dtype != u8
+                or v_scales.dtype != u8 or lengths.dtype != torch.int32
+                or (weights is not None and (weights.shape != (B, H, C)
+                                             or weights.dtype != torch.float32))):
+            raise ValueError("KV4Cache: shapes or types of the parts are not those of a cache of "
+                             f"(B, H, C, D) = {(B, H, C, D)}")
+        parts = (k_codes, k_scales, v_codes, v_scales, lengths)
+        for t in parts if weights is None else parts + (weights,):
+            if t.device != dev or not t.is_contiguous():
+                raise ValueError(f"KV4Cache: the parts must be contiguous and on {dev}")
+        if dev.type != "cuda":
             raise ValueError("KV4Cache: the parts must be on a GPU (HIP) device")
         self = cls.__new__(cls)
         self._blob = None
-        self._parts = (k_codes, k_scales, v_codes, v_scales, lengths)
+        self._parts = parts
         self.weights = weights
         self._bind(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
                    v_scales.data_ptr(), lengths.data_ptr(), B, H, D, C, dtype, dev)
@@ -194,11 +197,29 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _ready(t: torch.Tensor) -> torch.Tensor:
-    """t, or a copy, with rows as the C entries take them: also a contiguous t that
-    starts off 16 bytes."""
-    t = _packed(t)
-    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+# stride arrays (only read) of the last calls: finding one is quicker than making it
+_strides = lru_cache(maxsize=64)(_lib.strides4)
+
+
+@lru_cache(maxsize=64)
+def _dense(T: int, H: int, D: int):
+    return _lib.strides4((T * H * D, H * D, D, 1))
+
+
+def _operand(t: torch.Tensor):
+    """(t, or a copy, with rows as the C entries take them, its stride array). A
+    contiguous t's dimensions of 1 may have any stride, and it may start off 16 bytes."""
+    if not t.is_contiguous():
+        x = _packed(t)
+        if x is t:
+            return t, _strides(t.stride())
+        t = x
+    if t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t, _dense(t.shape[1], t.shape[2], t.shape[3])
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _window(window) -> int:
@@ -207,7 +228,7 @@ def _window(window) -> int:
 
 def _call(cache: KV4Cache, fn, *args) -> None:
     """fn(*args, stream) with the cache's device current: the launches go to it."""
-    if torch.cuda.current_device() == cache.device.index:
+    if _current_device() == cache.device.index:
         _lib.check(fn(*args, _lib.stream(cache)))
     else:
         with torch.cuda.device(cache.device):
@@ -230,9 +251,9 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, *,
         raise ValueError(f"kv4_append: {T} positions into a cache of {cache.capacity}")
     if T == 0:
         return
-    k, v = _ready(k), _ready(v)
+    (k, ks), (v, vs) = _operand(k), _operand(v)
     _call(cache, _lib.lib().ttcd_kv4_append, cache._ref, k.data_ptr(), v.data_ptr(), T,
-          _lib.strides4(k.stride()), _lib.strides4(v.stride()), _ptr(counts),
+          ks, vs, _ptr(counts),
           _ptr(cache.weights), _DT[cache.dtype])
 
 
@@ -244,8 +265,9 @@ def kv4_read(cache: KV4Cache, count: int) -> tuple[torch.Tensor, torch.Tensor]:
     count = int(count)
     if count < 0:
         raise ValueError(f"kv4_read: count must be >= 0, got {count}")
-    k, v = (torch.empty(cache.batch, count, cache.kv_heads, cache.head_dim, dtype=cache.dtype,
-                        device=cache.device) for _ in range(2))
+    k = torch.empty(cache.batch, count, cache.kv_heads, cache.head_dim, dtype=cache.dtype,
+                    device=cache.device)
+    v = torch.empty_like(k)
     if count:
         _call(cache, _lib.lib().ttcd_kv4_read, cache._ref, k.data_ptr(), v.data_ptr(), count,
               _DT[cache.dtype])
@@ -268,7 +290,7 @@ def kv4_attn(q: torch.Tensor, cache: KV4Cache, window: int | None = None, *,
     if window is not None and window == 0:
         raise ValueError("kv4_attn: window must be >= 1, or None / < 0 for none")
     B, T, H, D = q.shape
-    q = _ready(q)
+    q, qs = _operand(q)
     o = torch.empty(B, T, H, D, dtype=q.dtype, device=q.device)
     lse = torch.empty(B, H, T, dtype=torch.float32, device=q.device) if return_lse else None
     if T > 0:
@@ -276,7 +298,7 @@ def kv4_attn(q: torch.Tensor, cache: KV4Cache, window: int | None = None, *,
         n = L.ttcd_kv4_attn_workspace_bytes(cache._ref, T, H, W) if split_keys else 0
         work = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
         _call(cache, L.ttcd_kv4_attn_fwd, cache._ref, q.data_ptr(), o.data_ptr(), _ptr(lse), T, H,
-              _lib.strides4(q.stride()), _lib.strides4(o.stride()), _ptr(counts), W, D ** -0.5,
+              qs, _dense(T, H, D), _ptr(counts), W, D ** -0.5,
               _DT[q.dtype], _ptr(work), n)
     return (o, lse) if return_lse else o
 
@@ -308,9 +330,9 @@ def kv4_key_weights(q: torch.Tensor, cache: KV4Cache, lse: torch.Tensor,
                          "16-byte aligned")
     if T == 0:
         return out if accumulate else out.zero_()
-    q, lse = _ready(q), lse.contiguous()
+    (q, qs), lse = _operand(q), lse.contiguous()
     _call(cache, _lib.lib().ttcd_kv4_key_weights_fwd, cache._ref, q.data_ptr(), lse.data_ptr(),
-          out.data_ptr(), T, H, _lib.strides4(q.stride()), _ptr(counts), _window(window),
+          out.data_ptr(), T, H, qs, _ptr(counts), _window(window),
           D ** -0.5, int(bool(accumulate)), _DT[q.dtype])
     return out
 
