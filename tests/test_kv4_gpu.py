@@ -431,6 +431,37 @@ def test_prefill_decode_evict_and_on(gpu, dtype, D, Hq, H):
     assert torch.allclose(c.weights.double().cpu(), acc, rtol=1e-3, atol=1e-6)
 
 
+def test_two_calls_at_once_on_one_cache(gpu):
+    """Reads of one cache on two streams, each with its own workspace: the results of
+    the calls one after the other, every time."""
+    c, _ = _pair(2, 2, 128, 8192, BF, (8192, 6000))
+    qs = [_rand(i, 2, t, 8, 128).cuda() for i, t in ((1, 1), (2, 100))]
+    want = [kv4_attn(q, c, return_lse=True) for q in qs]
+    ww = [kv4_key_weights(q, c, l) for q, (_, l) in zip(qs, want)]
+    streams = [torch.cuda.Stream() for _ in qs]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(20):
+        for s, q, (_, l) in zip(streams, qs, want):
+            with torch.cuda.stream(s):
+                got.append((*kv4_attn(q, c, return_lse=True), kv4_key_weights(q, c, l)))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        for x, y in zip(g, (*want[i % 2], ww[i % 2])):
+            assert torch.equal(x, y)
+
+
+def test_caches_made_in_inference_mode(gpu):
+    with torch.inference_mode():
+        c = KV4Cache(1, 1, 64, 64, weights=True)
+        kv4_append(c, *[_rand(1, 1, 5, 1, 64).cuda()] * 2)
+    c.reset()
+    assert c.lengths.tolist() == [0]
+    kv4_append(c, *[_rand(1, 1, 5, 1, 64).cuda()] * 2)
+    assert c.lengths.tolist() == [5]
+
+
 def test_another_stream(gpu):
     c, r = _pair(1, 2, 64, 256, BF, (200,))
     k, v, q = (_rand(i, 1, 9, h, 64).cuda() for i, h in ((1, 2), (2, 2), (3, 4)))

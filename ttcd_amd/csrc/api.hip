@@ -1203,9 +1203,6 @@ int kv4_window(int window) {
   return window <= 0 ? 0 : (window < ttcd::kKv4MaxLength ? window : ttcd::kKv4MaxLength);
 }
 
-#ifndef KV4_UNSPLIT
-#define KV4_UNSPLIT 40
-#endif
 struct Kv4Plan {
   int row_tiles, nrb, parts;
 };
@@ -1227,7 +1224,7 @@ Kv4Plan kv4_plan(const ttcd_kv4_cache* c, int Tq, int Hq, int window) {
   const int64_t tiles = keys / 32 + 1, groups = (int64_t)c->batch * c->kv_heads * p.nrb;
   int64_t parts = 1;
   if (p.row_tiles < 8) {
-    if (tiles > KV4_UNSPLIT) parts = std::min((1024 + groups - 1) / groups, tiles / 16);
+    if (tiles > 40) parts = std::min((1024 + groups - 1) / groups, tiles / 16);
   } else if (tiles > 32) {
     parts = std::min(512 / groups, tiles / 8);
   }

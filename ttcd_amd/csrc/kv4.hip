@@ -727,13 +727,13 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
     u32x4 c[2];
     uint32_t s[2];
   };
-  Codes kc, vc;
+  Codes kc, vc;  // loaded, to be converted
   // the slot of a tile's 16 keys of this wavefront: its halves may lie apart where
   // the ring ends, a multiple of 32 slots from anything
   auto slot_of = [&](int tile) __attribute__((always_inline)) {
     return (int)((uint32_t)(tile * kBlockKeys + wave * 16) % (uint32_t)C);
   };
-  auto load_k = [&](int tile) __attribute__((always_inline)) {
+  auto load_k = [&](Codes& kc, int tile) __attribute__((always_inline)) {
     const int64_t row = (int64_t)bh * C + slot_of(tile) + (lane & 15);
     const uint8_t* src = a.c.kc + row * (D / 2) + kq * (D / 8);
     if constexpr (D == 128) {
@@ -745,7 +745,7 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
     }
     kc.s[0] = a.c.ks[row * (D / 32) + kq * (D / 4) / 32];
   };
-  auto load_v = [&](int tile) __attribute__((always_inline)) {
+  auto load_v = [&](Codes& vc, int tile) __attribute__((always_inline)) {
     const int64_t g = (((int64_t)bh * C + slot_of(tile)) >> 2) + half;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -753,7 +753,7 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
       vc.s[i] = *reinterpret_cast<const uint32_t*>(a.c.vs + ((g + 2 * i) * (D / 32) + vw / 4) * 4);
     }
   };
-  auto store_k = [&](int tile) __attribute__((always_inline)) {
+  auto store_k = [&](const Codes& kc, int tile) __attribute__((always_inline)) {
     char* dst = smem + (tile & 1) * TILE + (km >> 5) * (32 * D * 2) + (km & 31) * 16;
     const float s = scale_of(kc.s[0]);
 #pragma unroll
@@ -762,7 +762,7 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
       *reinterpret_cast<u32x4*>(dst + c * 512) = values8<T>(kc.c[0][i], s);
     }
   };
-  auto store_v = [&](int tile) __attribute__((always_inline)) {
+  auto store_v = [&](const Codes& vc, int tile) __attribute__((always_inline)) {
     char* dst = smem + (2 + (tile & 1)) * TILE + wave * (16 * D * 2) + lane * 16;
     uint32_t w[8];
     float s[8];
@@ -859,23 +859,24 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
         o[i] = mfma32<T>(vf, p[j], o[i]);
       }
     if constexpr (kMore) {
-      store_k(tile + 2);
-      store_v(tile + 1);
-      load_k(min(tile + 3, t1 - 1));
-      load_v(min(tile + 2, t1 - 1));
+      store_k(kc, tile + 2);
+      store_v(vc, tile + 1);
+      load_k(kc, min(tile + 3, t1 - 1));
+      load_v(vc, min(tile + 2, t1 - 1));
       settle(next, tile + 1);
       __syncthreads();
     }
   };
   if (t0 < t1) {
-    load_k(t0);
-    load_v(t0);
-    store_k(t0);
-    store_v(t0);
-    load_k(min(t0 + 1, t1 - 1));
-    load_v(min(t0 + 1, t1 - 1));
-    store_k(t0 + 1);
-    load_k(min(t0 + 2, t1 - 1));
+    Codes k0, v0, k1;  // what the first turns need, all asked for at once
+    load_k(k0, t0);
+    load_v(v0, t0);
+    load_k(k1, min(t0 + 1, t1 - 1));
+    load_v(vc, min(t0 + 1, t1 - 1));
+    load_k(kc, min(t0 + 2, t1 - 1));
+    store_k(k0, t0);
+    store_v(v0, t0);
+    store_k(k1, t0 + 1);
     __syncthreads();
     scores(sa, t0);
     settle(sa, t0);

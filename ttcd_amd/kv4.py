@@ -155,9 +155,10 @@ class KV4Cache:
 
     def reset(self) -> None:
         """Forget every position."""
-        self.lengths.zero_()
-        if self.weights is not None:
-            self.weights.zero_()
+        with torch.inference_mode():  # a cache made in inference mode is reset outside it too
+            self.lengths.zero_()
+            if self.weights is not None:
+                self.weights.zero_()
 
 
 def _cache(cache, fn: str) -> KV4Cache:
