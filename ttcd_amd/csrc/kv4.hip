@@ -893,23 +893,28 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
     }
   }
 
-  // Accumulator element e of block i: row rho = 8 (e / 4) + 4 half + e % 4, that is
-  // channel 8 (rho % W) + MB (rho / W) + i: 8 in a row a word.
-  if (row >= a.Tq * a.G) return;
   const bool none = rr.lo > rr.hi;  // saw the tiles that nobody's mask cuts
   l = none ? 0.f : l + __shfl_xor(l, 32);
   m = none ? -INFINITY : m - Fmt<T>::kBias;
-  const int64_t at = ((int64_t)part * a.c.B * a.c.H + bh) * ((int64_t)a.Tq * a.G) + row;
-  if (half == 0) {
+  const int rows = a.Tq * a.G, wrow0 = row0 + wave * 32;
+  const int64_t at0 = ((int64_t)part * a.c.B * a.c.H + bh) * (int64_t)rows;
+  if (half == 0 && row < rows) {
     if (a.parts > 1) {
-      a.part_ml[2 * at] = m;
-      a.part_ml[2 * at + 1] = l;
+      a.part_ml[2 * (at0 + row)] = m;
+      a.part_ml[2 * (at0 + row) + 1] = l;
     } else if (a.lse != nullptr) {
       a.lse[((int64_t)b * a.G * a.c.H + head) * a.Tq + t] =
           l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
     }
   }
+  // The wavefront's 32 rows through its quarter of the stages, chunk c of 16 bytes at
+  // c ^ (row % chunks): a lane has pieces of one row, a line is written by as many
+  // lanes as it has chunks.
+  __syncthreads();  // every stage is read
+  char* const rows_at = smem + wave * TILE;
   const float inv = 1.f / l;
+  // Accumulator element e of block i: row rho = 8 (e / 4) + 4 half + e % 4, that is
+  // channel 8 (rho % W) + MB (rho / W) + i: 8 in a row a word.
 #pragma unroll
   for (int wi = 0; wi < W / 2; ++wi) {  // the lane's words: those with bit 2 as its half
     const int w = 8 * (wi >> 2) + 4 * half + (wi & 3);
@@ -921,18 +926,39 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
       x[c] = o[c % MB][e];
     }
     if (a.parts > 1) {
-      if (l != 0.f) {  // an empty part is not read
-        float* dst = a.part + at * D + 8 * w;
-        *reinterpret_cast<f32x4*>(dst) = f32x4{x[0], x[1], x[2], x[3]};
-        *reinterpret_cast<f32x4*>(dst + 4) = f32x4{x[4], x[5], x[6], x[7]};
-      }
+      char* const dst = rows_at + n * (D * 4);
+      *reinterpret_cast<f32x4*>(dst + ((2 * w) ^ (n & (2 * W - 1))) * 16) =
+          f32x4{x[0], x[1], x[2], x[3]};
+      *reinterpret_cast<f32x4*>(dst + ((2 * w + 1) ^ (n & (2 * W - 1))) * 16) =
+          f32x4{x[4], x[5], x[6], x[7]};
     } else {
       u32x4 y;
 #pragma unroll
       for (int c = 0; c < 4; ++c)
         y[c] = l == 0.f ? 0u : pair_of<T>(x[2 * c] * inv, x[2 * c + 1] * inv);
-      *reinterpret_cast<u32x4*>(static_cast<T*>(a.o) + b * a.o_sb + t * a.o_st + head * a.o_sh +
-                                8 * w) = y;
+      *reinterpret_cast<u32x4*>(rows_at + n * (D * 2) + (w ^ (n & (W - 1))) * 16) = y;
+    }
+  }
+  __syncthreads();
+  if (a.parts > 1) {
+    constexpr int CH = 2 * W;
+#pragma unroll
+    for (int i = 0; i < CH / 2; ++i) {
+      const int r = i * (64 / CH) + lane / CH, c = lane % CH;
+      if (wrow0 + r < rows)  // of a part without keys too, which is not read
+        *reinterpret_cast<u32x4*>(a.part + (at0 + wrow0 + r) * D + 4 * c) =
+            *reinterpret_cast<const u32x4*>(rows_at + r * (D * 4) + (c ^ (r & (CH - 1))) * 16);
+    }
+  } else {
+    constexpr int CH = W;
+#pragma unroll
+    for (int i = 0; i < CH / 2; ++i) {
+      const int r = i * (64 / CH) + lane / CH, c = lane % CH;
+      const int to = (wrow0 + r) / a.G, ho = h * a.G + (wrow0 + r) - to * a.G;
+      if (wrow0 + r < rows)
+        *reinterpret_cast<u32x4*>(static_cast<T*>(a.o) + b * a.o_sb + to * a.o_st + ho * a.o_sh +
+                                  8 * c) =
+            *reinterpret_cast<const u32x4*>(rows_at + r * (D * 2) + (c ^ (r & (CH - 1))) * 16);
     }
   }
 }
