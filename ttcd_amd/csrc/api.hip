@@ -1209,6 +1209,21 @@ struct Kv4Plan {
 
 // Workgroups over rows and keys. The lengths are on the GPU: parts go by the most
 // keys that a row block can see, and each takes its share of what there is.
+//
+// Up to 32 rows a key / value head (a token, or a few): kernels of 8 wavefronts with 16
+// or 32 rows that stream the keys, bound by those: parts for 1024 workgroups, but 16
+// tiles of 32 keys each at the least, two a wavefront (us, one token, 16/8 heads of
+// 128: 8 sequences of 4096 keys 15.5, with 8 tiles 19.6; 32 of up to 16384 63, for 512
+// workgroups 68; one of 8192 9.5, with 32 tiles 12.0), and none for up to 40 tiles,
+// where the second launch costs more than it saves (1024 keys 7.5, split 9.0; 2048
+// 9.0 split; 704 6.5).
+//
+// More: 128 rows a workgroup and tiles of 64 keys, of which a turn takes so many us
+// with a CU to itself and so many for each of two that share one. What a split adds is
+// its launch, its rows and its sums, written and read. Measured (us, 16/8 heads of
+// 128): 300 queries on an 8192 window in 3 parts 83, 6 52, 10 48, 12 (taken) 45, 16 54;
+// 1000 queries in 1 part 207, 2 127, 3 119, 4 (taken) 102; 64 queries of 32 sequences
+// on a 960 window in 1 part (taken) 31, 2 61.
 Kv4Plan kv4_plan(const ttcd_kv4_cache* c, int Tq, int Hq, int window) {
   const int G = Hq / c->kv_heads;
   const int64_t rows = (int64_t)Tq * G;
@@ -1221,14 +1236,28 @@ Kv4Plan kv4_plan(const ttcd_kv4_cache* c, int Tq, int Hq, int window) {
     const int64_t span = (int64_t)window + (rb + G - 1) / G;
     keys = span < keys ? span : keys;
   }
-  const int64_t tiles = keys / 32 + 1, groups = (int64_t)c->batch * c->kv_heads * p.nrb;
+  const int64_t groups = (int64_t)c->batch * c->kv_heads * p.nrb;
   int64_t parts = 1;
   if (p.row_tiles < 8) {
+    const int64_t tiles = keys / 32 + 1;
     if (tiles > 40) parts = std::min((1024 + groups - 1) / groups, tiles / 16);
-  } else if (tiles > 32) {
-    parts = std::min(512 / groups, tiles / 8);
+    parts = std::min(std::max(parts, (int64_t)1), (int64_t)ttcd::kKv4MaxParts);
+  } else {
+    const int64_t tiles = keys / 64 + 1;
+    const int64_t most = std::min({512 / groups, tiles / 4, (int64_t)ttcd::kKv4MaxParts});
+    const double all_rows = (double)c->batch * Hq * Tq, bytes = all_rows * (c->head_dim + 2) * 4;
+    const double alone = c->head_dim == 128 ? 1.5 : 1.0, shared = c->head_dim == 128 ? 2.2 : 1.35;
+    double least = 0;
+    for (int64_t n = 1; n == 1 || n <= most; ++n) {
+      const double turns = (double)tiles / n + 1;
+      double t = turns * (groups * n <= 256 ? alone : shared);
+      if (n > 1) t += 3.0 + n * bytes / 7e6 + all_rows * 5e-4;
+      if (n > 1 && t >= least) continue;
+      least = t;
+      parts = n;
+    }
   }
-  p.parts = (int)std::min(std::max(parts, (int64_t)1), (int64_t)ttcd::kKv4MaxParts);
+  p.parts = (int)parts;
   return p;
 }
 
