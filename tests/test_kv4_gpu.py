@@ -335,6 +335,20 @@ def test_key_weights_match_64_bits(gpu, B, T, Hq, H, D, C, lengths, window, coun
     assert ((w.double().sum(-1).cpu() - seen).abs() <= 1e-3 * seen).all()
 
 
+@pytest.mark.parametrize("T,Hq,D,dtype", [(70, 1, 64, BF), (100, 2, 128, HF), (7, 2, 64, BF)])
+def test_a_nan_query_weighs_only_what_it_sees(gpu, T, Hq, D, dtype):
+    c, r = _pair(1, 1, D, 192, dtype, (130,))
+    q = _rand(2, 1, T, Hq, D, dtype=dtype)
+    _, lse = kv4_attn(q.cuda(), c, return_lse=True)
+    good = kv4_key_weights(q.cuda(), c, lse)
+    q[0, 3, 0, 1] = math.nan
+    _, lse = kv4_attn(q.cuda(), c, return_lse=True)
+    w = kv4_key_weights(q.cuda(), c, lse)
+    pos = 130 - T + 3
+    assert torch.isnan(w[0, 0, :pos + 1]).all()
+    assert torch.equal(w[0, 0, pos + 1:], good[0, 0, pos + 1:])
+
+
 # ------------------------------------------------------------------- eviction
 
 def _evict_case(c, r, w, keep, recent, out=None):

@@ -313,9 +313,10 @@ hipError_t launch_read(const Kv4ReadArgs& a, hipStream_t st) {
 // of 32 keys: S^T = K Q^T (16x16x32: keys x rows), online softmax over the
 // registers, O^T = V^T P^T with P as it lies after the first product (the keys
 // of a lane's quarter are the 8 that the second product wants from it, in the
-// order in which it then reads V). The 4 wavefronts of a workgroup take every
-// fourth tile of its part of the keys and are added through LDS; the parts of a
-// row are added by a second launch.
+// order in which it then reads V). The 8 wavefronts of a workgroup take every
+// eighth tile of its part of the keys and are added through LDS; the parts of a
+// row are added by a second launch (by the last workgroup to end, it cost 7 us more
+// of 63 with write-through stores, and fences between the XCDs' caches 400).
 //
 // The reference maximum of a row moves only where a score exceeds it by more
 // than 8 (log2): up to then probabilities stay under 2^8, and the four
@@ -1194,7 +1195,7 @@ __global__ __launch_bounds__(256, 4) void kv4_weights_rows_kernel(Kv4WeightsArgs
 // Many rows: a wavefront holds 64 keys and sweeps the rows; 64 rows at a time go
 // through LDS, for the workgroup's 4 wavefronts, the next ones loaded a turn ahead
 // (each wavefront loading 16 rows for itself, a turn ahead too, waited for them: 66
-// us for 512 queries on 16384 keys, 16/8 heads of 128, against KKK). Rows of 2 D
+// us for 512 queries on 16384 keys, 16/8 heads of 128, against 53). Rows of 2 D
 // bytes, chunk c of 16 at c ^ (row % 16), so that 16 rows' reads spread over the banks.
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void kv4_weights_kernel(Kv4WeightsArgs a) {
@@ -1255,7 +1256,10 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_kernel(Kv4WeightsArgs a) {
   float lse_n = 0.f;  // of row row0 + tid, threads 0 .. 63
   auto fetch = [&](int row0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < PASS; ++i) qn[i] = *reinterpret_cast<const u32x4*>(q_l[i]);
+    for (int i = 0; i < PASS; ++i) {
+      qn[i] = *reinterpret_cast<const u32x4*>(q_l[i]);
+      if (row_l[i] >= row_end) qn[i] = u32x4{0u, 0u, 0u, 0u};  // whatever the row before holds
+    }
     if (wave == 0) {
       const int row = min(row0 + lane, row_end - 1), t = row / a.G;
       lse_n = a.lse[((int64_t)bh * a.G + row - t * a.G) * a.Tq + t] * kLog2e;
