@@ -155,7 +155,9 @@ __device__ __forceinline__ int count_of(const int32_t* counts, int b, int T) {
 // threads, each with 8 channels of one of them: 16 bytes in, 4 out, of a key and
 // of a value. Threads go by channel first for the keys and by slot first for the
 // values, as either lies in the cache, so a wavefront's stores are whole lines.
-// The 4 threads of a block find its largest magnitude by two shuffles.
+// The 4 threads of a block find its largest magnitude by two shuffles. Bound by its
+// traffic and by its launch: 4096 positions of 8 heads of 128 take 7.0 us (21 MB, 3.0
+// TB/s, of which some 3 us are any launch's); a token of 32 sequences 3.5.
 template <typename T>
 __device__ __forceinline__ uint32_t quantise8(u32x4 x, int d1, int d2, uint32_t* scale) {
   // NaN counts as 0: the format holds none
@@ -258,7 +260,8 @@ hipError_t launch_append(const Kv4AppendArgs& a, hipStream_t st) {
 // ---------------------------------------------------------------------------
 // Read back the last `count` positions. A thread takes 8 channels of the 4
 // slots of a group: 16 bytes of value codes in one load, 4 rows of 16 bytes out
-// for keys and for values each.
+// for keys and for values each. Bound by its traffic: 16384 positions of 2 x 8 heads of
+// 128, 170 MB, in 27.0 us (6.3 TB/s).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void read_kernel(Kv4ReadArgs a) {
   constexpr int R = D / 8, BL = D / 32;
@@ -324,6 +327,12 @@ hipError_t launch_read(const Kv4ReadArgs& a, hipStream_t st) {
 // the inputs' type for the product, as the prefill kernels round it; sums and
 // statistics are fp32. In f16 the reference is 7 lower (probabilities up to
 // 2^15), so that small ones keep 7 bits more above f16's least step.
+//
+// Bound by the codes it reads: a token of 32 sequences of up to 16384 keys, 16/8 heads
+// of 128, 294 MB in 57 us (5.2 TB/s), and 4.8 for the sum of its 4 parts. Loads are 16
+// bytes a lane straight into operands, a tile ahead; nothing is staged, as nothing is
+// shared. With 4 wavefronts a workgroup the parts and their sums double (64.9 against
+// 63.5 us in all; one token of 257 keys 5.2 against 4.8).
 constexpr int kRowWaves = 8;
 
 template <int D>
@@ -647,7 +656,15 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Kv4AttnArgs a)
 // One turn folds tile t: the scores of t + 1 are issued against the exponentials
 // of t, then the second product of t against the conversion of K(t + 2) and
 // V(t + 1) from codes that were loaded a turn before. Two stages of each in LDS
-// and one barrier a turn.
+// and one barrier a turn. The last turn is code of its own, so that the others have
+// no branch between products and exponentials (279 -> 272 us).
+//
+// Bound by the matrix pipe and the exponentials, which take about as long: 4096
+// queries on an 8192 window, 16/8 heads of 128, 261 us, 1053 TFLOP/s (a large library
+// product reaches 1226 on the same card). Two workgroups a CU, 64 KiB of LDS and 256
+// registers each. 64 rows a wavefront, which would halve the operand reads, spill
+// (1169 us); every wavefront converting for itself, without LDS, took 476; scheduling
+// groups of a product, a read and 6 VALU operations 277 to 289.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 template <typename T>
@@ -967,7 +984,7 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
 // The parts of a row, at most 64: every wavefront finds their weights, a part a
 // lane; D / 4 threads with 4 channels each in every one of the 256 / (D / 4) groups
 // share the sums between them. (One thread after the other over the parts took 29
-// us for 103 of them.)
+// us for 103 of them; 64 of 30 rows take 3.9, 12 of 9600 rows, 61 MB, 9.0.)
 template <typename T, int D>
 __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4AttnArgs a) {
   constexpr int TH = D / 4, GR = 256 / TH;
@@ -1115,7 +1132,8 @@ __device__ __forceinline__ void store_weights(const Kv4WeightsArgs& a, float (&w
 }
 
 // Up to 16 rows (a token's, or a few tokens'): they stay in registers and the keys
-// stream by, the next ones loaded ahead.
+// stream by, the next ones loaded ahead. Bound by its traffic: a token of 8 sequences
+// of up to 16000 keys, 43 MB, 13.0 us (a workgroup for every 256 keys: 22).
 template <typename T, int D>
 __global__ __launch_bounds__(256, 4) void kv4_weights_rows_kernel(Kv4WeightsArgs a) {
   constexpr int STEPS = D / 32, NK = 4, GROUP = 16 * NK;
@@ -1383,7 +1401,9 @@ hipError_t launch_weights_typed(const Kv4WeightsArgs& a, hipStream_t st) {
 // positions that stay, in order. Wavefronts own runs of keys, so a key's place
 // is the count of kept ones before it: in the wavefront by ballot, over the
 // wavefronts by one sum. A capacity of up to 64 keys a thread is read once, into
-// registers (REGS of them); a longer one at every pass (REGS = 0).
+// registers (REGS of them); a longer one at every pass (REGS = 0). Bound by a CU's
+// VALU and its waits for LDS and barriers, as there are few heads: 16 of 32768 keys
+// 34 us, read at every pass 53.
 constexpr int kSelThreads = 1024;
 
 // Weights in the order of unsigned numbers between 0 and 2^32 - 1, NaN before all
@@ -1529,7 +1549,9 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(Kv4EvictArgs a)
 }
 
 // The kept rows, 4 new slots to D / 8 threads: a thread takes 32 channels of one
-// of the keys, 8 channels of the 4 values.
+// of the keys, 8 channels of the 4 values. Bound by its traffic: half of 32768 keys of
+// 2 x 8 heads, 36 MB in (and as much again beside it in the same lines) and 36 out, 24
+// us (4 bytes a lane of the keys: 37).
 template <int D>
 __global__ __launch_bounds__(256) void kv4_gather_kernel(Kv4EvictArgs a) {
   constexpr int R = D / 8, BL = D / 32;
