@@ -984,7 +984,7 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
 // The parts of a row, at most 64: every wavefront finds their weights, a part a
 // lane; D / 4 threads with 4 channels each in every one of the 256 / (D / 4) groups
 // share the sums between them. (One thread after the other over the parts took 29
-// us for 103 of them; 64 of 30 rows take 3.9, 12 of 9600 rows, 61 MB, 9.0.)
+// us for 103 of them; 64 of 30 rows take 3.9.)
 template <typename T, int D>
 __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4AttnArgs a) {
   constexpr int TH = D / 4, GR = 256 / TH;
@@ -1036,6 +1036,68 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4AttnArgs a) {
         l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
+// The same with few parts (up to 16) of many rows (1024 and more): a wavefront has a
+// row to itself, D / 64 channels a lane, and no other to wait for (us, the sum's share
+// of all: 4 parts of 16000 rows 104 -> 99; fewer rows leave too few wavefronts: 16 of
+// 16 rows 9.5 -> 10.8).
+template <typename T, int D>
+__global__ __launch_bounds__(256) void kv4_combine_rows_kernel(Kv4AttnArgs a) {
+  constexpr int CL = D / 64;
+  const int rows = a.Tq * a.G;
+  const int64_t all = (int64_t)a.c.B * a.c.H * rows;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t id = (int64_t)blockIdx.x * 4 + wave;
+  if (id >= all) return;
+  const int bh = (int)(id / rows), row = (int)(id - (int64_t)bh * rows);
+  const int b = bh / a.c.H, h = bh - b * a.c.H;
+  float m = -INFINITY, l = 0.f;
+  if (lane < a.parts) {
+    const float* ml = a.part_ml + 2 * (lane * all + id);
+    m = ml[0];
+    l = ml[1];
+  }
+  float top = m;
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+  float f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
+  const bool empty = l == 0.f;  // such a part's sums are not there
+  l = empty ? 0.f : l * f;
+  f = empty ? -1.f : f;
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) l += __shfl_xor(l, d);
+  l = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(l)));
+  float o[CL];
+#pragma unroll
+  for (int i = 0; i < CL; ++i) o[i] = 0.f;
+  const float* src = a.part + id * D + CL * lane;
+  for (int p0 = 0; p0 < a.parts; p0 += 4) {
+    float x[4][CL];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < CL; ++i) x[j][i] = src[min(p0 + j, a.parts - 1) * all * D + i];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // an empty part, or one past the last, holds anything
+      const float w = __shfl(f, p0 + j);
+      if (p0 + j < a.parts && !(w < 0.f))
+#pragma unroll
+        for (int i = 0; i < CL; ++i) o[i] = fmaf(x[j][i], w, o[i]);
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int t = row / a.G, head = h * a.G + row - t * a.G;
+  T* dst = static_cast<T*>(a.o) + b * a.o_sb + t * a.o_st + head * a.o_sh + CL * lane;
+  if constexpr (CL == 2)
+    *reinterpret_cast<uint32_t*>(dst) = pair_of<T>(o[0] * inv, o[1] * inv);
+  else
+    *dst = static_cast<T>(o[0] * inv);
+  if (a.lse != nullptr && lane == 0)
+    a.lse[((int64_t)b * a.G * a.c.H + head) * a.Tq + t] =
+        l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
 template <typename T, int D>
 hipError_t launch_attn_typed(const Kv4AttnArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)a.parts * a.nrb * a.c.B * a.c.H));
@@ -1048,7 +1110,11 @@ hipError_t launch_attn_typed(const Kv4AttnArgs& a, hipStream_t st) {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.parts == 1) return e;
   const int64_t rows = (int64_t)a.c.B * a.c.H * a.G * a.Tq;
-  hipLaunchKernelGGL((kv4_combine_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, st, a);
+  if (a.parts <= 16 && rows >= 1024)
+    hipLaunchKernelGGL((kv4_combine_rows_kernel<T, D>), dim3((unsigned)((rows + 3) / 4)),
+                       dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((kv4_combine_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
