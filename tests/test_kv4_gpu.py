@@ -335,6 +335,27 @@ def test_key_weights_match_64_bits(gpu, B, T, Hq, H, D, C, lengths, window, coun
     assert ((w.double().sum(-1).cpu() - seen).abs() <= 1e-3 * seen).all()
 
 
+@pytest.mark.parametrize("T,Hq,window", [(1, 2, 40), (1, 2, None), (9, 2, 33), (30, 2, 20), (90, 4, 64)])
+@pytest.mark.parametrize("dtype,D", [(BF, 128), (HF, 64)])
+def test_values_that_no_query_sees_may_be_nan(gpu, T, Hq, window, dtype, D):
+    """NaN scales, as no append leaves, in positions before every query's window and in
+    slots past the end."""
+    c, r = _pair(1, 2, D, 256, dtype, (200,))
+    seen = 256 if window is None else window + T - 1
+    for t, shape in ((c.k_scales, None), (c.v_scales, True)):
+        x = t if shape is None else t.transpose(3, 4).flatten(2, 3)
+        hidden = torch.ones(256, dtype=torch.bool)
+        hidden[max(0, 200 - seen):200] = False
+        x = x.clone()
+        x[:, :, hidden.cuda()] = 255
+        t.copy_(x if shape is None else x.unflatten(2, (64, 4)).transpose(3, 4))
+    q = _rand(4, 1, T, Hq, D, dtype=dtype)
+    o, lse = kv4_attn(q.cuda(), c, window, return_lse=True)
+    _check_attn(r, q, o, lse, window, None)
+    w = kv4_key_weights(q.cuda(), c, lse, window)
+    assert torch.isfinite(w).all() and (w[..., 200:] == 0).all()
+
+
 @pytest.mark.parametrize("T,Hq,D,dtype", [(70, 1, 64, BF), (100, 2, 128, HF), (7, 2, 64, BF)])
 def test_a_nan_query_weighs_only_what_it_sees(gpu, T, Hq, D, dtype):
     c, r = _pair(1, 1, D, 192, dtype, (130,))
@@ -563,6 +584,27 @@ def test_offsets_past_32_bits(gpu):
     assert torch.allclose(w[-1][:, at.cuda()].double().cpu(), want[:, :40], rtol=1e-4, atol=1e-9)
     new, index, _ = kv4_evict(c, w, 20, 4, out=KV4Cache(B, H, D, 32))
     assert new.lengths.tolist()[-1] == 20 and int(index[-1].max()) == C + 22
+
+
+@pytest.mark.parametrize("D,dtype", [(64, BF), (64, HF), (128, BF), (128, HF)])
+@pytest.mark.parametrize("T", [1, 12])
+def test_caches_past_the_last_level_cache(gpu, D, dtype, T):
+    """A cache of more than 128 MiB is read past the caches: the bits of a small one with
+    the same window of positions."""
+    H, Hq, start = 8, 16, 262144 * 3 - 20
+    big, small = KV4Cache(1, H, D, 262144, dtype), KV4Cache(1, H, D, 128, dtype)
+    k, v = _rand(1, 1, 90, H, D, dtype=dtype).cuda(), _rand(2, 1, 90, H, D, dtype=dtype).cuda()
+    q = _rand(3, 1, T, Hq, D, dtype=dtype).cuda()
+    out = []
+    for c in (big, small):
+        c.lengths.fill_(start)
+        kv4_append(c, k, v)
+        out.append(kv4_attn(q, c, 60, return_lse=True) + kv4_read(c, 90))
+    for x, y in zip(*out):
+        assert torch.equal(x, y)
+    r = kv4_ref.Ref(1, H, D, 128, dtype)
+    r.append(k, v)
+    _check_attn(r, q, out[0][0], out[0][1], 60, None)
 
 
 def test_refusals(gpu):

@@ -329,11 +329,23 @@ hipError_t launch_read(const Kv4ReadArgs& a, hipStream_t st) {
 // 2^15), so that small ones keep 7 bits more above f16's least step.
 //
 // Bound by the codes it reads: a token of 32 sequences of up to 16384 keys, 16/8 heads
-// of 128, 294 MB in 57 us (5.2 TB/s), and 4.8 for the sum of its 4 parts. Loads are 16
+// of 128, 294 MB in 53 us (5.6 TB/s), and 4.8 for the sum of its 4 parts. Loads are 16
 // bytes a lane straight into operands, a tile ahead; nothing is staged, as nothing is
 // shared. With 4 wavefronts a workgroup the parts and their sums double (64.9 against
 // 63.5 us in all; one token of 257 keys 5.2 against 4.8).
+//
+// FAR: a cache that the last-level cache cannot hold beside anything else is read past
+// the caches (the token of 32 sequences 64 -> 59 us), a smaller one through them (44 MB,
+// as it may be there from the call before: 18.6 us, past them 19.4).
 constexpr int kRowWaves = 8;
+
+template <bool FAR, typename V>
+__device__ __forceinline__ V codes(const V* p) {
+  if constexpr (FAR)
+    return __builtin_nontemporal_load(p);
+  else
+    return *p;
+}
 
 template <int D>
 struct KvTile {
@@ -367,8 +379,8 @@ __device__ __forceinline__ void transpose_pair(const uint32_t (&w)[8], const flo
 template <typename T, int D, int NT>
 __device__ __forceinline__ void fold_tile(RowState<T, D, NT>& st, const KvTile<D>& kv,
                                           const u32x4 (&q)[NT][D / 32], float c, int p0, bool masked,
-                                          const int (&lo)[NT], const int (&hi)[NT], int len,
-                                          int lane) {
+                                          const int (&lo)[NT], const int (&hi)[NT], int any_lo,
+                                          int any_hi, int lane) {
   constexpr int STEPS = D / 32, NM = D / 16;
   const int quarter = lane >> 4;
   f32x4 s[NT][2];
@@ -393,8 +405,9 @@ __device__ __forceinline__ void fold_tile(RowState<T, D, NT>& st, const KvTile<D
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
           if (p < lo[nt] || p > hi[nt]) s[nt][g][e] = -INFINITY;
-        // past the sequence's end a slot holds anything: make it finite
-        if (p >= len) {
+        // what no row sees may be anything, and a slot without a position is: make it
+        // finite, for 0 times it to be 0
+        if (p < any_lo || p > any_hi) {
           if (g == 0)
             vs0 &= ~(255u << (8 * e));
           else
@@ -478,7 +491,7 @@ __device__ __forceinline__ RowRange row_range(int t, int n_new, int len, int C, 
   return {lo, pos};
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, bool FAR>
 __global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Kv4AttnArgs a) {
   constexpr int STEPS = D / 32, NM = D / 16, RB = 16 * NT, R = D / 8;
   __shared__ float so[kRowWaves][16][D + 4];
@@ -537,14 +550,15 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Kv4AttnArgs a)
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           if constexpr (D == 128) {
-            kv.k[g] = *reinterpret_cast<const u32x4*>(k0 + (k_at + 16 * g * (D / 2)));
+            kv.k[g] = codes<FAR>(reinterpret_cast<const u32x4*>(k0 + (k_at + 16 * g * (D / 2))));
           } else {
-            const u32x2 half = *reinterpret_cast<const u32x2*>(k0 + (k_at + 16 * g * (D / 2)));
+            const u32x2 half =
+                codes<FAR>(reinterpret_cast<const u32x2*>(k0 + (k_at + 16 * g * (D / 2))));
             kv.k[g][0] = half[0];
             kv.k[g][1] = half[1];
           }
           kv.ks[g] = s0[ks_at + 16 * g * (D / 32)];
-          kv.v[g] = *reinterpret_cast<const u32x4*>(v0 + (v_at + 16 * g * (D / 2)));
+          kv.v[g] = codes<FAR>(reinterpret_cast<const u32x4*>(v0 + (v_at + 16 * g * (D / 2))));
           kv.vs[g] = *reinterpret_cast<const uint32_t*>(t0 + (vs_at + 16 * g * (D / 32)));
         }
       };
@@ -553,7 +567,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Kv4AttnArgs a)
       int slot = (int)((uint32_t)(tile * 32) % (uint32_t)C);
       auto fold = [&](const KvTile<D>& kv) __attribute__((always_inline)) {
         const bool masked = tile * 32 < last.lo || tile * 32 + 31 > first.hi;
-        fold_tile<T, D, NT>(st, kv, q, a.c_log2, tile * 32, masked, lo, hi, len, lane);
+        fold_tile<T, D, NT>(st, kv, q, a.c_log2, tile * 32, masked, lo, hi, first.lo, last.hi, lane);
         tile += kRowWaves;
       };
       auto next = [&](KvTile<D>& kv) __attribute__((always_inline)) {
@@ -713,8 +727,8 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
   f32x16 o[MB];
 #pragma unroll
   for (int i = 0; i < MB; ++i) o[i] = f32x16{};
-  // tiles [t0, t1) of 64 keys that the workgroup folds
-  int t0 = 0, t1 = 0;
+  // tiles [t0, t1) of 64 keys that the workgroup folds, and the keys that any row sees
+  int t0 = 0, t1 = 0, any_lo = 0, any_hi = -1;
   const int t_lo = row0 / a.G, t_hi = min((row0 + RB - 1) / a.G, n_new - 1);
   if (t_lo <= t_hi) {
     const RowRange first = row_range(t_lo, n_new, len, C, a.window);
@@ -724,6 +738,8 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
       const int per = (tiles + a.parts - 1) / a.parts;
       t0 = tile_lo + part * per;
       t1 = min(t0 + per, tile_lo + tiles);
+      any_lo = first.lo;
+      any_hi = last.hi;
     }
   }
   // the keys that all rows of this wavefront see
@@ -784,8 +800,7 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
     char* dst = smem + (2 + (tile & 1)) * TILE + wave * (16 * D * 2) + lane * 16;
     uint32_t w[8];
     float s[8];
-    // a slot past the sequence's end holds anything: make it finite
-    const int past = len - (tile * kBlockKeys + wave * 16 + 4 * half);  // keys of the lane before it
+    const int p = tile * kBlockKeys + wave * 16 + 4 * half;  // the lane's first key
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       w[e] = vc.c[0][e] >> (vk * 4 * MB);
@@ -793,11 +808,13 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
     }
     scales4(vc.s[0], s);
     scales4(vc.s[1], s + 4);
-    if (tile * kBlockKeys + kBlockKeys > len) {
+    // what no row sees may be anything, and a slot without a position is: make it
+    // finite, for 0 times it to be 0
+    if (tile * kBlockKeys < any_lo || tile * kBlockKeys + kBlockKeys - 1 > any_hi) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[e] = e < past ? s[e] : 0.f;
-        s[4 + e] = 8 + e < past ? s[4 + e] : 0.f;
+        s[e] = p + e >= any_lo && p + e <= any_hi ? s[e] : 0.f;
+        s[4 + e] = p + 8 + e >= any_lo && p + 8 + e <= any_hi ? s[4 + e] : 0.f;
       }
     }
     u32x4 even, odd;
@@ -1101,10 +1118,17 @@ __global__ __launch_bounds__(256) void kv4_combine_rows_kernel(Kv4AttnArgs a) {
 template <typename T, int D>
 hipError_t launch_attn_typed(const Kv4AttnArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)a.parts * a.nrb * a.c.B * a.c.H));
-  if (a.row_tiles == 1)
-    hipLaunchKernelGGL((kv4_rows_kernel<T, D, 1>), grid, dim3(64 * kRowWaves), 0, st, a);
+  // codes and scales, against half of the 256 MiB of last-level cache
+  const bool far = (int64_t)a.c.B * a.c.H * a.c.C * (D + D / 16) > (int64_t(128) << 20);
+  const dim3 few(64 * kRowWaves);
+  if (a.row_tiles == 1 && far)
+    hipLaunchKernelGGL((kv4_rows_kernel<T, D, 1, true>), grid, few, 0, st, a);
+  else if (a.row_tiles == 1)
+    hipLaunchKernelGGL((kv4_rows_kernel<T, D, 1, false>), grid, few, 0, st, a);
+  else if (a.row_tiles == 2 && far)
+    hipLaunchKernelGGL((kv4_rows_kernel<T, D, 2, true>), grid, few, 0, st, a);
   else if (a.row_tiles == 2)
-    hipLaunchKernelGGL((kv4_rows_kernel<T, D, 2>), grid, dim3(64 * kRowWaves), 0, st, a);
+    hipLaunchKernelGGL((kv4_rows_kernel<T, D, 2, false>), grid, few, 0, st, a);
   else
     hipLaunchKernelGGL((kv4_block_kernel<T, D>), grid, dim3(256), 0, st, a);
   hipError_t e = hipGetLastError();

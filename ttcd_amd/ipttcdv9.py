@@ -370,7 +370,7 @@ class IPTTCDv9Prefill:
         act = torch.sigmoid(g) if c["gate_fn"] == "sigmoid" else F.silu(g)
         return on * act
 
-    def _ttt_attention(self, q, k, v, ctx: "_Prefill", held):
+    def _ttt_attention(self, q, k, v, ctx: "_Prefill | None" = None, held=None):
         """Teacher and student outputs of a TTT layer; k / v may be longer than q
         (a cached prefill: the queries are the last positions)."""
         if held is not None:
