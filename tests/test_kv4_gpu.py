@@ -433,6 +433,45 @@ def test_evict_into_another_cache(gpu):
         kv4_evict(c, w, 8, out=KV4Cache(2, 2, 64, 32, HF))
 
 
+def test_a_refused_eviction_changes_neither_cache(gpu):
+    c, _ = _pair(2, 2, 64, 64, BF, (64, 10), weights=True)
+    held = c.weights
+    held.fill_(3.0)
+    for keep, out in ((8, c), (8, KV4Cache(1, 2, 64, 64)), (8, KV4Cache(2, 2, 128, 64)),
+                      (33, KV4Cache(2, 2, 64, 32))):
+        had = out.weights
+        with pytest.raises(ValueError):
+            kv4_evict(c, None, keep, out=out)
+        assert out.weights is had and c.weights is held
+    assert (held == 3.0).all() and c.lengths.tolist() == [64, 10]
+
+
+def test_evict_by_the_weights_of_the_cache_written(gpu):
+    """The written cache keeps the new weights, also where its own were gone by."""
+    c, r = _pair(2, 2, 64, 64, BF, (64, 10))
+    out = KV4Cache(2, 2, 64, 64, weights=True)
+    w = torch.rand(2, 2, 64, device=gpu)
+    out.weights.copy_(w)
+    _, index, new = kv4_evict(c, out.weights, 20, 4, out=out)
+    want, ww = r.evict(w.cpu(), 20, 4)
+    assert torch.equal(index.cpu(), want) and torch.equal(new[..., :20].cpu(), ww)
+    assert out.weights is new
+
+
+def test_weights_that_do_not_fit_are_refused(gpu):
+    c = KV4Cache(2, 2, 64, 64, weights=True)
+    held = c.weights
+    for w in (torch.zeros(2, 2, 32, device=gpu), torch.zeros(2, 2, 64),
+              torch.zeros(2, 2, 64, device=gpu, dtype=HF),
+              torch.zeros(2, 2, 128, device=gpu)[..., ::2], [0.0]):
+        with pytest.raises(ValueError):
+            c.weights = w
+    assert c.weights is held
+    c.weights = None
+    kv4_append(c, *[_rand(1, 2, 4, 2, 64).cuda()] * 2)
+    assert c.lengths.tolist() == [4, 4]
+
+
 # ------------------------------------------------------------------- together
 
 @pytest.mark.parametrize("dtype,D,Hq,H", [(BF, 128, 4, 2), (HF, 64, 9, 3)])

@@ -153,6 +153,20 @@ class KV4Cache:
         """Positions that each sequence has had, int32 (batch,)."""
         return self._part(4)
 
+    @property
+    def weights(self) -> torch.Tensor | None:
+        """The slots' attention weights, (batch, kv_heads, capacity) fp32, if they are kept."""
+        return self._weights
+
+    @weights.setter
+    def weights(self, w: torch.Tensor | None) -> None:
+        shape = (self.batch, self.kv_heads, self.capacity)
+        if w is not None and (not isinstance(w, torch.Tensor) or w.shape != shape
+                              or w.dtype != torch.float32 or w.device != self.device
+                              or not w.is_contiguous()):
+            raise ValueError(f"KV4Cache: weights must be contiguous fp32 {shape} on {self.device}")
+        self._weights = w
+
     def reset(self) -> None:
         """Forget every position."""
         with torch.inference_mode():  # a cache made in inference mode is reset outside it too
@@ -330,7 +344,8 @@ def kv4_key_weights(q: torch.Tensor, cache: KV4Cache, lse: torch.Tensor,
         raise ValueError(f"kv4_key_weights: out must be contiguous fp32 {shape} on q's device, "
                          "16-byte aligned")
     if T == 0:
-        return out if accumulate else out.zero_()
+        with torch.inference_mode():
+            return out if accumulate else out.zero_()
     (q, qs), lse = _operand(q), lse.contiguous()
     _call(cache, _lib.lib().ttcd_kv4_key_weights_fwd, cache._ref, q.data_ptr(), lse.data_ptr(),
           out.data_ptr(), T, H, qs, _ptr(counts), _window(window),
@@ -349,7 +364,7 @@ def kv4_evict(cache: KV4Cache, weights: torch.Tensor | None, keep: int, recent: 
     a capacity >= keep) whose positions 0, 1, .. are the kept ones in their order;
     index (B, Hkv, keep) int32, the position that each had, -1 behind the last;
     and their weights by the new cache's slots, which are also ``new.weights`` if
-    the cache keeps weights. The old cache stays as it is."""
+    either cache keeps weights. The old cache stays as it is."""
     _cache(cache, "kv4_evict")
     weights = cache.weights if weights is None else weights
     keep, recent = int(keep), int(recent)
@@ -368,12 +383,11 @@ def kv4_evict(cache: KV4Cache, weights: torch.Tensor | None, keep: int, recent: 
                          f"{keep}, {recent}")
     weights = weights.contiguous()
     index = torch.empty(B, H, keep, dtype=torch.int32, device=cache.device)
-    if out.weights is not None and out.weights.data_ptr() != weights.data_ptr():
-        new_weights = out.weights
-    else:
+    new_weights = out.weights
+    if new_weights is None or new_weights.data_ptr() == weights.data_ptr():
         new_weights = torch.empty(B, H, out.capacity, dtype=torch.float32, device=cache.device)
-        if cache.weights is not None:
-            out.weights = new_weights
     _call(cache, _lib.lib().ttcd_kv4_evict, cache._ref, weights.data_ptr(), keep,
           min(recent, 2**31 - 1), out._ref, new_weights.data_ptr(), index.data_ptr())
+    if cache.weights is not None or out.weights is not None:
+        out.weights = new_weights
     return out, index, new_weights
