@@ -646,6 +646,18 @@ def test_caches_past_the_last_level_cache(gpu, D, dtype, T):
     _check_attn(r, q, out[0][0], out[0][1], 60, None)
 
 
+@pytest.mark.parametrize("weights", [False, True])
+def test_a_cache_of_given_parts_shares_them(gpu, weights):
+    c, _ = _pair(2, 2, 64, 64, BF, (64, 10), weights=weights)
+    d = KV4Cache.from_parts(c.k_codes, c.k_scales, c.v_codes, c.v_scales, c.lengths, BF,
+                            c.weights)
+    assert d.weights is c.weights and d.lengths is c.lengths
+    kv4_append(d, *[_rand(1, 2, 4, 2, 64).cuda()] * 2)
+    assert c.lengths.tolist() == [68, 14]
+    for x, y in zip(kv4_read(c, 64), kv4_read(d, 64)):
+        assert torch.equal(x, y)
+
+
 def test_refusals(gpu):
     c = KV4Cache(2, 2, 64, 64)
     x = _rand(1, 2, 4, 2, 64).cuda()

@@ -116,9 +116,9 @@ class KV4Cache:
         self = cls.__new__(cls)
         self._blob = None
         self._parts = parts
-        self.weights = weights
         self._bind(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
                    v_scales.data_ptr(), lengths.data_ptr(), B, H, D, C, dtype, dev)
+        self.weights = weights
         return self
 
     def _part(self, i: int) -> torch.Tensor:
