@@ -1492,9 +1492,14 @@ hipError_t launch_weights_typed(const Kv4WeightsArgs& a, hipStream_t st) {
 // is the count of kept ones before it: in the wavefront by ballot, over the
 // wavefronts by one sum. A capacity of up to 64 keys a thread is read once, into
 // registers (REGS of them); a longer one at every pass (REGS = 0). Bound by a CU's
-// VALU and its waits for LDS and barriers, as there are few heads: 16 of 32768 keys
-// 34 us, read at every pass 53.
+// latencies and VALU, as there are few heads: 16 of 32768 keys 19 to 22 us, of which 6 are
+// the loads (read at every pass 38); 8 of 131072, at every pass, 132. The loads of 8
+// keys are asked for together, also those of keys that are not there (each waited for by
+// itself, behind its condition: 33 and 174). Keys past a wavefront's run are skipped by
+// 8: with the copies of the rows 40 us, one by one 49; with none skipped 40, but 1001
+// keys in room for 32768 21 instead of 15.5.
 constexpr int kSelThreads = 1024;
+constexpr int kSelStep = 8;  // loads at once
 
 // Weights in the order of unsigned numbers between 0 and 2^32 - 1, NaN before all
 // of them; -0 is 0.
@@ -1502,6 +1507,11 @@ __device__ __forceinline__ uint32_t order_of(float w) {
   if (!(w == w)) return 1u;
   const uint32_t u = __float_as_uint(w + 0.f);
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+}
+
+// Of the lanes in m, how many come before this one.
+__device__ __forceinline__ int lanes_below(uint64_t m) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
 }
 
 template <int REGS>
@@ -1524,23 +1534,49 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(Kv4EvictArgs a)
   const int run = (n + WAVES * 64 - 1) / (WAVES * 64) * 64;  // keys of a wavefront
   const int j0 = wave * run + lane;
   // of the j-th oldest: an older key's weight, the most for a new one, 0 for none
-  auto weight = [&](int j) __attribute__((always_inline)) {
+  auto slot_of = [&](int j) __attribute__((always_inline)) {
     const int s = slot0 + j;
-    return j < cand ? order_of(wt[s >= C ? s - C : s]) : j < n ? 0xffffffffu : 0u;
+    return s >= C ? s - C : s;
+  };
+  auto order = [&](int j, float w) __attribute__((always_inline)) {
+    return j < cand ? order_of(w) : j < n ? 0xffffffffu : 0u;
+  };
+  constexpr int STEP = REGS > 0 && REGS < kSelStep ? REGS : kSelStep;
+  auto load = [&](float* w, int i0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < STEP; ++i) {  // in bounds: slot 0 for what is none of the older keys
+      const int j = j0 + (i0 + i) * 64;
+      w[i] = wt[j < cand ? slot_of(j) : 0];
+    }
+  };
+  // from the run's end on the keys are the next wavefront's: none here
+  auto value = [&](int i, float w) __attribute__((always_inline)) {
+    return i * 64 < run ? order(j0 + i * 64, w) : 0u;
   };
   uint32_t u[REGS > 0 ? REGS : 1];
   if constexpr (REGS > 0) {
+    float w[REGS];
 #pragma unroll
-    for (int i = 0; i < REGS; ++i)
-      if (i * 64 < run) u[i] = weight(j0 + i * 64);
+    for (int i0 = 0; i0 < REGS; i0 += STEP)
+      if (i0 * 64 < run) load(w + i0, i0);
+#pragma unroll
+    for (int i = 0; i < REGS; ++i) u[i] = value(i, w[i]);
   }
   auto each = [&](auto f) __attribute__((always_inline)) {
     if constexpr (REGS > 0) {
 #pragma unroll
-      for (int i = 0; i < REGS; ++i)
-        if (i * 64 < run) f(j0 + i * 64, u[i]);
+      for (int i0 = 0; i0 < REGS; i0 += STEP) {
+        if (i0 * 64 >= run) break;
+#pragma unroll
+        for (int i = i0; i < i0 + STEP; ++i) f(j0 + i * 64, u[i]);
+      }
     } else {
-      for (int i = 0; i < run; i += 64) f(j0 + i, weight(j0 + i));
+      for (int i0 = 0; i0 * 64 < run; i0 += STEP) {
+        float w[STEP];
+        load(w, i0);
+#pragma unroll
+        for (int i = 0; i < STEP; ++i) f(j0 + (i0 + i) * 64, value(i0 + i, w[i]));
+      }
     }
   };
 
@@ -1621,17 +1657,16 @@ __global__ __launch_bounds__(kSelThreads) void kv4_select_kernel(Kv4EvictArgs a)
   }
   eq_at = __builtin_amdgcn_readfirstlane(eq_at);
   at = __builtin_amdgcn_readfirstlane(at) + min(eq_at, (int)need);
-  const uint64_t below = (1ull << lane) - 1;
   int32_t* index = a.index + (int64_t)bh * a.keep;
   each([&](int j, uint32_t x) __attribute__((always_inline)) {
     bool stays = x > prefix;
-    const uint64_t eqs = __ballot(x == prefix);
-    if (eqs != 0 && need > 0) {
-      stays = stays || (x == prefix && eq_at + __popcll(eqs & below) < (int)need);
+    if (need > 0) {
+      const uint64_t eqs = __ballot(x == prefix);
+      stays = stays || (x == prefix && eq_at + lanes_below(eqs) < (int)need);
       eq_at += __popcll(eqs);
     }
     const uint64_t all = __ballot(stays);
-    if (stays) index[at + __popcll(all & below)] = first + j;
+    if (stays) index[at + lanes_below(all)] = first + j;
     at += __popcll(all);
   });
   for (int j = kept + tid; j < a.keep; j += kSelThreads) index[j] = -1;
@@ -1718,8 +1753,12 @@ hipError_t launch_kv4_weights(const Kv4WeightsArgs& a, Elem dtype, hipStream_t s
 
 hipError_t launch_kv4_evict(const Kv4EvictArgs& a, hipStream_t st) {
   const int heads = a.c.B * a.c.H;
+  // registers by the keys a thread may have: 1001 in room for 1024 take 6.2 us with one,
+  // 7.8 with 8, 11.2 read at every pass
   const int per = (a.c.C + kSelThreads - 1) / kSelThreads;
-  if (per <= 8)
+  if (per <= 1)
+    hipLaunchKernelGGL((kv4_select_kernel<1>), dim3(heads), dim3(kSelThreads), 0, st, a);
+  else if (per <= 8)
     hipLaunchKernelGGL((kv4_select_kernel<8>), dim3(heads), dim3(kSelThreads), 0, st, a);
   else if (per <= 32)
     hipLaunchKernelGGL((kv4_select_kernel<32>), dim3(heads), dim3(kSelThreads), 0, st, a);
