@@ -495,8 +495,9 @@ ttcd_status ttcd_ttt_scan_fwd(const void* dw, const void* w_cur, float lr, void*
  * 4-byte aligned. Position p of a sequence is in slot p % capacity; the last
  * `capacity` positions are held. capacity: a multiple of 32 up to 2^30; head_dim
  * 64 or 128. A cache that is not `const` below is written; a call that writes one
- * may not overlap in time with another on it. No call reads a slot that holds no
- * position into a result, so a new cache needs its lengths set to 0 and no more.
+ * may not overlap in time with another on it. No call lets a slot that holds no
+ * position, nor one that no query of the call sees, into a result, so a new cache
+ * needs its lengths set to 0 and no more.
  */
 typedef struct ttcd_kv4_cache {
   void* k_codes;
