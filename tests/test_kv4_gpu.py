@@ -599,6 +599,31 @@ def test_a_captured_step_decodes_on(gpu):
     assert torch.allclose(c.weights.double().cpu(), acc, rtol=1e-3, atol=1e-6)
 
 
+def test_a_captured_eviction_goes_by_the_lengths_it_finds(gpu):
+    """Replays over other lengths, weights and rows, with eager calls between them."""
+    C, keep = 2080, 600
+    c = KV4Cache(2, 2, 64, C)
+    out = KV4Cache(2, 2, 64, C)
+    w = torch.zeros(2, 2, C, device=gpu)
+    kv4_evict(c, w, keep, 9, out=out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        _, index, nw = kv4_evict(c, w, keep, 9, out=out)
+        k, v = kv4_read(out, keep)
+    for i, lengths in enumerate(((2000, 3), (600, 601), (0, 2080), (5000, 1100))):
+        held, r = _pair(2, 2, 64, C, BF, lengths, seed=50 + i)
+        for name in ("k_codes", "k_scales", "v_codes", "v_scales", "lengths"):
+            getattr(c, name).copy_(getattr(held, name))
+        w.copy_(torch.rand(2, 2, C, generator=torch.Generator().manual_seed(i)))
+        g.replay()
+        torch.cuda.synchronize()
+        wi, ww = r.evict(w.cpu(), keep, 9)
+        assert torch.equal(index.cpu(), wi) and torch.equal(nw[..., :keep].cpu(), ww)
+        for x, y in zip((k, v), r.take(wi, C).read(keep)):
+            assert torch.equal(x.cpu(), y)
+
+
 def test_offsets_past_32_bits(gpu):
     """Codes of more than 4 GiB: the last sequence's rows lie behind them."""
     B, H, D, C = 66, 8, 128, 131072
