@@ -823,8 +823,8 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
     *reinterpret_cast<u32x4*>(dst + 1024) = odd;
     if constexpr (MB == 4) {
       transpose_pair<T, 1>(w, s, &even, &odd);
-      *reinterpret_cast<u32x4*>(dst + 2048) = even;
-      *reinterpret_cast<u32x4*>(dst + 3072) = odd;
+      *reinterpret_cast<u32x4*>(dst + 2 * 1024) = even;
+      *reinterpret_cast<u32x4*>(dst + 3 * 1024) = odd;
     }
   };
 
