@@ -613,6 +613,13 @@ ttcd_status ttcd_attn_schedule_coverage(int T, int dual, int window_s,
 ttcd_status ttcd_attn_block_coverage(int npair, int nqb, int ngrp, int packed,
                                      int32_t* counts, int64_t xcd_work[8]);
 
+/* Host-only replay of the order in which a workgroup of the 4-bit cache's attention of
+ * many rows fills and reads its stages in LDS over key tiles t0 .. t1 - 1 (no GPU
+ * needed): TTCD_ERR_UNSUPPORTED if a stage is read and written, or written twice, with no
+ * barrier between the two, if a read finds another tile than the one it is to find, or if
+ * not every tile is folded once and in order. */
+ttcd_status ttcd_kv4_block_stages(int t0, int t1);
+
 #ifdef __cplusplus
 }
 #endif

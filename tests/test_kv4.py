@@ -156,3 +156,13 @@ def test_model_cache_arguments():
         c.reserve(34, 64)
     with pytest.raises(NotImplementedError):
         IPTTCDv9Cache(bits=4, capacity=64, keep=8).reserve(1, 32)
+
+
+def test_no_stage_is_rewritten_while_it_may_be_read():
+    """The many-row attention's order of loads, conversions, products and barriers, by the
+    code that the kernel runs (kv4_sweep.h)."""
+    f = _lib.lib().ttcd_kv4_block_stages
+    for t0 in range(4):
+        for n in range(1, 40):
+            assert f(t0, t0 + n) == 0, (t0, n, _lib.lib().ttcd_last_error())
+    assert f(3, 3) == f(-1, 4) == f(2, 1) == INV

@@ -66,6 +66,7 @@ EXPORTS = (
     "ttcd_kv4_evict",
     "ttcd_attn_schedule_coverage",
     "ttcd_attn_block_coverage",
+    "ttcd_kv4_block_stages",
 )
 
 _i32 = ctypes.c_int
@@ -185,6 +186,7 @@ _SIGS = {
     "ttcd_attn_schedule_coverage": (_i32, [
         _i32, _i32, _i32, _i32, _i32, _vp, _vp]),
     "ttcd_attn_block_coverage": (_i32, [_i32, _i32, _i32, _i32, _vp, _vp]),
+    "ttcd_kv4_block_stages": (_i32, [_i32, _i32]),
 }
 
 _lock = threading.Lock()

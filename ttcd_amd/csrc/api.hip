@@ -12,6 +12,7 @@
 #include <mutex>
 
 #include "internal.h"
+#include "kv4_sweep.h"
 #include "schedule.h"
 #include "ttcd.h"
 
@@ -1545,6 +1546,48 @@ ttcd_status ttcd_attn_block_coverage(int npair, int nqb, int ngrp, int packed, i
     counts[((int64_t)pair * nqb + qb) * ngrp + grp] += 1;
     xcd_work[g % ttcd::kXcd] += packed == 2 ? 1 : (int64_t)(qb + 1) * (packed == 3 ? pair + 1 : 1);
   }
+  return ok();
+}
+
+ttcd_status ttcd_kv4_block_stages(int t0, int t1) {
+  if (t0 < 0 || t1 <= t0) return fail(TTCD_ERR_INVALID_ARGUMENT, "need 0 <= t0 < t1");
+  struct Stage {
+    int holds = -1, written = -1, read = -1;  // a tile; intervals between barriers
+  } k[2], v[2];
+  int interval = 0, folded = t0, bad = -1;
+  auto load = [&](int& codes, int tile) {
+    if (tile < t0 || tile >= t1) bad = tile;
+    codes = tile;
+  };
+  auto store = [&](Stage* stages, int codes, int tile) {
+    Stage& s = stages[tile & 1];
+    if (s.read == interval || s.written == interval) bad = tile;
+    s.holds = codes;
+    s.written = interval;
+  };
+  auto read = [&](Stage* stages, int tile) {
+    Stage& s = stages[tile & 1];
+    if (s.holds != tile || s.written == interval) bad = tile;
+    s.read = interval;
+  };
+  int s0 = -1, s1 = -1;  // whose scores these are
+  ttcd::kv4_sweep<int>(
+      t0, t1, s0, s1, load, load, [&](int codes, int tile) { store(k, codes, tile); },
+      [&](int codes, int tile) { store(v, codes, tile); },
+      [&](int& s, int tile) {
+        read(k, tile);
+        s = tile;
+      },
+      [&](int& s, int tile) {
+        if (s != tile) bad = tile;
+      },
+      [&](int& s, int tile) {
+        read(v, tile);
+        if (s != tile || tile != folded++) bad = tile;
+      },
+      [&] { ++interval; });
+  if (bad >= 0 || folded != t1)
+    return fail(TTCD_ERR_UNSUPPORTED, "stage error: tile %d of %d .. %d", bad, t0, t1 - 1);
   return ok();
 }
 

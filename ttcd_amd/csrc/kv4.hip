@@ -23,6 +23,7 @@
 #include <stdint.h>
 
 #include "internal.h"
+#include "kv4_sweep.h"
 
 namespace ttcd {
 namespace {
@@ -34,11 +35,6 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
-template <bool V>
-struct Bool {
-  static constexpr bool value = V;
-};
 
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kLog2e = 1.44269504088896341f;
@@ -667,11 +663,9 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Kv4AttnArgs a)
 // (every read and write is 16 bytes a lane and 512 in a row). S^T = K Q^T, then
 // O^T = V^T P^T with P as it lies after the first product.
 //
-// One turn folds tile t: the scores of t + 1 are issued against the exponentials
-// of t, then the second product of t against the conversion of K(t + 2) and
-// V(t + 1) from codes that were loaded a turn before. Two stages of each in LDS
-// and one barrier a turn. The last turn is code of its own, so that the others have
-// no branch between products and exponentials (279 -> 272 us).
+// The order of loads, conversions, products and barriers is kv4_sweep.h's; two stages of
+// each in LDS and one barrier a turn. (With a branch for the last turn 279 us, as code of
+// its own 272.)
 //
 // Bound by the matrix pipe and the exponentials, which take about as long: 4096
 // queries on an 8192 window, 16/8 heads of 128, 261 us, 1053 TFLOP/s (a large library
@@ -761,7 +755,6 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
     u32x4 c[2];
     uint32_t s[2];
   };
-  Codes kc, vc;  // loaded, to be converted
   // the slot of a tile's 16 keys of this wavefront: its halves may lie apart where
   // the ring ends, a multiple of 32 slots from anything
   auto slot_of = [&](int tile) __attribute__((always_inline)) {
@@ -867,11 +860,8 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
       for (int i = 0; i < MB; ++i) o[i] *= f;
     }
   };
-  // Tiles past the last are read and written as the last: memory that is there, and
-  // stages that nothing reads any more.
-  auto turn = [&](f32x16 (&s)[2], f32x16 (&next)[2], int tile, auto more) __attribute__((always_inline)) {
-    constexpr bool kMore = decltype(more)::value;
-    if constexpr (kMore) scores(next, tile + 1);
+  // adds a tile's probabilities times its values
+  auto fold = [&](f32x16 (&s)[2], int tile) __attribute__((always_inline)) {
     u32x4 p[4];
     const float ref = m == -INFINITY ? 0.f : m - Fmt<T>::kBias;
 #pragma unroll
@@ -893,40 +883,10 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
         const u32x4 vf = *reinterpret_cast<const u32x4*>(src + j * (16 * D * 2) + i * 1024);
         o[i] = mfma32<T>(vf, p[j], o[i]);
       }
-    if constexpr (kMore) {
-      store_k(kc, tile + 2);
-      store_v(vc, tile + 1);
-      load_k(kc, min(tile + 3, t1 - 1));
-      load_v(vc, min(tile + 2, t1 - 1));
-      settle(next, tile + 1);
-      __syncthreads();
-    }
   };
-  if (t0 < t1) {
-    Codes k0, v0, k1;  // what the first turns need, all asked for at once
-    load_k(k0, t0);
-    load_v(v0, t0);
-    load_k(k1, min(t0 + 1, t1 - 1));
-    load_v(vc, min(t0 + 1, t1 - 1));
-    load_k(kc, min(t0 + 2, t1 - 1));
-    store_k(k0, t0);
-    store_v(v0, t0);
-    store_k(k1, t0 + 1);
-    __syncthreads();
-    scores(sa, t0);
-    settle(sa, t0);
-    int tile = t0;
-    for (; tile + 2 < t1; tile += 2) {
-      turn(sa, sb, tile, Bool<true>());
-      turn(sb, sa, tile + 1, Bool<true>());
-    }
-    if (tile + 1 < t1) {
-      turn(sa, sb, tile, Bool<true>());
-      turn(sb, sa, tile + 1, Bool<false>());
-    } else {
-      turn(sa, sb, tile, Bool<false>());
-    }
-  }
+  if (t0 < t1)
+    kv4_sweep<Codes>(t0, t1, sa, sb, load_k, load_v, store_k, store_v, scores, settle, fold,
+                     [] { __syncthreads(); });
 
   const bool none = rr.lo > rr.hi;  // saw the tiles that nobody's mask cuts
   l = none ? 0.f : l + __shfl_xor(l, 32);
