@@ -166,3 +166,26 @@ def test_no_stage_is_rewritten_while_it_may_be_read():
         for n in range(1, 40):
             assert f(t0, t0 + n) == 0, (t0, n, _lib.lib().ttcd_last_error())
     assert f(3, 3) == f(-1, 4) == f(2, 1) == INV
+
+
+def test_a_student_window_over_dropped_keys_is_refused():
+    """The newest `recent` of the kept keys, and what came after them, are in a row."""
+    from ttcd_amd import IPTTCDv9Cache
+    c = IPTTCDv9Cache(bits=4, capacity=512, keep=100, recent=20)
+    c._spare = object()  # no layers: nothing is evicted but in the counts
+    c.reserve(256, None, 256)
+    c.advance(90)
+    c.reserve(256, None, 256)  # nothing dropped yet: the student sees all there is
+    c.advance(170)
+    assert (c.seen, c.held, c.run) == (260, 100, 20)
+    c.reserve(256, None, 21)
+    c.reserve(1, None)
+    with pytest.raises(NotImplementedError, match="student"):
+        c.reserve(256, None, 22)
+    c.advance(1)
+    with pytest.raises(NotImplementedError, match="student"):
+        c.reserve(256, None, 22)
+    assert (c.seen, c.held, c.run) == (261, 100, 20)
+    c = IPTTCDv9Cache(bits=4, capacity=64)
+    c.advance(500)  # a ring has dropped no key between others
+    c.reserve(9, 32, 32)

@@ -155,3 +155,51 @@ def test_refusals():
     mask[0, 0] = 0
     with pytest.raises(NotImplementedError, match="mask"):
         model.forward(ids, cache=M.IPTTCDv9Cache(bits=4, capacity=64), attention_mask=mask)
+
+
+def _student_rows(monkeypatch, model, ids, chunks, cache):
+    """What the student of TTT layer 0 gives in each of the calls."""
+    rows, real = [], kv4.kv4_attn
+
+    def attn(q, held, window=None, **kw):
+        out = real(q, held, window, **kw)
+        if window == model.window_s:
+            rows.append(out)
+        return out
+
+    monkeypatch.setattr(kv4, "kv4_attn", attn)
+    a = 0
+    for n in chunks:
+        model.forward(ids[:, a:a + n], cache=cache)
+        a += n
+    monkeypatch.setattr(kv4, "kv4_attn", real)
+    return rows
+
+
+@pytest.mark.parametrize("path", M.PATHS)
+def test_the_student_sees_positions_of_its_window_after_an_eviction(monkeypatch, path):
+    """Layer 0's queries, keys and values do not depend on attention, so its student over a
+    cache that dropped keys has to give what it gives over one that holds all of them, but
+    for the order of its sums: a rounding of the probabilities and of the result each, off
+    by half a step of 2^-8 on either side, of values of at most max |v|."""
+    cfg = dict(TINY, ttt_layers=[0], window_size=None)
+    model = M.IPTTCDv9Prefill(cfg, M.init_weights(cfg, DEV, seed=14), path=path)
+    span, chunks = model.window_s, (400, 1, 300)
+    ids = _ids(1, sum(chunks), seed=15).to(DEV)
+    whole = FourBits(capacity=sum(chunks))
+    want = _student_rows(monkeypatch, model, ids, chunks, whole)
+    cut = FourBits(capacity=sum(chunks), keep=span + 30, recent=span - 1)
+    got = _student_rows(monkeypatch, model, ids, chunks, cut)
+    assert cut.kv4[0].lengths.tolist() == [span + 30]
+    assert [x.shape[1] for x in got] == [400, 300] and len(want) == 2
+    top = max(kv4.kv4_read(whole.kv4[0], sum(chunks))[1].abs().max().item(), 1e-6)
+    for x, y in zip(got, want):
+        assert (x.float() - y.float()).abs().max().item() <= 4 * 2.0 ** -8 * top
+    short = FourBits(capacity=sum(chunks), keep=span + 30, recent=span - 2)
+    for a, n in ((0, 400), (400, 1)):
+        model.forward(ids[:, a:a + n], cache=short)
+    held = [c.lengths.tolist() for c in short.kv4.values()]
+    with pytest.raises(NotImplementedError, match="student"):
+        model.forward(ids[:, 401:], cache=short)
+    assert short.seen == 401 and [c.lengths.tolist() for c in short.kv4.values()] == held
+    model.forward(ids[:, 401:410], cache=short)  # fewer than a chunk: no student

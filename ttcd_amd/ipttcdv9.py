@@ -456,7 +456,9 @@ class IPTTCDv9Prefill:
                 raise NotImplementedError("a cached prefill with a padding mask or packed "
                                           "sequences")
             cache.check(B, self.Hkv, self.D, self.dtype, self.dev)
-            cache.reserve(T, None if self.window_t < 0 else self.window_t)
+            # a TTT layer's student attends in calls of a chunk and more
+            student = self.window_s if self.ttt and T >= self.cfg["ttt_chunk"] else None
+            cache.reserve(T, None if self.window_t < 0 else self.window_t, student)
             ctx.cache, ctx.offset = cache, cache.seen
             attention_mask = None
         if attention_mask is not None:
@@ -549,7 +551,9 @@ class IPTTCDv9Cache:
     tokens (or as many as the prompt has), full-causal attention room for every
     token that is kept. keep: after a call that leaves more, each layer's kv heads
     keep that many keys, the newest `recent` and those with the largest sum of
-    attention weights so far (full-causal models only)."""
+    attention weights so far (full-causal models only; the student window of a TTT
+    layer counts positions, so a call of ttt_chunk tokens and more on such a cache
+    needs recent and keep of the student window less one)."""
 
     def __init__(self, bits: int = 16, capacity: int | None = None, keep: int | None = None,
                  recent: int = 0):
@@ -567,6 +571,7 @@ class IPTTCDv9Cache:
         self.capacity = None if capacity is None else -(-int(capacity) // 32) * 32
         self.seen = 0
         self.held = 0  # positions in a 4-bit layer's cache (more have wrapped off a window's)
+        self.run = 0   # of them the newest with none dropped between
         self.kv: dict[int, tuple[torch.Tensor, torch.Tensor]] = {}
         self.kv4: dict[int, _kv4.KV4Cache] = {}
         self._spare: _kv4.KV4Cache | None = None
@@ -579,13 +584,19 @@ class IPTTCDv9Cache:
                              f"this prefill needs {shape}")
         self._shape = shape
 
-    def reserve(self, T: int, window: int | None) -> None:
-        """Refuse T more tokens that a 4-bit cache has no room for."""
+    def reserve(self, T: int, window: int | None, student: int | None = None) -> None:
+        """Refuse T more tokens that a 4-bit cache has no room for, or whose student
+        window (of a TTT layer, None if none runs) reaches over dropped keys."""
         if self.bits != 4:
             return
         if self.keep is not None and window is not None:
             raise NotImplementedError("dropping keys of a windowed model: the window counts "
                                       "positions, and those of the kept keys are not in a row")
+        if student is not None and self.run < min(student - 1, self.seen):
+            raise NotImplementedError(
+                f"a TTT layer's student window of {student} over a cache that dropped keys: "
+                f"only the newest {self.run} held positions are in a row (recent={self.recent} "
+                f"of keep={self.keep}; it takes {student - 1})")
         need = self.held + T
         if window is not None:
             need = min(need, window + T - 1)
@@ -621,6 +632,7 @@ class IPTTCDv9Cache:
         if self.bits != 4:
             return
         self.held += T
+        self.run += T
         if self.keep is None or self.held <= self.keep:
             return
         if self._spare is None:
@@ -629,6 +641,7 @@ class IPTTCDv9Cache:
             self.kv4[i], _, _ = _kv4.kv4_evict(old, None, self.keep, self.recent, out=self._spare)
             self._spare = old
         self.held = self.keep
+        self.run = min(self.run, self.recent, self.keep)
 
     def extend(self, layer: int, k: torch.Tensor, v: torch.Tensor, keep: int | None):
         """Keys / values for layer's attention: the cached ones, then k / v of
