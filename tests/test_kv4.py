@@ -189,3 +189,19 @@ def test_a_student_window_over_dropped_keys_is_refused():
     c = IPTTCDv9Cache(bits=4, capacity=64)
     c.advance(500)  # a ring has dropped no key between others
     c.reserve(9, 32, 32)
+
+
+def test_room_for_a_student_window_wider_than_the_teachers():
+    """The student's rows would see as much of their window as the ring happens to hold."""
+    from ttcd_amd import IPTTCDv9Cache
+    c = IPTTCDv9Cache(bits=4, capacity=320)
+    c.reserve(256, 64, 256)  # the prompt's first tokens: all of them are there
+    c.advance(256)
+    c.reserve(256, 64)       # no student runs: the teacher's window and the call
+    with pytest.raises(ValueError, match="positions"):
+        c.reserve(256, 64, 256)
+    big = IPTTCDv9Cache(bits=4, capacity=511)
+    big.advance(5000)
+    big.reserve(256, 64, 256)
+    with pytest.raises(ValueError, match="positions"):
+        big.reserve(256, 64, 258)

@@ -203,3 +203,22 @@ def test_the_student_sees_positions_of_its_window_after_an_eviction(monkeypatch,
         model.forward(ids[:, 401:], cache=short)
     assert short.seen == 401 and [c.lengths.tolist() for c in short.kv4.values()] == held
     model.forward(ids[:, 401:410], cache=short)  # fewer than a chunk: no student
+
+
+def test_a_student_window_wider_than_the_teachers_needs_its_room(monkeypatch):
+    """With too small a ring the call is refused before it writes. With room, the student
+    of layer 0 gives what it gives in one call, but for four half steps as above."""
+    cfg = dict(TINY, ttt_layers=[0], window_size=64)  # student window 256
+    model = M.IPTTCDv9Prefill(cfg, M.init_weights(cfg, DEV, seed=16), path="stock")
+    ids = _ids(1, 768, seed=17).to(DEV)
+    cache = M.IPTTCDv9Cache(bits=4, capacity=64 + 256)
+    model.forward(ids[:, :256], cache=cache)
+    with pytest.raises(ValueError, match="positions"):
+        model.forward(ids[:, 256:512], cache=cache)
+    assert cache.seen == 256 and cache.kv4[0].lengths.tolist() == [256]
+    whole = FourBits(capacity=768)
+    want = _student_rows(monkeypatch, model, ids, (768,), whole)[0]
+    got = _student_rows(monkeypatch, model, ids, (256,) * 3, FourBits(capacity=511))
+    top = max(kv4.kv4_read(whole.kv4[0], 768)[1].abs().max().item(), 1e-6)
+    d = (torch.cat(got, 1).float() - want.float()).abs().max().item()
+    assert d <= 4 * 2.0 ** -8 * top

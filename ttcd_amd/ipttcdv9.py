@@ -548,8 +548,8 @@ class IPTTCDv9Cache:
 
     bits=4 holds them in 4 bits (ttcd_amd.kv4), `capacity` positions a layer,
     allocated once: a window needs window_size + T - 1 of them for calls of T
-    tokens (or as many as the prompt has), full-causal attention room for every
-    token that is kept. keep: after a call that leaves more, each layer's kv heads
+    tokens (or as many as the prompt has; a TTT layer's student window takes the place
+    of a smaller window_size), full-causal attention room for every token that is kept. keep: after a call that leaves more, each layer's kv heads
     keep that many keys, the newest `recent` and those with the largest sum of
     attention weights so far (full-causal models only; the student window of a TTT
     layer counts positions, so a call of ttt_chunk tokens and more on such a cache
@@ -599,7 +599,7 @@ class IPTTCDv9Cache:
                 f"of keep={self.keep}; it takes {student - 1})")
         need = self.held + T
         if window is not None:
-            need = min(need, window + T - 1)
+            need = min(need, max(window, student or 0) + T - 1)
         if max(need, T) > self.capacity:
             raise ValueError(f"IPTTCDv9Cache: {T} more tokens need {max(need, T)} positions of "
                              f"{self.capacity}")
