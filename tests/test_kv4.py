@@ -205,3 +205,21 @@ def test_room_for_a_student_window_wider_than_the_teachers():
     big.reserve(256, 64, 256)
     with pytest.raises(ValueError, match="positions"):
         big.reserve(256, 64, 258)
+
+
+def test_a_cache_whose_last_call_did_not_end_is_refused(monkeypatch):
+    """Its first layers hold the call's positions and the others do not."""
+    from ttcd_amd import IPTTCDv9Cache, kv4
+    monkeypatch.setattr(kv4, "KV4Cache", lambda *a, **kw: object())
+    monkeypatch.setattr(kv4, "kv4_append", lambda held, k, v: None)
+    c = IPTTCDv9Cache(bits=4, capacity=64)
+    c.check(1, 2, 64, torch.bfloat16, "cpu")
+    for layers in (2, 1):  # a call of both layers, and one that ends behind the first
+        c.reserve(5, None)
+        for i in range(layers):
+            c.append(i, None, None)
+        if layers == 2:
+            c.advance(5)
+    with pytest.raises(RuntimeError, match="did not end"):
+        c.reserve(5, None)
+    assert (c.seen, c.held) == (5, 5)

@@ -222,3 +222,23 @@ def test_a_student_window_wider_than_the_teachers_needs_its_room(monkeypatch):
     top = max(kv4.kv4_read(whole.kv4[0], 768)[1].abs().max().item(), 1e-6)
     d = (torch.cat(got, 1).float() - want.float()).abs().max().item()
     assert d <= 4 * 2.0 ** -8 * top
+
+
+def test_a_call_that_raised_between_layers_leaves_no_usable_cache(monkeypatch):
+    model = M.IPTTCDv9Prefill(TINY, M.init_weights(TINY, DEV, seed=9))
+    ids = _ids(1, 40, seed=1).to(DEV)
+    cache = M.IPTTCDv9Cache(bits=4, capacity=128)
+    model.forward(ids[:, :20], cache=cache)
+    real = M.IPTTCDv9Prefill.layer
+
+    def layer(self, i, *a):
+        if i == 1:
+            raise MemoryError
+        return real(self, i, *a)
+
+    monkeypatch.setattr(M.IPTTCDv9Prefill, "layer", layer)
+    with pytest.raises(MemoryError):
+        model.forward(ids[:, 20:], cache=cache)
+    monkeypatch.setattr(M.IPTTCDv9Prefill, "layer", real)
+    with pytest.raises(RuntimeError, match="did not end"):
+        model.forward(ids[:, 20:], cache=cache)

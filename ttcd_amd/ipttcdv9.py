@@ -572,6 +572,7 @@ class IPTTCDv9Cache:
         self.seen = 0
         self.held = 0  # positions in a 4-bit layer's cache (more have wrapped off a window's)
         self.run = 0   # of them the newest with none dropped between
+        self._open = False  # a call has written some of the 4-bit layers and not ended
         self.kv: dict[int, tuple[torch.Tensor, torch.Tensor]] = {}
         self.kv4: dict[int, _kv4.KV4Cache] = {}
         self._spare: _kv4.KV4Cache | None = None
@@ -589,6 +590,9 @@ class IPTTCDv9Cache:
         window (of a TTT layer, None if none runs) reaches over dropped keys."""
         if self.bits != 4:
             return
+        if self._open:
+            raise RuntimeError("IPTTCDv9Cache: the last call on this cache did not end, so its "
+                               "layers hold different positions; start a new one")
         if self.keep is not None and window is not None:
             raise NotImplementedError("dropping keys of a windowed model: the window counts "
                                       "positions, and those of the kept keys are not in a row")
@@ -609,6 +613,7 @@ class IPTTCDv9Cache:
         held = self.kv4.get(layer)
         if held is None:
             held = self.kv4[layer] = self._new()
+        self._open = True
         _kv4.kv4_append(held, k, v)
         return held
 
@@ -633,15 +638,16 @@ class IPTTCDv9Cache:
             return
         self.held += T
         self.run += T
-        if self.keep is None or self.held <= self.keep:
-            return
-        if self._spare is None:
-            self._spare = self._new()
-        for i, old in self.kv4.items():
-            self.kv4[i], _, _ = _kv4.kv4_evict(old, None, self.keep, self.recent, out=self._spare)
-            self._spare = old
-        self.held = self.keep
-        self.run = min(self.run, self.recent, self.keep)
+        if self.keep is not None and self.held > self.keep:
+            if self._spare is None:
+                self._spare = self._new()
+            for i, old in self.kv4.items():
+                self.kv4[i], _, _ = _kv4.kv4_evict(old, None, self.keep, self.recent,
+                                                   out=self._spare)
+                self._spare = old
+            self.held = self.keep
+            self.run = min(self.run, self.recent, self.keep)
+        self._open = False
 
     def extend(self, layer: int, k: torch.Tensor, v: torch.Tensor, keep: int | None):
         """Keys / values for layer's attention: the cached ones, then k / v of
