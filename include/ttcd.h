@@ -574,10 +574,10 @@ ttcd_status ttcd_kv4_key_weights_fwd(const ttcd_kv4_cache* cache, const void* q,
  * than any number). They become positions 0, 1, .. of `out`, in their order, whose
  * lengths are set to their number. weights: (batch, kv_heads, capacity) fp32 by
  * slot. out: another cache of the same batch, kv_heads and head_dim and a capacity
- * >= keep, none of its memory shared with `cache`. new_weights: (batch, kv_heads,
- * out->capacity) fp32 or NULL: the kept keys' weights, 0 behind them. index:
- * (batch, kv_heads, keep) int32: the position that each new one had, -1 behind the
- * last. 1 <= keep, 0 <= recent.
+ * >= keep. new_weights: (batch, kv_heads, out->capacity) fp32 or NULL: the kept keys'
+ * weights, 0 behind them. index: (batch, kv_heads, keep) int32: the position that each
+ * new one had, -1 behind the last. 1 <= keep, 0 <= recent. What is written (out's parts,
+ * new_weights, index) may share no memory with itself or with what is read.
  */
 ttcd_status ttcd_kv4_evict(const ttcd_kv4_cache* cache, const float* weights, int keep,
                            int recent, ttcd_kv4_cache* out, float* new_weights, int32_t* index,

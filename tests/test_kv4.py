@@ -223,3 +223,40 @@ def test_a_cache_whose_last_call_did_not_end_is_refused(monkeypatch):
     with pytest.raises(RuntimeError, match="did not end"):
         c.reserve(5, None)
     assert (c.seen, c.held) == (5, 5)
+
+
+def test_eviction_refuses_any_shared_memory():
+    """Not only the same pointers: ranges that overlap."""
+    kc, ks, vc, vs = 2 * 2 * 64 * 32, 2 * 2 * 64 * 2, 2 * 2 * 64 * 32, 2 * 2 * 64 * 2
+    w, index, lens = 2 * 2 * 64 * 4, 2 * 2 * 8 * 4, 8
+
+    def spread(base):
+        at, out = base, {}
+        for name, n in (("k_codes", kc), ("k_scales", ks), ("v_codes", vc), ("v_scales", vs),
+                        ("lengths", lens)):
+            out[name], at = at, at + -(-n // 16) * 16
+        return out, at
+
+    old, end = spread(P)
+    new, last = spread(end + w)
+    parts = [(old[n], size) for n, size in zip(old, (kc, ks, vc, vs, lens))] + [(end, w)]
+    nw, idx = last, last + w
+    f = _lib.lib().ttcd_kv4_evict
+
+    def call(**over):
+        a = dict(new, nw=nw, idx=idx, **{})
+        a.update(over)
+        return f(_struct(**old), end, 8, 2, _struct(**{n: a[n] for n in new}), a["nw"], a["idx"],
+                 None)
+
+    for name, size in (("k_codes", kc), ("k_scales", ks), ("v_codes", vc), ("v_scales", vs),
+                       ("lengths", lens), ("nw", w), ("idx", index)):
+        for at, n in parts:
+            # the last and the first 16 bytes (or all) of what is read
+            for over in (at + n - min(n, 16), at - size + min(size, 16)):
+                if over % 16 == 0 and over > 0:
+                    assert call(**{name: over}) == INV, (name, hex(over))
+                    assert b"share" in _lib.lib().ttcd_last_error()
+    for name, size in (("k_codes", kc), ("v_scales", vs), ("lengths", lens), ("idx", index)):
+        assert call(**{name: nw + 16}) == INV  # written twice
+    assert call(idx=nw - 16) == INV

@@ -717,3 +717,23 @@ def test_refusals(gpu):
     c.lengths.fill_(5)
     c.reset()
     assert c.lengths.tolist() == [0, 0]
+
+
+def test_evict_into_a_cache_that_shares_its_weights(gpu):
+    """The old cache stays as it is: the written one, whose weights are the old one's (or a
+    part of the memory that is read), gets new ones."""
+    both = torch.rand(2, 3, 2, 64, device=gpu)
+    own = both.flatten()[:2 * 2 * 64].view(2, 2, 64)       # the old cache's
+    other = both.flatten()[3 * 64:7 * 64].view(2, 2, 64)   # overlaps it
+    for held, given, target in ((own, torch.rand(2, 2, 64, device=gpu), own), (own, None, other),
+                                (None, own, other)):
+        c, r = _pair(2, 2, 64, 64, BF, (64, 10))
+        c.weights = held
+        out = KV4Cache(2, 2, 64, 64)
+        out.weights = target
+        was, go_by = both.clone(), (held if given is None else given).clone()
+        _, index, new = kv4_evict(c, given, 20, 4, out=out)
+        want, ww = r.evict(go_by.cpu(), 20, 4)
+        assert torch.equal(both, was)
+        assert torch.equal(index.cpu(), want) and torch.equal(new[..., :20].cpu(), ww)
+        assert out.weights is new and c.weights is held

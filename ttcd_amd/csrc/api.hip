@@ -1266,6 +1266,23 @@ size_t kv4_part_bytes(const ttcd_kv4_cache* c, int Tq, int Hq) {
   return (size_t)c->batch * Tq * Hq * (c->head_dim + 2) * sizeof(float);
 }
 
+struct Span {
+  const void* at;  // null: none
+  int64_t bytes;
+};
+bool overlap(const Span& a, const Span& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+  return x && y && x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)a.bytes;
+}
+void kv4_spans(const ttcd_kv4_cache* c, Span spans[5]) {
+  const int64_t n = (int64_t)c->batch * c->kv_heads * c->capacity * c->head_dim;
+  spans[0] = {c->k_codes, n / 2};
+  spans[1] = {c->k_scales, n / 32};
+  spans[2] = {c->v_codes, n / 2};
+  spans[3] = {c->v_scales, n / 32};
+  spans[4] = {c->lengths, (int64_t)c->batch * 4};
+}
+
 }  // namespace
 
 ttcd_status ttcd_kv4_append(ttcd_kv4_cache* cache, const void* k, const void* v, int T,
@@ -1412,10 +1429,21 @@ ttcd_status ttcd_kv4_evict(const ttcd_kv4_cache* cache, const float* weights, in
     return fail(TTCD_ERR_INVALID_ARGUMENT,
                 "need 1 <= keep <= out's capacity and recent >= 0 (got %d, %d, %d)", keep,
                 out->capacity, recent);
-  if (out->k_codes == cache->k_codes || out->k_scales == cache->k_scales ||
-      out->v_codes == cache->v_codes || out->v_scales == cache->v_scales ||
-      out->lengths == cache->lengths || new_weights == weights)
-    return fail(TTCD_ERR_INVALID_ARGUMENT, "out must not share memory with the cache");
+  const int64_t heads = (int64_t)cache->batch * cache->kv_heads;
+  Span read[6], written[7];
+  kv4_spans(cache, read);
+  read[5] = {weights, heads * cache->capacity * 4};
+  kv4_spans(out, written);
+  written[5] = {new_weights, heads * out->capacity * 4};
+  written[6] = {index, heads * keep * 4};
+  for (int i = 0; i < 7; ++i) {
+    for (const Span& r : read)
+      if (overlap(written[i], r))
+        return fail(TTCD_ERR_INVALID_ARGUMENT, "out must not share memory with the cache");
+    for (int j = 0; j < i; ++j)
+      if (overlap(written[i], written[j]))
+        return fail(TTCD_ERR_INVALID_ARGUMENT, "out's parts must not share memory");
+  }
   ttcd::Kv4EvictArgs a = {};
   a.c = kv4(cache);
   a.out = kv4(out);

@@ -208,6 +208,14 @@ def _counts(counts, cache: KV4Cache, fn: str):
     return counts.contiguous()
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor | None) -> bool:
+    """Whether two contiguous tensors share memory."""
+    if b is None:
+        return False
+    x, y = a.data_ptr(), b.data_ptr()
+    return x < y + b.numel() * b.element_size() and y < x + a.numel() * a.element_size()
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -384,7 +392,9 @@ def kv4_evict(cache: KV4Cache, weights: torch.Tensor | None, keep: int, recent: 
     weights = weights.contiguous()
     index = torch.empty(B, H, keep, dtype=torch.int32, device=cache.device)
     new_weights = out.weights
-    if new_weights is None or new_weights.data_ptr() == weights.data_ptr():
+    # the weights that are read, and the old cache's, stay as they are
+    if (new_weights is None or _overlap(new_weights, weights)
+            or _overlap(new_weights, cache.weights)):
         new_weights = torch.empty(B, H, out.capacity, dtype=torch.float32, device=cache.device)
     _call(cache, _lib.lib().ttcd_kv4_evict, cache._ref, weights.data_ptr(), keep,
           min(recent, 2**31 - 1), out._ref, new_weights.data_ptr(), index.data_ptr())
