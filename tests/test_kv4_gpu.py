@@ -737,3 +737,29 @@ def test_evict_into_a_cache_that_shares_its_weights(gpu):
         assert torch.equal(both, was)
         assert torch.equal(index.cpu(), want) and torch.equal(new[..., :20].cpu(), ww)
         assert out.weights is new and c.weights is held
+
+
+def test_gradients_are_refused_and_not_dropped(gpu):
+    c = KV4Cache(2, 2, 64, 64, weights=True)
+    x, q = _rand(1, 2, 4, 2, 64).cuda(), _rand(1, 2, 4, 4, 64).cuda()
+    kv4_append(c, x, x)
+    _, lse = kv4_attn(q, c, return_lse=True)
+    w = torch.rand(2, 2, 64, device=gpu, requires_grad=True)
+
+    def given():
+        c.weights = w
+
+    calls = (lambda: kv4_key_weights(q, c, lse.clone().requires_grad_()),
+             lambda: kv4_key_weights(q, c, lse, out=w),
+             lambda: kv4_key_weights(q[:, :0], c, lse[:, :, :0], out=w),
+             lambda: kv4_evict(c, w, 8), given)
+    was = w.detach().clone()
+    for f in calls:
+        with pytest.raises(RuntimeError, match="forward-only"):
+            f()
+    assert torch.equal(w.detach(), was) and c.weights is not w
+    with torch.no_grad():
+        for f in calls[:1] + calls[3:]:
+            f()
+    with pytest.raises(ValueError):
+        kv4_key_weights(q, c, lse, out=[0.0])

@@ -165,6 +165,8 @@ class KV4Cache:
                               or w.dtype != torch.float32 or w.device != self.device
                               or not w.is_contiguous()):
             raise ValueError(f"KV4Cache: weights must be contiguous fp32 {shape} on {self.device}")
+        if w is not None:
+            _forward_only(w, "KV4Cache")
         self._weights = w
 
     def reset(self) -> None:
@@ -181,6 +183,12 @@ def _cache(cache, fn: str) -> KV4Cache:
     return cache
 
 
+def _forward_only(t: torch.Tensor, fn: str) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{fn} is forward-only: autograd / gradient inputs are not supported; "
+                           "call it under torch.no_grad() or torch.inference_mode()")
+
+
 def _rows(t, cache: KV4Cache, name: str, fn: str, heads: int | None) -> None:
     """The checks of a (B, T, heads, D) operand (heads None: any multiple of the cache's)."""
     if not isinstance(t, torch.Tensor) or t.dim() != 4:
@@ -194,9 +202,7 @@ def _rows(t, cache: KV4Cache, name: str, fn: str, heads: int | None) -> None:
         raise ValueError(f"{fn}: {name} must be {cache.dtype} as the cache, got {t.dtype}")
     if t.device != cache.device:
         raise ValueError(f"{fn}: {name} must be on the cache's device")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"{fn} is forward-only: autograd / gradient inputs are not supported; "
-                           "call it under torch.no_grad() or torch.inference_mode()")
+    _forward_only(t, fn)
 
 
 def _counts(counts, cache: KV4Cache, fn: str):
@@ -342,15 +348,17 @@ def kv4_key_weights(q: torch.Tensor, cache: KV4Cache, lse: torch.Tensor,
     if (not isinstance(lse, torch.Tensor) or lse.shape != (B, H, T)
             or lse.dtype != torch.float32 or lse.device != q.device):
         raise ValueError(f"kv4_key_weights: lse must be fp32 ({B}, {H}, {T}) on q's device")
+    _forward_only(lse, "kv4_key_weights")
     shape = (B, cache.kv_heads, cache.capacity)
     if out is None:
         if accumulate:
             raise ValueError("kv4_key_weights: accumulate needs out")
         out = torch.empty(shape, dtype=torch.float32, device=q.device)
-    elif (out.shape != shape or out.dtype != torch.float32 or out.device != q.device
+    elif (not isinstance(out, torch.Tensor) or out.shape != shape or out.dtype != torch.float32 or out.device != q.device
           or not out.is_contiguous() or out.data_ptr() % 16):
         raise ValueError(f"kv4_key_weights: out must be contiguous fp32 {shape} on q's device, "
                          "16-byte aligned")
+    _forward_only(out, "kv4_key_weights")
     if T == 0:
         with torch.inference_mode():
             return out if accumulate else out.zero_()
@@ -380,6 +388,7 @@ def kv4_evict(cache: KV4Cache, weights: torch.Tensor | None, keep: int, recent: 
     if (not isinstance(weights, torch.Tensor) or weights.shape != (B, H, C)
             or weights.dtype != torch.float32 or weights.device != cache.device):
         raise ValueError(f"kv4_evict: weights must be fp32 ({B}, {H}, {C}) on the cache's device")
+    _forward_only(weights, "kv4_evict")
     if out is None:
         out = KV4Cache.__new__(KV4Cache)
         out._alloc(B, H, cache.head_dim, C, cache.dtype, cache.device)  # the call sets its lengths
