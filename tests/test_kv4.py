@@ -260,3 +260,15 @@ def test_eviction_refuses_any_shared_memory():
     for name, size in (("k_codes", kc), ("v_scales", vs), ("lengths", lens), ("idx", index)):
         assert call(**{name: nw + 16}) == INV  # written twice
     assert call(idx=nw - 16) == INV
+
+
+def test_rows_past_64_bits_are_refused():
+    """Rows whose number, or whose blocks', wraps around to 0: each ended the process with a
+    division by it."""
+    one, many = _struct(batch=1, kv_heads=1), _struct(batch=16, kv_heads=1)
+    f = _lib.lib().ttcd_kv4_attn_workspace_bytes
+    assert f(one, 1 << 30, 512, 0) == f(many, 1 << 30, 1 << 30, 0) == 0
+    assert f(one, (1 << 31) - 1, (1 << 31) - 1, 0) == 0
+    assert _attn(c=many, Tq=1 << 30, Hq=1 << 30) == UNSUP
+    assert _weights(c=many, Tq=1 << 30, Hq=1 << 30) == UNSUP
+    assert _attn(c=one, Tq=1 << 30, Hq=512) == UNSUP

@@ -1188,15 +1188,19 @@ ttcd_status check_kv4_strides(const void* p, const int64_t* s) {
   return TTCD_OK;
 }
 
+// A workgroup a row of the sum over the parts. (By a division: batch * Hq * Tq may pass 64
+// bits, and rows that wrapped around to none ended the process in kv4_plan.)
+bool kv4_rows_fit(const ttcd_kv4_cache* c, int Tq, int Hq) {
+  return (int64_t)Hq * Tq <= (0x7fffffffLL - 1024) / c->batch;
+}
+
 ttcd_status check_kv4_rows(const ttcd_kv4_cache* c, int Tq, int Hq) {
   if (Tq < 1 || Hq < 1)
     return fail(TTCD_ERR_INVALID_ARGUMENT, "need Tq, Hq >= 1 (got %d, %d)", Tq, Hq);
   if (Hq % c->kv_heads != 0)
     return fail(TTCD_ERR_INVALID_ARGUMENT, "Hq (%d) must be a multiple of kv_heads (%d)", Hq,
                 c->kv_heads);
-  // a workgroup a row of the sum over the parts
-  if ((int64_t)c->batch * Hq * Tq > 0x7fffffffLL - 1024)
-    return fail(TTCD_ERR_UNSUPPORTED, "grid too large");
+  if (!kv4_rows_fit(c, Tq, Hq)) return fail(TTCD_ERR_UNSUPPORTED, "grid too large");
   return TTCD_OK;
 }
 
@@ -1333,7 +1337,7 @@ ttcd_status ttcd_kv4_read(const ttcd_kv4_cache* cache, void* k, void* v, int cou
 size_t ttcd_kv4_attn_workspace_bytes(const ttcd_kv4_cache* cache, int Tq, int Hq, int window) {
   if (!cache || cache->batch < 1 || cache->kv_heads < 1 || Tq < 1 || Hq < cache->kv_heads ||
       Hq % cache->kv_heads != 0 || (cache->head_dim != 64 && cache->head_dim != 128) ||
-      cache->capacity < 32)
+      cache->capacity < 32 || !kv4_rows_fit(cache, Tq, Hq))
     return 0;
   const Kv4Plan p = kv4_plan(cache, Tq, Hq, kv4_window(window));
   return p.parts > 1 ? p.parts * kv4_part_bytes(cache, Tq, Hq) : 0;

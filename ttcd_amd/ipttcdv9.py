@@ -549,11 +549,13 @@ class IPTTCDv9Cache:
     bits=4 holds them in 4 bits (ttcd_amd.kv4), `capacity` positions a layer,
     allocated once: a window needs window_size + T - 1 of them for calls of T
     tokens (or as many as the prompt has; a TTT layer's student window takes the place
-    of a smaller window_size), full-causal attention room for every token that is kept. keep: after a call that leaves more, each layer's kv heads
-    keep that many keys, the newest `recent` and those with the largest sum of
-    attention weights so far (full-causal models only; the student window of a TTT
-    layer counts positions, so a call of ttt_chunk tokens and more on such a cache
-    needs recent and keep of the student window less one)."""
+    of a smaller window_size), full-causal attention room for every token that is kept.
+    keep: after a call that leaves more, each layer's kv heads keep that many keys, the
+    newest `recent` and those with the largest sum of attention weights so far
+    (full-causal models only; the student window of a TTT layer counts positions, so a
+    call of ttt_chunk tokens and more on such a cache needs recent and keep of the
+    student window less one). A call that raises between its layers leaves a cache that
+    the next one refuses."""
 
     def __init__(self, bits: int = 16, capacity: int | None = None, keep: int | None = None,
                  recent: int = 0):

@@ -354,8 +354,8 @@ def kv4_key_weights(q: torch.Tensor, cache: KV4Cache, lse: torch.Tensor,
         if accumulate:
             raise ValueError("kv4_key_weights: accumulate needs out")
         out = torch.empty(shape, dtype=torch.float32, device=q.device)
-    elif (not isinstance(out, torch.Tensor) or out.shape != shape or out.dtype != torch.float32 or out.device != q.device
-          or not out.is_contiguous() or out.data_ptr() % 16):
+    elif (not isinstance(out, torch.Tensor) or out.shape != shape or out.dtype != torch.float32
+          or out.device != q.device or not out.is_contiguous() or out.data_ptr() % 16):
         raise ValueError(f"kv4_key_weights: out must be contiguous fp32 {shape} on q's device, "
                          "16-byte aligned")
     _forward_only(out, "kv4_key_weights")
