@@ -489,8 +489,11 @@ ttcd_status ttcd_ttt_scan_fwd(const void* dw, const void* w_cur, float lr, void*
  *   v_codes  (batch, kv_heads, capacity / 4, head_dim / 8, 4, 4): the 4-byte
  *            words of 8 channels of 4 neighbouring slots side by side
  *   v_scales (batch, kv_heads, capacity / 4, head_dim / 32, 4)
- *   lengths  (batch) int32: the positions that a sequence has had, up to 2^30
- *            (entries outside [0, 2^30] are taken as the nearest bound)
+ *   lengths  (batch) int32: the positions that a sequence has had; an append that
+ *            passes 2^30 takes a multiple of the capacity off, so that slots and
+ *            distances stay and at least `capacity` remain (capacities above 2^29 have
+ *            no such length: their sequences end at 2^30 positions). Entries outside
+ *            [0, 2^30] are taken as the nearest bound.
  * all contiguous, k_codes and v_codes 16-byte aligned, v_scales and lengths
  * 4-byte aligned. Position p of a sequence is in slot p % capacity; the last
  * `capacity` positions are held. capacity: a multiple of 32 up to 2^30; head_dim

@@ -763,3 +763,39 @@ def test_gradients_are_refused_and_not_dropped(gpu):
             f()
     with pytest.raises(ValueError):
         kv4_key_weights(q, c, lse, out=[0.0])
+
+
+@pytest.mark.parametrize("C,H,D,steps", [(64, 2, 64, (3, 4, 1, 1, 60, 64)),
+                                         (96, 1, 128, (1, 1, 1, 1, 1, 1, 1, 70)),
+                                         (512, 8, 128, (300, 1, 500, 2))])
+def test_a_ring_goes_on_past_the_largest_length(gpu, C, H, D, steps):
+    """Every call as over the same rows at the start of a sequence: append by one workgroup
+    a sequence and by many, attention of a few and of many rows, key weights, eviction."""
+    B, start = 2, torch.tensor([2 ** 30 - C - 5, 2 ** 30 - C - 200])
+    c, r = KV4Cache(B, H, D, C), kv4_ref.Ref(B, H, D, C)
+    c.lengths.copy_(start)
+    total = 0
+    for i, T in enumerate((C, *steps)):
+        k, v = _rand(3 * i, B, T, H, D), _rand(3 * i + 1, B, T, H, D)
+        kv4_append(c, k.cuda(), v.cuda())
+        r.append(k, v)
+        total += T
+        n = c.lengths.cpu().long()
+        assert (n <= 2 ** 30).all() and (n >= C).all() and ((n - start - total) % C == 0).all()
+        for x, y in zip(kv4_read(c, C), r.read(C)):
+            assert torch.equal(x.cpu(), y)
+        q = _rand(3 * i + 2, B, T, 2 * H, D)
+        o, lse = kv4_attn(q.cuda(), c, 50, return_lse=True)
+        _check_attn(r, q, o, lse, 50, None)
+        w = kv4_key_weights(q.cuda(), c, lse, 50).double().cpu()
+        want = r.key_weights(q, lse, 50)
+        for b in range(B):  # the oracle's positions count from 0
+            assert torch.allclose(w[b], want[b].roll(int(start[b]) % C, -1), rtol=1e-4, atol=1e-9)
+    assert (n < start + total).any()  # a length has dropped
+    w = torch.rand(B, H, C, generator=torch.Generator().manual_seed(C))
+    new, index, _ = kv4_evict(c, w.cuda(), C // 2, 5)
+    at = torch.stack([w[b].roll(-(int(start[b]) % C), -1) for b in range(B)])
+    want, _ = r.evict(at, C // 2, 5)
+    assert torch.equal(index.cpu() - (n - total)[:, None, None].int(), want)
+    for x, y in zip(kv4_read(new, C // 2), r.take(want, C).read(C // 2)):
+        assert torch.equal(x.cpu(), y)

@@ -146,6 +146,17 @@ __device__ __forceinline__ int count_of(const int32_t* counts, int b, int T) {
   return n < 0 ? 0 : (n > T ? T : n);
 }
 
+// The length of a sequence after n more positions. One that passes the limit drops by a
+// multiple of the capacity to no less than the capacity: what is held, in which slot and
+// how far before what else stays as it is, and a ring may go on for ever. (Of a capacity
+// above half the limit there is no such length; it stays at the limit.)
+__device__ __forceinline__ int length_after(int len, int n, int C) {
+  const uint32_t total = (uint32_t)len + (uint32_t)n;
+  if (total <= (uint32_t)kKv4MaxLength) return (int)total;
+  if (C > kKv4MaxLength / 2) return kKv4MaxLength;
+  return C + (int)(total % (uint32_t)C);
+}
+
 // ---------------------------------------------------------------------------
 // Append. 4 slots in a row (a word group of the values) of one head are D / 2
 // threads, each with 8 channels of one of them: 16 bytes in, 4 out, of a key and
@@ -225,7 +236,7 @@ __global__ __launch_bounds__(SMALL ? 1024 : 256) void append_kernel(Kv4AppendArg
       append_words<T, D>(a, b, g % a.c.H, len, n_new, g / a.c.H, i % PER);
     }
     __syncthreads();  // every thread has read the length
-    if (threadIdx.x == 0) a.c.len[b] = len + n_new;
+    if (threadIdx.x == 0) a.c.len[b] = length_after(len, n_new, a.c.C);
   } else {
     const int g = (int)(((int64_t)blockIdx.x * 256 + threadIdx.x) / PER);
     if (g < groups * a.c.H)
@@ -235,7 +246,8 @@ __global__ __launch_bounds__(SMALL ? 1024 : 256) void append_kernel(Kv4AppendArg
 
 __global__ void advance_kernel(Kv4AppendArgs a) {
   const int b = blockIdx.x * 256 + threadIdx.x;
-  if (b < a.c.B) a.c.len[b] = length_of(a.c.len, b) + count_of(a.counts, b, a.T);
+  if (b < a.c.B)
+    a.c.len[b] = length_after(length_of(a.c.len, b), count_of(a.counts, b, a.T), a.c.C);
 }
 
 template <typename T, int D>

@@ -150,7 +150,8 @@ class KV4Cache:
 
     @property
     def lengths(self) -> torch.Tensor:
-        """Positions that each sequence has had, int32 (batch,)."""
+        """Positions that each sequence has had, int32 (batch,); past 2^30 less a multiple
+        of the capacity (at least that many remain)."""
         return self._part(4)
 
     @property
