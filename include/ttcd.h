@@ -481,8 +481,9 @@ ttcd_status ttcd_ttt_scan_fwd(const void* dw, const void* w_cur, float lr, void*
  * byte e + 127: the least with no magnitude over 6 * 2^e, e in [-125, 125] for
  * BF16 and in [-23, 13] for F16 (so every held value is a number of the type). A
  * value is 4 bits, a sign (8) and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (codes 0 to
- * 7), rounded to nearest, ties to the even code; what is larger, infinities among
- * it, is held as 6 * 2^e, NaN as 0.
+ * 7), rounded to nearest, ties to the even code. The bound on e wins over the rest:
+ * magnitudes above 6 * 2^13 (F16) or 6 * 2^125 (BF16), infinities among them, are held
+ * as that (finite ones lose up to a quarter). NaN is held as 0.
  *   k_codes  (batch, kv_heads, capacity, head_dim / 2) bytes, channel 2i in the
  *            low half of byte i and 2i + 1 in the high one
  *   k_scales (batch, kv_heads, capacity, head_dim / 32)

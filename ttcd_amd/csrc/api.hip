@@ -1218,10 +1218,12 @@ struct Kv4Plan {
 // Up to 32 rows a key / value head (a token, or a few): kernels of 8 wavefronts with 16
 // or 32 rows that stream the keys, bound by those: parts for 1024 workgroups, but 16
 // tiles of 32 keys each at the least, two a wavefront (us, one token, 16/8 heads of
-// 128: 8 sequences of 4096 keys 15.5, with 8 tiles 19.6; 32 of up to 16384 63, for 512
-// workgroups 68; one of 8192 9.5, with 32 tiles 12.0), and none for up to 40 tiles,
-// where the second launch costs more than it saves (1024 keys 7.5, split 9.0; 2048
-// 9.0 split; 704 6.5).
+// 128: 8 sequences of 4096 keys 15.5, with 8 tiles 19.6; one of 8192 9.4, with 32 tiles
+// 12.0), and none for up to 40 tiles, where the second launch costs more than it saves
+// (1024 keys 7.5, split 9.0; 2048 9.0 split; 704 6.5). Parts for 512 workgroups are
+// better for large batches and worse for few sequences (1024 and 512: 32 of up to 16384
+// keys 58 and 55, 8 of 16384 36 and 31, 3 of 16384 21.6 and 22.0, 2 of 65001 with 15/5
+// heads of 64 18.4 and 19.4; the others above the same).
 //
 // More: 128 rows a workgroup and tiles of 64 keys, of which a turn takes so many us
 // with a CU to itself and so many for each of two that share one. What a split adds is

@@ -4,9 +4,10 @@
 //
 // Format. Blocks of 32 channels of one position share a power of two 2^e
 // (byte e + 127); a value is a sign and one of 0, .5, 1, 1.5, 2, 3, 4, 6
-// (e2m1), rounded to nearest even. e is the least with no value over 6 2^e, so
-// nothing but an infinity is clipped: the largest value of a block weighs most
-// in a dot product. Scales are powers of two because every held value is then
+// (e2m1), rounded to nearest even. e is the least with no value over 6 2^e: the
+// largest value of a block weighs most in a dot product. Clipped is only what lies
+// above 6 times the largest 2^e: infinities, f16 above 49152 (65504, the largest,
+// loses a quarter) and bf16 above 1.5 2^127. Scales are powers of two because every held value is then
 // exact in bf16 and f16 (the range of e sees to that, below): gfx950 converts
 // pairs of codes to either in one instruction, products with q are exact in an
 // MFMA, and no code depends on how a division rounds.
@@ -343,8 +344,11 @@ hipError_t launch_read(const Kv4ReadArgs& a, hipStream_t st) {
 // 63.5 us in all; one token of 257 keys 5.2 against 4.8).
 //
 // FAR: a cache that the last-level cache cannot hold beside anything else is read past
-// the caches (the token of 32 sequences 64 -> 59 us), a smaller one through them (44 MB,
-// as it may be there from the call before: 18.6 us, past them 19.4).
+// the caches (us, two of them in turn: the token of 32 sequences 63 -> 58, of 8 of 16384
+// keys, 143 MB, 39 -> 37), a smaller one through them. Of 44 MB that pays where it is
+// there from the call before (18.4 us, past them 18.9) and not where 350 MB of others
+// have passed by (20.5, past them 19.7), as a model's other layers do; 9 MB the same (9.4
+// and 9.8; 10.2 and 9.7). By the capacity: the lengths are on the GPU.
 constexpr int kRowWaves = 8;
 
 template <bool FAR, typename V>
@@ -680,7 +684,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Kv4AttnArgs a)
 // its own 272.)
 //
 // Bound by the matrix pipe and the exponentials, which take about as long: 4096
-// queries on an 8192 window, 16/8 heads of 128, 261 us, 1053 TFLOP/s (a large library
+// queries on an 8192 window, 16/8 heads of 128, 256 us, 1074 TFLOP/s (a large library
 // product reaches 1226 on the same card). Two workgroups a CU, 64 KiB of LDS and 256
 // registers each. 64 rows a wavefront, which would halve the operand reads, spill
 // (1169 us); every wavefront converting for itself, without LDS, took 476; scheduling
@@ -1000,7 +1004,6 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4AttnArgs a) {
   for (int d = 1; d < 64; d *= 2) l += __shfl_xor(l, d);
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   const float* src = a.part + id * D + 4 * d4;
-#pragma unroll 4
   for (int p0 = 0; p0 < a.parts; p0 += GR) {
     const int p = p0 + g;
     const float w = __shfl(f, p & 63);
