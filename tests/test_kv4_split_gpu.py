@@ -156,3 +156,60 @@ def test_evict_of_caches_of_8193_to_32768_slots(gpu, C, lengths, keep, recent):
     odd[..., ::7], odd[..., 5::11], odd[..., 6::11] = -0.0, math.nan, -math.inf
     for x in (w.log().square(), ties, odd, torch.zeros(2, 1, C)):
         _evict_case(c, r, x.cuda(), keep, recent)
+
+
+def test_graphs_of_split_calls_replay_at_once(gpu):
+    """One call of each kernel and sum captured, each graph with its workspace, replayed on
+    streams of their own over one cache, several times, with eager calls between."""
+    c, r = _pair(2, 2, 128, 8192, BF, (8192, 6000))
+    qs = [_rand(i, 2, T, 8, 128) for i, T in ((1, 1), (2, 7), (3, 10), (4, 130))]
+    want = [kv4_attn(q.cuda(), c, return_lse=True) for q in qs]
+    graphs, inputs = [], [q.cuda() for q in qs]
+    for q, x, w in zip(qs, inputs, want):
+        assert _parts(c, q.shape[1], 8, None) > 1
+        _check_attn(r, q, *w, None, None)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = kv4_attn(x, c, return_lse=True)
+        graphs.append((g, out))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        torch.cuda.synchronize()
+        for s, (g, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                for _ in range(4):
+                    g.replay()
+        torch.cuda.synchronize()
+        for (_, out), w in zip(graphs, want):
+            for x, y in zip(out, w):
+                assert torch.equal(x, y)
+                x.zero_()
+        assert torch.equal(kv4_attn(inputs[3], c), want[3][0])
+
+
+def test_a_captured_follow_up_goes_by_the_lengths_it_finds(gpu):
+    """Append of a chunk (lengths by a second launch), split attention of many rows, key
+    weights: each replay is the next chunk, over the ring's end and past empty parts."""
+    B, T, Hq, H, D, C = 2, 130, 8, 4, 64, 2048
+    c, r = _pair(B, H, D, C, HF, (1900, 3), weights=True)
+    assert 1 < _parts(c, T, Hq, None) <= 16
+    k, v, q = (torch.zeros(B, T, h, D, dtype=HF, device=gpu) for h in (H, H, Hq))
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        kv4_append(c, k, v)
+        o, lse = kv4_attn(q, c, return_lse=True)
+        w = kv4_key_weights(q, c, lse)
+    for i in range(4):
+        new = [_rand(7 * i + j, B, T, h, D, dtype=HF) for j, h in enumerate((H, H, Hq))]
+        for x, y in zip((k, v, q), new):
+            x.copy_(y)
+        g.replay()
+        torch.cuda.synchronize()
+        r.append(new[0], new[1])
+        _check_attn(r, new[2], o, lse, None, None)
+        seen = torch.full((B, H), T * Hq / H, dtype=torch.float64)
+        assert ((w.double().sum(-1).cpu() - seen).abs() <= 1e-3 * seen).all()
+        for x, y in zip(kv4_attn(q, c, return_lse=True), (o, lse)):
+            assert torch.equal(x, y)
