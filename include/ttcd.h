@@ -621,7 +621,7 @@ ttcd_status ttcd_attn_block_coverage(int npair, int nqb, int ngrp, int packed,
  * many rows fills and reads its stages in LDS over key tiles t0 .. t1 - 1 (no GPU
  * needed): TTCD_ERR_UNSUPPORTED if a stage is read and written, or written twice, with no
  * barrier between the two, if a read finds another tile than the one it is to find, or if
- * not every tile is folded once and in order. */
+ * not every tile is folded once and in order. 0 <= t0 < t1 <= 2^30. */
 ttcd_status ttcd_kv4_block_stages(int t0, int t1);
 
 #ifdef __cplusplus

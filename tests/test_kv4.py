@@ -165,7 +165,8 @@ def test_no_stage_is_rewritten_while_it_may_be_read():
     for t0 in range(4):
         for n in range(1, 40):
             assert f(t0, t0 + n) == 0, (t0, n, _lib.lib().ttcd_last_error())
-    assert f(3, 3) == f(-1, 4) == f(2, 1) == INV
+    assert f((1 << 30) - 9, 1 << 30) == 0
+    assert f(3, 3) == f(-1, 4) == f(2, 1) == f(0, (1 << 31) - 1) == INV
 
 
 def test_a_student_window_over_dropped_keys_is_refused():

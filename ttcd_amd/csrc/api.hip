@@ -1584,7 +1584,8 @@ ttcd_status ttcd_attn_block_coverage(int npair, int nqb, int ngrp, int packed, i
 }
 
 ttcd_status ttcd_kv4_block_stages(int t0, int t1) {
-  if (t0 < 0 || t1 <= t0) return fail(TTCD_ERR_INVALID_ARGUMENT, "need 0 <= t0 < t1");
+  if (t0 < 0 || t1 <= t0 || t1 > ttcd::kKv4MaxLength)
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "need 0 <= t0 < t1 <= 2^30");
   struct Stage {
     int holds = -1, written = -1, read = -1;  // a tile; intervals between barriers
   } k[2], v[2];

@@ -7,9 +7,9 @@
 // (e2m1), rounded to nearest even. e is the least with no value over 6 2^e: the
 // largest value of a block weighs most in a dot product. Clipped is only what lies
 // above 6 times the largest 2^e: infinities, f16 above 49152 (65504, the largest,
-// loses a quarter) and bf16 above 1.5 2^127. Scales are powers of two because every held value is then
-// exact in bf16 and f16 (the range of e sees to that, below): gfx950 converts
-// pairs of codes to either in one instruction, products with q are exact in an
+// loses a quarter) and bf16 above 1.5 2^127. Scales are powers of two because every
+// held value is then exact in bf16 and f16 (the range of e sees to that, below): gfx950
+// converts pairs of codes to either in one instruction, products with q are exact in an
 // MFMA, and no code depends on how a division rounds.
 //
 // Position p is in slot p % C, C a multiple of 32, so 32 positions from a
