@@ -588,6 +588,88 @@ ttcd_status ttcd_kv4_evict(const ttcd_kv4_cache* cache, const float* weights, in
                            void* stream);
 
 /*
+ * Attention of the nodes of a tree of drafted tokens. parents: (batch, N) int32, the
+ * node that each follows, before it (-1: none; what does not come before its node is
+ * taken as none). `draft` is a second cache that holds the nodes' own keys and values,
+ * node i in slot i (ttcd_kv4_append of all N to an empty one), of the cache's batch,
+ * kv_heads and head_dim, with a capacity >= N. Node i of sequence b is at position
+ * lengths[b] + depth(i) and sees the held keys of the cache after that less window
+ * (window <= 0: all), and of itself and its ancestors those whose depth is more than
+ * depth(i) - window. Sequence b has the first counts[b] (NULL: N) nodes, of those that
+ * draft's lengths[b] counts. q, o: (batch, N, Hq, head_dim); rows behind the last node
+ * get o = 0 and lse = -inf. The rest, and the workspace, as in ttcd_kv4_attn_fwd.
+ * N <= 256.
+ */
+size_t ttcd_kv4_tree_attn_workspace_bytes(const ttcd_kv4_cache* cache, int N, int Hq,
+                                          int window);
+ttcd_status ttcd_kv4_tree_attn_fwd(const ttcd_kv4_cache* cache, const ttcd_kv4_cache* draft,
+                                   const void* q, void* o, float* lse, int N, int Hq,
+                                   const int64_t q_stride[4], const int64_t o_stride[4],
+                                   const int32_t* parents, const int32_t* counts, int window,
+                                   float sm_scale, ttcd_dtype dtype, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+
+/*
+ * The draft's slots path[b, 0 .. counts[b]) become, bit by bit, the next positions of
+ * sequence b of the cache, whose lengths count them. path: (batch, P) int32, entries
+ * outside the draft's capacity taken as the nearest bound; counts: device int32[batch],
+ * clamped to [0, P], or NULL: P. weights as in ttcd_kv4_append. reset_draft != 0: the
+ * draft's lengths become 0. 1 <= P <= both capacities; the two share no memory.
+ */
+ttcd_status ttcd_kv4_commit(ttcd_kv4_cache* cache, ttcd_kv4_cache* draft, const int32_t* path,
+                            const int32_t* counts, int P, float* weights, int reset_draft,
+                            void* stream);
+
+/*
+ * Rotary embedding at given positions: the first 2 * num_freq channels of every head in
+ * pairs (i, num_freq + i), interleaved != 0: (2i, 2i + 1), turned by position *
+ * inv_freq[i] (inverse != 0: back) and multiplied by scale; the others copied. The angle
+ * is exact for any position below 2^53. q: (B, T, Hq, D), k: (B, T, Hkv, D), Hkv = 0:
+ * none; outputs of the same shapes, which may be the inputs (same strides). Strides of
+ * any sign and size but d-stride 1; 16-byte accesses are made where all allow it.
+ * positions: int32, or int64 with positions_64 != 0, at b * position_stride[0] + t *
+ * position_stride[1]; NULL: offset + t. D <= 1024. dtype BF16, F16 or F32.
+ */
+ttcd_status ttcd_rope_fwd(const void* q, const void* k, void* q_out, void* k_out,
+                          const float* inv_freq, int num_freq, const void* positions,
+                          int positions_64, const int64_t position_stride[2], int64_t offset,
+                          int B, int T, int Hq, int Hkv, int D, const int64_t q_stride[4],
+                          const int64_t k_stride[4], const int64_t q_out_stride[4],
+                          const int64_t k_out_stride[4], int interleaved, int inverse,
+                          float scale, ttcd_dtype dtype, void* stream);
+
+/*
+ * A token from every row of logits (R, V) of BF16 or F16, V <= 2^20, rows row_stride
+ * elements apart. Tokens rank by logit, of equal ones the lower index first; the weight
+ * of one is exp((logit - highest) / temperature). Kept are the first top_k (0: all), of
+ * those the shortest run with at least top_p (>= 1: all) of their sum, of those the ones
+ * with at least min_p of the highest weight; tokens[r] is the first whose running sum
+ * exceeds uniform[r] (in [0, 1)) times the sum of all kept, logprobs[r] (or NULL) the
+ * log of its weight's share of that sum. temperature 0: the first. -infinity and NaN are no
+ * candidates; a row without one gets token -1 and -infinity; of infinities each weighs
+ * 1. Weights and sums are 64 bits. Settings are one value for all rows, or device arrays
+ * (R) where not NULL (then a temperature or top_p not above 0 is 0 or keeps one token, a
+ * top_k below 1 keeps all, as a NaN does, and a min_p above 1 is 1).
+ */
+ttcd_status ttcd_sample_fwd(const void* logits, int64_t row_stride, int R, int V,
+                            const float* uniform, const float* temperatures, double temperature,
+                            const int32_t* top_ks, int top_k, const float* top_ps, double top_p,
+                            const float* min_ps, double min_p, int64_t* tokens, float* logprobs,
+                            ttcd_dtype dtype, void* stream);
+
+/*
+ * The nodes of a tree that agree with what was picked: from node 0 (whose token is
+ * given) to its first child whose token was picked at it, and on. parents as in
+ * ttcd_kv4_tree_attn_fwd; tokens, picked: (B, N) int64, the token of each node and the
+ * one that followed it; counts: device int32[B] or NULL. path: (B, N) int32, the nodes in
+ * order, -1 behind the last; accepted: (B), their number; next: (B) int64, what was
+ * picked at the last (-1 of a sequence without nodes). N <= 256.
+ */
+ttcd_status ttcd_tree_accept(const int32_t* parents, const int64_t* tokens,
+                             const int64_t* picked, const int32_t* counts, int32_t* path,
+                             int32_t* accepted, int64_t* next, int B, int N, void* stream);
+
+/*
  * Host-only schedule check (no GPU work). Replays the attention kernels'
  * exact tile/phase schedule for one (b, h) slice of length T and adds, for
  * every (query i, key j) pair the kernel would fold into each output, one

@@ -64,6 +64,12 @@ EXPORTS = (
     "ttcd_kv4_attn_fwd",
     "ttcd_kv4_key_weights_fwd",
     "ttcd_kv4_evict",
+    "ttcd_kv4_tree_attn_workspace_bytes",
+    "ttcd_kv4_tree_attn_fwd",
+    "ttcd_kv4_commit",
+    "ttcd_rope_fwd",
+    "ttcd_sample_fwd",
+    "ttcd_tree_accept",
     "ttcd_attn_schedule_coverage",
     "ttcd_attn_block_coverage",
     "ttcd_kv4_block_stages",
@@ -75,6 +81,7 @@ _vp = ctypes.c_void_p
 _fp = ctypes.c_void_p  # float* passed as a raw address
 _i64x4 = ctypes.POINTER(ctypes.c_int64)
 _i64x3 = ctypes.POINTER(ctypes.c_int64)
+_i64x2 = ctypes.POINTER(ctypes.c_int64)
 
 
 class KV4CacheStruct(ctypes.Structure):
@@ -183,6 +190,19 @@ _SIGS = {
     "ttcd_kv4_key_weights_fwd": (_i32, [
         _kv4, _vp, _fp, _fp, _i32, _i32, _i64x4, _vp, _i32, ctypes.c_float, _i32, _i32, _vp]),
     "ttcd_kv4_evict": (_i32, [_kv4, _fp, _i32, _i32, _kv4, _fp, _vp, _vp]),
+    "ttcd_kv4_tree_attn_workspace_bytes": (ctypes.c_size_t, [_kv4, _i32, _i32, _i32]),
+    "ttcd_kv4_tree_attn_fwd": (_i32, [
+        _kv4, _kv4, _vp, _vp, _fp, _i32, _i32, _i64x4, _i64x4, _vp, _vp, _i32, ctypes.c_float,
+        _i32, _vp, ctypes.c_size_t, _vp]),
+    "ttcd_kv4_commit": (_i32, [_kv4, _kv4, _vp, _vp, _i32, _fp, _i32, _vp]),
+    "ttcd_rope_fwd": (_i32, [
+        _vp, _vp, _vp, _vp, _fp, _i32, _vp, _i32, _i64x2, _i64,
+        _i32, _i32, _i32, _i32, _i32, _i64x4, _i64x4, _i64x4, _i64x4,
+        _i32, _i32, ctypes.c_float, _i32, _vp]),
+    "ttcd_sample_fwd": (_i32, [
+        _vp, _i64, _i32, _i32, _fp, _fp, ctypes.c_double, _vp, _i32, _fp, ctypes.c_double,
+        _fp, ctypes.c_double, _vp, _fp, _i32, _vp]),
+    "ttcd_tree_accept": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp]),
     "ttcd_attn_schedule_coverage": (_i32, [
         _i32, _i32, _i32, _i32, _i32, _vp, _vp]),
     "ttcd_attn_block_coverage": (_i32, [_i32, _i32, _i32, _i32, _vp, _vp]),
@@ -224,6 +244,7 @@ def lib() -> ctypes.CDLL:
 
 _Strides4 = ctypes.c_int64 * 4
 _Strides3 = ctypes.c_int64 * 3
+_Strides2 = ctypes.c_int64 * 2
 
 
 def strides4(strides) -> ctypes.Array:
@@ -232,6 +253,10 @@ def strides4(strides) -> ctypes.Array:
 
 def strides3(strides) -> ctypes.Array:
     return _Strides3(*strides)
+
+
+def strides2(strides) -> ctypes.Array:
+    return _Strides2(*strides)
 
 
 # torch's own accessor of the current stream's handle: torch.cuda.current_stream
@@ -244,6 +269,19 @@ def stream(t) -> int:
     if _raw_stream is not None:
         return _raw_stream(t.device.index)
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def call(t, fn, *args) -> None:
+    """fn(*args, stream), checked, with t's device (a tensor's, or what has one) current:
+    the launches go to it."""
+    if _current_device() == t.device.index:
+        check(fn(*args, stream(t)))
+    else:
+        with torch.cuda.device(t.device):
+            check(fn(*args, stream(t)))
 
 
 def check(status: int) -> None:

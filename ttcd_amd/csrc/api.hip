@@ -824,6 +824,76 @@ ttcd_status ttcd_rope_table_fwd(void* cos_table, void* sin_table, const float* i
                   "rope table launch");
 }
 
+ttcd_status ttcd_rope_fwd(const void* q, const void* k, void* q_out, void* k_out,
+                          const float* inv_freq, int num_freq, const void* positions,
+                          int positions_64, const int64_t position_stride[2], int64_t offset,
+                          int B, int T, int Hq, int Hkv, int D, const int64_t q_stride[4],
+                          const int64_t k_stride[4], const int64_t q_out_stride[4],
+                          const int64_t k_out_stride[4], int interleaved, int inverse,
+                          float scale, ttcd_dtype dtype, void* stream) {
+  if (!q || !q_out || !inv_freq) return fail(TTCD_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (Hkv < 0 || (Hkv > 0 && (!k || !k_out)))
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "null tensor pointer (k, Hkv = %d)", Hkv);
+  if (!q_stride || !q_out_stride || (Hkv > 0 && (!k_stride || !k_out_stride)) ||
+      (positions && !position_stride))
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "null stride array");
+  if (B < 1 || T < 1 || Hq < 1)
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "B, T, Hq must be >= 1 (got %d, %d, %d)", B, T, Hq);
+  if (D < 2 || D > 1024) return fail(TTCD_ERR_UNSUPPORTED, "head_dim %d not in 2 .. 1024", D);
+  if (num_freq < 1 || 2 * (int64_t)num_freq > D)
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "need 1 <= num_freq <= head_dim / 2 (got %d of %d)",
+                num_freq, D);
+  if ((unsigned)dtype > TTCD_DTYPE_F32) return fail(TTCD_ERR_INVALID_ARGUMENT, "unknown dtype");
+  if (!isfinite(scale)) return fail(TTCD_ERR_INVALID_ARGUMENT, "scale must be finite");
+  const int64_t heads = (int64_t)Hq + Hkv;
+  if ((int64_t)B * T > 0x7fffffffLL || heads * D > (1 << 28) ||
+      (int64_t)B * T > 0x7fffffffLL * 512 / (heads * D))
+    return fail(TTCD_ERR_UNSUPPORTED, "grid too large");
+  const int64_t* all[4] = {q_stride, q_out_stride, Hkv > 0 ? k_stride : q_stride,
+                           Hkv > 0 ? k_out_stride : q_out_stride};
+  for (int t = 0; t < 4; ++t)
+    if (all[t][3] != 1)
+      return fail(TTCD_ERR_INVALID_ARGUMENT, "head_dim must be contiguous (d-stride 1)");
+  ttcd::RopeArgs a = {};
+  a.q = q;
+  a.q_out = q_out;
+  a.inv_freq = inv_freq;
+  a.positions = positions;
+  a.pos64 = positions_64 != 0;
+  a.inverse = inverse != 0;
+  if (positions) {
+    a.pos_sb = position_stride[0];
+    a.pos_st = position_stride[1];
+  }
+  a.offset = offset;
+  a.scale = scale;
+  a.Hq = Hq;
+  a.Hkv = Hkv;
+  a.D = D;
+  a.n = num_freq;
+  a.tokens = (int64_t)B * T;
+  a.T = ttcd::make_fast_div(T);
+  a.q_sb = q_stride[0];
+  a.q_st = q_stride[1];
+  a.q_sh = q_stride[2];
+  a.qo_sb = q_out_stride[0];
+  a.qo_st = q_out_stride[1];
+  a.qo_sh = q_out_stride[2];
+  if (Hkv > 0) {
+    a.k = k;
+    a.k_out = k_out;
+    a.k_sb = k_stride[0];
+    a.k_st = k_stride[1];
+    a.k_sh = k_stride[2];
+    a.ko_sb = k_out_stride[0];
+    a.ko_st = k_out_stride[1];
+    a.ko_sh = k_out_stride[2];
+  }
+  return from_hip(ttcd::launch_rope(a, interleaved != 0, elem(dtype),
+                                    static_cast<hipStream_t>(stream)),
+                  "rope launch");
+}
+
 ttcd_status ttcd_qk_norm_rope_fwd(const void* q, const void* k, void* q_out, void* k_out,
                                   const void* q_norm_w, const void* k_norm_w, ttcd_dtype w_dtype,
                                   float eps, const void* cos_table, const void* sin_table,
@@ -1460,6 +1530,167 @@ ttcd_status ttcd_kv4_evict(const ttcd_kv4_cache* cache, const float* weights, in
   a.recent = recent;
   return from_hip(ttcd::launch_kv4_evict(a, static_cast<hipStream_t>(stream)),
                   "kv4 eviction launch");
+}
+
+namespace {
+
+// The draft that a tree's nodes lie in, next to the cache of their sequences.
+ttcd_status check_draft(const ttcd_kv4_cache* cache, const ttcd_kv4_cache* draft) {
+  if (draft->batch != cache->batch || draft->kv_heads != cache->kv_heads ||
+      draft->head_dim != cache->head_dim)
+    return fail(TTCD_ERR_INVALID_ARGUMENT,
+                "the draft must have the cache's batch, kv_heads and head_dim");
+  Span ours[5], theirs[5];
+  kv4_spans(cache, ours);
+  kv4_spans(draft, theirs);
+  for (const Span& x : ours)
+    for (const Span& y : theirs)
+      if (overlap(x, y))
+        return fail(TTCD_ERR_INVALID_ARGUMENT, "the draft must not share memory with the cache");
+  return TTCD_OK;
+}
+
+}  // namespace
+
+size_t ttcd_kv4_tree_attn_workspace_bytes(const ttcd_kv4_cache* cache, int N, int Hq,
+                                          int window) {
+  return N > ttcd::kTreeNodes ? 0 : ttcd_kv4_attn_workspace_bytes(cache, N, Hq, window);
+}
+
+ttcd_status ttcd_kv4_tree_attn_fwd(const ttcd_kv4_cache* cache, const ttcd_kv4_cache* draft,
+                                   const void* q, void* o, float* lse, int N, int Hq,
+                                   const int64_t q_stride[4], const int64_t o_stride[4],
+                                   const int32_t* parents, const int32_t* counts, int window,
+                                   float sm_scale, ttcd_dtype dtype, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  ttcd_status st = check_kv4(cache);
+  if (st == TTCD_OK) st = check_kv4(draft);
+  if (st == TTCD_OK) st = check_draft(cache, draft);
+  if (st == TTCD_OK) st = check_kv4_dtype(dtype);
+  if (st == TTCD_OK) st = check_kv4_strides(q, q_stride);
+  if (st == TTCD_OK) st = check_kv4_strides(o, o_stride);
+  if (st == TTCD_OK) st = check_kv4_rows(cache, N, Hq);
+  if (st != TTCD_OK) return st;
+  if (!parents) return fail(TTCD_ERR_INVALID_ARGUMENT, "null parents pointer");
+  if (N > ttcd::kTreeNodes)
+    return fail(TTCD_ERR_UNSUPPORTED, "%d nodes: at most %d", N, ttcd::kTreeNodes);
+  if (N > draft->capacity)
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "%d nodes in a draft of capacity %d", N,
+                draft->capacity);
+  if (!(sm_scale > 0.f) || !isfinite(sm_scale))
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "sm_scale must be finite and > 0");
+  ttcd::Kv4TreeArgs a = {};
+  a.c = kv4(cache);
+  a.d = kv4(draft);
+  a.parents = parents;
+  a.q = q;
+  a.o = o;
+  a.lse = lse;
+  a.counts = counts;
+  a.q_sb = q_stride[0];
+  a.q_st = q_stride[1];
+  a.q_sh = q_stride[2];
+  a.o_sb = o_stride[0];
+  a.o_st = o_stride[1];
+  a.o_sh = o_stride[2];
+  a.Tq = N;
+  a.G = Hq / cache->kv_heads;
+  a.window = kv4_window(window);
+  a.c_log2 = sm_scale * 1.4426950408889634f;
+  const Kv4Plan p = kv4_plan(cache, N, Hq, a.window);
+  a.row_tiles = p.row_tiles;
+  a.nrb = p.nrb;
+  a.parts = 1;
+  const size_t part = kv4_part_bytes(cache, N, Hq);
+  if (p.parts > 1 && workspace && aligned16(workspace) && workspace_bytes >= p.parts * part) {
+    a.parts = p.parts;
+    a.part = static_cast<float*>(workspace);
+    a.part_ml = a.part + p.parts * (part / sizeof(float) / (cache->head_dim + 2)) * cache->head_dim;
+  }
+  return from_hip(ttcd::launch_kv4_tree_attn(a, elem(dtype), static_cast<hipStream_t>(stream)),
+                  "kv4 tree attention launch");
+}
+
+ttcd_status ttcd_kv4_commit(ttcd_kv4_cache* cache, ttcd_kv4_cache* draft, const int32_t* path,
+                            const int32_t* counts, int P, float* weights, int reset_draft,
+                            void* stream) {
+  ttcd_status st = check_kv4(cache);
+  if (st == TTCD_OK) st = check_kv4(draft);
+  if (st == TTCD_OK) st = check_draft(cache, draft);
+  if (st != TTCD_OK) return st;
+  if (!path) return fail(TTCD_ERR_INVALID_ARGUMENT, "null path pointer");
+  if (P < 1 || P > cache->capacity || P > draft->capacity)
+    return fail(TTCD_ERR_INVALID_ARGUMENT,
+                "need 1 <= P <= the capacities (got P=%d, capacities %d and %d)", P,
+                cache->capacity, draft->capacity);
+  if ((int64_t)P * cache->kv_heads * (cache->head_dim / 8) > 0x7fffffffLL)
+    return fail(TTCD_ERR_UNSUPPORTED, "grid too large");
+  ttcd::Kv4CommitArgs a = {};
+  a.c = kv4(cache);
+  a.d = kv4(draft);
+  a.path = path;
+  a.counts = counts;
+  a.weights = weights;
+  a.P = P;
+  a.reset = reset_draft != 0;
+  return from_hip(ttcd::launch_kv4_commit(a, static_cast<hipStream_t>(stream)),
+                  "kv4 commit launch");
+}
+
+ttcd_status ttcd_sample_fwd(const void* logits, int64_t row_stride, int R, int V,
+                            const float* uniform, const float* temperatures, double temperature,
+                            const int32_t* top_ks, int top_k, const float* top_ps, double top_p,
+                            const float* min_ps, double min_p, int64_t* tokens, float* logprobs,
+                            ttcd_dtype dtype, void* stream) {
+  if (!logits || !uniform || !tokens)
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (R < 1 || V < 1)
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "need R, V >= 1 (got %d, %d)", R, V);
+  if (V > ttcd::kSampleVocab)
+    return fail(TTCD_ERR_UNSUPPORTED, "%d tokens a row: at most %d", V, ttcd::kSampleVocab);
+  if (dtype != TTCD_DTYPE_BF16 && dtype != TTCD_DTYPE_F16)
+    return fail(TTCD_ERR_UNSUPPORTED, "logits must be bf16 or f16");
+  if (row_stride < 0) return fail(TTCD_ERR_INVALID_ARGUMENT, "row stride must be >= 0");
+  if (reinterpret_cast<uintptr_t>(logits) & 1u)
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "logits must be 2-byte aligned");
+  if (!temperatures && !(temperature >= 0))
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "temperature must be >= 0");
+  if (!top_ks && top_k < 0) return fail(TTCD_ERR_INVALID_ARGUMENT, "top_k must be >= 0");
+  if (!top_ps && !(top_p > 0)) return fail(TTCD_ERR_INVALID_ARGUMENT, "top_p must be > 0");
+  if (!min_ps && !(min_p >= 0 && min_p <= 1))
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "min_p must be in 0 .. 1");
+  ttcd::SampleArgs a = {};
+  a.logits = logits;
+  a.st = row_stride;
+  a.R = R;
+  a.V = V;
+  a.uniform = uniform;
+  a.temperatures = temperatures;
+  a.temperature = temperature;
+  a.top_ks = top_ks;
+  a.top_k = top_k;
+  a.top_ps = top_ps;
+  a.top_p = top_p;
+  a.min_ps = min_ps;
+  a.min_p = min_p;
+  a.tokens = tokens;
+  a.logprobs = logprobs;
+  return from_hip(ttcd::launch_sample(a, elem(dtype), static_cast<hipStream_t>(stream)),
+                  "sample launch");
+}
+
+ttcd_status ttcd_tree_accept(const int32_t* parents, const int64_t* tokens,
+                             const int64_t* picked, const int32_t* counts, int32_t* path,
+                             int32_t* accepted, int64_t* next, int B, int N, void* stream) {
+  if (!parents || !tokens || !picked || !path || !accepted || !next)
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (B < 1 || N < 1)
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "need B, N >= 1 (got %d, %d)", B, N);
+  if (N > ttcd::kTreeNodes)
+    return fail(TTCD_ERR_UNSUPPORTED, "%d nodes: at most %d", N, ttcd::kTreeNodes);
+  const ttcd::AcceptArgs a = {parents, tokens, picked, counts, path, accepted, next, B, N};
+  return from_hip(ttcd::launch_tree_accept(a, static_cast<hipStream_t>(stream)),
+                  "tree accept launch");
 }
 
 ttcd_status ttcd_attn_schedule_coverage(int T, int dual, int window_s, int window_t,

@@ -1,6 +1,6 @@
 // internal.h - launcher interface between the C ABI (api.hip) and the
 // gfx950 kernels (attn.hip, conv.hip, merge.hip, prologue.hip, epilogue.hip,
-// ttt.hip, linear.hip, kv4.hip).
+// ttt.hip, linear.hip, kv4.hip, rope.hip, sample.hip).
 // Not part of the ABI.
 #pragma once
 
@@ -86,6 +86,29 @@ hipError_t launch_qk_norm_rope(const PrologueArgs& a, Elem dtype, Elem wt, hipSt
 // cos/sin tables: row t, column i = cos/sin(fp32(t) * inv_freq[i]) rounded to dtype.
 hipError_t launch_rope_table(void* cos_t, void* sin_t, const float* inv_freq, int rows, int half,
                              Elem dtype, hipStream_t stream);
+
+// Rotary embedding at given positions (rope.hip).
+struct RopeArgs {
+  const void* q;
+  const void* k;         // Hkv = 0: none
+  void* q_out;
+  void* k_out;
+  const float* inv_freq; // (n)
+  const void* positions; // int32, or int64 where pos64; null: offset + t
+  bool pos64, inverse;
+  int64_t pos_sb, pos_st;
+  int64_t offset;
+  float scale;
+  int Hq, Hkv, D, n;
+  int64_t tokens;        // B * T, below 2^31
+  FastDiv T;
+  FastDiv per_token, per_head, div_n;  // tasks, and frequencies (set by the launcher)
+  int64_t q_sb, q_st, q_sh;
+  int64_t k_sb, k_st, k_sh;
+  int64_t qo_sb, qo_st, qo_sh;
+  int64_t ko_sb, ko_st, ko_sh;
+};
+hipError_t launch_rope(const RopeArgs& a, bool pairs, Elem dtype, hipStream_t stream);
 
 // Teacher and student residual add + RMSNorm of the attention outputs (epilogue.hip).
 hipError_t launch_dual_residual_rmsnorm(const void* a_t, const void* a_s, const void* res,
@@ -262,5 +285,53 @@ struct Kv4EvictArgs {
   int keep, recent;
 };
 hipError_t launch_kv4_evict(const Kv4EvictArgs& a, hipStream_t stream);
+
+struct Kv4CommitArgs {
+  Kv4Cache c, d;          // the cache, and the draft that the nodes come from
+  const int32_t* path;    // (B, P) slots of the draft
+  const int32_t* counts;  // (B), or null: P
+  float* weights;         // (B, H, C), or null: 0 in the slots that are written
+  int P;
+  bool reset;             // the draft's lengths become 0
+};
+hipError_t launch_kv4_commit(const Kv4CommitArgs& a, hipStream_t stream);
+
+constexpr int kTreeNodes = 256;  // at most, of a sequence's tree
+
+// Attention of a tree's nodes: Tq nodes, their own keys in the cache d, node i in slot i.
+struct Kv4TreeArgs : Kv4AttnArgs {
+  Kv4Cache d;
+  const int32_t* parents;  // (B, Tq)
+};
+hipError_t launch_kv4_tree_attn(const Kv4TreeArgs& a, Elem dtype, hipStream_t stream);
+
+// A token from each row of logits (sample.hip). A setting is its array's, or the value.
+struct SampleArgs {
+  const void* logits;  // (R, V), row stride st
+  int64_t st;
+  int R, V;
+  const float* uniform;  // (R)
+  const float *temperatures, *top_ps, *min_ps;
+  const int32_t* top_ks;
+  double temperature, top_p, min_p;
+  int top_k;
+  int64_t* tokens;   // (R)
+  float* logprobs;   // (R), or null
+};
+constexpr int kSampleVocab = 1 << 20;  // at most, of a row
+hipError_t launch_sample(const SampleArgs& a, Elem dtype, hipStream_t stream);
+
+// The nodes of a tree that agree with what was picked (sample.hip).
+struct AcceptArgs {
+  const int32_t* parents;  // (B, N)
+  const int64_t* tokens;   // (B, N)
+  const int64_t* picked;   // (B, N)
+  const int32_t* counts;   // (B), or null: N
+  int32_t* path;           // (B, N)
+  int32_t* accepted;       // (B)
+  int64_t* next;           // (B)
+  int B, N;
+};
+hipError_t launch_tree_accept(const AcceptArgs& a, hipStream_t stream);
 
 }  // namespace ttcd

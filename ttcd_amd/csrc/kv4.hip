@@ -23,6 +23,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "internal.h"
 #include "kv4_sweep.h"
 
@@ -351,6 +353,11 @@ hipError_t launch_read(const Kv4ReadArgs& a, hipStream_t st) {
 // and 9.8; 10.2 and 9.7). By the capacity: the lengths are on the GPU.
 constexpr int kRowWaves = 8;
 
+template <typename Args>
+constexpr bool is_tree = false;
+template <>
+constexpr bool is_tree<Kv4TreeArgs> = true;
+
 template <bool FAR, typename V>
 __device__ __forceinline__ V codes(const V* p) {
   if constexpr (FAR)
@@ -388,11 +395,30 @@ __device__ __forceinline__ void transpose_pair(const uint32_t (&w)[8], const flo
   }
 }
 
-template <typename T, int D, int NT>
+// What a tile's rows see of it: keys lo .. hi of each row's, any_lo .. any_hi of anyone's.
+template <int NT>
+struct RangeMask {
+  const int (&lo)[NT], (&hi)[NT];
+  int p0, any_lo, any_hi;
+  __device__ __forceinline__ bool row(int nt, int key) const {
+    return p0 + key >= lo[nt] && p0 + key <= hi[nt];
+  }
+  __device__ __forceinline__ bool any(int key) const {
+    return p0 + key >= any_lo && p0 + key <= any_hi;
+  }
+};
+// The same as a bit a key.
+template <int NT>
+struct BitMask {
+  uint32_t rows[NT], all;
+  __device__ __forceinline__ bool row(int nt, int key) const { return (rows[nt] >> key) & 1; }
+  __device__ __forceinline__ bool any(int key) const { return (all >> key) & 1; }
+};
+
+template <typename T, int D, int NT, typename Mask>
 __device__ __forceinline__ void fold_tile(RowState<T, D, NT>& st, const KvTile<D>& kv,
-                                          const u32x4 (&q)[NT][D / 32], float c, int p0, bool masked,
-                                          const int (&lo)[NT], const int (&hi)[NT], int any_lo,
-                                          int any_hi, int lane) {
+                                          const u32x4 (&q)[NT][D / 32], float c, bool masked,
+                                          const Mask& mask, int lane) {
   constexpr int STEPS = D / 32, NM = D / 16;
   const int quarter = lane >> 4;
   f32x4 s[NT][2];
@@ -413,13 +439,13 @@ __device__ __forceinline__ void fold_tile(RowState<T, D, NT>& st, const KvTile<D
     for (int g = 0; g < 2; ++g)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int p = p0 + 16 * g + 4 * quarter + e;
+        const int key = 16 * g + 4 * quarter + e;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
-          if (p < lo[nt] || p > hi[nt]) s[nt][g][e] = -INFINITY;
+          if (!mask.row(nt, key)) s[nt][g][e] = -INFINITY;
         // what no row sees may be anything, and a slot without a position is: make it
         // finite, for 0 times it to be 0
-        if (p < any_lo || p > any_hi) {
+        if (!mask.any(key)) {
           if (g == 0)
             vs0 &= ~(255u << (8 * e));
           else
@@ -503,11 +529,87 @@ __device__ __forceinline__ RowRange row_range(int t, int n_new, int len, int C, 
   return {lo, pos};
 }
 
-template <typename T, int D, int NT, bool FAR>
-__global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Kv4AttnArgs a) {
+// A tree's nodes (kv4_tree_attn): node i of a sequence is at position length + depth(i), and
+// sees the cache up to the window before that, itself and its ancestors, keys of the draft.
+// Ancestors are bits: after s steps a node has those of 2^s, itself among them, and knows
+// the one after the last, so 8 steps are enough for 256 nodes, and the depth's logarithm
+// is what it takes (walking up one by one would wait for LDS at every node of a chain).
+struct TreeBits {
+  uint32_t up[kTreeNodes][kTreeNodes / 32];
+  int depth[kTreeNodes], next[kTreeNodes];
+};
+template <int THREADS>
+__device__ __forceinline__ void tree_bits(TreeBits& tree, const int32_t* parents, int n) {
+  static_assert(THREADS >= kTreeNodes, "a thread a node");
+  constexpr int WORDS = kTreeNodes / 32;
+  const int i = threadIdx.x;
+  int next = -1;
+  if (i < n) {
+    next = parents[i];
+    if (next >= i || next < 0) next = -1;  // a parent comes before its node
+  }
+  if (i < kTreeNodes) {
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) tree.up[i][w] = w == i / 32 ? 1u << (i % 32) : 0u;
+    tree.depth[i] = next >= 0;
+    tree.next[i] = next;
+  }
+  while (__syncthreads_or(next >= 0)) {  // a node's next falls by half its distance at least
+    uint32_t up[WORDS];
+    int depth = 0, after = -1;
+    if (next >= 0) {
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) up[w] = tree.up[next][w];
+      depth = tree.depth[next];
+      after = tree.next[next];
+    }
+    __syncthreads();
+    if (next >= 0) {
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) tree.up[i][w] |= up[w];
+      tree.depth[i] += depth;
+      tree.next[i] = next = after;
+    }
+  }
+}
+
+// Bits lo .. hi of a word, those of them that there are.
+__device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
+  if (lo > hi || hi < 0 || lo > 31) return 0u;
+  return (0xffffffffu << max(lo, 0)) & (0xffffffffu >> (31 - min(hi, 31)));
+}
+
+// Node i's ancestors among nodes 32 w .. 32 w + 31, those that the window reaches.
+__device__ __forceinline__ uint32_t ancestors_in(const TreeBits& tree, int i, int w, int n,
+                                                 int window) {
+  if (i >= n) return 0u;
+  uint32_t m = tree.up[i][w];
+  if (window > 0 && tree.depth[i] >= window) {
+    uint32_t left = m;
+    while (left != 0) {
+      const int e = __builtin_ctz(left);
+      left &= left - 1;
+      if (tree.depth[i] - tree.depth[32 * w + e] >= window) m &= ~(1u << e);
+    }
+  }
+  return m;
+}
+
+__device__ __forceinline__ RowRange node_range(int i, int n, int depth, int len, int C, int W) {
+  if (i >= n) return {1, 0};
+  int lo = max(0, len - C);
+  if (W > 0) lo = max(lo, len + depth - W + 1);
+  return {lo, len - 1};
+}
+
+template <typename T, int D, int NT, bool FAR, typename Args>
+__global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Args a) {
+  constexpr bool TREE = is_tree<Args>;
   constexpr int STEPS = D / 32, NM = D / 16, RB = 16 * NT, R = D / 8;
-  __shared__ float so[kRowWaves][16][D + 4];
+  __shared__ __attribute__((aligned(16))) float so[kRowWaves][16][D + 4];
   __shared__ float sml[kRowWaves][RB][2];
+  static_assert(sizeof(TreeBits) <= sizeof(so), "the tree lies where the sums come later");
+  TreeBits& tree = *reinterpret_cast<TreeBits*>(&so);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int quarter = lane >> 4, n = lane & 15;
@@ -515,7 +617,9 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Kv4AttnArgs a)
   const int rest = blockIdx.x / a.parts;
   const int rb = rest % a.nrb, bh = rest / a.nrb;
   const int b = bh / a.c.H, h = bh % a.c.H;
-  const int len = length_of(a.c.len, b), n_new = count_of(a.counts, b, a.Tq);
+  const int len = length_of(a.c.len, b);
+  int n_new = count_of(a.counts, b, a.Tq);
+  if constexpr (TREE) n_new = min(n_new, length_of(a.d.len, b));
   const int row0 = rb * RB, C = a.c.C;
 
   u32x4 q[NT][STEPS];
@@ -528,21 +632,40 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Kv4AttnArgs a)
                    (int64_t)(h * a.G + row % a.G) * a.q_sh + quarter * (D / 4);
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) q[nt][i] = *reinterpret_cast<const u32x4*>(src + 8 * i);
-    const RowRange rr = row_range(row / a.G, n_new, len, C, a.window);
-    lo[nt] = rr.lo;
-    hi[nt] = rr.hi;
+    if constexpr (!TREE) {
+      const RowRange rr = row_range(row / a.G, n_new, len, C, a.window);
+      lo[nt] = rr.lo;
+      hi[nt] = rr.hi;
+    }
     st.m[nt] = -INFINITY;
     st.l[nt] = 0.f;
 #pragma unroll
     for (int i = 0; i < NM; ++i) st.o[nt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
+  if constexpr (TREE) {
+    tree_bits<64 * kRowWaves>(tree, a.parents + (int64_t)b * a.Tq, n_new);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int node = (row0 + 16 * nt + n) / a.G;
+      const RowRange rr = node_range(node, n_new, tree.depth[min(node, kTreeNodes - 1)], len, C,
+                                     a.window);
+      lo[nt] = rr.lo;
+      hi[nt] = rr.hi;
+    }
+  }
   // the block's keys, and those that all its rows see
   const int t_lo = row0 / a.G, t_hi = min((row0 + RB - 1) / a.G, n_new - 1);
   if (t_lo <= t_hi) {
-    const RowRange first = row_range(t_lo, n_new, len, C, a.window);
-    const RowRange last = row_range(t_hi, n_new, len, C, a.window);
-    if (first.lo <= last.hi) {
-      const int tile_lo = first.lo >> 5, tiles = (last.hi >> 5) - tile_lo + 1;
+    // (of a tree: bounds of all its rows' ranges, from a root to the deepest that there could be)
+    const RowRange first = TREE ? node_range(0, n_new, 0, len, C, a.window)
+                                : row_range(t_lo, n_new, len, C, a.window);
+    const RowRange last = TREE ? node_range(0, n_new, n_new - 1, len, C, a.window)
+                               : row_range(t_hi, n_new, len, C, a.window);
+    if (TREE || first.lo <= last.hi) {
+      const int tile_lo = first.lo >> 5;
+      // of the cache; a tree's draft follows
+      const int held = first.lo <= last.hi ? (last.hi >> 5) - tile_lo + 1 : 0;
+      const int tiles = TREE ? held + ((n_new + 31) >> 5) : held;
       const int per = (tiles + a.parts - 1) / a.parts;
       const int t0 = tile_lo + part * per, t1 = min(t0 + per, tile_lo + tiles);
       // a lane's place in 16 keys' rows; the rest of an address is the wavefront's
@@ -554,11 +677,20 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Kv4AttnArgs a)
       const uint8_t* const ks = a.c.ks + row * (D / 32);
       const uint8_t* const vc = a.c.vc + row * (D / 2);
       const uint8_t* const vs = a.c.vs + row * (D / 32);
-      auto load = [&](KvTile<D>& kv, int slot) __attribute__((always_inline)) {
-        const uint8_t* const k0 = kc + (int64_t)slot * (D / 2);
-        const uint8_t* const s0 = ks + (int64_t)slot * (D / 32);
-        const uint8_t* const v0 = vc + (int64_t)slot * (D / 2);
-        const uint8_t* const t0 = vs + (int64_t)slot * (D / 32);
+      auto load = [&](KvTile<D>& kv, int at, int slot) __attribute__((always_inline)) {
+        const uint8_t* k0 = kc + (int64_t)slot * (D / 2);
+        const uint8_t* s0 = ks + (int64_t)slot * (D / 32);
+        const uint8_t* v0 = vc + (int64_t)slot * (D / 2);
+        const uint8_t* t0 = vs + (int64_t)slot * (D / 32);
+        if constexpr (TREE) {
+          if (at >= tile_lo + held) {
+            const int64_t node = (int64_t)bh * a.d.C + (at - tile_lo - held) * 32;
+            k0 = a.d.kc + node * (D / 2);
+            s0 = a.d.ks + node * (D / 32);
+            v0 = a.d.vc + node * (D / 2);
+            t0 = a.d.vs + node * (D / 32);
+          }
+        }
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           if constexpr (D == 128) {
@@ -578,18 +710,36 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Kv4AttnArgs a)
       int tile = t0 + wave;
       int slot = (int)((uint32_t)(tile * 32) % (uint32_t)C);
       auto fold = [&](const KvTile<D>& kv) __attribute__((always_inline)) {
-        const bool masked = tile * 32 < last.lo || tile * 32 + 31 > first.hi;
-        fold_tile<T, D, NT>(st, kv, q, a.c_log2, tile * 32, masked, lo, hi, first.lo, last.hi, lane);
+        if constexpr (TREE) {
+          const int node = (tile - tile_lo - held) * 32;  // the draft's first, from 0 on
+          const bool masked = node >= 0 || tile * 32 < last.lo || tile * 32 + 31 > first.hi;
+          BitMask<NT> mask = {};
+          if (masked) {
+            const int p0 = tile * 32;
+            mask.all = node >= 0 ? bits_between(0, n_new - 1 - node)
+                                 : bits_between(first.lo - p0, last.hi - p0);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mask.rows[nt] = node >= 0 ? ancestors_in(tree, (row0 + 16 * nt + n) / a.G, node >> 5,
+                                                       n_new, a.window)
+                                        : bits_between(lo[nt] - p0, hi[nt] - p0);
+          }
+          fold_tile<T, D, NT>(st, kv, q, a.c_log2, masked, mask, lane);
+        } else {
+          const bool masked = tile * 32 < last.lo || tile * 32 + 31 > first.hi;
+          const RangeMask<NT> mask = {lo, hi, tile * 32, first.lo, last.hi};
+          fold_tile<T, D, NT>(st, kv, q, a.c_log2, masked, mask, lane);
+        }
         tile += kRowWaves;
       };
       auto next = [&](KvTile<D>& kv) __attribute__((always_inline)) {
         if (tile + kRowWaves >= t1) return;
         slot += step;
         if (slot >= C) slot -= C;
-        load(kv, slot);
+        load(kv, tile + kRowWaves, slot);
       };
       KvTile<D> kv[2];
-      if (tile < t1) load(kv[0], slot);
+      if (tile < t1) load(kv[0], tile, slot);
       while (tile < t1) {
         next(kv[1]);
         fold(kv[0]);
@@ -599,6 +749,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Kv4AttnArgs a)
       }
     }
   }
+  if constexpr (TREE) __syncthreads();  // the tree is read
   // add the wavefronts
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -606,7 +757,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Kv4AttnArgs a)
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     // a row that the sequence lacks saw the tiles that nobody's mask cuts
-    const bool none = lo[nt] > hi[nt];
+    const bool none = TREE ? (row0 + 16 * nt + n) / a.G >= n_new : lo[nt] > hi[nt];
     if (quarter == 0) {
       sml[wave][16 * nt + n][0] = none ? -INFINITY : st.m[nt] - Fmt<T>::kBias;
       sml[wave][16 * nt + n][1] = none ? 0.f : l;
@@ -706,8 +857,9 @@ __device__ __forceinline__ f32x16 mfma32<_Float16>(u32x4 a, u32x4 b, f32x16 c) {
 
 constexpr int kBlockKeys = 64;
 
-template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
+template <typename T, int D, typename Args>
+__global__ __launch_bounds__(256, 2) void kv4_block_kernel(Args a) {
+  constexpr bool TREE = is_tree<Args>;
   constexpr int KS = D / 16;  // steps of 16 channels
   constexpr int MB = D / 32;  // blocks of 32 channels
   constexpr int W = D / 8;    // words of 8 channels
@@ -721,7 +873,9 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
   const int rest = blockIdx.x / a.parts;
   const int rb = rest % a.nrb, bh = rest / a.nrb;
   const int b = bh / a.c.H, h = bh - b * a.c.H;
-  const int len = length_of(a.c.len, b), n_new = count_of(a.counts, b, a.Tq);
+  const int len = length_of(a.c.len, b);
+  int n_new = count_of(a.counts, b, a.Tq);
+  if constexpr (TREE) n_new = min(n_new, length_of(a.d.len, b));
   const int row0 = rb * RB, C = a.c.C;
 
   const int row = row0 + wave * 32 + n, t = min(row / a.G, a.Tq - 1), head = h * a.G + row % a.G;
@@ -732,19 +886,33 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < KS; ++i) q[i] = *reinterpret_cast<const u32x4*>(src + 16 * i);
   }
-  const RowRange rr = row_range(row / a.G, n_new, len, C, a.window);
+  RowRange rr;
+  __shared__ std::conditional_t<TREE, TreeBits, char> tree[1];
+  if constexpr (TREE) {
+    tree_bits<256>(tree[0], a.parents + (int64_t)b * a.Tq, n_new);
+    const int node = row / a.G;
+    rr = node_range(node, n_new, tree[0].depth[min(node, kTreeNodes - 1)], len, C, a.window);
+  } else {
+    rr = row_range(row / a.G, n_new, len, C, a.window);
+  }
   float m = -INFINITY, l = 0.f;
   f32x16 o[MB];
 #pragma unroll
   for (int i = 0; i < MB; ++i) o[i] = f32x16{};
   // tiles [t0, t1) of 64 keys that the workgroup folds, and the keys that any row sees
   int t0 = 0, t1 = 0, any_lo = 0, any_hi = -1;
+  int draft = 0;  // the first tile of a tree's draft, behind the cache's
   const int t_lo = row0 / a.G, t_hi = min((row0 + RB - 1) / a.G, n_new - 1);
   if (t_lo <= t_hi) {
-    const RowRange first = row_range(t_lo, n_new, len, C, a.window);
-    const RowRange last = row_range(t_hi, n_new, len, C, a.window);
-    if (first.lo <= last.hi) {
-      const int tile_lo = first.lo / kBlockKeys, tiles = last.hi / kBlockKeys - tile_lo + 1;
+    const RowRange first = TREE ? node_range(0, n_new, 0, len, C, a.window)
+                                : row_range(t_lo, n_new, len, C, a.window);
+    const RowRange last = TREE ? node_range(0, n_new, n_new - 1, len, C, a.window)
+                               : row_range(t_hi, n_new, len, C, a.window);
+    if (TREE || first.lo <= last.hi) {
+      const int tile_lo = first.lo / kBlockKeys;
+      const int held = first.lo <= last.hi ? last.hi / kBlockKeys - tile_lo + 1 : 0;
+      const int tiles = TREE ? held + (n_new + kBlockKeys - 1) / kBlockKeys : held;
+      draft = tile_lo + held;
       const int per = (tiles + a.parts - 1) / a.parts;
       t0 = tile_lo + part * per;
       t1 = min(t0 + per, tile_lo + tiles);
@@ -758,8 +926,10 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
     const int w0 = (row0 + wave * 32) / a.G;
     const int w1 = min((row0 + wave * 32 + 31) / a.G, n_new - 1);
     if (w0 <= w1) {
-      in_lo = row_range(w1, n_new, len, C, a.window).lo;
-      in_hi = row_range(w0, n_new, len, C, a.window).hi;
+      in_lo = (TREE ? node_range(0, n_new, n_new - 1, len, C, a.window)
+                    : row_range(w1, n_new, len, C, a.window)).lo;
+      in_hi = (TREE ? node_range(0, n_new, 0, len, C, a.window)
+                    : row_range(w0, n_new, len, C, a.window)).hi;
     }
   }
 
@@ -776,9 +946,24 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
   auto slot_of = [&](int tile) __attribute__((always_inline)) {
     return (int)((uint32_t)(tile * kBlockKeys + wave * 16) % (uint32_t)C);
   };
+  // the cache that a tile lies in, and its 16 keys' row there
+  auto cache_of = [&](int tile) __attribute__((always_inline)) {
+    if constexpr (TREE) return tile >= draft ? a.d : a.c;
+    return a.c;
+  };
+  auto row_of = [&](int tile) __attribute__((always_inline)) {
+    if constexpr (TREE) {
+      // what lies behind the draft's end wraps: memory that is there, and no row sees it
+      if (tile >= draft)
+        return (int64_t)bh * a.d.C + (int)((uint32_t)((tile - draft) * kBlockKeys + wave * 16) %
+                                           (uint32_t)a.d.C);
+    }
+    return (int64_t)bh * C + slot_of(tile);
+  };
   auto load_k = [&](Codes& kc, int tile) __attribute__((always_inline)) {
-    const int64_t row = (int64_t)bh * C + slot_of(tile) + (lane & 15);
-    const uint8_t* src = a.c.kc + row * (D / 2) + kq * (D / 8);
+    const Kv4Cache from = cache_of(tile);
+    const int64_t row = row_of(tile) + (lane & 15);
+    const uint8_t* src = from.kc + row * (D / 2) + kq * (D / 8);
     if constexpr (D == 128) {
       kc.c[0] = *reinterpret_cast<const u32x4*>(src);
     } else {
@@ -786,14 +971,15 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
       kc.c[0][0] = x[0];
       kc.c[0][1] = x[1];
     }
-    kc.s[0] = a.c.ks[row * (D / 32) + kq * (D / 4) / 32];
+    kc.s[0] = from.ks[row * (D / 32) + kq * (D / 4) / 32];
   };
   auto load_v = [&](Codes& vc, int tile) __attribute__((always_inline)) {
-    const int64_t g = (((int64_t)bh * C + slot_of(tile)) >> 2) + half;
+    const Kv4Cache from = cache_of(tile);
+    const int64_t g = (row_of(tile) >> 2) + half;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      vc.c[i] = *reinterpret_cast<const u32x4*>(a.c.vc + ((g + 2 * i) * W + vw) * 16);
-      vc.s[i] = *reinterpret_cast<const uint32_t*>(a.c.vs + ((g + 2 * i) * (D / 32) + vw / 4) * 4);
+      vc.c[i] = *reinterpret_cast<const u32x4*>(from.vc + ((g + 2 * i) * W + vw) * 16);
+      vc.s[i] = *reinterpret_cast<const uint32_t*>(from.vs + ((g + 2 * i) * (D / 32) + vw / 4) * 4);
     }
   };
   auto store_k = [&](const Codes& kc, int tile) __attribute__((always_inline)) {
@@ -819,7 +1005,14 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
     scales4(vc.s[1], s + 4);
     // what no row sees may be anything, and a slot without a position is: make it
     // finite, for 0 times it to be 0
-    if (tile * kBlockKeys < any_lo || tile * kBlockKeys + kBlockKeys - 1 > any_hi) {
+    if (TREE && tile >= draft) {
+      const int i = p - draft * kBlockKeys;  // the lane's first node
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[e] = i + e < n_new ? s[e] : 0.f;
+        s[4 + e] = i + 8 + e < n_new ? s[4 + e] : 0.f;
+      }
+    } else if (tile * kBlockKeys < any_lo || tile * kBlockKeys + kBlockKeys - 1 > any_hi) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         s[e] = p + e >= any_lo && p + e <= any_hi ? s[e] : 0.f;
@@ -851,7 +1044,19 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
   // masks tile's scores and moves the reference where they exceed it by 2^8
   auto settle = [&](f32x16 (&s)[2], int tile) __attribute__((always_inline)) {
     const int p0 = tile * kBlockKeys;
-    if (p0 < in_lo || p0 + kBlockKeys - 1 > in_hi) {
+    if (TREE && tile >= draft) {
+      if constexpr (TREE) {
+        uint32_t seen[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+          seen[kb] = ancestors_in(tree[0], row / a.G, 2 * (tile - draft) + kb, n_new, a.window);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (!((seen[kb] >> (8 * (e >> 2) + 4 * half + (e & 3))) & 1)) s[kb][e] = -INFINITY;
+      }
+    } else if (p0 < in_lo || p0 + kBlockKeys - 1 > in_hi) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -904,7 +1109,8 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Kv4AttnArgs a) {
     kv4_sweep<Codes>(t0, t1, sa, sb, load_k, load_v, store_k, store_v, scores, settle, fold,
                      [] { __syncthreads(); });
 
-  const bool none = rr.lo > rr.hi;  // saw the tiles that nobody's mask cuts
+  // saw the tiles that nobody's mask cuts
+  const bool none = TREE ? row / a.G >= n_new : rr.lo > rr.hi;
   l = none ? 0.f : l + __shfl_xor(l, 32);
   m = none ? -INFINITY : m - Fmt<T>::kBias;
   const int rows = a.Tq * a.G, wrow0 = row0 + wave * 32;
@@ -1090,30 +1296,31 @@ __global__ __launch_bounds__(256) void kv4_combine_rows_kernel(Kv4AttnArgs a) {
         l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-template <typename T, int D>
-hipError_t launch_attn_typed(const Kv4AttnArgs& a, hipStream_t st) {
+template <typename T, int D, typename Args>
+hipError_t launch_attn_typed(const Args& a, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)a.parts * a.nrb * a.c.B * a.c.H));
   // codes and scales, against half of the 256 MiB of last-level cache
   const bool far = (int64_t)a.c.B * a.c.H * a.c.C * (D + D / 16) > (int64_t(128) << 20);
   const dim3 few(64 * kRowWaves);
   if (a.row_tiles == 1 && far)
-    hipLaunchKernelGGL((kv4_rows_kernel<T, D, 1, true>), grid, few, 0, st, a);
+    hipLaunchKernelGGL((kv4_rows_kernel<T, D, 1, true, Args>), grid, few, 0, st, a);
   else if (a.row_tiles == 1)
-    hipLaunchKernelGGL((kv4_rows_kernel<T, D, 1, false>), grid, few, 0, st, a);
+    hipLaunchKernelGGL((kv4_rows_kernel<T, D, 1, false, Args>), grid, few, 0, st, a);
   else if (a.row_tiles == 2 && far)
-    hipLaunchKernelGGL((kv4_rows_kernel<T, D, 2, true>), grid, few, 0, st, a);
+    hipLaunchKernelGGL((kv4_rows_kernel<T, D, 2, true, Args>), grid, few, 0, st, a);
   else if (a.row_tiles == 2)
-    hipLaunchKernelGGL((kv4_rows_kernel<T, D, 2, false>), grid, few, 0, st, a);
+    hipLaunchKernelGGL((kv4_rows_kernel<T, D, 2, false, Args>), grid, few, 0, st, a);
   else
-    hipLaunchKernelGGL((kv4_block_kernel<T, D>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((kv4_block_kernel<T, D, Args>), grid, dim3(256), 0, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.parts == 1) return e;
   const int64_t rows = (int64_t)a.c.B * a.c.H * a.G * a.Tq;
   if (a.parts <= 16 && rows >= 1024)
     hipLaunchKernelGGL((kv4_combine_rows_kernel<T, D>), dim3((unsigned)((rows + 3) / 4)),
-                       dim3(256), 0, st, a);
+                       dim3(256), 0, st, static_cast<const Kv4AttnArgs&>(a));
   else
-    hipLaunchKernelGGL((kv4_combine_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((kv4_combine_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, st,
+                       static_cast<const Kv4AttnArgs&>(a));
   return hipGetLastError();
 }
 
@@ -1696,7 +1903,88 @@ __global__ __launch_bounds__(256) void kv4_gather_kernel(Kv4EvictArgs a) {
   if (r < BL) *reinterpret_cast<uint32_t*>(a.out.vs + (gn * BL + r) * 4) = vsw;
 }
 
+// ---------------------------------------------------------------------------
+// Commit: nodes of a draft become the next positions of their sequences, bit by bit.
+// D / 8 threads a node and head: a word of its value each, and D / 32 of them 16 bytes of
+// its key and the scales. A node of 8 heads of 128 is 1088 bytes: bound by the launch.
+template <int D>
+__device__ __forceinline__ void commit_words(const Kv4CommitArgs& a, int b, int h, int len, int i,
+                                             int r) {
+  constexpr int R = D / 8, BL = D / 32;
+  const int node = min(max(a.path[(int64_t)b * a.P + i], 0), a.d.C - 1);
+  const int64_t bh = (int64_t)b * a.c.H + h;
+  const int64_t src = bh * a.d.C + node;
+  const int64_t dst = bh * a.c.C + ((uint32_t)len + (uint32_t)i) % (uint32_t)a.c.C;
+  const int es = src & 3, ed = dst & 3;
+  *reinterpret_cast<uint32_t*>(a.c.vc + (((dst >> 2) * R + r) * 4 + ed) * 4) =
+      *reinterpret_cast<const uint32_t*>(a.d.vc + (((src >> 2) * R + r) * 4 + es) * 4);
+  if (r < BL) {
+    *reinterpret_cast<u32x4*>(a.c.kc + (dst * BL + r) * 16) =
+        *reinterpret_cast<const u32x4*>(a.d.kc + (src * BL + r) * 16);
+    a.c.ks[dst * BL + r] = a.d.ks[src * BL + r];
+    a.c.vs[((dst >> 2) * BL + r) * 4 + ed] = a.d.vs[((src >> 2) * BL + r) * 4 + es];
+  }
+  if (a.weights != nullptr && r == 0) a.weights[dst] = 0.f;
+}
+
+// A sequence's lengths are written by the workgroup that has read its length, so with SMALL
+// it has all of the sequence's nodes; else they are another launch's.
+template <int D, bool SMALL>
+__global__ __launch_bounds__(SMALL ? 1024 : 256) void commit_kernel(Kv4CommitArgs a) {
+  constexpr int R = D / 8;
+  const int b = SMALL ? blockIdx.x : blockIdx.y;
+  const int len = length_of(a.c.len, b), n = count_of(a.counts, b, a.P);
+  const int items = n * a.c.H * R;
+  for (int64_t i = (SMALL ? 0 : (int64_t)blockIdx.x * 256) + threadIdx.x; i < items;
+       i += SMALL ? 1024 : (int64_t)gridDim.x * 256) {
+    const int node = (int)i / R;
+    commit_words<D>(a, b, node % a.c.H, len, node / a.c.H, (int)i % R);
+  }
+  if constexpr (SMALL) {
+    __syncthreads();  // every thread has read the length
+    if (threadIdx.x == 0) {
+      a.c.len[b] = length_after(len, n, a.c.C);
+      if (a.reset) a.d.len[b] = 0;
+    }
+  }
+}
+
+__global__ void commit_lengths_kernel(Kv4CommitArgs a) {
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b < a.c.B) {
+    a.c.len[b] = length_after(length_of(a.c.len, b), count_of(a.counts, b, a.P), a.c.C);
+    if (a.reset) a.d.len[b] = 0;
+  }
+}
+
+template <int D>
+hipError_t launch_commit_typed(const Kv4CommitArgs& a, hipStream_t st) {
+  const int64_t items = (int64_t)a.P * a.c.H * (D / 8);
+  if (items <= 8 * 1024) {
+    hipLaunchKernelGGL((commit_kernel<D, true>), dim3(a.c.B), dim3(1024), 0, st, a);
+    return hipGetLastError();
+  }
+  hipLaunchKernelGGL((commit_kernel<D, false>), dim3((unsigned)((items + 255) / 256), a.c.B),
+                     dim3(256), 0, st, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(commit_lengths_kernel, dim3((a.c.B + 255) / 256), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
 }  // namespace
+
+hipError_t launch_kv4_commit(const Kv4CommitArgs& a, hipStream_t st) {
+  return a.c.D == 128 ? launch_commit_typed<128>(a, st) : launch_commit_typed<64>(a, st);
+}
+
+hipError_t launch_kv4_tree_attn(const Kv4TreeArgs& a, Elem dtype, hipStream_t st) {
+  if (dtype == Elem::BF16)
+    return a.c.D == 128 ? launch_attn_typed<__bf16, 128>(a, st)
+                        : launch_attn_typed<__bf16, 64>(a, st);
+  return a.c.D == 128 ? launch_attn_typed<_Float16, 128>(a, st)
+                      : launch_attn_typed<_Float16, 64>(a, st);
+}
 
 hipError_t launch_kv4_append(const Kv4AppendArgs& a, Elem dtype, hipStream_t st) {
   if (dtype == Elem::BF16)

@@ -8,6 +8,9 @@
     kv4_key_weights(q, cache, lse, window)  the attention weight of each key
     kv4_evict(cache, weights, keep, recent) the cache without the least of them
     kv4_read(cache, count)                  the held values
+    kv4_tree_attn(q, cache, draft, parents) attention of a tree of drafted tokens, whose
+        own keys and values are in a second cache
+    kv4_commit(cache, draft, path, counts)  accepted ones move into the cache
 
 The reference keeps bf16 keys and values (fla's attn_state, fla/models/utils.py:
 35-96) and has no counterpart; window conventions are those of window_attn
@@ -249,20 +252,8 @@ def _operand(t: torch.Tensor):
     return t, _dense(t.shape[1], t.shape[2], t.shape[3])
 
 
-_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-
-
 def _window(window) -> int:
     return 0 if window is None or window < 0 else int(min(window, 2**31 - 1))
-
-
-def _call(cache: KV4Cache, fn, *args) -> None:
-    """fn(*args, stream) with the cache's device current: the launches go to it."""
-    if _current_device() == cache.device.index:
-        _lib.check(fn(*args, _lib.stream(cache)))
-    else:
-        with torch.cuda.device(cache.device):
-            _lib.check(fn(*args, _lib.stream(cache)))
 
 
 def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, *,
@@ -282,7 +273,7 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, *,
     if T == 0:
         return
     (k, ks), (v, vs) = _operand(k), _operand(v)
-    _call(cache, _lib.lib().ttcd_kv4_append, cache._ref, k.data_ptr(), v.data_ptr(), T,
+    _lib.call(cache, _lib.lib().ttcd_kv4_append, cache._ref, k.data_ptr(), v.data_ptr(), T,
           ks, vs, _ptr(counts),
           _ptr(cache.weights), _DT[cache.dtype])
 
@@ -299,7 +290,7 @@ def kv4_read(cache: KV4Cache, count: int) -> tuple[torch.Tensor, torch.Tensor]:
                     device=cache.device)
     v = torch.empty_like(k)
     if count:
-        _call(cache, _lib.lib().ttcd_kv4_read, cache._ref, k.data_ptr(), v.data_ptr(), count,
+        _lib.call(cache, _lib.lib().ttcd_kv4_read, cache._ref, k.data_ptr(), v.data_ptr(), count,
               _DT[cache.dtype])
     return k, v
 
@@ -327,7 +318,7 @@ def kv4_attn(q: torch.Tensor, cache: KV4Cache, window: int | None = None, *,
         L, W = _lib.lib(), _window(window)
         n = L.ttcd_kv4_attn_workspace_bytes(cache._ref, T, H, W) if split_keys else 0
         work = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-        _call(cache, L.ttcd_kv4_attn_fwd, cache._ref, q.data_ptr(), o.data_ptr(), _ptr(lse), T, H,
+        _lib.call(cache, L.ttcd_kv4_attn_fwd, cache._ref, q.data_ptr(), o.data_ptr(), _ptr(lse), T, H,
               qs, _dense(T, H, D), _ptr(counts), W, D ** -0.5,
               _DT[q.dtype], _ptr(work), n)
     return (o, lse) if return_lse else o
@@ -364,7 +355,7 @@ def kv4_key_weights(q: torch.Tensor, cache: KV4Cache, lse: torch.Tensor,
         with torch.inference_mode():
             return out if accumulate else out.zero_()
     (q, qs), lse = _operand(q), lse.contiguous()
-    _call(cache, _lib.lib().ttcd_kv4_key_weights_fwd, cache._ref, q.data_ptr(), lse.data_ptr(),
+    _lib.call(cache, _lib.lib().ttcd_kv4_key_weights_fwd, cache._ref, q.data_ptr(), lse.data_ptr(),
           out.data_ptr(), T, H, qs, _ptr(counts), _window(window),
           D ** -0.5, int(bool(accumulate)), _DT[q.dtype])
     return out
@@ -406,8 +397,85 @@ def kv4_evict(cache: KV4Cache, weights: torch.Tensor | None, keep: int, recent: 
     if (new_weights is None or _overlap(new_weights, weights)
             or _overlap(new_weights, cache.weights)):
         new_weights = torch.empty(B, H, out.capacity, dtype=torch.float32, device=cache.device)
-    _call(cache, _lib.lib().ttcd_kv4_evict, cache._ref, weights.data_ptr(), keep,
+    _lib.call(cache, _lib.lib().ttcd_kv4_evict, cache._ref, weights.data_ptr(), keep,
           min(recent, 2**31 - 1), out._ref, new_weights.data_ptr(), index.data_ptr())
     if cache.weights is not None or out.weights is not None:
         out.weights = new_weights
     return out, index, new_weights
+
+
+TREE_NODES = 256  # of a sequence, at most
+
+
+def _draft(draft, cache: KV4Cache, fn: str) -> KV4Cache:
+    if not isinstance(draft, KV4Cache):
+        raise ValueError(f"{fn}: draft must be a KV4Cache")
+    if (draft.batch != cache.batch or draft.kv_heads != cache.kv_heads
+            or draft.head_dim != cache.head_dim or draft.dtype != cache.dtype
+            or draft.device != cache.device):
+        raise ValueError(f"{fn}: draft must have the cache's batch, kv heads, head_dim, dtype and "
+                         "device")
+    return draft
+
+
+def _nodes(t, cache: KV4Cache, name: str, fn: str, n: int | None = None) -> torch.Tensor:
+    if (not isinstance(t, torch.Tensor) or t.dim() != 2 or t.shape[0] != cache.batch
+            or (n is not None and t.shape[1] != n) or t.dtype != torch.int32
+            or t.device != cache.device):
+        raise ValueError(f"{fn}: {name} must be int32 ({cache.batch}, "
+                         f"{'N' if n is None else n}) on the cache's device")
+    return t.contiguous()
+
+
+def kv4_tree_attn(q: torch.Tensor, cache: KV4Cache, draft: KV4Cache, parents: torch.Tensor,
+                  window: int | None = None, *, counts: torch.Tensor | None = None,
+                  return_lse: bool = False, split_keys: bool = True):
+    """Attention of the nodes of a tree of drafted tokens, q (B, N, H, D), N <= 256: node i
+    follows node parents[b, i] < i ((B, N) int32; -1: none) and is at position length +
+    depth, behind the cache's. It sees the cache's held keys of the `window` (None or < 0:
+    all) positions up to its own and, within those, itself and its ancestors, which `draft`
+    holds: kv4_append all nodes to an empty second cache first, node i is in its slot i
+    (counts[b] of them: the first). So a chain of nodes sees what the same tokens would
+    that kv4_append adds to the cache itself, and the cache stays as it is until kv4_commit.
+    Returns o like q, and with ``return_lse`` lse, fp32 natural-log (B, H, N); rows behind
+    the last node get o = 0 and lse = -inf. ``split_keys`` as in kv4_attn."""
+    fn = "kv4_tree_attn"
+    _draft(draft, _cache(cache, fn), fn)
+    _rows(q, cache, "q", fn, None)
+    counts = _counts(counts, cache, fn)
+    if window is not None and window == 0:
+        raise ValueError(f"{fn}: window must be >= 1, or None / < 0 for none")
+    B, N, H, D = q.shape
+    parents = _nodes(parents, cache, "parents", fn, N)
+    if N > TREE_NODES or N > draft.capacity:
+        raise ValueError(f"{fn}: {N} nodes, need at most {min(TREE_NODES, draft.capacity)} (a "
+                         f"draft's capacity, and {TREE_NODES})")
+    q, qs = _operand(q)
+    o = torch.empty(B, N, H, D, dtype=q.dtype, device=q.device)
+    lse = torch.empty(B, H, N, dtype=torch.float32, device=q.device) if return_lse else None
+    if N > 0:
+        L, W = _lib.lib(), _window(window)
+        n = L.ttcd_kv4_tree_attn_workspace_bytes(cache._ref, N, H, W) if split_keys else 0
+        work = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        _lib.call(cache, L.ttcd_kv4_tree_attn_fwd, cache._ref, draft._ref, q.data_ptr(),
+                  o.data_ptr(), _ptr(lse), N, H, qs, _dense(N, H, D), parents.data_ptr(),
+                  _ptr(counts), W, D ** -0.5, _DT[q.dtype], _ptr(work), n)
+    return (o, lse) if return_lse else o
+
+
+def kv4_commit(cache: KV4Cache, draft: KV4Cache, path: torch.Tensor,
+               counts: torch.Tensor | None = None, *, reset: bool = False) -> None:
+    """The draft's slots path[b, :counts[b]] ((B, P) int32; counts None: all P) become the
+    next positions of sequence b, the same bits, and its lengths count them. path's other
+    entries may be anything. P at most the capacity of either. ``reset``: the draft is
+    empty afterwards."""
+    fn = "kv4_commit"
+    _draft(draft, _cache(cache, fn), fn)
+    path = _nodes(path, cache, "path", fn)
+    counts = _counts(counts, cache, fn)
+    P = path.shape[1]
+    if P < 1 or P > min(cache.capacity, draft.capacity):
+        raise ValueError(f"{fn}: need 1 to {min(cache.capacity, draft.capacity)} nodes (the "
+                         f"capacities), got {P}")
+    _lib.call(cache, _lib.lib().ttcd_kv4_commit, cache._ref, draft._ref, path.data_ptr(),
+              _ptr(counts), P, _ptr(cache.weights), int(bool(reset)))
