@@ -123,6 +123,20 @@ def test_the_least_and_largest_numbers(gpu):
                 _check(x, u, **kw)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_zero_without_a_sign_alone_and_nan_above_all(gpu, dtype):
+    x = -_logits(4, 6, 3001, dtype).abs() - 0.5
+    x[0, 5::7] = -0.0
+    x[1, 17] = -0.0
+    x[2, 100] = NAN
+    x[3] = NAN
+    x[3, 2999] = -2.0
+    x[4, ::2] = -NAN
+    x[5, 1:] = NAN
+    for kw in (dict(), dict(top_k=9), dict(top_p=0.5), dict(min_p=0.9), dict(temperature=0)):
+        _check(x, _uniform(2, 6), **kw)
+
+
 def test_ties_go_to_the_lower_index(gpu):
     x = torch.zeros(12, 24, dtype=BF)
     x[:, 3::4] = 1.0

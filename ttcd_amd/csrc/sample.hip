@@ -11,8 +11,15 @@
 // every value that occurs, in 64 bits, as are all sums. Counting is exact in any order, so
 // a row's token does not depend on how its sums are laid out. A workgroup takes a row: it
 // counts the values in LDS (16 bits a count, 128 KiB), finds the last kept value and the
-// drawn one with how many of its tokens come before the drawn token, and reads the row
-// again for the token itself.
+// drawn one with how many of its tokens come before the drawn token, and looks for that
+// one in the row, most of which is still in registers.
+//
+// Of a row of 151936 bf16 logits alone (25 us on a CU): zeroing 0.8 us, counting 12.2 (LDS
+// atomics: 11 cycles for 64 tokens), sums of the values' weights 4.9 (f16, whose rows have
+// 8 times the values, 14.7: 64-bit arithmetic), cuts and draw 3.7 (one wavefront's
+// latencies), the token 2.6. 256 rows, 78 MB: 33 us, of which counting, at the rate of the
+// memory (4.4 TB/s), is 17.6. Reading the row again for the token took 9.3 of 256 rows and
+// 3.5 of one; the order of a value taken while counting, instead of its bits, 4 more.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -23,94 +30,129 @@ namespace ttcd {
 namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef int16_t s16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kSampleThreads = 1024;
 constexpr int kSampleWaves = kSampleThreads / 64;
 constexpr int kBlocks = 512;     // of 128 values, 64 words of 2 counts
-constexpr int kHeavy = 8192;     // a count above this moves to the list
-constexpr int kHeavyMost = kSampleVocab / kHeavy;
+constexpr int kBlocksWave = kBlocks / kSampleWaves;
+constexpr uint32_t kHeavy = 8192;  // a count of this and more moves to the list
+constexpr uint32_t kHeavyBits = (0x10000u - kHeavy) * 0x10001u;  // that such a count has some of
+constexpr int kHeavyMost = kSampleVocab / kHeavy + 1;
+// Vectors of a thread between two looks at the counts: 7 turns of 1024 of them, with what a
+// count may have by then, are below 65536.
+constexpr int kStretch = 7;
+constexpr int kHeld = 2 * kStretch;  // that stay in registers
+constexpr int kTurnsMost = kSampleVocab / 8 / kSampleThreads + 1;
 
-// The order of a 16-bit value, the largest (infinity) 0, those up to kLast numbers above
-// -infinity, then -infinity and NaN.
+// The order of a 16-bit value is 0x7fff less its bits, of a negative one its bits: the
+// largest come first. Infinity is kFirst, the last number above -infinity kLast; outside of
+// those lie -infinity and NaN.
+constexpr uint32_t kZero = 0x7fff;  // the order of +0; that of -0 is the next
 template <typename T>
 struct Order;
 template <>
 struct Order<__bf16> {
-  static constexpr uint32_t kInf = 0x7f80;
+  static constexpr uint32_t kFirst = 0x7fff - 0x7f80, kLast = 0x7fff + 0x7f80;
 };
 template <>
 struct Order<_Float16> {
-  static constexpr uint32_t kInf = 0x7c00;
+  static constexpr uint32_t kFirst = 0x7fff - 0x7c00, kLast = 0x7fff + 0x7c00;
 };
-template <typename T>
-constexpr uint32_t first_of() { return 0x7fffu - Order<T>::kInf; }  // before the shift
-template <typename T>
-constexpr uint32_t last_of() { return 0x7fffu + Order<T>::kInf - first_of<T>(); }
-template <typename T>
-constexpr uint32_t zero_of() { return 0x7fffu - first_of<T>(); }  // of +0; -0 is the next
-
-// Both halves of a word. A positive value's bits turn around below 0x7fff, a negative one's
-// are in order as they are.
-template <typename T>
-__device__ __forceinline__ uint32_t order_pair(uint32_t x) {
-  const uint32_t sign = (x >> 15) & 0x00010001u;
-  const uint32_t o = x ^ ((sign << 15) - sign) ^ 0x7fff7fffu;
-  constexpr uint32_t f = first_of<T>();
-  // halves apart: the lower one's borrow stays its own
-  return ((o - (f << 16)) & 0xffff0000u) | ((o - f) & 0xffffu);
+__device__ __forceinline__ uint32_t bits_of(uint32_t order) {
+  return order <= kZero ? kZero - order : order;
 }
-
-// The value of an order.
 template <typename T>
 __device__ __forceinline__ double value_of(uint32_t order) {
-  const uint32_t o = order + first_of<T>();
-  const uint16_t bits = (uint16_t)(o < 0x8000u ? o ^ 0x7fffu : o);
-  return (double)static_cast<float>(__builtin_bit_cast(T, bits));
+  return (double)static_cast<float>(__builtin_bit_cast(T, (uint16_t)bits_of(order)));
 }
 
+// Lanes of a row of 16 by N before (0 where there is none) or around.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xf, 0xf, true);
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint64_t lo = dpp<CTRL>((uint32_t)u), hi = dpp<CTRL>((uint32_t)(u >> 32));
+  return __builtin_bit_cast(double, hi << 32 | lo);
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t x, int lane) {
+  return __builtin_amdgcn_readlane(x, lane);
+}
+__device__ __forceinline__ double lane_of(double x, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint64_t lo = lane_of((uint32_t)u, lane), hi = lane_of((uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, hi << 32 | lo);
+}
 // Sums over the lanes before this one (all: over all of them).
 template <typename V>
 __device__ __forceinline__ V scan_before(V x, int lane, V* all = nullptr) {
-  V sum = x;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const V o = __shfl_up(sum, d);
-    if (lane >= d) sum += o;
-  }
-  if (all != nullptr) *all = __shfl(sum, 63);
-  const V before = __shfl_up(sum, 1);
-  return lane == 0 ? V(0) : before;
+  x += dpp<0x111>(x);  // row_shr:1, 2, 4, 8
+  x += dpp<0x112>(x);
+  x += dpp<0x114>(x);
+  x += dpp<0x118>(x);
+  const V a = lane_of(x, 15), b = a + lane_of(x, 31), c = b + lane_of(x, 47);
+  if (all != nullptr) *all = c + lane_of(x, 63);
+  return dpp<0x111>(x) + (lane < 16 ? V(0) : lane < 32 ? a : lane < 48 ? b : c);
+}
+template <typename V>
+__device__ __forceinline__ V sum_of(V x) {
+  x += dpp<0x121>(x);  // row_ror:1, 2, 4, 8
+  x += dpp<0x122>(x);
+  x += dpp<0x124>(x);
+  x += dpp<0x128>(x);
+  return lane_of(x, 0) + lane_of(x, 16) + (lane_of(x, 32) + lane_of(x, 48));
 }
 
-template <typename T>
 struct Row {
-  uint32_t* hist;       // [32768] counts of orders 2 i and 2 i + 1
-  double* sums;         // [kBlocks] of weights before a block of 128 orders, ..
-  double* block;        // .. and of its own
+  uint32_t* hist;       // [32768] counts of the values of bits 2 i and 2 i + 1
+  double* sums;         // [kBlocks] of weights up to and with a block of 128 orders
   uint32_t* counts;     // the same of tokens
-  uint32_t* tokens;
+  uint32_t* tokens;     // of the block alone
   uint32_t* heavy;      // [2 kHeavyMost] order, count
-  uint32_t nheavy;
-  double top, t;        // the highest logit, and the temperature
+  uint32_t nheavy, first, last;  // kFirst, kLast
+  const double* powers; // [64] of 2^(i / 64)
+  double top, per_t;    // the highest logit, and 1 / temperature
 
-  __device__ __forceinline__ double weight(uint32_t order) const {
-    const double x = value_of<T>(order);
-    return x == top ? 1.0 : exp((x - top) / t);
+  // exp(y), y <= 0: 2^(k / 64) times the exponential of what is left, at most ln 2 / 128, by
+  // its series up to the fifth power (the sixth is below 2^-54; what ln 2 / 64 lacks in 53
+  // bits is worth 2^-55 |y|).
+  __device__ __forceinline__ double weight_at(double x) const {
+    if (top > 1e300) return x == top ? 1.0 : 0.0;  // infinity
+    const double y = fmax((x - top) * per_t, -800.0);  // 0 from there on
+    const double k = rint(y * 92.332482616893656877);  // 64 / ln 2
+    const double r = fma(-k, 0.010830424696249145, y);
+    double e = fma(r, 1.0 / 120, 1.0 / 24);
+    e = fma(e, r, 1.0 / 6);
+    e = fma(e, r, 0.5);
+    e = fma(e, r, 1.0);
+    const int n = (int)k;
+    const double p = powers[n & 63];
+    return ldexp(fma(p * r, e, p), n >> 6);
   }
-  // The counts of the orders 2 i and 2 i + 1, 0 for what is no number.
-  __device__ __forceinline__ void count(int i, uint32_t* c0, uint32_t* c1) const {
-    const uint32_t w = hist[i];
+  template <typename T>
+  __device__ __forceinline__ double weight(uint32_t order) const {
+    return weight_at(value_of<T>(order));
+  }
+  // The word of the counts of orders 2 i (in the low half) and 2 i + 1.
+  __device__ __forceinline__ uint32_t word(int i) const {
+    const uint32_t w = hist[i <= (int)kZero / 2 ? kZero / 2 - i : i];
+    return i <= (int)kZero / 2 ? w << 16 | w >> 16 : w;
+  }
+  // Those counts, 0 for what is no number.
+  __device__ __forceinline__ void count(uint32_t w, uint32_t order, uint32_t* c0,
+                                        uint32_t* c1) const {
     uint32_t a = w & 0xffffu, b = w >> 16;
+#pragma unroll 1
     for (uint32_t j = 0; j < nheavy; ++j) {
-      if (heavy[2 * j] == 2u * i) a += heavy[2 * j + 1];
-      if (heavy[2 * j] == 2u * i + 1) b += heavy[2 * j + 1];
+      if (heavy[2 * j] == order) a += heavy[2 * j + 1];
+      if (heavy[2 * j] == order + 1) b += heavy[2 * j + 1];
     }
-    if (2 * i == (int)zero_of<T>()) {  // -0 is 0
-      a += b;
-      b = 0;
-    }
-    *c0 = 2u * i <= last_of<T>() ? a : 0;
-    *c1 = 2u * i + 1 <= last_of<T>() ? b : 0;
+    *c0 = order >= first && order <= last ? a : 0;
+    *c1 = order + 1 >= first && order + 1 <= last ? b : 0;
   }
 };
 
@@ -123,22 +165,21 @@ struct Place {
   double weight;    // of one
 };
 
-// The first value that comes and, with its own tokens, reaches what is asked for, of those
-// up to `limit`, which comes itself (limit if none does): by tokens, by the sum of weights,
-// or by more than the sum. One wavefront.
+// The first value that comes and, with its own tokens, reaches what is asked for (the last
+// up to `limit` if none does): by tokens, by the sum of weights, or by more than the sum.
+// One wavefront. first, last: blocks, of which limit's is the last or comes after it.
 enum class By { Tokens, Sum, More };
 template <typename T>
-__device__ __forceinline__ Place find(const Row<T>& row, By by, uint32_t rank, double sum,
-                                      uint32_t limit, int lane) {
+__device__ __forceinline__ Place find(const Row& row, By by, uint32_t rank, double sum,
+                                      uint32_t limit, int first, int last, int lane) {
   auto reached = [&](uint32_t r, double s) __attribute__((always_inline)) {
     return by == By::Tokens ? r >= rank : by == By::Sum ? s >= sum : s > sum;
   };
-  int blk = limit >> 7;
-  for (int b0 = 0; b0 < (int)(limit >> 7); b0 += 64) {
-    const int b = b0 + lane;
-    const uint32_t n = row.tokens[b];
-    const bool hit = b < (int)(limit >> 7) && n > 0 &&
-                     reached(row.counts[b] + n, row.sums[b] + row.block[b]);
+  last = min(last, (int)(limit >> 7));
+  int blk = last;
+  for (int b0 = first; b0 < last; b0 += 64) {
+    const int b = min(b0 + lane, kBlocks - 1);
+    const bool hit = b0 + lane < last && row.tokens[b] > 0 && reached(row.counts[b], row.sums[b]);
     const uint64_t hits = __ballot(hit);
     if (hits != 0) {
       blk = b0 + __builtin_ctzll(hits);
@@ -146,25 +187,27 @@ __device__ __forceinline__ Place find(const Row<T>& row, By by, uint32_t rank, d
     }
   }
   uint32_t c0, c1;
-  row.count(blk * 64 + lane, &c0, &c1);
   const uint32_t o0 = blk * 128 + 2 * lane;
+  row.count(row.word(blk * 64 + lane), o0, &c0, &c1);
   if (o0 > limit) c0 = 0;
   if (o0 + 1 > limit) c1 = 0;
-  const double w0 = c0 ? row.weight(o0) : 0.0, w1 = c1 ? row.weight(o0 + 1) : 0.0;
-  const uint32_t r0 = row.counts[blk] + scan_before<uint32_t>(c0 + c1, lane);
-  const double s0 = row.sums[blk] + scan_before<double>(c0 * w0 + c1 * w1, lane);
+  const double w0 = row.weight<T>(o0), w1 = row.weight<T>(o0 + 1);
+  const uint32_t r0 = (blk == 0 ? 0 : row.counts[blk - 1]) + scan_before<uint32_t>(c0 + c1, lane);
+  const double s0 =
+      (blk == 0 ? 0.0 : row.sums[blk - 1]) +
+      scan_before<double>((c0 ? c0 * w0 : 0.0) + (c1 ? c1 * w1 : 0.0), lane);
   const uint32_t r1 = r0 + c0;
-  const double s1 = s0 + c0 * w0;
+  const double s1 = s0 + (c0 ? c0 * w0 : 0.0);
   const bool hit0 = c0 && reached(r1, s1), hit1 = c1 && reached(r1 + c1, s1 + c1 * w1);
   const uint64_t hits = __ballot(hit0 || hit1), there = __ballot(c0 || c1);
-  const int at = hits != 0 ? __builtin_ctzll(hits) : 63 - __builtin_clzll(there);
+  const int at = hits != 0 ? __builtin_ctzll(hits) : there != 0 ? 63 - __builtin_clzll(there) : 0;
   const bool second = hits != 0 ? !hit0 : c1 != 0;  // in the lane that counts
   Place p;
-  p.order = __shfl(second ? o0 + 1 : o0, at);
-  p.count = __shfl(second ? c1 : c0, at);
-  p.before = __shfl(second ? s1 : s0, at);
-  p.rank = __shfl(second ? r1 : r0, at);
-  p.weight = __shfl(second ? w1 : w0, at);
+  p.order = lane_of(second ? o0 + 1 : o0, at);
+  p.count = lane_of(second ? c1 : c0, at);
+  p.before = lane_of(second ? s1 : s0, at);
+  p.rank = lane_of(second ? r1 : r0, at);
+  p.weight = lane_of(second ? w1 : w0, at);
   return p;
 }
 
@@ -181,16 +224,22 @@ struct Span {
 template <typename T>
 __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
   __shared__ __attribute__((aligned(16))) uint32_t hist[32768];
-  __shared__ double sums[kBlocks], block[kBlocks];
+  __shared__ double sums[kBlocks], powers[64];
   __shared__ uint32_t counts[kBlocks], ntok[kBlocks];
-  __shared__ uint32_t heavy[2 * kHeavyMost], nheavy, best;
-  __shared__ uint32_t drawn, skip, many, seen[kSampleWaves];
+  __shared__ uint32_t heavy[2 * kHeavyMost], nheavy, least;
+  __shared__ int most;
+  __shared__ uint32_t drawn, skip, many, seen[kTurnsMost * kSampleWaves];
+  constexpr uint32_t kFirst = Order<T>::kFirst, kLast = Order<T>::kLast;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = blockIdx.x, V = a.V;
   const uint16_t* row = static_cast<const uint16_t*>(a.logits) + r * a.st;
   const Span span(row, V);
-  const u32x4* body = reinterpret_cast<const u32x4*>(row + span.head);
+  // the i-th vector
+  const char* const body_at = reinterpret_cast<const char*>(row + span.head);
+  auto body = [&](int i) __attribute__((always_inline)) {
+    return *reinterpret_cast<const u32x4*>(body_at + (uint32_t)i * 16u);
+  };
   const int rest = V - 8 * span.vectors;  // elements outside of the vectors
   // the i-th of those
   auto loose = [&](int i) __attribute__((always_inline)) {
@@ -200,66 +249,127 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     *reinterpret_cast<u32x4*>(hist + 4 * (i * kSampleThreads + tid)) = u32x4{0u, 0u, 0u, 0u};
+  if (tid < 64) powers[tid] = exp2(tid / 64.0);
   if (tid == 0) {
     nheavy = 0;
-    best = 0xffffu;
+    least = 0xffffu;
+    most = -0x8000;
   }
   __syncthreads();
 
-  // Count. No count passes 65535: a stretch ends before one can, and those above kHeavy
-  // then move to the list.
-  uint32_t least = 0xffffu;
-  auto add = [&](uint32_t o) __attribute__((always_inline)) {
-    atomicAdd(hist + (o >> 1), 1u + (o & 1u) * 0xffffu);
-    least = min(least, o);
+  // Count, by bits. No count passes 65535: a stretch ends before one can, and those of
+  // kHeavy and more then move to the list. The highest number is the highest of the bits as
+  // signed 16-bit numbers, or the lowest without a sign if all are negative.
+  u16x2 lowest = {0xffff, 0xffff};
+  s16x2 highest = {-0x8000, -0x8000};
+  auto add = [&](uint32_t at, uint32_t odd) __attribute__((always_inline)) {
+    atomicAdd(reinterpret_cast<uint32_t*>(reinterpret_cast<char*>(hist) + at), odd * 0xffffu + 1u);
   };
   auto add_pair = [&](uint32_t x) __attribute__((always_inline)) {
-    const uint32_t o = order_pair<T>(x);
-    add(o & 0xffffu);
-    add(o >> 16);
+    add((x << 1) & 0x1fffcu, x & 1u);
+    add((x >> 15) & 0x1fffcu, (x >> 16) & 1u);
+    lowest = __builtin_elementwise_min(lowest, __builtin_bit_cast(u16x2, x));
+    highest = __builtin_elementwise_max(highest, __builtin_bit_cast(s16x2, x));
   };
-  if (tid < rest) add(order_pair<T>(row[loose(tid)]) & 0xffffu);
-  int done = rest, from = 0;  // elements since the last look, and vectors
-  while (from < span.vectors) {
-    const int to = min(span.vectors, from + (65535 - done) / 8);
-    for (int i = from + tid; i < to; i += kSampleThreads) {
-      const u32x4 x = body[i];
+  auto add_vector = [&](const u32x4& v) __attribute__((always_inline)) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) add_pair(x[j]);
-    }
-    from = to;
-    done = kHeavy;
-    if (from < span.vectors) {
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int at = 4 * (i * kSampleThreads + tid);
-        const u32x4 w = *reinterpret_cast<const u32x4*>(hist + at);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t lo = w[e] & 0xffffu, hi = w[e] >> 16;
-          if (lo <= kHeavy && hi <= kHeavy) continue;
-          if (lo > kHeavy) {
-            const uint32_t j = atomicAdd(&nheavy, 1u);
-            heavy[2 * j] = 2 * (at + e);
-            heavy[2 * j + 1] = lo;
-          }
-          if (hi > kHeavy) {
-            const uint32_t j = atomicAdd(&nheavy, 1u);
-            heavy[2 * j] = 2 * (at + e) + 1;
-            heavy[2 * j + 1] = hi;
-          }
-          hist[at + e] = (lo > kHeavy ? 0u : lo) | (hi > kHeavy ? 0u : hi << 16);
-        }
+    for (int e = 0; e < 4; ++e) add_pair(v[e]);
+  };
+  auto look = [&]() {
+    __syncthreads();
+#pragma unroll 1
+    for (int at = 4 * tid; at < 32768; at += 4 * kSampleThreads) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(hist + at);
+      if (((w[0] | w[1] | w[2] | w[3]) & kHeavyBits) == 0) continue;
+      for (int i = 0; i < 8; ++i) {  // the counts of 8 values
+        const uint32_t word = hist[at + i / 2], n = i % 2 ? word >> 16 : word & 0xffffu;
+        if (n < kHeavy) continue;
+        const uint32_t bits = 2 * at + i, j = atomicAdd(&nheavy, 1u);
+        heavy[2 * j] = bits < 0x8000u ? kZero - bits : bits;
+        heavy[2 * j + 1] = n;
+        hist[at + i / 2] = i % 2 ? word & 0xffffu : word & 0xffff0000u;
       }
-      __syncthreads();
     }
+    __syncthreads();
+  };
+  if (tid < rest) {
+    const uint32_t x = row[loose(tid)];
+    add((x << 1) & 0x1fffcu, x & 1u);
+    const uint32_t both = x | x << 16;
+    lowest = __builtin_elementwise_min(lowest, __builtin_bit_cast(u16x2, both));
+    highest = __builtin_elementwise_max(highest, __builtin_bit_cast(s16x2, both));
+  }
+  // the row's first vectors stay in registers (a turn that the row does not reach: the first)
+  u32x4 held[kHeld];
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j) {
+    const int i = j * kSampleThreads + tid;
+    held[j] = span.vectors > 0 ? body(i < span.vectors ? i : 0) : u32x4{};
   }
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) least = min(least, (uint32_t)__shfl_xor((int)least, d));
-  if (lane == 0) atomicMin(&best, least);
+  for (int j = 0; j < kHeld; ++j) {
+    if (j == kStretch && span.vectors > j * kSampleThreads) look();
+    if (j * kSampleThreads + tid < span.vectors) add_vector(held[j]);
+  }
+  for (int from = kHeld * kSampleThreads; from < span.vectors; from += kStretch * kSampleThreads) {
+    u32x4 x[kStretch];
+#pragma unroll
+    for (int j = 0; j < kStretch; ++j)
+      x[j] = body(min(from + j * kSampleThreads + tid, span.vectors - 1));
+    look();
+#pragma unroll
+    for (int j = 0; j < kStretch; ++j)
+      if (from + j * kSampleThreads + tid < span.vectors) add_vector(x[j]);
+  }
+  {
+    uint32_t lo = min((uint32_t)lowest[0], (uint32_t)lowest[1]);
+    int hi = max((int)highest[0], (int)highest[1]);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      lo = min(lo, (uint32_t)__shfl_xor((int)lo, d));
+      hi = max(hi, __shfl_xor(hi, d));
+    }
+    if (lane == 0) {
+      atomicMin(&least, lo);
+      atomicMax(&most, hi);
+    }
+  }
   __syncthreads();
-  if (best > last_of<T>()) {  // no number above -infinity
+  // -0 counts as 0: its count, to that of 0, or to the list where that could pass 65535
+  if (tid == 0) {
+    for (uint32_t j = 0; j < nheavy; ++j)
+      if (heavy[2 * j] == kZero + 1) heavy[2 * j] = kZero;
+    const uint32_t w = hist[0x4000], z = hist[0], n = w & 0xffffu;
+    if (n > 0) {
+      hist[0x4000] = w & 0xffff0000u;
+      if (n + (z & 0xffffu) <= 0xffffu) {
+        hist[0] = z + n;
+      } else {
+        heavy[2 * nheavy] = kZero;
+        heavy[2 * nheavy + 1] = n;
+        ++nheavy;
+      }
+    }
+  }
+  __syncthreads();
+
+  Row x = {hist, sums, counts, ntok, heavy, 0, kFirst, kLast, powers, 0.0, 0.0};
+  x.nheavy = __builtin_amdgcn_readfirstlane(nheavy);
+  uint32_t best = most >= 0 ? kZero - most : least;
+  if (best < kFirst) {  // a NaN: the first number there is
+    uint32_t first = 0xffffu;
+    for (int i = lane; i < 32768; i += 64) {
+      uint32_t c0, c1;
+      x.count(x.word(i), 2 * i, &c0, &c1);
+      first = min(first, c0 ? 2u * i : c1 ? 2u * i + 1 : 0xffffu);
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) first = min(first, (uint32_t)__shfl_xor((int)first, d));
+    best = first;
+  }
+  if (best == kZero + 1) best = kZero;
+  best = __builtin_amdgcn_readfirstlane(best);
+  if (best > kLast) {  // no number above -infinity
     if (tid == 0) {
       a.tokens[r] = -1;
       if (a.logprobs != nullptr) a.logprobs[r] = -INFINITY;
@@ -275,49 +385,74 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
     t = 1.0;
     top_k = 1;
   }
-  Row<T> x = {hist, sums, block, counts, ntok, heavy, nheavy, value_of<T>(best), t};
-  for (int b = wave; b < kBlocks; b += kSampleWaves) {
-    uint32_t c0, c1;
-    x.count(b * 64 + lane, &c0, &c1);
-    uint32_t n = 0;
-    double s = 0.0;
-    if (__any(c0 + c1 > 0)) {
-      n = c0 + c1;
-      if (c0) s = c0 * x.weight(b * 128 + 2 * lane);
-      if (c1) s += c1 * x.weight(b * 128 + 2 * lane + 1);
+  x.top = value_of<T>(best);
+  x.per_t = 1.0 / t;
+  const int first = best >> 7;
+  // Sums of blocks, in turns of the wavefronts. First which there are, by 8 words at once.
+  auto block_of = [&](int j) __attribute__((always_inline)) { return j * kSampleWaves + wave; };
+  uint32_t some = x.nheavy > 0 ? 0xffffffffu : 0u;
+#pragma unroll 1
+  for (int j0 = 0; j0 < kBlocksWave; j0 += 8) {
+    uint32_t w[8];
 #pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        n += __shfl_xor(n, d);
-        s += __shfl_xor(s, d);
-      }
-    }
+    for (int j = 0; j < 8; ++j) w[j] = x.word(block_of(j0 + j) * 64 + lane);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) some |= (__ballot(w[j] != 0) != 0 ? 1u : 0u) << (j0 + j);
+  }
+  // A block's values are a step apart, so a weight's quotient to the next is the block's: lane
+  // j has that of the wavefront's j-th. (No other number shares infinity's block.)
+  const uint32_t begin = block_of(lane % kBlocksWave) * 128;
+  const double step = exp((value_of<T>(begin + 1) - value_of<T>(begin)) * x.per_t);
+  if (lane < kBlocksWave) {
+    ntok[block_of(lane)] = 0;
+    sums[block_of(lane)] = 0.0;
+  }
+  while (some != 0) {
+    const int j = __builtin_ctz(some), b = block_of(j);
+    some &= some - 1;
+    const uint32_t o = b * 128 + 2 * lane;
+    uint32_t c0, c1;
+    x.count(x.word(o / 2), o, &c0, &c1);
+    const double w0 = x.weight<T>(o);
+    const double w1 = o + 1 == best ? 1.0 : w0 * lane_of(step, j);  // what weighs 1 does exactly
+    const uint32_t n = sum_of(c0 + c1);
+    const double s = sum_of((c0 ? c0 * w0 : 0.0) + (c1 ? c1 * w1 : 0.0));
     if (lane == 0) {
       ntok[b] = n;
-      block[b] = s;
+      sums[b] = s;
     }
   }
   __syncthreads();
   if (wave == 0) {
-    uint32_t all = 0;
-    double total = 0.0;
-    for (int b0 = 0; b0 < kBlocks; b0 += 64) {
-      uint32_t n;
-      double s;
-      const uint32_t nb = all + scan_before<uint32_t>(ntok[b0 + lane], lane, &n);
-      const double sb = total + scan_before<double>(block[b0 + lane], lane, &s);
-      counts[b0 + lane] = nb;
-      sums[b0 + lane] = sb;
-      all += n;
-      total += s;
+    // running sums over the blocks, 8 a lane
+    constexpr int PER = kBlocks / 64;
+    uint32_t n[PER], all = 0, bits = 0;
+    double s[PER], total = 0.0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      n[i] = ntok[PER * lane + i];
+      s[i] = sums[PER * lane + i];
+      bits |= (n[i] > 0 ? 1u : 0u) << i;
+      all = n[i] += all;
+      total = s[i] += total;
     }
+    const uint32_t before_n = scan_before<uint32_t>(all, lane, &all);
+    const double before_s = scan_before<double>(total, lane, &total);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      counts[PER * lane + i] = n[i] + before_n;
+      sums[PER * lane + i] = s[i] + before_s;
+    }
+    const int end = 63 - __builtin_clzll(__ballot(bits != 0));  // the last lane with tokens
+    const int final = PER * end + 31 - __builtin_clz(lane_of(bits, end));  // and block
     // The kept tokens end in the value `last`, with `ends` of its own; their sum is total.
     // One cut after the other, then the draw (a loop, for find to be there once).
-    uint32_t last = last_of<T>(), ends = 0;
+    uint32_t last = kLast, ends = 0xffffffffu;
     Place p = {};
     double want = 0.0;
-    enum { kAll, kTopK, kTopP, kMinP, kDraw, kStages };
+    enum { kTopK, kTopP, kMinP, kDraw, kStages };
 #pragma unroll 1
-    for (int stage = kAll; stage < kStages; ++stage) {
+    for (int stage = kTopK; stage < kStages; ++stage) {
       By by = By::Tokens;
       uint32_t rank = all;
       if (stage == kTopK) {
@@ -333,24 +468,23 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
         uint32_t lo = best;
         for (uint32_t step = 1024; step > 0; step = step == 1024 ? 16 : step == 16 ? 1 : 0) {
           const uint32_t o = lo + step * (lane + 1);
-          lo += step * (uint32_t)__popcll(__ballot(o <= last_of<T>() && x.weight(o) >= min_p));
+          const bool in = o <= kLast && x.weight<T>(min(o, kLast)) >= min_p;
+          lo += step * (uint32_t)__popcll(__ballot(in));
         }
         if (lo >= last) continue;
         uint32_t c0, c1;
-        x.count((lo >> 7) * 64 + lane, &c0, &c1);
         const uint32_t o0 = (lo & ~127u) + 2 * lane;
-        rank = (o0 <= lo ? c0 : 0) + (o0 + 1 <= lo ? c1 : 0);
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) rank += __shfl_xor(rank, d);
-        rank += counts[lo >> 7];
+        x.count(x.word(o0 / 2), o0, &c0, &c1);
+        rank = sum_of((o0 <= lo ? c0 : 0) + (o0 + 1 <= lo ? c1 : 0));
+        if (lo >= 128) rank += counts[(lo >> 7) - 1];
       } else if (stage == kDraw) {
         by = By::More;
         want = (double)a.uniform[r] * total;
       }
-      p = find<T>(x, by, rank, want, last, lane);
+      p = find<T>(x, by, rank, want, last, first, final, lane);
       uint32_t m = rank - p.rank;
       if (stage == kTopP) {
-        const uint32_t most = p.order == last ? ends : p.count;
+        const uint32_t most = p.order == last ? min(ends, p.count) : p.count;
         const double need = ceil((want - p.before) / p.weight);
         m = need < 1.0 ? 1u : need < (double)most ? (uint32_t)need : most;
         // the quotient is rounded: the least m by the sums themselves
@@ -363,7 +497,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
         total = p.before + m * p.weight;
       }
     }
-    const uint32_t mine = p.order == last ? ends : p.count;
+    const uint32_t mine = p.order == last ? min(ends, p.count) : p.count;
     const double j = floor((want - p.before) / p.weight);
     uint32_t at = j < 1.0 ? 0u : j < (double)mine ? (uint32_t)j : mine - 1;
     if (at > 0 && p.before + at * p.weight > want) --at;
@@ -377,70 +511,95 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
   }
   __syncthreads();
 
-  // The skip-th token of the drawn value. -0 counts as 0.
-  const uint32_t want = drawn;
-  uint32_t left = skip;
-  const bool zero = want == zero_of<T>();
-  auto is = [&](uint32_t o) __attribute__((always_inline)) {
-    return o == want || (zero && o == want + 1);
+  // The skip-th token of the drawn value, of either zero for 0.
+  const uint32_t pattern = drawn == kZero ? 0u : bits_of(drawn);
+  const uint32_t keep = drawn == kZero ? 0x7fffu : 0xffffu;
+  const uint32_t pattern2 = pattern * 0x10001u, keep2 = keep * 0x10001u;
+  auto is = [&](uint32_t bits) __attribute__((always_inline)) { return (bits & keep) == pattern; };
+  // bits 15 and 31: whether the halves are the pattern
+  auto equal = [&](uint32_t w) __attribute__((always_inline)) {
+    const uint32_t z = (w & keep2) ^ pattern2;
+    return ~(((z & 0x7fff7fffu) + 0x7fff7fffu) | z | 0x7fff7fffu);
   };
-  // bit i: element i of a vector
+  // which elements of a vector, a bit each
   auto matches = [&](const u32x4& v) __attribute__((always_inline)) {
     uint32_t m = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t o = order_pair<T>(v[j]);
-      m |= (is(o & 0xffffu) ? 1u : 0u) << (2 * j) | (is(o >> 16) ? 2u : 0u) << (2 * j);
+      const uint32_t e = equal(v[j]);
+      m |= ((e >> 15) & 1u) << (2 * j) | (e >> 31) << (2 * j + 1);
     }
     return m;
   };
-  if (many == 1) {
-    if (tid < rest && is(order_pair<T>(row[loose(tid)]) & 0xffffu)) a.tokens[r] = loose(tid);
-    for (int i = tid; i < span.vectors; i += kSampleThreads) {
-      const uint32_t m = matches(body[i]);
-      if (m) a.tokens[r] = span.head + 8 * i + __builtin_ctz(m);
+  // the vector of a turn, from a register or from memory (in a turn that the row does not
+  // reach, another)
+  const int turns = (span.vectors + kSampleThreads - 1) / kSampleThreads;
+  auto each = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j)
+      if (j < turns) f(j, held[j]);
+    for (int j0 = kHeld; j0 < turns; j0 += kStretch) {
+      u32x4 v[kStretch];
+#pragma unroll
+      for (int j = 0; j < kStretch; ++j)
+        v[j] = body(min((j0 + j) * kSampleThreads + tid, span.vectors - 1));
+#pragma unroll
+      for (int j = 0; j < kStretch; ++j)
+        if (j0 + j < turns) f(j0 + j, v[j]);
+    }
+  };
+  // The one there is, or, in their order, the loose ones before the vectors, the vectors by
+  // turns and wavefronts, the loose ones behind.
+  const bool one = many == 1;
+  if (one && tid < rest && is(row[loose(tid)])) a.tokens[r] = loose(tid);
+  each([&](int j, const u32x4& v) __attribute__((always_inline)) {
+    const int i = j * kSampleThreads + tid;
+    uint32_t n = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) n += __popc(equal(v[e]));
+    if (i >= span.vectors) n = 0;
+    if (one) {
+      if (n) a.tokens[r] = span.head + 8 * i + __builtin_ctz(matches(v));
+    } else {
+      n = sum_of(n);
+      if (lane == 0) seen[j * kSampleWaves + wave] = n;
+    }
+  });
+  if (one) return;
+  __syncthreads();
+  if (wave != 0) return;
+  const bool mine = lane < rest && is(row[loose(lane)]);
+  const uint64_t heads = __ballot(mine && lane < span.head);
+  const uint64_t tails = __ballot(mine && lane >= span.head);
+  const uint64_t below = (1ull << lane) - 1;
+  uint32_t left = skip;
+  if (left < (uint32_t)__popcll(heads)) {
+    if (((heads >> lane) & 1) && (uint32_t)__popcll(heads & below) == left)
+      a.tokens[r] = loose(lane);
+    return;
+  }
+  left -= __popcll(heads);
+  for (int e0 = 0; e0 < turns * kSampleWaves; e0 += 64) {
+    const uint32_t n = e0 + lane < turns * kSampleWaves ? seen[e0 + lane] : 0;
+    uint32_t all;
+    const uint32_t before = scan_before<uint32_t>(n, lane, &all);
+    if (left >= all) {
+      left -= all;
+      continue;
+    }
+    const int at = __builtin_ctzll(__ballot(left >= before && left < before + n));
+    left -= lane_of(before, at);
+    const int i = (e0 + at) * 64 + lane;  // the 64 vectors of that turn and wavefront
+    const uint32_t m = i < span.vectors ? matches(body(i)) : 0;
+    const uint32_t prior = scan_before<uint32_t>(__popc(m), lane);
+    if (left >= prior && left < prior + __popc(m)) {
+      uint32_t bits = m;
+      for (uint32_t k = left - prior; k > 0; --k) bits &= bits - 1;
+      a.tokens[r] = span.head + 8 * i + __builtin_ctz(bits);
     }
     return;
   }
-  // In their order: the loose ones before the vectors, a run of vectors a wavefront, the
-  // loose ones behind. The wavefront whose run it is in reads it once more.
-  const int run = (span.vectors + kSampleWaves - 1) / kSampleWaves;
-  const int lo = min(wave * run, span.vectors), hi = min(lo + run, span.vectors);
-  uint32_t n = 0;
-  for (int i = lo + lane; i < hi; i += 64) n += __popc(matches(body[i]));
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) n += __shfl_xor(n, d);
-  if (lane == 0) seen[wave] = n;
-  __syncthreads();
-  const bool mine = lane < rest && is(order_pair<T>(row[loose(lane)]) & 0xffffu);
-  const uint64_t heads = __ballot(mine && lane < span.head), tails = __ballot(mine && lane >= span.head);
-  const uint64_t below = (1ull << lane) - 1;
-  uint32_t before = __popcll(heads);
-  if (wave == 0 && ((heads >> lane) & 1) && (uint32_t)__popcll(heads & below) == left)
-    a.tokens[r] = loose(lane);
-  for (int w = 0; w < wave; ++w) before += seen[w];
-  if (left >= before && left < before + n) {
-    left -= before;
-    for (int i0 = lo; i0 < hi; i0 += 64) {
-      const uint32_t m = i0 + lane < hi ? matches(body[i0 + lane]) : 0;
-      uint32_t all;
-      const uint32_t prior = scan_before<uint32_t>(__popc(m), lane, &all);
-      if (left < all) {
-        if (left >= prior && left < prior + __popc(m)) {
-          uint32_t bits = m;
-          for (uint32_t k = left - prior; k > 0; --k) bits &= bits - 1;
-          a.tokens[r] = span.head + 8 * (i0 + lane) + __builtin_ctz(bits);
-        }
-        break;
-      }
-      left -= all;
-    }
-  }
-  if (wave == kSampleWaves - 1) {
-    before += n;
-    if (((tails >> lane) & 1) && left == before + (uint32_t)__popcll(tails & below))
-      a.tokens[r] = loose(lane);
-  }
+  if (((tails >> lane) & 1) && left == (uint32_t)__popcll(tails & below)) a.tokens[r] = loose(lane);
 }
 
 // The walk over a tree: from node 0 to its first child whose token was picked at it, and on.
