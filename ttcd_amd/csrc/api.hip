@@ -1534,6 +1534,37 @@ ttcd_status ttcd_kv4_evict(const ttcd_kv4_cache* cache, const float* weights, in
 
 namespace {
 
+struct Kv4TreePlan {
+  int row_tiles, nrb, units, least;
+  size_t bytes;  // of the workspace; 0: no split
+};
+
+// The same for a tree, whose parts the kernels deal to the sequences by their lengths: up to
+// 64 of them, a lane each, to share 512 workgroups, two a CU (us, nodes and sequences of up to
+// 16000 keys, 16/8 heads of 128, with 256, 512 and 768: 16 of 8 30, 31, 36; 8 of 32 94, 59,
+// 60; 64 of 8 76, 64, 70; 256 of 1 59, 54, 66). As many parts to every sequence took 50 for
+// the first of these. No split up to 40 tiles of 32 keys, or 8 of 64: the sum of the parts
+// costs more than it saves.
+Kv4TreePlan kv4_tree_plan(const ttcd_kv4_cache* c, int N, int Hq, int window) {
+  const int64_t rows = (int64_t)N * (Hq / c->kv_heads);
+  Kv4TreePlan p = {};
+  p.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 8;
+  const int rb = 16 * p.row_tiles;
+  const bool block = p.row_tiles == 8;
+  p.nrb = (int)((rows + rb - 1) / rb);
+  int64_t keys = c->capacity;
+  if (window > 0 && window < keys) keys = window;
+  const int64_t tiles = (keys + N) / (block ? 64 : 32) + 2;  // of a sequence, at most
+  if (tiles <= (block ? 8 : 40) || c->batch > 64) return p;
+  p.least = 4;
+  const int64_t groups = (int64_t)c->kv_heads * p.nrb, all = (tiles + p.least - 1) / p.least;
+  const int64_t units = std::min((512 + groups - 1) / groups, c->batch * all);
+  p.units = (int)std::max(units, (int64_t)c->batch + 1);
+  p.bytes = (size_t)p.units * c->kv_heads * rows * (c->head_dim + 2) * sizeof(float) +
+            (size_t)c->batch * 2 * sizeof(int32_t);
+  return p;
+}
+
 // The draft that a tree's nodes lie in, next to the cache of their sequences.
 ttcd_status check_draft(const ttcd_kv4_cache* cache, const ttcd_kv4_cache* draft) {
   if (draft->batch != cache->batch || draft->kv_heads != cache->kv_heads ||
@@ -1554,7 +1585,12 @@ ttcd_status check_draft(const ttcd_kv4_cache* cache, const ttcd_kv4_cache* draft
 
 size_t ttcd_kv4_tree_attn_workspace_bytes(const ttcd_kv4_cache* cache, int N, int Hq,
                                           int window) {
-  return N > ttcd::kTreeNodes ? 0 : ttcd_kv4_attn_workspace_bytes(cache, N, Hq, window);
+  if (!cache || cache->batch < 1 || cache->kv_heads < 1 || N < 1 || N > ttcd::kTreeNodes ||
+      Hq < cache->kv_heads || Hq % cache->kv_heads != 0 ||
+      (cache->head_dim != 64 && cache->head_dim != 128) || cache->capacity < 32 ||
+      !kv4_rows_fit(cache, N, Hq))
+    return 0;
+  return kv4_tree_plan(cache, N, Hq, kv4_window(window)).bytes;
 }
 
 ttcd_status ttcd_kv4_tree_attn_fwd(const ttcd_kv4_cache* cache, const ttcd_kv4_cache* draft,
@@ -1597,15 +1633,16 @@ ttcd_status ttcd_kv4_tree_attn_fwd(const ttcd_kv4_cache* cache, const ttcd_kv4_c
   a.G = Hq / cache->kv_heads;
   a.window = kv4_window(window);
   a.c_log2 = sm_scale * 1.4426950408889634f;
-  const Kv4Plan p = kv4_plan(cache, N, Hq, a.window);
+  const Kv4TreePlan p = kv4_tree_plan(cache, N, Hq, a.window);
   a.row_tiles = p.row_tiles;
   a.nrb = p.nrb;
   a.parts = 1;
-  const size_t part = kv4_part_bytes(cache, N, Hq);
-  if (p.parts > 1 && workspace && aligned16(workspace) && workspace_bytes >= p.parts * part) {
-    a.parts = p.parts;
+  if (p.bytes > 0 && workspace && aligned16(workspace) && workspace_bytes >= p.bytes) {
+    a.units = p.units;
+    a.least = p.least;
     a.part = static_cast<float*>(workspace);
-    a.part_ml = a.part + p.parts * (part / sizeof(float) / (cache->head_dim + 2)) * cache->head_dim;
+    a.part_ml = a.part + (size_t)p.units * Hq * N * cache->head_dim;
+    a.shares = reinterpret_cast<int32_t*>(a.part_ml + (size_t)p.units * Hq * N * 2);
   }
   return from_hip(ttcd::launch_kv4_tree_attn(a, elem(dtype), static_cast<hipStream_t>(stream)),
                   "kv4 tree attention launch");

@@ -296,12 +296,18 @@ struct Kv4CommitArgs {
 };
 hipError_t launch_kv4_commit(const Kv4CommitArgs& a, hipStream_t stream);
 
-constexpr int kTreeNodes = 256;  // at most, of a sequence's tree
+// At most, of a sequence's tree. A multiple of every count of rows that a workgroup takes, so
+// none of a workgroup's rows is of a node past that.
+constexpr int kTreeNodes = 256;
 
 // Attention of a tree's nodes: Tq nodes, their own keys in the cache d, node i in slot i.
 struct Kv4TreeArgs : Kv4AttnArgs {
   Kv4Cache d;
   const int32_t* parents;  // (B, Tq)
+  int units;  // > 0 (then B < units, B <= 64): parts of all sequences together, dealt by their
+              // lengths; part, part_ml: (units, H, Tq * G, ..)
+  int least;  // tiles of a part, at the least
+  int32_t* shares;  // (B, 2) the first part of a sequence, and how many it has
 };
 hipError_t launch_kv4_tree_attn(const Kv4TreeArgs& a, Elem dtype, hipStream_t stream);
 

@@ -27,6 +27,7 @@
 
 #include "internal.h"
 #include "kv4_sweep.h"
+#include "wave.h"
 
 namespace ttcd {
 namespace {
@@ -352,6 +353,7 @@ hipError_t launch_read(const Kv4ReadArgs& a, hipStream_t st) {
 // have passed by (20.5, past them 19.7), as a model's other layers do; 9 MB the same (9.4
 // and 9.8; 10.2 and 9.7). By the capacity: the lengths are on the GPU.
 constexpr int kRowWaves = 8;
+constexpr int kTreeWaves = 4;  // of a workgroup over a tree's rows
 
 template <typename Args>
 constexpr bool is_tree = false;
@@ -530,16 +532,18 @@ __device__ __forceinline__ RowRange row_range(int t, int n_new, int len, int C, 
 }
 
 // A tree's nodes (kv4_tree_attn): node i of a sequence is at position length + depth(i), and
-// sees the cache up to the window before that, itself and its ancestors, keys of the draft.
-// Ancestors are bits: after s steps a node has those of 2^s, itself among them, and knows
-// the one after the last, so 8 steps are enough for 256 nodes, and the depth's logarithm
-// is what it takes (walking up one by one would wait for LDS at every node of a chain).
+// sees the cache up to the window before that, itself and its ancestors, keys of the draft,
+// those of them that the window reaches. They are bits: after s steps a node has those of
+// 2^s, itself among them, and knows the one after the last, so 8 steps are enough for 256
+// nodes, and the depth's logarithm is what it takes (walking up one by one would wait for LDS
+// at every node of a chain). Nodes behind the last see nothing.
 struct TreeBits {
   uint32_t up[kTreeNodes][kTreeNodes / 32];
   int depth[kTreeNodes], next[kTreeNodes];
 };
 template <int THREADS>
-__device__ __forceinline__ void tree_bits(TreeBits& tree, const int32_t* parents, int n) {
+__device__ __forceinline__ void tree_bits(TreeBits& tree, const int32_t* parents, int n,
+                                          int window) {
   static_assert(THREADS >= kTreeNodes, "a thread a node");
   constexpr int WORDS = kTreeNodes / 32;
   const int i = threadIdx.x;
@@ -550,7 +554,7 @@ __device__ __forceinline__ void tree_bits(TreeBits& tree, const int32_t* parents
   }
   if (i < kTreeNodes) {
 #pragma unroll
-    for (int w = 0; w < WORDS; ++w) tree.up[i][w] = w == i / 32 ? 1u << (i % 32) : 0u;
+    for (int w = 0; w < WORDS; ++w) tree.up[i][w] = w == i / 32 && i < n ? 1u << (i % 32) : 0u;
     tree.depth[i] = next >= 0;
     tree.next[i] = next;
   }
@@ -571,28 +575,26 @@ __device__ __forceinline__ void tree_bits(TreeBits& tree, const int32_t* parents
       tree.next[i] = next = after;
     }
   }
+  if (window > 0 && window < n) {
+    if (i < n && tree.depth[i] >= window) {
+      const int least = tree.depth[i] - window + 1;
+      for (int w = 0; w <= i / 32; ++w) {
+        uint32_t left = tree.up[i][w];
+        while (left != 0) {
+          const int e = __builtin_ctz(left);
+          left &= left - 1;
+          if (tree.depth[32 * w + e] < least) tree.up[i][w] &= ~(1u << e);
+        }
+      }
+    }
+    __syncthreads();
+  }
 }
 
 // Bits lo .. hi of a word, those of them that there are.
 __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
   if (lo > hi || hi < 0 || lo > 31) return 0u;
   return (0xffffffffu << max(lo, 0)) & (0xffffffffu >> (31 - min(hi, 31)));
-}
-
-// Node i's ancestors among nodes 32 w .. 32 w + 31, those that the window reaches.
-__device__ __forceinline__ uint32_t ancestors_in(const TreeBits& tree, int i, int w, int n,
-                                                 int window) {
-  if (i >= n) return 0u;
-  uint32_t m = tree.up[i][w];
-  if (window > 0 && tree.depth[i] >= window) {
-    uint32_t left = m;
-    while (left != 0) {
-      const int e = __builtin_ctz(left);
-      left &= left - 1;
-      if (tree.depth[i] - tree.depth[32 * w + e] >= window) m &= ~(1u << e);
-    }
-  }
-  return m;
 }
 
 __device__ __forceinline__ RowRange node_range(int i, int n, int depth, int len, int C, int W) {
@@ -602,21 +604,93 @@ __device__ __forceinline__ RowRange node_range(int i, int n, int depth, int len,
   return {lo, len - 1};
 }
 
+// A workgroup's share: part `part` of sequence b's tiles, those from `part * tiles` on, and
+// where its sums go, row 0's place among the parts' rows.
+struct Share {
+  int b, h, rb, part, parts;
+  int tiles;      // of a part; 0: those there are, dealt evenly
+  int64_t sums;
+};
+template <int KEYS>
+__device__ __forceinline__ Share share_of(const Kv4AttnArgs& a, int id, int) {
+  const int part = id % a.parts, rest = id / a.parts;
+  const int rb = rest % a.nrb, bh = rest / a.nrb;
+  const int b = bh / a.c.H;
+  return {b, bh - b * a.c.H, rb, part, a.parts, 0,
+          ((int64_t)part * a.c.B * a.c.H + bh) * ((int64_t)a.Tq * a.G)};
+}
+
+// How a tree's sequences share their parts: as many tiles of KEYS keys to each part, whatever
+// the sequence, so that a batch of mixed lengths ends at once. A lane a sequence.
+struct TreeShares {
+  uint32_t first, parts;  // of the lane's sequence
+  int tiles;              // of a part
+};
+template <int KEYS>
+__device__ __forceinline__ TreeShares tree_shares(const Kv4TreeArgs& a, int lane) {
+  uint32_t tiles = 0;
+  if (lane < a.c.B) {
+    const int len = length_of(a.c.len, lane);
+    const int n = min(count_of(a.counts, lane, a.Tq), length_of(a.d.len, lane));
+    if (n > 0) {
+      const RowRange keys = node_range(0, n, 0, len, a.c.C, a.window);
+      tiles = (n + KEYS - 1) / KEYS;
+      if (keys.lo <= keys.hi) tiles += keys.hi / KEYS - keys.lo / KEYS + 1;
+    }
+  }
+  // The least tiles a part with which there are no more parts than units: between all of
+  // them full, and every sequence's last one short.
+  const uint32_t all = sum_of(tiles), most = max_of(tiles), units = a.units, B = a.c.B;
+  uint32_t lo = max(max((all + units - 1) / units, (most + kKv4MaxParts - 1) / kKv4MaxParts),
+                    (uint32_t)a.least);
+  uint32_t hi = max(lo, (all + units - B - 1) / (units - B));
+  while (lo < hi) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (sum_of((tiles + mid - 1) / mid) <= units)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  TreeShares s;
+  s.tiles = lo;
+  s.parts = (tiles + s.tiles - 1) / s.tiles;
+  s.first = scan_before<uint32_t>(s.parts, lane);
+  return s;
+}
+template <int KEYS>
+__device__ __forceinline__ Share share_of(const Kv4TreeArgs& a, int id, int lane) {
+  if (a.units == 0) return share_of<KEYS>(static_cast<const Kv4AttnArgs&>(a), id, lane);
+  const TreeShares s = tree_shares<KEYS>(a, lane);
+  if (id == 0 && threadIdx.x < a.c.B) {  // for the sums of the parts
+    a.shares[2 * lane] = s.first;
+    a.shares[2 * lane + 1] = s.parts;
+  }
+  const uint32_t unit = id % a.units;
+  const int rest = id / a.units, rb = rest % a.nrb, h = rest / a.nrb;
+  const uint64_t mine = __ballot(unit - s.first < s.parts);
+  if (mine == 0) return {-1, h, rb, 0, 0, 0, 0};
+  const int b = __builtin_ctzll(mine);
+  return {b, h, rb, (int)(unit - lane_of(s.first, b)), (int)lane_of(s.parts, b), s.tiles,
+          ((int64_t)unit * a.c.H + h) * ((int64_t)a.Tq * a.G)};
+}
+
 template <typename T, int D, int NT, bool FAR, typename Args>
-__global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Args a) {
+__global__ __launch_bounds__(64 * (is_tree<Args> ? kTreeWaves : kRowWaves),
+                             is_tree<Args> ? 4 - NT : 1) void kv4_rows_kernel(Args a) {
   constexpr bool TREE = is_tree<Args>;
+  constexpr int WAVES = TREE ? kTreeWaves : kRowWaves;
   constexpr int STEPS = D / 32, NM = D / 16, RB = 16 * NT, R = D / 8;
-  __shared__ __attribute__((aligned(16))) float so[kRowWaves][16][D + 4];
-  __shared__ float sml[kRowWaves][RB][2];
+  __shared__ __attribute__((aligned(16))) float so[WAVES][16][D + 4];
+  __shared__ float sml[WAVES][RB][2];
   static_assert(sizeof(TreeBits) <= sizeof(so), "the tree lies where the sums come later");
   TreeBits& tree = *reinterpret_cast<TreeBits*>(&so);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int quarter = lane >> 4, n = lane & 15;
-  const int part = blockIdx.x % a.parts;
-  const int rest = blockIdx.x / a.parts;
-  const int rb = rest % a.nrb, bh = rest / a.nrb;
-  const int b = bh / a.c.H, h = bh % a.c.H;
+  const Share mine = share_of<32>(a, blockIdx.x, lane);
+  const int part = mine.part, parts = mine.parts, b = mine.b, h = mine.h, bh = b * a.c.H + h;
+  const int rb = mine.rb;
+  if (TREE && b < 0) return;
   const int len = length_of(a.c.len, b);
   int n_new = count_of(a.counts, b, a.Tq);
   if constexpr (TREE) n_new = min(n_new, length_of(a.d.len, b));
@@ -642,17 +716,6 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Args a) {
 #pragma unroll
     for (int i = 0; i < NM; ++i) st.o[nt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  if constexpr (TREE) {
-    tree_bits<64 * kRowWaves>(tree, a.parents + (int64_t)b * a.Tq, n_new);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int node = (row0 + 16 * nt + n) / a.G;
-      const RowRange rr = node_range(node, n_new, tree.depth[min(node, kTreeNodes - 1)], len, C,
-                                     a.window);
-      lo[nt] = rr.lo;
-      hi[nt] = rr.hi;
-    }
-  }
   // the block's keys, and those that all its rows see
   const int t_lo = row0 / a.G, t_hi = min((row0 + RB - 1) / a.G, n_new - 1);
   if (t_lo <= t_hi) {
@@ -661,12 +724,19 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Args a) {
                                 : row_range(t_lo, n_new, len, C, a.window);
     const RowRange last = TREE ? node_range(0, n_new, n_new - 1, len, C, a.window)
                                : row_range(t_hi, n_new, len, C, a.window);
+    if constexpr (TREE) {  // of rows whose tiles nothing cuts
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        lo[nt] = 0;
+        hi[nt] = len - 1;
+      }
+    }
     if (TREE || first.lo <= last.hi) {
       const int tile_lo = first.lo >> 5;
       // of the cache; a tree's draft follows
       const int held = first.lo <= last.hi ? (last.hi >> 5) - tile_lo + 1 : 0;
       const int tiles = TREE ? held + ((n_new + 31) >> 5) : held;
-      const int per = (tiles + a.parts - 1) / a.parts;
+      const int per = TREE && mine.tiles > 0 ? mine.tiles : (tiles + parts - 1) / parts;
       const int t0 = tile_lo + part * per, t1 = min(t0 + per, tile_lo + tiles);
       // a lane's place in 16 keys' rows; the rest of an address is the wavefront's
       const int word = D == 128 ? n : n >> 1;
@@ -706,7 +776,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Args a) {
           kv.vs[g] = *reinterpret_cast<const uint32_t*>(t0 + (vs_at + 16 * g * (D / 32)));
         }
       };
-      const int step = kRowWaves * 32 % C;
+      const int step = WAVES * 32 % C;
       int tile = t0 + wave;
       int slot = (int)((uint32_t)(tile * 32) % (uint32_t)C);
       auto fold = [&](const KvTile<D>& kv) __attribute__((always_inline)) {
@@ -720,8 +790,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Args a) {
                                  : bits_between(first.lo - p0, last.hi - p0);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mask.rows[nt] = node >= 0 ? ancestors_in(tree, (row0 + 16 * nt + n) / a.G, node >> 5,
-                                                       n_new, a.window)
+              mask.rows[nt] = node >= 0 ? tree.up[(row0 + 16 * nt + n) / a.G][node >> 5]
                                         : bits_between(lo[nt] - p0, hi[nt] - p0);
           }
           fold_tile<T, D, NT>(st, kv, q, a.c_log2, masked, mask, lane);
@@ -730,22 +799,43 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Args a) {
           const RangeMask<NT> mask = {lo, hi, tile * 32, first.lo, last.hi};
           fold_tile<T, D, NT>(st, kv, q, a.c_log2, masked, mask, lane);
         }
-        tile += kRowWaves;
+        tile += WAVES;
       };
+      // AHEAD tiles are on their way while one is folded
+      constexpr int AHEAD = TREE ? 2 : 1;
       auto next = [&](KvTile<D>& kv) __attribute__((always_inline)) {
-        if (tile + kRowWaves >= t1) return;
+        if (tile + AHEAD * WAVES >= t1) return;
         slot += step;
         if (slot >= C) slot -= C;
-        load(kv, tile + kRowWaves, slot);
+        load(kv, tile + AHEAD * WAVES, slot);
       };
-      KvTile<D> kv[2];
+      KvTile<D> kv[AHEAD + 1];
       if (tile < t1) load(kv[0], tile, slot);
+      if constexpr (TREE) {
+        if (tile + WAVES < t1) {
+          slot += step;
+          if (slot >= C) slot -= C;
+          load(kv[1], tile + WAVES, slot);
+        }
+        // the tree where a tile of the part needs it: the draft's, and those that the window cuts
+        if (t0 < t1 && (t1 > tile_lo + held || t0 * 32 < last.lo)) {
+          tree_bits<64 * WAVES>(tree, a.parents + (int64_t)b * a.Tq, n_new, a.window);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const int node = (row0 + 16 * nt + n) / a.G;
+            const RowRange rr = node_range(node, n_new, tree.depth[node], len, C, a.window);
+            lo[nt] = rr.lo;
+            hi[nt] = rr.hi;
+          }
+        }
+      }
       while (tile < t1) {
-        next(kv[1]);
-        fold(kv[0]);
-        if (tile >= t1) break;
-        next(kv[0]);
-        fold(kv[1]);
+#pragma unroll
+        for (int i = 0; i <= AHEAD; ++i) {
+          next(kv[(i + AHEAD) % (AHEAD + 1)]);
+          fold(kv[i]);
+          if (tile >= t1) break;
+        }
       }
     }
   }
@@ -773,26 +863,26 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_rows_kernel(Args a) {
       for (int i = 0; i < NM; ++i)
         so[wave][n][NM * (4 * quarter + e) + i] = st.o[nt][i][e];
     __syncthreads();
-    constexpr int PER = D * 16 / (64 * kRowWaves);  // channels a thread
+    constexpr int PER = D * 16 / (64 * WAVES);  // channels a thread
     constexpr int TPR = D / PER;                    // threads a row
     const int r = threadIdx.x / TPR, d0 = (threadIdx.x % TPR) * PER;
     const int row = row0 + 16 * nt + r;
     if (row < a.Tq * a.G) {
       float m = -INFINITY, l = 0.f, o[PER];
 #pragma unroll
-      for (int w = 0; w < kRowWaves; ++w) m = fmaxf(m, sml[w][16 * nt + r][0]);
+      for (int w = 0; w < WAVES; ++w) m = fmaxf(m, sml[w][16 * nt + r][0]);
       const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int i = 0; i < PER; ++i) o[i] = 0.f;
 #pragma unroll
-      for (int w = 0; w < kRowWaves; ++w) {
+      for (int w = 0; w < WAVES; ++w) {
         const float f = __builtin_amdgcn_exp2f(sml[w][16 * nt + r][0] - ref);
         l = fmaf(sml[w][16 * nt + r][1], f, l);
 #pragma unroll
         for (int i = 0; i < PER; ++i) o[i] = fmaf(so[w][r][d0 + i], f, o[i]);
       }
-      if (a.parts > 1) {
-        const int64_t at = ((int64_t)part * a.c.B * a.c.H + bh) * ((int64_t)a.Tq * a.G) + row;
+      if (parts > 1) {
+        const int64_t at = mine.sums + row;
         if (threadIdx.x % TPR == 0) {
           a.part_ml[2 * at] = m;
           a.part_ml[2 * at + 1] = l;
@@ -869,10 +959,10 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Args a) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, n = lane & 31;
-  const int part = blockIdx.x % a.parts;
-  const int rest = blockIdx.x / a.parts;
-  const int rb = rest % a.nrb, bh = rest / a.nrb;
-  const int b = bh / a.c.H, h = bh - b * a.c.H;
+  const Share mine = share_of<kBlockKeys>(a, blockIdx.x, lane);
+  const int part = mine.part, parts = mine.parts, b = mine.b, h = mine.h, bh = b * a.c.H + h;
+  const int rb = mine.rb;
+  if (TREE && b < 0) return;
   const int len = length_of(a.c.len, b);
   int n_new = count_of(a.counts, b, a.Tq);
   if constexpr (TREE) n_new = min(n_new, length_of(a.d.len, b));
@@ -888,13 +978,10 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Args a) {
   }
   RowRange rr;
   __shared__ std::conditional_t<TREE, TreeBits, char> tree[1];
-  if constexpr (TREE) {
-    tree_bits<256>(tree[0], a.parents + (int64_t)b * a.Tq, n_new);
-    const int node = row / a.G;
-    rr = node_range(node, n_new, tree[0].depth[min(node, kTreeNodes - 1)], len, C, a.window);
-  } else {
+  if constexpr (TREE)
+    rr = {0, len - 1};  // of rows whose tiles no window cuts
+  else
     rr = row_range(row / a.G, n_new, len, C, a.window);
-  }
   float m = -INFINITY, l = 0.f;
   f32x16 o[MB];
 #pragma unroll
@@ -913,11 +1000,19 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Args a) {
       const int held = first.lo <= last.hi ? last.hi / kBlockKeys - tile_lo + 1 : 0;
       const int tiles = TREE ? held + (n_new + kBlockKeys - 1) / kBlockKeys : held;
       draft = tile_lo + held;
-      const int per = (tiles + a.parts - 1) / a.parts;
+      const int per = TREE && mine.tiles > 0 ? mine.tiles : (tiles + parts - 1) / parts;
       t0 = tile_lo + part * per;
       t1 = min(t0 + per, tile_lo + tiles);
       any_lo = first.lo;
       any_hi = last.hi;
+      if constexpr (TREE) {
+        // the tree where a tile of the part needs it: the draft's, and those that the window cuts
+        if (t0 < t1 && (t1 > draft || t0 * kBlockKeys < last.lo)) {
+          tree_bits<256>(tree[0], a.parents + (int64_t)b * a.Tq, n_new, a.window);
+          const int node = row / a.G;
+          rr = node_range(node, n_new, tree[0].depth[node], len, C, a.window);
+        }
+      }
     }
   }
   // the keys that all rows of this wavefront see
@@ -1044,17 +1139,18 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Args a) {
   // masks tile's scores and moves the reference where they exceed it by 2^8
   auto settle = [&](f32x16 (&s)[2], int tile) __attribute__((always_inline)) {
     const int p0 = tile * kBlockKeys;
-    if (TREE && tile >= draft) {
-      if constexpr (TREE) {
-        uint32_t seen[2];
+    if constexpr (TREE) {
+      if (tile >= draft || p0 < in_lo || p0 + kBlockKeys - 1 > in_hi) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-          seen[kb] = ancestors_in(tree[0], row / a.G, 2 * (tile - draft) + kb, n_new, a.window);
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < 2; ++kb) {
+          const uint32_t seen =
+              (tile >= draft ? tree[0].up[row / a.G][2 * (tile - draft) + kb]
+                             : bits_between(rr.lo - p0 - 32 * kb, rr.hi - p0 - 32 * kb)) >>
+              (4 * half);
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if (!((seen[kb] >> (8 * (e >> 2) + 4 * half + (e & 3))) & 1)) s[kb][e] = -INFINITY;
+            if (!(seen & (1u << (8 * (e >> 2) + (e & 3))))) s[kb][e] = -INFINITY;
+        }
       }
     } else if (p0 < in_lo || p0 + kBlockKeys - 1 > in_hi) {
 #pragma unroll
@@ -1114,9 +1210,9 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Args a) {
   l = none ? 0.f : l + __shfl_xor(l, 32);
   m = none ? -INFINITY : m - Fmt<T>::kBias;
   const int rows = a.Tq * a.G, wrow0 = row0 + wave * 32;
-  const int64_t at0 = ((int64_t)part * a.c.B * a.c.H + bh) * (int64_t)rows;
+  const int64_t at0 = mine.sums;
   if (half == 0 && row < rows) {
-    if (a.parts > 1) {
+    if (parts > 1) {
       a.part_ml[2 * (at0 + row)] = m;
       a.part_ml[2 * (at0 + row) + 1] = l;
     } else if (a.lse != nullptr) {
@@ -1142,7 +1238,7 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Args a) {
       const int e = 4 * ((8 * (wi >> 2) + W * (c / MB)) >> 3) + (wi & 3);
       x[c] = o[c % MB][e];
     }
-    if (a.parts > 1) {
+    if (parts > 1) {
       char* const dst = rows_at + n * (D * 4);
       *reinterpret_cast<f32x4*>(dst + ((2 * w) ^ (n & (2 * W - 1))) * 16) =
           f32x4{x[0], x[1], x[2], x[3]};
@@ -1157,7 +1253,7 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Args a) {
     }
   }
   __syncthreads();
-  if (a.parts > 1) {
+  if (parts > 1) {
     constexpr int CH = 2 * W;
 #pragma unroll
     for (int i = 0; i < CH / 2; ++i) {
@@ -1184,17 +1280,36 @@ __global__ __launch_bounds__(256, 2) void kv4_block_kernel(Args a) {
 // lane; D / 4 threads with 4 channels each in every one of the 256 / (D / 4) groups
 // share the sums between them. (One thread after the other over the parts took 29
 // us for 103 of them; 64 of 30 rows take 3.9.)
-template <typename T, int D>
-__global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4AttnArgs a) {
+//
+// Where they are: `parts` rows `all` apart, the first `id`.
+struct Parts {
+  int parts;
+  int64_t id, all;
+};
+__device__ __forceinline__ Parts parts_of(const Kv4AttnArgs& a, int bh, int row) {
+  const int64_t rows = (int64_t)a.Tq * a.G;
+  return {a.parts, bh * rows + row, a.c.B * a.c.H * rows};
+}
+__device__ __forceinline__ Parts parts_of(const Kv4TreeArgs& a, int bh, int row) {
+  const int64_t rows = (int64_t)a.Tq * a.G;
+  const int b = bh / a.c.H, h = bh - b * a.c.H;
+  return {a.shares[2 * b + 1], ((int64_t)a.shares[2 * b] * a.c.H + h) * rows + row,
+          a.c.H * rows};
+}
+
+template <typename T, int D, typename Args>
+__global__ __launch_bounds__(256) void kv4_combine_kernel(Args a) {
   constexpr int TH = D / 4, GR = 256 / TH;
   __shared__ f32x4 so[GR][TH];
   const int rows = a.Tq * a.G;
-  const int64_t id = blockIdx.x, all = (int64_t)a.c.B * a.c.H * rows;
   const int bh = blockIdx.x / rows, row = blockIdx.x - bh * rows;
   const int b = bh / a.c.H, h = bh - b * a.c.H;
   const int d4 = threadIdx.x % TH, g = threadIdx.x / TH, lane = threadIdx.x & 63;
+  const Parts in = parts_of(a, bh, row);
+  if (is_tree<Args> && in.parts == 1) return;  // written by the part
+  const int64_t id = in.id, all = in.all;
   float m = -INFINITY, l = 0.f;
-  if (lane < a.parts) {
+  if (lane < in.parts) {
     const float* ml = a.part_ml + 2 * (lane * all + id);
     m = ml[0];
     l = ml[1];
@@ -1210,10 +1325,10 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4AttnArgs a) {
   for (int d = 1; d < 64; d *= 2) l += __shfl_xor(l, d);
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   const float* src = a.part + id * D + 4 * d4;
-  for (int p0 = 0; p0 < a.parts; p0 += GR) {
+  for (int p0 = 0; p0 < in.parts; p0 += GR) {
     const int p = p0 + g;
     const float w = __shfl(f, p & 63);
-    if (p < a.parts && !(w < 0.f)) {
+    if (p < in.parts && !(w < 0.f)) {
       const f32x4 v = *reinterpret_cast<const f32x4*>(src + p * all * D);
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = fmaf(v[e], w, o[e]);
@@ -1238,48 +1353,50 @@ __global__ __launch_bounds__(256) void kv4_combine_kernel(Kv4AttnArgs a) {
 // row to itself, D / 64 channels a lane, and no other to wait for (us, the sum's share
 // of all: 4 parts of 16000 rows 104 -> 99; fewer rows leave too few wavefronts: 16 of
 // 16 rows 9.5 -> 10.8).
-template <typename T, int D>
-__global__ __launch_bounds__(256) void kv4_combine_rows_kernel(Kv4AttnArgs a) {
-  constexpr int CL = D / 64;
+template <typename T, int D, typename Args>
+__global__ __launch_bounds__(256) void kv4_combine_rows_kernel(Args a) {
+  constexpr int CL = D / 64, LANES = is_tree<Args> ? 64 : 16;  // of parts, at most
   const int rows = a.Tq * a.G;
-  const int64_t all = (int64_t)a.c.B * a.c.H * rows;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t id = (int64_t)blockIdx.x * 4 + wave;
-  if (id >= all) return;
-  const int bh = (int)(id / rows), row = (int)(id - (int64_t)bh * rows);
+  const int64_t out = (int64_t)blockIdx.x * 4 + wave;
+  if (out >= (int64_t)a.c.B * a.c.H * rows) return;
+  const int bh = (int)(out / rows), row = (int)(out - (int64_t)bh * rows);
   const int b = bh / a.c.H, h = bh - b * a.c.H;
+  const Parts in = parts_of(a, bh, row);
+  if (is_tree<Args> && in.parts == 1) return;  // written by the part
+  const int64_t id = in.id, all = in.all;
   float m = -INFINITY, l = 0.f;
-  if (lane < a.parts) {
+  if (lane < in.parts) {
     const float* ml = a.part_ml + 2 * (lane * all + id);
     m = ml[0];
     l = ml[1];
   }
   float top = m;
 #pragma unroll
-  for (int d = 1; d < 16; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+  for (int d = 1; d < LANES; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
   float f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
   const bool empty = l == 0.f;  // such a part's sums are not there
   l = empty ? 0.f : l * f;
   f = empty ? -1.f : f;
 #pragma unroll
-  for (int d = 1; d < 16; d *= 2) l += __shfl_xor(l, d);
+  for (int d = 1; d < LANES; d *= 2) l += __shfl_xor(l, d);
   l = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(l)));
   float o[CL];
 #pragma unroll
   for (int i = 0; i < CL; ++i) o[i] = 0.f;
   const float* src = a.part + id * D + CL * lane;
-  for (int p0 = 0; p0 < a.parts; p0 += 4) {
+  for (int p0 = 0; p0 < in.parts; p0 += 4) {
     float x[4][CL];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int i = 0; i < CL; ++i) x[j][i] = src[min(p0 + j, a.parts - 1) * all * D + i];
+      for (int i = 0; i < CL; ++i) x[j][i] = src[min(p0 + j, in.parts - 1) * all * D + i];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       // an empty part, or one past the last, holds anything
       const float w = __shfl(f, p0 + j);
-      if (p0 + j < a.parts && !(w < 0.f))
+      if (p0 + j < in.parts && !(w < 0.f))
 #pragma unroll
         for (int i = 0; i < CL; ++i) o[i] = fmaf(x[j][i], w, o[i]);
     }
@@ -1298,10 +1415,18 @@ __global__ __launch_bounds__(256) void kv4_combine_rows_kernel(Kv4AttnArgs a) {
 
 template <typename T, int D, typename Args>
 hipError_t launch_attn_typed(const Args& a, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)a.parts * a.nrb * a.c.B * a.c.H));
+  int64_t groups = (int64_t)a.parts * a.nrb * a.c.B * a.c.H;
+  int parts = a.parts;  // of a row
+  if constexpr (is_tree<Args>) {
+    if (a.units > 0) {
+      groups = (int64_t)a.units * a.nrb * a.c.H;
+      parts = (a.units + a.c.B - 1) / a.c.B;  // on average (more than 1)
+    }
+  }
+  const dim3 grid((unsigned)groups);
   // codes and scales, against half of the 256 MiB of last-level cache
   const bool far = (int64_t)a.c.B * a.c.H * a.c.C * (D + D / 16) > (int64_t(128) << 20);
-  const dim3 few(64 * kRowWaves);
+  const dim3 few(64 * (is_tree<Args> ? kTreeWaves : kRowWaves));
   if (a.row_tiles == 1 && far)
     hipLaunchKernelGGL((kv4_rows_kernel<T, D, 1, true, Args>), grid, few, 0, st, a);
   else if (a.row_tiles == 1)
@@ -1313,14 +1438,14 @@ hipError_t launch_attn_typed(const Args& a, hipStream_t st) {
   else
     hipLaunchKernelGGL((kv4_block_kernel<T, D, Args>), grid, dim3(256), 0, st, a);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.parts == 1) return e;
+  if (e != hipSuccess || parts == 1) return e;
   const int64_t rows = (int64_t)a.c.B * a.c.H * a.G * a.Tq;
-  if (a.parts <= 16 && rows >= 1024)
-    hipLaunchKernelGGL((kv4_combine_rows_kernel<T, D>), dim3((unsigned)((rows + 3) / 4)),
-                       dim3(256), 0, st, static_cast<const Kv4AttnArgs&>(a));
+  if (parts <= 16 && rows >= 1024)
+    hipLaunchKernelGGL((kv4_combine_rows_kernel<T, D, Args>), dim3((unsigned)((rows + 3) / 4)),
+                       dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL((kv4_combine_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, st,
-                       static_cast<const Kv4AttnArgs&>(a));
+    hipLaunchKernelGGL((kv4_combine_kernel<T, D, Args>), dim3((unsigned)rows), dim3(256), 0, st,
+                       a);
   return hipGetLastError();
 }
 

@@ -451,7 +451,7 @@ def kv4_tree_attn(q: torch.Tensor, cache: KV4Cache, draft: KV4Cache, parents: to
         raise ValueError(f"{fn}: {N} nodes, need at most {min(TREE_NODES, draft.capacity)} (a "
                          f"draft's capacity, and {TREE_NODES})")
     q, qs = _operand(q)
-    o = torch.empty(B, N, H, D, dtype=q.dtype, device=q.device)
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty(B, H, N, dtype=torch.float32, device=q.device) if return_lse else None
     if N > 0:
         L, W = _lib.lib(), _window(window)

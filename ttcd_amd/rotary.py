@@ -15,6 +15,7 @@ a cached key's position from it, and a gradient through the embedding.
 from __future__ import annotations
 
 import math
+from functools import lru_cache
 
 import torch
 
@@ -22,6 +23,10 @@ from . import _lib
 
 _DT = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16,
        torch.float32: _lib.DTYPE_F32}
+
+# stride arrays (only read) of the last calls: finding one is quicker than making it
+_strides4 = lru_cache(maxsize=64)(_lib.strides4)
+_strides2 = lru_cache(maxsize=64)(_lib.strides2)
 
 
 def rope_frequencies(dim: int, base: float, scaling: dict | None = None, device=None,
@@ -105,50 +110,59 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor,
     position * inv_freq[i], times scale; the other channels as they are. positions: int32 or
     int64, (B, T) or (T,), on q's device; None: offset .. offset + T - 1. bf16, f16 or f32;
     inv_freq fp32. ``inverse`` turns back. Returns new contiguous (q, k), or q alone."""
-    for name, t in (("q", q), ("k", k), ("inv_freq", inv_freq), ("positions", positions)):
-        if t is None and name in ("k", "positions"):
-            continue
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise ValueError(f"rope: {name} must be a tensor on a GPU (HIP) device")
-        if t.device != q.device:
-            raise ValueError(f"rope: {name} must be on q's device")
-        if torch.is_grad_enabled() and t.requires_grad:
-            raise RuntimeError("rope is forward-only: autograd / gradient inputs are not supported; "
-                               "call it under torch.no_grad() (inverse=True is its gradient)")
-    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2]
-                                           or k.shape[3] != q.shape[3] or k.dtype != q.dtype)):
-        raise ValueError(f"rope: q and k must be (B, T, H, D) of the same B, T, D and dtype, got "
-                         f"{tuple(q.shape)}, {None if k is None else tuple(k.shape)}")
+    if (not isinstance(q, torch.Tensor) or not q.is_cuda or q.dim() != 4
+            or not isinstance(inv_freq, torch.Tensor) or not inv_freq.is_cuda):
+        raise ValueError("rope: q (B, T, H, D) and inv_freq must be tensors on a GPU (HIP) device")
     B, T, Hq, D = q.shape
-    if q.dtype not in _DT:
-        raise ValueError(f"rope: q and k must be bf16, f16 or f32, got {q.dtype}")
+    dev, dtype = q.device, q.dtype
+    code = _DT.get(dtype)
+    if code is None:
+        raise ValueError(f"rope: q and k must be bf16, f16 or f32, got {dtype}")
     n = inv_freq.numel()
-    if inv_freq.dim() != 1 or inv_freq.dtype != torch.float32 or n < 1 or 2 * n > D:
-        raise ValueError(f"rope: inv_freq must be fp32 (n,), 1 <= n <= {D // 2}, got "
+    if (inv_freq.dim() != 1 or inv_freq.dtype != torch.float32 or inv_freq.device != dev or n < 1
+            or 2 * n > D):
+        raise ValueError(f"rope: inv_freq must be fp32 (n,), 1 <= n <= {D // 2}, on q's device, got "
                          f"{tuple(inv_freq.shape)} {inv_freq.dtype}")
-    inv_freq = inv_freq.contiguous()
-    steps = None
+    Hkv = 0
+    if k is not None:
+        if (not isinstance(k, torch.Tensor) or k.dim() != 4 or k.dtype != dtype or k.device != dev
+                or k.shape[0] != B or k.shape[1] != T or k.shape[3] != D):
+            raise ValueError(f"rope: k must be (B, T, H, D) with q's B, T, D = {(B, T, D)}, dtype "
+                             f"and device, got {k}")
+        Hkv = k.shape[2]
+    if torch.is_grad_enabled() and (q.requires_grad or inv_freq.requires_grad
+                                    or (k is not None and k.requires_grad)):
+        raise RuntimeError("rope is forward-only: autograd / gradient inputs are not supported; "
+                           "call it under torch.no_grad() (inverse=True is its gradient)")
+    at = steps = None
+    wide = 0
     if positions is not None:
-        if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in (
-                (B, T), (T,)):
-            raise ValueError(f"rope: positions must be int32 or int64 ({B}, {T}) or ({T},), got "
-                             f"{tuple(positions.shape)} {positions.dtype}")
-        steps = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
-    q, k = (t if t is None or t.stride(3) == 1 else t.contiguous() for t in (q, k))
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    if k is not None and k.shape[2] and not Hq:
+        if (not isinstance(positions, torch.Tensor) or positions.device != dev
+                or positions.dtype not in (torch.int32, torch.int64)
+                or positions.shape not in ((B, T), (T,))):
+            raise ValueError(f"rope: positions must be int32 or int64 ({B}, {T}) or ({T},) on q's "
+                             "device")
+        steps = positions.stride()
+        steps = _strides2(steps if len(steps) == 2 else (0,) + steps)
+        at, wide = positions.data_ptr(), int(positions.dtype == torch.int64)
+    if Hkv and not Hq:
         raise ValueError("rope: q has no heads")
-    if q.numel():
-        has_k = k is not None and k.shape[2] > 0
-        _lib.call(
-            q, _lib.lib().ttcd_rope_fwd, q.data_ptr(), k.data_ptr() if has_k else None,
-            q_out.data_ptr(), k_out.data_ptr() if has_k else None, inv_freq.data_ptr(), n,
-            None if positions is None else positions.data_ptr(),
-            int(positions is not None and positions.dtype == torch.int64),
-            None if steps is None else _lib.strides2(steps), int(offset), B, T, Hq,
-            k.shape[2] if has_k else 0, D, _lib.strides4(q.stride()),
-            _lib.strides4(k.stride()) if has_k else None, _lib.strides4(q_out.stride()),
-            _lib.strides4(k_out.stride()) if has_k else None, int(bool(interleaved)),
-            int(bool(inverse)), float(scale), _DT[q.dtype])
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    if inv_freq.stride(0) != 1:
+        inv_freq = inv_freq.contiguous()
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = k_at = k_to = k_strides = k_dense = None
+    if k is not None:
+        if k.stride(3) != 1:
+            k = k.contiguous()
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+        if Hkv:
+            k_at, k_to = k.data_ptr(), k_out.data_ptr()
+            k_strides, k_dense = _strides4(k.stride()), _strides4(k_out.stride())
+    if B and T and Hq:
+        _lib.call(q, _lib.lib().ttcd_rope_fwd, q.data_ptr(), k_at, q_out.data_ptr(), k_to,
+                  inv_freq.data_ptr(), n, at, wide, steps, offset, B, T, Hq, Hkv, D,
+                  _strides4(q.stride()), k_strides, _strides4(q_out.stride()), k_dense,
+                  int(interleaved), int(inverse), scale, code)
     return q_out if k is None else (q_out, k_out)

@@ -73,8 +73,8 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0, top_
     if logits.stride(-1) != 1 or logits.dim() > 2:
         logits = logits.reshape(R, V).contiguous()  # leading dimensions that merge: no copy
     uniform = uniform.contiguous()
-    tokens = torch.empty(rows, dtype=torch.int64, device=dev)
-    logprobs = torch.empty(rows, dtype=torch.float32, device=dev) if return_logprob else None
+    tokens = torch.empty_like(uniform, dtype=torch.int64)
+    logprobs = torch.empty_like(uniform) if return_logprob else None
     if R:
         _lib.call(logits, _lib.lib().ttcd_sample_fwd, logits.data_ptr(),
                   logits.stride(0) if logits.dim() == 2 else 0, R, V, uniform.data_ptr(),
@@ -105,14 +105,14 @@ def tree_accept(parents: torch.Tensor, tokens: torch.Tensor, picked: torch.Tenso
     if counts is not None and (not isinstance(counts, torch.Tensor) or counts.shape != (B,)
                                or counts.dtype != torch.int32 or counts.device != dev):
         raise ValueError(f"tree_accept: counts must be int32 ({B},) on the parents' device")
-    path = torch.empty(B, N, dtype=torch.int32, device=dev)
-    accepted = torch.empty(B, dtype=torch.int32, device=dev)
-    following = torch.empty(B, dtype=torch.int64, device=dev)
     if N < 1:
         raise ValueError("tree_accept: trees of no nodes")
+    parents, tokens, picked = parents.contiguous(), tokens.contiguous(), picked.contiguous()
+    counts = None if counts is None else counts.contiguous()
+    path = torch.empty_like(parents)
+    accepted = parents.new_empty(B) if counts is None else torch.empty_like(counts)
+    following = picked.new_empty(B)
     if B:
-        parents, tokens, picked = parents.contiguous(), tokens.contiguous(), picked.contiguous()
-        counts = None if counts is None else counts.contiguous()
         _lib.call(parents, _lib.lib().ttcd_tree_accept, parents.data_ptr(), tokens.data_ptr(),
                   picked.data_ptr(), _ptr(counts), path.data_ptr(), accepted.data_ptr(),
                   following.data_ptr(), B, N)
