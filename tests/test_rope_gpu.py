@@ -12,7 +12,7 @@ import torch
 
 import ttcd_amd
 from oracle import drafted_ref
-from ttcd_amd import rope, rope_frequencies
+from ttcd_amd import _lib, rope, rope_frequencies
 
 pytestmark = pytest.mark.gpu
 
@@ -37,7 +37,8 @@ def _check(x, y, inv, pos, **kw):
 @pytest.mark.parametrize("dtype", [BF, HF, SF])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("D,n", [(128, 64), (128, 32), (64, 8), (64, 30), (80, 40), (80, 11),
-                                 (256, 128), (2, 1), (7, 3), (96, 24), (1024, 512)])
+                                 (256, 128), (2, 1), (7, 3), (96, 24), (1024, 512), (64, 7),
+                                 (96, 13), (16, 5), (8, 1)])
 @pytest.mark.parametrize("B,T", [(1, 1), (3, 37)])
 def test_layouts(gpu, dtype, interleaved, D, n, B, T):
     q, k = _rand(1, B, T, 3, D, dtype=dtype).cuda(), _rand(2, B, T, 2, D, dtype=dtype).cuda()
@@ -131,6 +132,20 @@ def test_agrees_with_the_prologue(gpu):
     for x, y in zip(ttcd_amd.qk_norm_rope(q, k, None, None, 0.0, cos, sin), rope(q, k, inv)):
         # u (|x0| + |x1|) of the tables, u |y| of either result, |y| <= 2 ** 0.5 max |x|
         assert (x.double() - y.double()).abs().max() <= 5 * U[BF] * q.abs().max().double()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D,n", [(64, 32), (64, 7), (96, 5), (10, 5)])
+def test_outputs_in_place(gpu, interleaved, D, n):
+    """The C entry writes over its inputs, the border of what turns within a vector or not."""
+    q, k = _rand(1, 2, 33, 3, D).cuda(), _rand(2, 2, 33, 2, D).cuda()
+    inv, _ = rope_frequencies(2 * n, 1e4, device="cuda")
+    want = rope(q, k, inv, offset=3, interleaved=interleaved)
+    qs, ks = (_lib.strides4(x.stride()) for x in (q, k))
+    _lib.check(_lib.lib().ttcd_rope_fwd(
+        q.data_ptr(), k.data_ptr(), q.data_ptr(), k.data_ptr(), inv.data_ptr(), n, None, 0, None, 3,
+        2, 33, 3, 2, D, qs, ks, qs, ks, int(interleaved), 0, 1.0, _lib.DTYPE_BF16, _lib.stream(q)))
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
 
 
 def test_empty_and_another_stream_and_a_graph(gpu):

@@ -65,9 +65,28 @@ struct Vec {
   T e[N];
 };
 
-// VE elements of 16 bytes (all sizes, strides and addresses allow it), or 1. PAIRS:
-// interleaved.
+// The rotation of a vector whose channels the border of what turns may cut: the halves' partners
+// one by one from the head (lines that are there), interleaved ones from the vector.
 template <typename T, int VE, bool PAIRS>
+__device__ __forceinline__ Vec<T, VE> rotate_cut(const Vec<T, VE>& x, const T* head, int d0, int n,
+                                                 const float2* turn) {
+  Vec<T, VE> y = x;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    const int d = d0 + e;
+    if (d >= 2 * n) break;
+    const bool second = PAIRS ? d % 2 : d >= n;
+    const float2 cs = turn[PAIRS ? d / 2 : second ? d - n : d];
+    const T other = PAIRS ? x.e[e ^ 1] : head[second ? d - n : d + n];
+    const float v = static_cast<float>(x.e[e]), w = static_cast<float>(other);
+    y.e[e] = static_cast<T>(second ? fmaf(w, cs.y, v * cs.x) : fmaf(v, cs.x, -(w * cs.y)));
+  }
+  return y;
+}
+
+// VE elements of 16 bytes (all strides and addresses allow it), or 1. PAIRS: interleaved. CUT:
+// the border of what turns lies within a vector.
+template <typename T, int VE, bool PAIRS, bool CUT>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a) {
   typedef Vec<T, VE> V __attribute__((aligned(VE * sizeof(T))));
   extern __shared__ float2 turns[];  // (tokens, n)
@@ -75,13 +94,15 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a) {
   const int64_t first = (int64_t)blockIdx.x * kRopeTasks;
   const int64_t token0 = first / a.per_token.d;
   const int at0 = (int)(first - token0 * a.per_token.d);
-  constexpr int R = PAIRS && VE > 1 ? 1 : 2;  // vectors of a task
-  const int turning = PAIRS && VE > 1 ? 2 * n / VE : n / VE;  // tasks of a head that turn
+  constexpr int R = CUT || (PAIRS && VE > 1) ? 1 : 2;  // vectors of a task
+  // tasks of a head that turn
+  const int turning = CUT ? (2 * n + VE - 1) / VE : PAIRS && VE > 1 ? 2 * n / VE : n / VE;
 
   V x[kRopeIter][2];
   int64_t dst[kRopeIter];
   int pair[kRopeIter], step[kRopeIter], tok[kRopeIter];
   T* out[kRopeIter];
+  const T* in[kRopeIter];
 #pragma unroll
   for (int it = 0; it < kRopeIter; ++it) {
     const int local = at0 + it * kRopeThreads + threadIdx.x;
@@ -100,7 +121,12 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a) {
                    : static_cast<T*>(a.q_out) + b * a.qo_sb + t * a.qo_st + h * a.qo_sh;
     // where the task's first vector lies, how far the second, and the first pair (-1: a copy)
     int d0;
-    if (u < turning) {
+    in[it] = src;
+    if (CUT) {
+      pair[it] = u < turning ? 0 : -1;
+      d0 = u * VE;
+      step[it] = 0;
+    } else if (u < turning) {
       pair[it] = PAIRS && VE > 1 ? u * VE / 2 : u * VE;
       d0 = PAIRS ? u * VE * (VE > 1 ? 1 : 2) : u * VE;
       step[it] = PAIRS ? 1 : n;
@@ -131,7 +157,10 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a) {
     if (out[it] == nullptr) continue;
     V y0 = x[it][0], y1 = y0;
     if constexpr (R == 2) y1 = x[it][1];
-    if (pair[it] >= 0) {
+    if (CUT) {
+      if (pair[it] >= 0)
+        y0 = rotate_cut<T, VE, PAIRS>(x[it][0], in[it], (int)dst[it], n, turns + tok[it] * n);
+    } else if (pair[it] >= 0) {
       const float2* turn = turns + tok[it] * n + pair[it];
       auto rotate = [&](float2 cs, T& e0, T& e1) __attribute__((always_inline)) {
         const float v0 = static_cast<float>(e0), v1 = static_cast<float>(e1);
@@ -152,12 +181,12 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a) {
   }
 }
 
-template <typename T, int VE>
+template <typename T, int VE, bool CUT>
 hipError_t launch_layout(const RopeArgs& args, bool pairs, hipStream_t st) {
   RopeArgs a = args;
   // tasks of a head: of the channels that turn, then copies
   const int turning = pairs && VE > 1 ? 2 * a.n / VE : a.n / VE;
-  const int per_head = turning + (a.D - 2 * a.n) / VE;
+  const int per_head = CUT ? a.D / VE : turning + (a.D - 2 * a.n) / VE;
   const int per_token = per_head * (a.Hq + a.Hkv);
   a.per_head = make_fast_div(per_head);
   a.per_token = make_fast_div(per_token);
@@ -168,26 +197,32 @@ hipError_t launch_layout(const RopeArgs& args, bool pairs, hipStream_t st) {
   const int64_t span = std::min((int64_t)(kRopeTasks - 1 + per_token - 1) / per_token + 1, a.tokens);
   const size_t lds = (size_t)span * a.n * sizeof(float2);
   if (pairs)
-    hipLaunchKernelGGL((rope_kernel<T, VE, true>), dim3((unsigned)blocks), dim3(kRopeThreads), lds,
+    hipLaunchKernelGGL((rope_kernel<T, VE, true, CUT>), dim3((unsigned)blocks), dim3(kRopeThreads), lds,
                        st, a);
   else
-    hipLaunchKernelGGL((rope_kernel<T, VE, false>), dim3((unsigned)blocks), dim3(kRopeThreads),
+    hipLaunchKernelGGL((rope_kernel<T, VE, false, CUT>), dim3((unsigned)blocks), dim3(kRopeThreads),
                        lds, st, a);
   return hipGetLastError();
 }
 
-// Vectors where every one of them lies within a head's channels on one side of every border
-// and at a multiple of 16 bytes.
+// Vectors where heads are whole ones at multiples of 16 bytes: two of them a task where the
+// border of what turns is one of theirs too, else with a partner read apart, which needs
+// outputs that are not the inputs (12382 tokens of 6 heads of 64, 7 pairs each: 11.2 us, one
+// element a task 17.5).
 template <typename T>
 hipError_t launch_typed(const RopeArgs& a, bool pairs, hipStream_t st) {
   constexpr int VE = 16 / sizeof(T);
   const int64_t strides[] = {a.q_sb,  a.q_st,  a.q_sh,  a.k_sb,  a.k_st,  a.k_sh,
                              a.qo_sb, a.qo_st, a.qo_sh, a.ko_sb, a.ko_st, a.ko_sh};
-  bool wide = a.D % VE == 0 && (pairs ? 2 * a.n : a.n) % VE == 0;
+  bool wide = a.D % VE == 0;
   for (int64_t s : strides) wide = wide && s % VE == 0;
   for (const void* p : {a.q, a.k, (const void*)a.q_out, (const void*)a.k_out})
     wide = wide && (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
-  return wide ? launch_layout<T, VE>(a, pairs, st) : launch_layout<T, 1>(a, pairs, st);
+  if (!wide) return launch_layout<T, 1, false>(a, pairs, st);
+  if ((pairs ? 2 * a.n : a.n) % VE == 0) return launch_layout<T, VE, false>(a, pairs, st);
+  if (a.q == a.q_out || (a.k != nullptr && a.k == a.k_out))
+    return launch_layout<T, 1, false>(a, pairs, st);
+  return launch_layout<T, VE, true>(a, pairs, st);
 }
 
 }  // namespace

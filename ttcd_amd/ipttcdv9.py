@@ -76,6 +76,11 @@ forward() with one token a call. With keep=.. a full-causal model's layers drop
 the keys of least accumulated attention weight after a call that leaves more
 than that. The reference has neither.
 
+Drafted tokens: forward(.., tree=parents) takes the nodes of a tree (kv4_tree_attn) over such a
+cache of one sequence instead of its next tokens, and leaves it as it is; cache.accept() then
+moves the accepted ones into it. generate() samples a text, a token a call or, with a callable
+that drafts, as many as a tree of them agree with.
+
 Not covered (raise NotImplementedError): qkv_bias, non-causal TTT conv,
 ttt_weight_renorm, Muon, normalised TTT features or proj-diff,
 ttt_output_use_teacher_conv, l2 softmax, a cache together with a padding
@@ -92,6 +97,7 @@ from . import attn as _attn
 from . import epilogue as _epi
 from . import kv4 as _kv4
 from . import prologue as _pro
+from . import sampling as _sampling
 from . import ttt as _ttt
 from .linear import project
 
@@ -327,6 +333,8 @@ class IPTTCDv9Prefill:
         """The teacher window within each row's unpadded tokens / each packed
         sequence (fla Attention's varlen path) or over whole rows; over a 4-bit
         cache's keys where the layer has one."""
+        if ctx.tree is not None:
+            return _kv4.kv4_tree_attn(q, held, ctx.cache.drafts[ctx.layer], ctx.tree, self.window_t)
         if held is not None:
             return ctx.cache.attend(q, held, self.window_t)
         if ctx.cu_seqlens is None:
@@ -401,8 +409,11 @@ class IPTTCDv9Prefill:
         xa = x  # attn_norm output: the gate's input
         q, k, v = self._qkv(i, x, ctx)
         held = None  # a 4-bit cache of this layer, this chunk in it
+        ctx.layer = i
         if ctx.cache is not None:
-            if ctx.cache.bits == 4:
+            if ctx.tree is not None:
+                held = ctx.cache.draft(i, k, v)
+            elif ctx.cache.bits == 4:
                 held = ctx.cache.append(i, k, v)
             else:
                 # the cached keys of earlier chunks, then this chunk's (Tk >= T)
@@ -442,12 +453,14 @@ class IPTTCDv9Prefill:
         return residual, y
 
     def _prefill_context(self, B: int, T: int, attention_mask, cu_seqlens,
-                         cache: "IPTTCDv9Cache | None" = None) -> "_Prefill":
+                         cache: "IPTTCDv9Cache | None" = None, tree=None) -> "_Prefill":
         """_use_fast_prefill_path (modeling_ipttcdv9.py:562-574) and what the
         fallback needs: unpad indices and cu_seqlens for a padding mask,
         per-sequence rotary tables for packed sequences; the rotary offset and
         the cache of a cached prefill."""
         ctx = _Prefill()
+        if tree is not None and not isinstance(cache, IPTTCDv9Cache):
+            raise ValueError("a tree of drafted tokens needs an IPTTCDv9Cache")
         if cache is not None:
             if not isinstance(cache, IPTTCDv9Cache):
                 raise ValueError("cache must be an IPTTCDv9Cache")
@@ -461,6 +474,8 @@ class IPTTCDv9Prefill:
             cache.reserve(T, None if self.window_t < 0 else self.window_t, student)
             ctx.cache, ctx.offset = cache, cache.seen
             attention_mask = None
+            if tree is not None:
+                self._tree_context(ctx, B, T, tree)
         if attention_mask is not None:
             if attention_mask.shape != (B, T):
                 raise ValueError(f"attention_mask must be (B, T) = ({B}, {T}), got "
@@ -492,33 +507,131 @@ class IPTTCDv9Prefill:
                     and ctx.cu_seqlens is None)
         return ctx
 
+    def _tree_context(self, ctx: "_Prefill", B: int, T: int, tree) -> None:
+        """The parents on the GPU, and rotary rows of each node's position: the tokens seen and
+        its depth."""
+        if B != 1:
+            raise NotImplementedError("a tree of drafted tokens for more than one sequence: the "
+                                      "cache counts the tokens of all together")
+        if ctx.cache.bits != 4 or ctx.cache.keep is not None:
+            raise NotImplementedError("a tree of drafted tokens over other than a 4-bit cache that "
+                                      "keeps its keys")
+        if T > _kv4.TREE_NODES or (self.ttt and T >= self.cfg["ttt_chunk"]):
+            raise ValueError(f"a tree of {T} nodes: at most {_kv4.TREE_NODES}, and fewer than a "
+                             "TTT layer's ttt_chunk")
+        parents = [int(p) for p in (tree.flatten().tolist() if isinstance(tree, torch.Tensor)
+                                    else tree)]
+        if len(parents) != T or any(not -1 <= p < i for i, p in enumerate(parents)):
+            raise ValueError(f"tree must be the {T} nodes' parents, each -1 or a node before")
+        depth = []
+        for p in parents:
+            depth.append(0 if p < 0 else depth[p] + 1)
+        ctx.tree = torch.tensor([parents], dtype=torch.int32, device=self.dev)
+        pos = torch.tensor(depth, device=self.dev) + ctx.offset
+        cos, sin = self.tables(ctx.offset + T)
+        ctx.tables, ctx.offset = (cos[pos], sin[pos]), 0
+        ctx.cache.begin_draft(T)
+
     @torch.inference_mode()
     def forward(self, input_ids: torch.Tensor, logits_to_keep: int = 1,
                 attention_mask: torch.Tensor | None = None,
                 cu_seqlens: torch.Tensor | None = None,
-                cache: "IPTTCDv9Cache | None" = None) -> torch.Tensor:
+                cache: "IPTTCDv9Cache | None" = None, tree=None) -> torch.Tensor:
         """Logits (B, logits_to_keep, vocab) of the prefill of `input_ids`
         (B, T), as IPTTCDForCausalLM(input_ids, logits_to_keep=...) returns them
         with fuse_linear_cross_entropy off (bench_prefill.py:73-74).
         attention_mask: the (B, T) 0/1 padding mask; cu_seqlens: packed
         sequences of a (1, T) batch (int32, 0 .. T); cache: an IPTTCDv9Cache
         holding the earlier chunks of the prompt (empty for the first), which
-        this call extends with its T tokens."""
+        this call extends with its T tokens. tree: the parents of T drafted tokens (a sequence
+        of ints or a tensor; node i follows node tree[i] < i, -1 what the cache holds), of which
+        the logits of all come back; cache.accept() then takes those to keep."""
         if input_ids.dim() != 2 or input_ids.device != self.dev:
             raise ValueError("input_ids must be (B, T) on the model's device")
         B, T = input_ids.shape
-        ctx = self._prefill_context(B, T, attention_mask, cu_seqlens, cache)
+        ctx = self._prefill_context(B, T, attention_mask, cu_seqlens, cache, tree)
         h = F.embedding(input_ids, self.w["model.embeddings.weight"])
         y = None
         for i in range(self.cfg["num_hidden_layers"]):
             h, y = self.layer(i, h, y, ctx)
-        if cache is not None:
+        if tree is not None:
+            logits_to_keep = T
+            cache.end_draft()
+        elif cache is not None:
             cache.advance(T)
         if logits_to_keep > 0:  # only the kept rows of the last block's output
             h, y = h[:, -logits_to_keep:], y[:, -logits_to_keep:]
         keep = h + y
         x = _epi.rmsnorm(keep.contiguous(), self.w["model.norm.weight"], self.cfg["norm_eps"])
         return F.linear(x, self.w["lm_head.weight"])
+
+
+    @torch.inference_mode()
+    def generate(self, input_ids: torch.Tensor, count: int, uniform: torch.Tensor | None = None, *,
+                 temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
+                 draft=None, cache: "IPTTCDv9Cache | None" = None) -> torch.Tensor:
+        """The `count` tokens after input_ids (1, T), (1, count) int64, each sampled
+        (ttcd_amd.sample, with these settings) by the uniform number of its place: fp32
+        (count,) on the model's device, None at temperature 0. cache: a 4-bit IPTTCDv9Cache with
+        room for it all, of which what it holds comes before input_ids (None: an own one);
+        it then holds all but the last token.
+
+        draft: a callable that gets the tokens so far (a list of ints, input_ids first) and the
+        most that are of use, and returns (parents, tokens) of drafted ones after them, lists
+        (parents: -1 the last token, or a drafted one before). They go through the model at
+        once, up to 255 of them, and those stay that are what is sampled at their place: the
+        text is the one of a token a call, as far as the roundings of the two agree."""
+        if input_ids.dim() != 2 or input_ids.shape[0] != 1 or input_ids.shape[1] < 1:
+            raise ValueError("generate: input_ids must be (1, T), T >= 1")
+        if count < 1:
+            raise ValueError(f"generate: count must be >= 1, got {count}")
+        if uniform is None:
+            if temperature != 0:
+                raise ValueError("generate: sampling needs a uniform number for every token")
+            uniform = torch.zeros(count, device=self.dev)
+        if uniform.shape != (count,):
+            raise ValueError(f"generate: uniform must be ({count},), got {tuple(uniform.shape)}")
+        T, most = input_ids.shape[1], _kv4.TREE_NODES
+        if self.ttt:
+            most = min(most, self.cfg["ttt_chunk"] - 1)
+        if cache is None:
+            room = T + count + most
+            if self.window_t >= 0:
+                room = min(room, max(self.window_t, self.window_s if self.ttt else 0) + max(T, most))
+            cache = IPTTCDv9Cache(bits=4, capacity=room)
+        kw = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        logits = self.forward(input_ids, cache=cache)[:, -1]
+        done = _sampling.sample(logits, uniform[:1], **kw).tolist()
+        prompt = input_ids[0].tolist() if draft is not None else []
+        while len(done) < count:
+            left = count - len(done)
+            # a drafted token after the next left - 1 is of no use: the one that follows them
+            # is sampled
+            parents, tokens = [], []
+            if draft is not None and left > 1:
+                parents, tokens = draft(prompt + done, left - 1)
+            parents, tokens = list(parents)[:most - 1], list(tokens)[:most - 1]
+            if len(parents) != len(tokens):
+                raise ValueError("generate: draft must return as many parents as tokens")
+            tree = [-1] + [int(p) + 1 for p in parents]
+            ids = torch.tensor([[done[-1]] + [int(t) for t in tokens]], device=self.dev)
+            if len(tree) == 1:
+                logits = self.forward(ids, cache=cache)[:, -1]
+                done += _sampling.sample(logits, uniform[len(done):len(done) + 1], **kw).tolist()
+                continue
+            logits = self.forward(ids, cache=cache, tree=tree)[0]
+            place = []
+            for p in tree:
+                place.append(len(done) if p < 0 else place[p] + 1)
+            # places past the last have no number; what is sampled there is not kept
+            at = torch.tensor(place, device=self.dev).clamp(max=count - 1)
+            picked = _sampling.sample(logits, uniform[at], **kw)[None]
+            path, accepted, following = _sampling.tree_accept(
+                torch.tensor([tree], dtype=torch.int32, device=self.dev), ids, picked)
+            n = min(cache.accept(path, accepted, most=left), left)
+            done += (ids[0, path[0, 1:n].long()].tolist()
+                     + [int(picked[0, path[0, n - 1]])])[:left]
+        return torch.tensor([done], device=self.dev)
 
 
 def patch_fused_attn(model: IPTTCDv9Prefill, kernel: str = "triton") -> int:
@@ -579,6 +692,9 @@ class IPTTCDv9Cache:
         self.kv4: dict[int, _kv4.KV4Cache] = {}
         self._spare: _kv4.KV4Cache | None = None
         self._shape = None
+        self.drafts: dict[int, _kv4.KV4Cache] = {}  # the nodes' keys and values
+        self._begun = self._nodes = 0  # nodes of the last tree; 0 until it ends, and accepted
+        self._drafted = False  # a layer's draft may hold some
 
     def check(self, B: int, Hkv: int, D: int, dtype, device) -> None:
         shape = (B, Hkv, D, dtype, torch.device(device))
@@ -618,6 +734,49 @@ class IPTTCDv9Cache:
         self._open = True
         _kv4.kv4_append(held, k, v)
         return held
+
+    def begin_draft(self, T: int) -> None:
+        """A tree of T nodes is about to go through the layers: their drafts are emptied of
+        one that was not accepted."""
+        if self._drafted:
+            for d in self.drafts.values():
+                d.reset()
+        self._nodes, self._begun, self._drafted = 0, T, True
+
+    def draft(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> "_kv4.KV4Cache":
+        """The layer's 4-bit cache, with the nodes' keys and values in its draft."""
+        held = self.kv4.get(layer)
+        if held is None:
+            held = self.kv4[layer] = self._new()
+        d, room = self.drafts.get(layer), -(-self._begun // 32) * 32
+        if d is None or d.capacity < room:
+            B, Hkv, D, dtype, device = self._shape
+            d = self.drafts[layer] = _kv4.KV4Cache(B, Hkv, D, room, dtype, device)
+        _kv4.kv4_append(d, k, v)
+        return held
+
+    def end_draft(self) -> None:
+        """The tree has gone through every layer."""
+        self._nodes = self._begun
+
+    def accept(self, path: torch.Tensor, accepted: torch.Tensor, most: int | None = None) -> int:
+        """The nodes path[0, :accepted[0]] of the last tree (as tree_accept gives them, `most`
+        of them at the most) become the sequence's next tokens in every layer. Returns how
+        many (a host synchronisation)."""
+        if not self._nodes:
+            raise RuntimeError("IPTTCDv9Cache: no tree of drafted tokens to accept from")
+        if path.shape != (1, self._nodes):
+            raise ValueError(f"IPTTCDv9Cache: path must be (1, {self._nodes}), got "
+                             f"{tuple(path.shape)}")
+        if most is not None:
+            accepted = accepted.clamp(max=most)
+        n = min(max(int(accepted[0]), 0), self._nodes)
+        self._open = True
+        for i, held in self.kv4.items():
+            _kv4.kv4_commit(held, self.drafts[i], path, accepted, reset=True)
+        self._nodes, self._drafted = 0, False
+        self.advance(n)
+        return n
 
     def _new(self) -> "_kv4.KV4Cache":
         B, Hkv, D, dtype, device = self._shape
@@ -674,6 +833,8 @@ class _Prefill:
         self.max_seqlen = 0
         self.tables = None        # per-token rotary rows for packed sequences
         self.cache = None         # IPTTCDv9Cache of a cached prefill
+        self.tree = None          # parents of drafted tokens, (1, N) int32
+        self.layer = 0            # the one that runs
         self.offset = 0           # rotary offset: tokens prefilled before this call
 
 
