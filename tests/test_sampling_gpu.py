@@ -70,6 +70,30 @@ def test_vocabularies(gpu, dtype, V):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
+def test_few_kept_of_many(gpu, dtype):
+    """Rows long enough for a bound under the first top_k: ordinary ones, all equal, all
+    negative, one peak beside nothing, the peak in the first vector, few numbers, NaN above."""
+    V = 40007
+    x = _logits(2, 9, V, dtype)
+    x[1] = 1.5
+    x[2] = -x[2].abs() - 1
+    x[3] = 0.0
+    x[3, 30000] = 9.0
+    x[4] = x[4].abs() * 0.01
+    x[4, 3] = 30.0
+    x[5, 100:] = -INF
+    x[6, 12345] = NAN
+    x[7] = torch.arange(V).flip(0).div(400).floor().to(dtype)
+    x[8, 20:] = 0.25
+    u = _uniform(3, 9)
+    for k in (1, 2, 20, 63, 64, 65, 300, 1023, 1024, 1025):
+        _check(x, u, top_k=k)
+        _check(x[:, 3:], 1 - u, temperature=0.6, top_k=k, top_p=0.9, min_p=0.01)
+    _check(x, u, temperature=0)
+    _check(x[:, :32770], u, top_k=[1, 5, 64, 0, 1024, 7, 9, 2000, 33])
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
 def test_values_that_come_often(gpu, dtype):
     """Counts past 16 bits, in the first stretch and over several: all equal, two values, a
     masked half."""

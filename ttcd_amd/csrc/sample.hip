@@ -17,9 +17,10 @@
 // Of a row of 151936 bf16 logits alone (25 us on a CU): zeroing 0.8 us, counting 12.2 (LDS
 // atomics: 11 cycles for 64 tokens), sums of the values' weights 4.9 (f16, whose rows have
 // 8 times the values, 14.7: 64-bit arithmetic), cuts and draw 3.7 (one wavefront's
-// latencies), the token 2.6. 256 rows, 78 MB: 33 us, of which counting, at the rate of the
+// latencies), the token 2.6. 256 rows, 78 MB: 35 us, of which counting, at the rate of the
 // memory (4.4 TB/s), is 17.6. Reading the row again for the token took 9.3 of 256 rows and
-// 3.5 of one; the order of a value taken while counting, instead of its bits, 4 more.
+// 3.5 of one (streamed three times, with half the registers: 40 us for 36 of 256 rows); the
+// order of a value taken while counting, instead of its bits, 4 more.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -45,6 +46,7 @@ constexpr int kHeavyMost = kSampleVocab / kHeavy + 1;
 // count may have by then, are below 65536.
 constexpr int kStretch = 7;
 constexpr int kHeld = 2 * kStretch;  // that stay in registers
+constexpr int kGroup = 3;  // turns that are streamed at once; two groups make a stretch
 constexpr int kTurnsMost = kSampleVocab / 8 / kSampleThreads + 1;
 
 // The order of a 16-bit value is 0x7fff less its bits, of a negative one its bits: the
@@ -189,7 +191,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
   __shared__ double sums[kBlocks], powers[64];
   __shared__ uint32_t counts[kBlocks], ntok[kBlocks];
   __shared__ uint32_t heavy[2 * kHeavyMost], nheavy, least;
-  __shared__ int most;
+  __shared__ int most, lowest_group, highest_group;
   __shared__ uint32_t drawn, skip, many, seen[kTurnsMost * kSampleWaves];
   constexpr uint32_t kFirst = Order<T>::kFirst, kLast = Order<T>::kLast;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -208,6 +210,15 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
     return i < span.head ? i : i + 8 * span.vectors;
   };
 
+  double t = a.temperatures != nullptr ? (double)a.temperatures[r] : a.temperature;
+  const double top_p = a.top_ps != nullptr ? (double)a.top_ps[r] : a.top_p;
+  const double min_p = a.min_ps != nullptr ? (double)a.min_ps[r] : a.min_p;
+  int top_k = a.top_ks != nullptr ? a.top_ks[r] : a.top_k;
+  if (!(t > 0.0)) {  // the first
+    t = 1.0;
+    top_k = 1;
+  }
+
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     *reinterpret_cast<u32x4*>(hist + 4 * (i * kSampleThreads + tid)) = u32x4{0u, 0u, 0u, 0u};
@@ -216,6 +227,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
     nheavy = 0;
     least = 0xffffu;
     most = -0x8000;
+    lowest_group = 0x7fff;
+    highest_group = -0x8000;
   }
   __syncthreads();
 
@@ -239,10 +252,18 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
   };
   auto look = [&]() {
     __syncthreads();
-#pragma unroll 1
-    for (int at = 4 * tid; at < 32768; at += 4 * kSampleThreads) {
-      const u32x4 w = *reinterpret_cast<const u32x4*>(hist + at);
-      if (((w[0] | w[1] | w[2] | w[3]) & kHeavyBits) == 0) continue;
+    uint32_t any[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {  // all on their way before the first is looked at
+      const u32x4 w = *reinterpret_cast<const u32x4*>(hist + 4 * (k * kSampleThreads + tid));
+      any[k] = (w[0] | w[1] | w[2] | w[3]) & kHeavyBits;
+    }
+    uint32_t where = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) where |= (any[k] != 0 ? 1u : 0u) << k;
+    while (where != 0) {
+      const int at = 4 * (__builtin_ctz(where) * kSampleThreads + tid);
+      where &= where - 1;
       for (int i = 0; i < 8; ++i) {  // the counts of 8 values
         const uint32_t word = hist[at + i / 2], n = i % 2 ? word >> 16 : word & 0xffffu;
         if (n < kHeavy) continue;
@@ -261,28 +282,97 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
     lowest = __builtin_elementwise_min(lowest, __builtin_bit_cast(u16x2, both));
     highest = __builtin_elementwise_max(highest, __builtin_bit_cast(s16x2, both));
   }
-  // the row's first vectors stay in registers (a turn that the row does not reach: the first)
+  auto highest_of = [&](const u32x4& v) __attribute__((always_inline)) {
+    // words by value: a cast of a vector's element takes its first
+    const uint32_t w[4] = {v[0], v[1], v[2], v[3]};
+    return __builtin_elementwise_max(
+        __builtin_elementwise_max(__builtin_bit_cast(s16x2, w[0]), __builtin_bit_cast(s16x2, w[1])),
+        __builtin_elementwise_max(__builtin_bit_cast(s16x2, w[2]), __builtin_bit_cast(s16x2, w[3])));
+  };
+  // the row's first vectors (a turn that the row does not reach: the first)
+  const int turns = (span.vectors + kSampleThreads - 1) / kSampleThreads;
   u32x4 held[kHeld];
 #pragma unroll
   for (int j = 0; j < kHeld; ++j) {
     const int i = j * kSampleThreads + tid;
     held[j] = span.vectors > 0 ? body(i < span.vectors ? i : 0) : u32x4{};
   }
+  // f(turn, number, vector) for the turns from `from` up to `end` (numbers past the last: the
+  // last vector), before(turn) ahead of each group of them; the next group is on its way.
+  auto stream = [&](int from, int end, auto before, auto f) __attribute__((always_inline)) {
+    if (from >= end) return;
+    u32x4 next[kGroup];
+    auto load = [&](int j0) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < kGroup; ++j)
+        next[j] = body(min((j0 + j) * kSampleThreads + tid, span.vectors - 1));
+    };
+    load(from);
+#pragma unroll 1
+    for (int j0 = from; j0 < end; j0 += kGroup) {
+      u32x4 now[kGroup];
+#pragma unroll
+      for (int j = 0; j < kGroup; ++j) now[j] = next[j];
+      if (j0 + kGroup < end) load(j0 + kGroup);
+      before(j0);
+#pragma unroll
+      for (int j = 0; j < kGroup; ++j)
+        if (j0 + j < end) f(j0 + j, (j0 + j) * kSampleThreads + tid, now[j]);
+    }
+  };
+  // Of few kept tokens most vectors hold none: with the row's first turns dealt to top_k groups
+  // or more, the least of the groups' highest logits is one that top_k tokens reach. Vectors
+  // without such a one are not counted (all of a counted one are: those below are past the
+  // cut). Groups of 16 threads, or one; by bits, so of a positive logit, and not of a NaN.
+  // 20 of 151936, without it and with: one bf16 row 27.5 and 26.7 us, 64 30.6 and 29.1, 256
+  // (read at the memory's rate) 35.7 and 36.1; f16, whose sums are the fewer, 64 rows 37.0
+  // and 33.7, 512 83.7 and 77.6. The first turns are all that a thread holds; of rows under 4
+  // of them the bound would be loose and the count short.
+  int bound = -0x8000;
+  if (top_k > 0 && top_k <= kSampleThreads && span.vectors >= 4 * kSampleThreads) {
+    s16x2 top = {-0x8000, -0x8000};
+    auto look_at = [&](int, int i, const u32x4& v) __attribute__((always_inline)) {
+      if (i < span.vectors) top = __builtin_elementwise_max(top, highest_of(v));
+    };
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) look_at(j, j * kSampleThreads + tid, held[j]);
+    int group = max((int)top[0], (int)top[1]);
+    if (top_k <= kSampleThreads / 16) {
+#pragma unroll
+      for (int d = 1; d < 16; d *= 2) group = max(group, __shfl_xor(group, d));
+    }
+    int low = group, high = group;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      low = min(low, __shfl_xor(low, d));
+      high = max(high, __shfl_xor(high, d));
+    }
+    if (lane == 0) {
+      atomicMin(&lowest_group, low);
+      atomicMax(&highest_group, high);
+    }
+    __syncthreads();
+    if (lowest_group > 0 && highest_group <= (int)(kZero - kFirst)) bound = lowest_group;
+  }
+  const s16x2 below2 = {(int16_t)(bound - 1), (int16_t)(bound - 1)};
+  auto counts_in = [&](const u32x4& v) __attribute__((always_inline)) {
+    const s16x2 m = __builtin_elementwise_max(highest_of(v), below2);
+    return bound < 0 ||
+           __builtin_bit_cast(uint32_t, m) != __builtin_bit_cast(uint32_t, below2);
+  };
+  auto count = [&](int, int i, const u32x4& v) __attribute__((always_inline)) {
+    if (i < span.vectors && counts_in(v)) add_vector(v);
+  };
 #pragma unroll
   for (int j = 0; j < kHeld; ++j) {
-    if (j == kStretch && span.vectors > j * kSampleThreads) look();
-    if (j * kSampleThreads + tid < span.vectors) add_vector(held[j]);
+    if (j == kStretch && turns > j) look();
+    count(j, j * kSampleThreads + tid, held[j]);
   }
-  for (int from = kHeld * kSampleThreads; from < span.vectors; from += kStretch * kSampleThreads) {
-    u32x4 x[kStretch];
-#pragma unroll
-    for (int j = 0; j < kStretch; ++j)
-      x[j] = body(min(from + j * kSampleThreads + tid, span.vectors - 1));
-    look();
-#pragma unroll
-    for (int j = 0; j < kStretch; ++j)
-      if (from + j * kSampleThreads + tid < span.vectors) add_vector(x[j]);
-  }
+  stream(kHeld, turns,
+         [&](int j) __attribute__((always_inline)) {
+           if ((j - kHeld) % (2 * kGroup) == 0) look();
+         },
+         count);
   {
     uint32_t lo = min((uint32_t)lowest[0], (uint32_t)lowest[1]);
     int hi = max((int)highest[0], (int)highest[1]);
@@ -339,14 +429,6 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
     return;
   }
 
-  double t = a.temperatures != nullptr ? (double)a.temperatures[r] : a.temperature;
-  const double top_p = a.top_ps != nullptr ? (double)a.top_ps[r] : a.top_p;
-  const double min_p = a.min_ps != nullptr ? (double)a.min_ps[r] : a.min_p;
-  int top_k = a.top_ks != nullptr ? a.top_ks[r] : a.top_k;
-  if (!(t > 0.0)) {  // the first
-    t = 1.0;
-    top_k = 1;
-  }
   x.top = value_of<T>(best);
   x.per_t = 1.0 / t;
   const int first = best >> 7;
@@ -493,29 +575,11 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
     }
     return m;
   };
-  // the vector of a turn, from a register or from memory (in a turn that the row does not
-  // reach, another)
-  const int turns = (span.vectors + kSampleThreads - 1) / kSampleThreads;
-  auto each = [&](auto f) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j)
-      if (j < turns) f(j, held[j]);
-    for (int j0 = kHeld; j0 < turns; j0 += kStretch) {
-      u32x4 v[kStretch];
-#pragma unroll
-      for (int j = 0; j < kStretch; ++j)
-        v[j] = body(min((j0 + j) * kSampleThreads + tid, span.vectors - 1));
-#pragma unroll
-      for (int j = 0; j < kStretch; ++j)
-        if (j0 + j < turns) f(j0 + j, v[j]);
-    }
-  };
   // The one there is, or, in their order, the loose ones before the vectors, the vectors by
   // turns and wavefronts, the loose ones behind.
   const bool one = many == 1;
   if (one && tid < rest && is(row[loose(tid)])) a.tokens[r] = loose(tid);
-  each([&](int j, const u32x4& v) __attribute__((always_inline)) {
-    const int i = j * kSampleThreads + tid;
+  auto seek = [&](int j, int i, const u32x4& v) __attribute__((always_inline)) {
     uint32_t n = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) n += __popc(equal(v[e]));
@@ -526,7 +590,11 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
       n = sum_of(n);
       if (lane == 0) seen[j * kSampleWaves + wave] = n;
     }
-  });
+  };
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j)
+    if (j < turns) seek(j, j * kSampleThreads + tid, held[j]);
+  stream(kHeld, turns, [](int) {}, seek);
   if (one) return;
   __syncthreads();
   if (wave != 0) return;
@@ -618,12 +686,15 @@ __global__ __launch_bounds__(64) void tree_accept_kernel(AcceptArgs a) {
 
 }  // namespace
 
-hipError_t launch_sample(const SampleArgs& a, Elem dtype, hipStream_t stream) {
-  if (dtype == Elem::BF16)
-    hipLaunchKernelGGL(sample_kernel<__bf16>, dim3(a.R), dim3(kSampleThreads), 0, stream, a);
-  else
-    hipLaunchKernelGGL(sample_kernel<_Float16>, dim3(a.R), dim3(kSampleThreads), 0, stream, a);
+template <typename T>
+hipError_t launch_sample_typed(const SampleArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL(sample_kernel<T>, dim3(a.R), dim3(kSampleThreads), 0, stream, a);
   return hipGetLastError();
+}
+
+hipError_t launch_sample(const SampleArgs& a, Elem dtype, hipStream_t stream) {
+  return dtype == Elem::BF16 ? launch_sample_typed<__bf16>(a, stream)
+                             : launch_sample_typed<_Float16>(a, stream);
 }
 
 hipError_t launch_tree_accept(const AcceptArgs& a, hipStream_t stream) {
