@@ -14,13 +14,15 @@
 // drawn one with how many of its tokens come before the drawn token, and looks for that
 // one in the row, most of which is still in registers.
 //
-// Of a row of 151936 bf16 logits alone (25 us on a CU): zeroing 0.8 us, counting 12.2 (LDS
-// atomics: 11 cycles for 64 tokens), sums of the values' weights 4.9 (f16, whose rows have
-// 8 times the values, 14.7: 64-bit arithmetic), cuts and draw 3.7 (one wavefront's
-// latencies), the token 2.6. 256 rows, 78 MB: 35 us, of which counting, at the rate of the
-// memory (4.4 TB/s), is 17.6. Reading the row again for the token took 9.3 of 256 rows and
-// 3.5 of one (streamed three times, with half the registers: 40 us for 36 of 256 rows); the
-// order of a value taken while counting, instead of its bits, 4 more.
+// Of a row of 151936 bf16 logits alone (24 us on a CU): zeroing 0.8 us, counting 12.2 (LDS
+// atomics: 11 cycles for 64 tokens), sums of the values' weights 3.5 (f16, whose rows have
+// 8 times the values, 7; 64 lanes a block with an exponential for every two values 4.9 and
+// 14.7), cuts and draw 3.7 (one wavefront's latencies), the token 2.6. 256 rows, 78 MB: 34
+// us, of which counting, at the rate of the memory (4.4 TB/s), is 17.6. Reading the row again
+// for the token took 9.3 of 256 rows and 3.5 of one; the order of a value taken while
+// counting, instead of its bits, 4 more. Not counting what a bound under the first top_k
+// leaves out (20 of 151936: one row 25.9 to 25.1 us, 64 29.0 to 28.1, 256 34.3 to 34.6) was
+// not worth its code.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -38,7 +40,6 @@ typedef int16_t s16x2 __attribute__((ext_vector_type(2)));
 constexpr int kSampleThreads = 1024;
 constexpr int kSampleWaves = kSampleThreads / 64;
 constexpr int kBlocks = 512;     // of 128 values, 64 words of 2 counts
-constexpr int kBlocksWave = kBlocks / kSampleWaves;
 constexpr uint32_t kHeavy = 8192;  // a count of this and more moves to the list
 constexpr uint32_t kHeavyBits = (0x10000u - kHeavy) * 0x10001u;  // that such a count has some of
 constexpr int kHeavyMost = kSampleVocab / kHeavy + 1;
@@ -105,6 +106,13 @@ struct Row {
   __device__ __forceinline__ uint32_t word(int i) const {
     const uint32_t w = hist[i <= (int)kZero / 2 ? kZero / 2 - i : i];
     return i <= (int)kZero / 2 ? w << 16 | w >> 16 : w;
+  }
+  // Four of them, of orders 8 i and on.
+  __device__ __forceinline__ u32x4 words(int i) const {
+    const bool up = 8 * i <= (int)kZero;
+    const u32x4 w = *reinterpret_cast<const u32x4*>(hist + (up ? (kZero - 7) / 2 - 4 * i : 4 * i));
+    auto turned = [](uint32_t v) __attribute__((always_inline)) { return v << 16 | v >> 16; };
+    return up ? u32x4{turned(w[3]), turned(w[2]), turned(w[1]), turned(w[0])} : w;
   }
   // Those counts, 0 for what is no number.
   __device__ __forceinline__ void count(uint32_t w, uint32_t order, uint32_t* c0,
@@ -191,7 +199,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
   __shared__ double sums[kBlocks], powers[64];
   __shared__ uint32_t counts[kBlocks], ntok[kBlocks];
   __shared__ uint32_t heavy[2 * kHeavyMost], nheavy, least;
-  __shared__ int most, lowest_group, highest_group;
+  __shared__ int most;
   __shared__ uint32_t drawn, skip, many, seen[kTurnsMost * kSampleWaves];
   constexpr uint32_t kFirst = Order<T>::kFirst, kLast = Order<T>::kLast;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -227,8 +235,6 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
     nheavy = 0;
     least = 0xffffu;
     most = -0x8000;
-    lowest_group = 0x7fff;
-    highest_group = -0x8000;
   }
   __syncthreads();
 
@@ -282,13 +288,6 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
     lowest = __builtin_elementwise_min(lowest, __builtin_bit_cast(u16x2, both));
     highest = __builtin_elementwise_max(highest, __builtin_bit_cast(s16x2, both));
   }
-  auto highest_of = [&](const u32x4& v) __attribute__((always_inline)) {
-    // words by value: a cast of a vector's element takes its first
-    const uint32_t w[4] = {v[0], v[1], v[2], v[3]};
-    return __builtin_elementwise_max(
-        __builtin_elementwise_max(__builtin_bit_cast(s16x2, w[0]), __builtin_bit_cast(s16x2, w[1])),
-        __builtin_elementwise_max(__builtin_bit_cast(s16x2, w[2]), __builtin_bit_cast(s16x2, w[3])));
-  };
   // the row's first vectors (a turn that the row does not reach: the first)
   const int turns = (span.vectors + kSampleThreads - 1) / kSampleThreads;
   u32x4 held[kHeld];
@@ -320,48 +319,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
         if (j0 + j < end) f(j0 + j, (j0 + j) * kSampleThreads + tid, now[j]);
     }
   };
-  // Of few kept tokens most vectors hold none: with the row's first turns dealt to top_k groups
-  // or more, the least of the groups' highest logits is one that top_k tokens reach. Vectors
-  // without such a one are not counted (all of a counted one are: those below are past the
-  // cut). Groups of 16 threads, or one; by bits, so of a positive logit, and not of a NaN.
-  // 20 of 151936, without it and with: one bf16 row 27.5 and 26.7 us, 64 30.6 and 29.1, 256
-  // (read at the memory's rate) 35.7 and 36.1; f16, whose sums are the fewer, 64 rows 37.0
-  // and 33.7, 512 83.7 and 77.6. The first turns are all that a thread holds; of rows under 4
-  // of them the bound would be loose and the count short.
-  int bound = -0x8000;
-  if (top_k > 0 && top_k <= kSampleThreads && span.vectors >= 4 * kSampleThreads) {
-    s16x2 top = {-0x8000, -0x8000};
-    auto look_at = [&](int, int i, const u32x4& v) __attribute__((always_inline)) {
-      if (i < span.vectors) top = __builtin_elementwise_max(top, highest_of(v));
-    };
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j) look_at(j, j * kSampleThreads + tid, held[j]);
-    int group = max((int)top[0], (int)top[1]);
-    if (top_k <= kSampleThreads / 16) {
-#pragma unroll
-      for (int d = 1; d < 16; d *= 2) group = max(group, __shfl_xor(group, d));
-    }
-    int low = group, high = group;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      low = min(low, __shfl_xor(low, d));
-      high = max(high, __shfl_xor(high, d));
-    }
-    if (lane == 0) {
-      atomicMin(&lowest_group, low);
-      atomicMax(&highest_group, high);
-    }
-    __syncthreads();
-    if (lowest_group > 0 && highest_group <= (int)(kZero - kFirst)) bound = lowest_group;
-  }
-  const s16x2 below2 = {(int16_t)(bound - 1), (int16_t)(bound - 1)};
-  auto counts_in = [&](const u32x4& v) __attribute__((always_inline)) {
-    const s16x2 m = __builtin_elementwise_max(highest_of(v), below2);
-    return bound < 0 ||
-           __builtin_bit_cast(uint32_t, m) != __builtin_bit_cast(uint32_t, below2);
-  };
   auto count = [&](int, int i, const u32x4& v) __attribute__((always_inline)) {
-    if (i < span.vectors && counts_in(v)) add_vector(v);
+    if (i < span.vectors) add_vector(v);
   };
 #pragma unroll
   for (int j = 0; j < kHeld; ++j) {
@@ -432,36 +391,43 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
   x.top = value_of<T>(best);
   x.per_t = 1.0 / t;
   const int first = best >> 7;
-  // Sums of blocks, in turns of the wavefronts. First which there are, by 8 words at once.
-  auto block_of = [&](int j) __attribute__((always_inline)) { return j * kSampleWaves + wave; };
-  uint32_t some = x.nheavy > 0 ? 0xffffffffu : 0u;
+  // Sums of blocks, 4 at a time in turns of the wavefronts: 16 lanes a block, 8 values a lane,
+  // one exponential for all 8, since a block's values are a step apart and a weight's quotient
+  // to the next is the block's. Lane j of a wavefront has that of its j-th block. (No other
+  // number shares infinity's block.)
+  constexpr int kTurns = kBlocks / 4 / kSampleWaves;
+  auto block_of = [&](int turn, int j) __attribute__((always_inline)) {
+    return 4 * (turn * kSampleWaves + wave) + j;
+  };
+  const uint32_t begin = block_of(lane / 4 % kTurns, lane % 4) * 128;
+  double step = exp((value_of<T>(begin + 1) - value_of<T>(begin)) * x.per_t);
+  if (!(step <= 1.0)) step = 0.0;  // where no numbers are
+  u32x4 words = x.words(block_of(0, 0) * 16 + lane);
 #pragma unroll 1
-  for (int j0 = 0; j0 < kBlocksWave; j0 += 8) {
-    uint32_t w[8];
+  for (int turn = 0; turn < kTurns; ++turn) {
+    const u32x4 w = words;
+    const int b = block_of(turn, lane / 16);
+    words = x.words(block_of(min(turn + 1, kTurns - 1), 0) * 16 + lane);
+    uint32_t n = 0;
+    double s = 0.0;
+    if (x.nheavy > 0 || __ballot((w[0] | w[1] | w[2] | w[3]) != 0) != 0) {
+      const double q = __shfl(step, 4 * turn + lane / 16);
+      const uint32_t o = b * 128 + 8 * (lane % 16);
+      double weight = x.weight<T>(max(o, best));  // 1 for best itself, exactly
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = x.word(block_of(j0 + j) * 64 + lane);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) some |= (__ballot(w[j] != 0) != 0 ? 1u : 0u) << (j0 + j);
-  }
-  // A block's values are a step apart, so a weight's quotient to the next is the block's: lane
-  // j has that of the wavefront's j-th. (No other number shares infinity's block.)
-  const uint32_t begin = block_of(lane % kBlocksWave) * 128;
-  const double step = exp((value_of<T>(begin + 1) - value_of<T>(begin)) * x.per_t);
-  if (lane < kBlocksWave) {
-    ntok[block_of(lane)] = 0;
-    sums[block_of(lane)] = 0.0;
-  }
-  while (some != 0) {
-    const int j = __builtin_ctz(some), b = block_of(j);
-    some &= some - 1;
-    const uint32_t o = b * 128 + 2 * lane;
-    uint32_t c0, c1;
-    x.count(x.word(o / 2), o, &c0, &c1);
-    const double w0 = x.weight<T>(o);
-    const double w1 = o + 1 == best ? 1.0 : w0 * lane_of(step, j);  // what weighs 1 does exactly
-    const uint32_t n = sum_of(c0 + c1);
-    const double s = sum_of((c0 ? c0 * w0 : 0.0) + (c1 ? c1 * w1 : 0.0));
-    if (lane == 0) {
+      for (int i = 0; i < 4; ++i) {
+        uint32_t c0, c1;
+        x.count(w[i], o + 2 * i, &c0, &c1);
+        n += c0 + c1;
+        s = fma((double)c0, weight, s);
+        if (o + 2 * i >= best) weight *= q;
+        s = fma((double)c1, weight, s);
+        if (o + 2 * i + 1 >= best) weight *= q;
+      }
+      n = sum_of_row(n);
+      s = sum_of_row(s);
+    }
+    if (lane % 16 == 0) {
       ntok[b] = n;
       sums[b] = s;
     }

@@ -37,12 +37,18 @@ __device__ __forceinline__ V scan_before(V x, int lane, V* all = nullptr) {
   if (all != nullptr) *all = c + lane_of(x, 63);
   return dpp<0x111>(x) + (lane < 16 ? V(0) : lane < 32 ? a : lane < 48 ? b : c);
 }
+// The sum over a row of 16 lanes, in each of them, and over all.
 template <typename V>
-__device__ __forceinline__ V sum_of(V x) {
+__device__ __forceinline__ V sum_of_row(V x) {
   x += dpp<0x121>(x);  // row_ror:1, 2, 4, 8
   x += dpp<0x122>(x);
   x += dpp<0x124>(x);
   x += dpp<0x128>(x);
+  return x;
+}
+template <typename V>
+__device__ __forceinline__ V sum_of(V x) {
+  x = sum_of_row(x);
   return lane_of(x, 0) + lane_of(x, 16) + (lane_of(x, 32) + lane_of(x, 48));
 }
 __device__ __forceinline__ uint32_t max_of(uint32_t x) {
