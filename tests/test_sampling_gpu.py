@@ -70,6 +70,19 @@ def test_vocabularies(gpu, dtype, V):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
+def test_temperatures_whose_quotient_is_infinite(gpu, dtype):
+    """The highest weigh 1 each and nothing else anything, down to the least temperature."""
+    x = _logits(7, 4, 1003, dtype)
+    x[1, [9, 500, 1002]] = 20.0
+    x[2] = -3.0
+    x[3, 700] = INF
+    u = torch.tensor([0.5, 0.7, 0.999, 0.2])
+    for t in (1e-30, 1e-299, 1e-309, 5e-324):
+        _check(x, u, temperature=t)
+        _check(x, u, temperature=t, top_p=0.9, min_p=0.5)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
 def test_few_kept_of_many(gpu, dtype):
     """Rows long enough for a bound under the first top_k: ordinary ones, all equal, all
     negative, one peak beside nothing, the peak in the first vector, few numbers, NaN above."""

@@ -389,7 +389,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
   }
 
   x.top = value_of<T>(best);
-  x.per_t = 1.0 / t;
+  x.per_t = fmin(1.0 / t, 1e300);  // finite: what is 0 stays 0
   const int first = best >> 7;
   // Sums of blocks, 4 at a time in turns of the wavefronts: 16 lanes a block, 8 values a lane,
   // one exponential for all 8, since a block's values are a step apart and a weight's quotient
