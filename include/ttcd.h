@@ -639,8 +639,8 @@ ttcd_status ttcd_rope_fwd(const void* q, const void* k, void* q_out, void* k_out
                           float scale, ttcd_dtype dtype, void* stream);
 
 /*
- * A token from every row of logits (R, V) of BF16 or F16, V <= 2^20, rows row_stride
- * elements apart. Tokens rank by logit, of equal ones the lower index first; the weight
+ * A token from every row of logits (R, V) of BF16 or F16, R < 2^22, V <= 2^20, rows
+ * row_stride elements apart. Tokens rank by logit, of equal ones the lower index first; the weight
  * of one is exp((logit - highest) / temperature). Kept are the first top_k (0: all), of
  * those the shortest run with at least top_p (>= 1: all) of their sum, of those the ones
  * with at least min_p of the highest weight; tokens[r] is the first whose running sum
@@ -663,7 +663,7 @@ ttcd_status ttcd_sample_fwd(const void* logits, int64_t row_stride, int R, int V
  * ttcd_kv4_tree_attn_fwd; tokens, picked: (B, N) int64, the token of each node and the
  * one that followed it; counts: device int32[B] or NULL. path: (B, N) int32, the nodes in
  * order, -1 behind the last; accepted: (B), their number; next: (B) int64, what was
- * picked at the last (-1 of a sequence without nodes). N <= 256.
+ * picked at the last (-1 of a sequence without nodes). B < 2^26, N <= 256.
  */
 ttcd_status ttcd_tree_accept(const int32_t* parents, const int64_t* tokens,
                              const int64_t* picked, const int32_t* counts, int32_t* path,

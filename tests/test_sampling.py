@@ -60,6 +60,9 @@ def test_bad_arguments():
     assert walk(a=None) == walk(b=None) == walk(c=None) == walk(d=None) == walk(e=None) == INV
     assert walk(f=None) == walk(B=0) == walk(N=0) == INV
     assert walk(N=257) == UNSUP
+    # more threads than a launch has
+    assert _sample(R=1 << 22) == _sample(R=2 ** 31 - 1) == UNSUP
+    assert walk(B=1 << 26) == walk(B=2 ** 31 - 1) == UNSUP
 
 
 def test_python_refuses_the_cpu():

@@ -1685,6 +1685,8 @@ ttcd_status ttcd_sample_fwd(const void* logits, int64_t row_stride, int R, int V
     return fail(TTCD_ERR_INVALID_ARGUMENT, "need R, V >= 1 (got %d, %d)", R, V);
   if (V > ttcd::kSampleVocab)
     return fail(TTCD_ERR_UNSUPPORTED, "%d tokens a row: at most %d", V, ttcd::kSampleVocab);
+  // a launch has fewer than 2^32 threads: 1024 a row
+  if (R >= 1 << 22) return fail(TTCD_ERR_UNSUPPORTED, "grid too large (%d rows)", R);
   if (dtype != TTCD_DTYPE_BF16 && dtype != TTCD_DTYPE_F16)
     return fail(TTCD_ERR_UNSUPPORTED, "logits must be bf16 or f16");
   if (row_stride < 0) return fail(TTCD_ERR_INVALID_ARGUMENT, "row stride must be >= 0");
@@ -1725,6 +1727,8 @@ ttcd_status ttcd_tree_accept(const int32_t* parents, const int64_t* tokens,
     return fail(TTCD_ERR_INVALID_ARGUMENT, "need B, N >= 1 (got %d, %d)", B, N);
   if (N > ttcd::kTreeNodes)
     return fail(TTCD_ERR_UNSUPPORTED, "%d nodes: at most %d", N, ttcd::kTreeNodes);
+  if (B >= 1 << 26)  // 64 threads a sequence
+    return fail(TTCD_ERR_UNSUPPORTED, "grid too large (%d sequences)", B);
   const ttcd::AcceptArgs a = {parents, tokens, picked, counts, path, accepted, next, B, N};
   return from_hip(ttcd::launch_tree_accept(a, static_cast<hipStream_t>(stream)),
                   "tree accept launch");

@@ -77,7 +77,8 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0, top_
     logprobs = torch.empty_like(uniform) if return_logprob else None
     if R:
         _lib.call(logits, _lib.lib().ttcd_sample_fwd, logits.data_ptr(),
-                  logits.stride(0) if logits.dim() == 2 else 0, R, V, uniform.data_ptr(),
+                  logits.stride(0) if logits.dim() == 2 else 0, min(R, 2 ** 31 - 1),
+                  min(V, 2 ** 31 - 1), uniform.data_ptr(),
                   _ptr(ts), float(t), _ptr(ks), min(int(k), 2 ** 31 - 1), _ptr(ps), float(p),
                   _ptr(ms), float(m), tokens.data_ptr(), _ptr(logprobs), _DT[logits.dtype])
     return (tokens, logprobs) if return_logprob else tokens
@@ -115,5 +116,6 @@ def tree_accept(parents: torch.Tensor, tokens: torch.Tensor, picked: torch.Tenso
     if B:
         _lib.call(parents, _lib.lib().ttcd_tree_accept, parents.data_ptr(), tokens.data_ptr(),
                   picked.data_ptr(), _ptr(counts), path.data_ptr(), accepted.data_ptr(),
-                  following.data_ptr(), B, N)
+                  following.data_ptr(), min(B, 2 ** 31 - 1),
+                  min(N, 2 ** 31 - 1))
     return path, accepted, following
