@@ -222,9 +222,42 @@ def test_refusals():
     m.forward(ids, cache=cache, tree=one)
     with pytest.raises(ValueError, match="path"):
         cache.accept(torch.zeros(1, 3, dtype=torch.int32, device=DEV), torch.ones(1, device=DEV))
+    # nothing was written: the right call still goes
+    for p, n in ((torch.zeros(1, 4, device=DEV), torch.ones(1, dtype=torch.int32, device=DEV)),
+                 (torch.zeros(1, 4, dtype=torch.int32, device=DEV), torch.ones(1, device=DEV)),
+                 (torch.zeros(1, 4, dtype=torch.int32, device=DEV),
+                  torch.ones(2, dtype=torch.int32, device=DEV))):
+        with pytest.raises(ValueError, match="int32"):
+            cache.accept(p, n)
+    path, n = torch.zeros(1, 4, dtype=torch.int32, device=DEV), torch.ones(1, dtype=torch.int32,
+                                                                            device=DEV)
+    assert cache.accept(path, n) == 1 and cache.seen == 1
+    # a tree that other tokens have passed is of another place
+    m.forward(ids, cache=cache, tree=one)
+    m.forward(ids, cache=cache)
+    with pytest.raises(RuntimeError, match="no tree"):
+        cache.accept(path, n)
+    assert cache.seen == 5
     u = torch.zeros(3, device=DEV)
     for bad in (lambda: m.generate(ids, 0, u), lambda: m.generate(ids, 3), lambda: m.generate(ids, 4, u),
                 lambda: m.generate(ids.expand(2, 4), 3, u),
-                lambda: m.generate(ids, 3, u, draft=lambda t, n: ([-1], []))):
+                lambda: m.generate(ids, 3, u, draft=lambda t, n: ([-1], [])),
+                lambda: m.generate(ids, 3, u, draft=lambda t, n: ([-2], [1])),
+                lambda: m.generate(ids, 3, u, draft=lambda t, n: ([0], [1])),
+                lambda: m.generate(ids, 3, u, draft=lambda t, n: ([-1], [-1])),
+                lambda: m.generate(ids, 3, u, draft=lambda t, n: ([-1], [m.cfg["vocab_size"]]))):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_logits_that_are_no_numbers_end_a_text():
+    """A token -1 goes into no embedding."""
+    m = _model({"window_size": None})
+    m.w = dict(m.w)
+    m.w["lm_head.weight"] = torch.full_like(m.w["lm_head.weight"], float("nan"))
+    u = torch.zeros(3, device=DEV)
+    ids = _ids(1, 4, 0).to(DEV)
+    assert m.generate(ids, 1, u[:1]).tolist() == [[-1]]
+    for draft in (None, lambda t, n: ([-1], [1])):
+        with pytest.raises(RuntimeError, match="no logit"):
+            m.generate(ids, 3, u, draft=draft)

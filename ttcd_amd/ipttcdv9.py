@@ -603,7 +603,10 @@ class IPTTCDv9Prefill:
         logits = self.forward(input_ids, cache=cache)[:, -1]
         done = _sampling.sample(logits, uniform[:1], **kw).tolist()
         prompt = input_ids[0].tolist() if draft is not None else []
+        vocab = self.cfg["vocab_size"]
         while len(done) < count:
+            if done[-1] < 0:
+                raise RuntimeError(f"generate: no logit for token {len(done) - 1} is a number")
             left = count - len(done)
             # a drafted token after the next left - 1 is of no use: the one that follows them
             # is sampled
@@ -613,6 +616,9 @@ class IPTTCDv9Prefill:
             parents, tokens = list(parents)[:most - 1], list(tokens)[:most - 1]
             if len(parents) != len(tokens):
                 raise ValueError("generate: draft must return as many parents as tokens")
+            if any(not 0 <= t < vocab for t in tokens) or any(p < -1 for p in parents):
+                raise ValueError(f"generate: draft must return tokens of 0 .. {vocab - 1} and "
+                                 "parents of -1 or a drafted token before")
             tree = [-1] + [int(p) + 1 for p in parents]
             ids = torch.tensor([[done[-1]] + [int(t) for t in tokens]], device=self.dev)
             if len(tree) == 1:
@@ -765,16 +771,18 @@ class IPTTCDv9Cache:
         many (a host synchronisation)."""
         if not self._nodes:
             raise RuntimeError("IPTTCDv9Cache: no tree of drafted tokens to accept from")
-        if path.shape != (1, self._nodes):
-            raise ValueError(f"IPTTCDv9Cache: path must be (1, {self._nodes}), got "
-                             f"{tuple(path.shape)}")
+        dev = self._shape[-1]
+        for name, t, shape in (("path", path, (1, self._nodes)), ("accepted", accepted, (1,))):
+            if t.shape != shape or t.dtype != torch.int32 or t.device.type != dev.type:
+                raise ValueError(f"IPTTCDv9Cache: {name} must be int32 {shape} on the GPU, got "
+                                 f"{t.dtype} {tuple(t.shape)}")
         if most is not None:
             accepted = accepted.clamp(max=most)
         n = min(max(int(accepted[0]), 0), self._nodes)
         self._open = True
         for i, held in self.kv4.items():
             _kv4.kv4_commit(held, self.drafts[i], path, accepted, reset=True)
-        self._nodes, self._drafted = 0, False
+        self._drafted = False
         self.advance(n)
         return n
 
@@ -793,8 +801,10 @@ class IPTTCDv9Cache:
         return o
 
     def advance(self, T: int) -> None:
-        """T tokens have gone through every layer."""
+        """T tokens have gone through every layer. A tree that was not accepted before is of
+        another place now."""
         self.seen += T
+        self._nodes = 0
         if self.bits != 4:
             return
         self.held += T
