@@ -580,7 +580,8 @@ class IPTTCDv9Prefill:
         most that are of use, and returns (parents, tokens) of drafted ones after them, lists
         (parents: -1 the last token, or a drafted one before). They go through the model at
         once, up to 255 of them, and those stay that are what is sampled at their place: the
-        text is the one of a token a call, as far as the roundings of the two agree."""
+        text is the one of a token a call, as far as the roundings of the two agree. Logits none
+        of which is a number end it with a RuntimeError (as the last token they are a -1)."""
         if input_ids.dim() != 2 or input_ids.shape[0] != 1 or input_ids.shape[1] < 1:
             raise ValueError("generate: input_ids must be (1, T), T >= 1")
         if count < 1:
