@@ -624,11 +624,12 @@ ttcd_status ttcd_kv4_commit(ttcd_kv4_cache* cache, ttcd_kv4_cache* draft, const 
  * Rotary embedding at given positions: the first 2 * num_freq channels of every head in
  * pairs (i, num_freq + i), interleaved != 0: (2i, 2i + 1), turned by position *
  * inv_freq[i] (inverse != 0: back) and multiplied by scale; the others copied. The angle
- * is exact for any position below 2^53. q: (B, T, Hq, D), k: (B, T, Hkv, D), Hkv = 0:
- * none; outputs of the same shapes, which may be the inputs (same strides). Strides of
- * any sign and size but d-stride 1; 16-byte accesses are made where all allow it.
- * positions: int32, or int64 with positions_64 != 0, at b * position_stride[0] + t *
- * position_stride[1]; NULL: offset + t. D <= 1024. dtype BF16, F16 or F32.
+ * is exact where neither it nor the position exceeds 2^53 in size. q: (B, T, Hq, D), k:
+ * (B, T, Hkv, D), Hkv = 0: none; outputs of the same shapes, which may be the inputs (same
+ * strides). Strides of any sign and size but d-stride 1; 16-byte accesses are made where
+ * all allow it. positions: int32, or int64 with positions_64 != 0, at b *
+ * position_stride[0] + t * position_stride[1]; NULL: offset + t. D <= 1024. dtype BF16, F16
+ * or F32.
  */
 ttcd_status ttcd_rope_fwd(const void* q, const void* k, void* q_out, void* k_out,
                           const float* inv_freq, int num_freq, const void* positions,

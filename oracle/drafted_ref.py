@@ -8,11 +8,38 @@ import math
 import torch
 
 
+def _arctan_of_reciprocal(x, one):
+    """arctan(1 / x) in units of 1 / one, by its series."""
+    total, term, k = 0, one // x, 1
+    while term:
+        total += term // k if k % 4 == 1 else -(term // k)
+        term //= x * x
+        k += 2
+    return total
+
+
+_BITS = 240
+# 2 pi = 8 (4 arctan(1 / 5) - arctan(1 / 239)), in units of 2^-_BITS
+_TURN = 8 * (4 * _arctan_of_reciprocal(5, 1 << _BITS) - _arctan_of_reciprocal(239, 1 << _BITS))
+
+
+def _angle(p, f):
+    """p f modulo 2 pi, the product in integers: it passes 53 bits for positions from 2^29 on."""
+    num, den = f.as_integer_ratio()
+    a = (p * num << _BITS) // den % _TURN
+    return math.ldexp(a - _TURN if 2 * a > _TURN else a, -_BITS)
+
+
 def rope(x, inv_freq, positions, interleaved=False, scale=1.0, inverse=False):
     """x (B, T, H, D) turned by positions (B, T), float64, and sum |x| |turn| of each pair."""
     n = inv_freq.numel()
     y, mag = x.double().clone(), torch.zeros(x.shape, dtype=torch.float64)
-    a = positions.double()[..., None] * inv_freq.double() * (-1 if inverse else 1)
+    if positions.numel() and positions.abs().max() >= 2 ** 29:
+        a = torch.tensor([[[_angle(p, f) for f in inv_freq.tolist()] for p in row]
+                          for row in positions.tolist()], dtype=torch.float64)
+    else:
+        a = positions.double()[..., None] * inv_freq.double()
+    a = a * (-1 if inverse else 1)
     turn = torch.polar(torch.full_like(a, scale), a)[:, :, None]
     i = torch.arange(n)
     re, im = (2 * i, 2 * i + 1) if interleaved else (i, n + i)

@@ -98,3 +98,22 @@ def test_python_refuses_the_cpu():
     x = torch.zeros(1, 2, 2, 64)
     with pytest.raises(ValueError, match="GPU"):
         ttcd_amd.rope(x, x, torch.ones(32))
+
+
+def test_the_oracles_far_angles():
+    """The oracle's turns of far positions against decimals of 90 digits: the product of a position
+    and a frequency passes 53 bits from 2^29 on."""
+    from decimal import Decimal, getcontext
+    getcontext().prec = 90
+    two_pi = 2 * Decimal("3.14159265358979323846264338327950288419716939937510"
+                         "582097494459230781640628620899862803482534211706798")
+    f = torch.tensor([1.0, 0.8659643, 0.0123, 1e-5])
+    pos = torch.tensor([[5, 2 ** 29 + 1, 2 ** 40 - 1, 2 ** 52 + 12345, 2 ** 53 - 1, -2 ** 53 + 3]])
+    x = torch.zeros(1, 6, 1, 8)
+    x[..., :4] = 1.0  # (cos, sin) of every pair
+    y, _ = drafted_ref.rope(x, f, pos)
+    for t, p in enumerate(pos[0].tolist()):
+        for i, w in enumerate(f.tolist()):
+            a = float((Decimal(p) * Decimal(w)) % two_pi)
+            assert abs(y[0, t, 0, i].item() - math.cos(a)) < 1e-14
+            assert abs(y[0, t, 0, 4 + i].item() - math.sin(a)) < 1e-14

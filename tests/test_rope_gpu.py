@@ -188,3 +188,19 @@ def test_refusals(gpu):
             call()
     with pytest.raises(RuntimeError, match="forward-only"):
         rope(q.requires_grad_(), None, inv)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_the_farthest_positions(gpu, interleaved):
+    """Where position * inv_freq passes 53 bits (2^29 with 24 bits of a frequency) the angle is
+    exact all the same: the oracle multiplies in integers. The same bounds as near by."""
+    pos = torch.tensor([[2 ** 29 + 1, 2 ** 31 + 7, 2 ** 40 - 1, -2 ** 45 + 9, 2 ** 50 + 3,
+                         2 ** 52 + 12345, 2 ** 53 - 1, 2 ** 53, -2 ** 53 + 1]])
+    x = _rand(1, 1, 9, 2, 128, dtype=SF).cuda()
+    for base in (1e4, 1e6):
+        inv, _ = rope_frequencies(128, base, device="cuda")
+        _check(x, rope(x, None, inv, pos.cuda(), interleaved=interleaved), inv, pos,
+               interleaved=interleaved)
+    start = 2 ** 53 - 9
+    _check(x, rope(x, None, inv, offset=start, interleaved=interleaved), inv,
+           start + torch.arange(9)[None], interleaved=interleaved)

@@ -3,10 +3,10 @@
 //
 // Pair i of the first 2 n channels, (x_i, x_{n+i}) or (x_2i, x_{2i+1}), turns by the
 // angle p f_i: y0 = x0 c - x1 s, y1 = x0 s + x1 c with c = scale cos, s = scale sin
-// (the inverse: by -p f_i); channels from 2 n on are copied. p f_i is taken in 64 bits
-// and brought into a quarter turn there (a float holds the angle of position 10^6 to
-// 0.03), cosine and sine of the rest in 32; the products are 32 bits, rounded to the
-// type once.
+// (the inverse: by -p f_i); channels from 2 n on are copied. p f_i is taken in 64 bits, its
+// product's remainder beside it (from position 2^29 on it has more than 53 bits), and brought
+// into a quarter turn there (a float holds the angle of position 10^6 to 0.03), cosine and
+// sine of the rest in 32; the products are 32 bits, rounded to the type once.
 //
 // A task is a vector of 16 bytes of a head (interleaved pairs, copies) or two of them
 // (halves); tasks run over heads and then tokens, 512 in a row a workgroup, two a
@@ -39,13 +39,18 @@ __device__ __forceinline__ double position(const RopeArgs& a, int b, int t) {
                  : (double)static_cast<const int32_t*>(a.positions)[at];
 }
 
-// cos and sin of a quarter turn's half at most, by their series: the next terms are
-// below 2^-29 there.
-__device__ __forceinline__ float2 cos_sin(double angle) {
+// cos and sin of p f. In a quarter turn's half at most, by their series: the next terms are
+// below 2^-29 there. Exact in p f, of which `lo` is what 53 bits lack, while it is below 2^53
+// in size: then k is a whole number that a double holds, though far out one that is up to 2
+// off, since 2 / pi is rounded, which a second step takes from the rest.
+__device__ __forceinline__ float2 cos_sin(double p, double f) {
+  const double angle = p * f, lo = fma(p, f, -angle);
   const double k = rint(angle * 0.63661977236758134308);  // 2 / pi
   // pi / 2 in two doubles, the second what the first lacks
   double r = fma(-k, 1.5707963267948965580, angle);
-  r = fma(-k, 6.1232339957367660359e-17, r);
+  r = fma(-k, 6.1232339957367660359e-17, r) + lo;
+  const double more = rint(r * 0.63661977236758134308);
+  r = fma(-more, 1.5707963267948965580, r);
   const float x = (float)r, x2 = x * x;
   float s = 2.7557319e-6f;
   s = fmaf(s, x2, -1.9841270e-4f);
@@ -58,7 +63,7 @@ __device__ __forceinline__ float2 cos_sin(double angle) {
   c = fmaf(c, x2, 4.1666667e-2f);
   c = fmaf(c, x2, -0.5f);
   c = fmaf(c, x2, 1.0f);
-  const int quarter = (int)(int64_t)k & 3;
+  const int quarter = (int)((int64_t)k + (int64_t)more) & 3;
   const float cs = quarter & 1 ? s : c, sn = quarter & 1 ? c : s;
   return {quarter == 1 || quarter == 2 ? -cs : cs, quarter >= 2 ? -sn : sn};
 }
@@ -148,7 +153,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a) {
     for (int i = threadIdx.x; i < tokens * n; i += kRopeThreads) {
       const int j = a.div_n.quot(i), f = i - j * n;
       const int token = (int)token0 + j, b = a.T.quot(token), t = token - b * (int)a.T.d;
-      float2 cs = cos_sin(position(a, b, t) * (double)a.inv_freq[f]);
+      float2 cs = cos_sin(position(a, b, t), (double)a.inv_freq[f]);
       cs.x *= a.scale;
       cs.y *= a.inverse ? -a.scale : a.scale;
       turns[i] = cs;
