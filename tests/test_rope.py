@@ -117,3 +117,13 @@ def test_the_oracles_far_angles():
             a = float((Decimal(p) * Decimal(w)) % two_pi)
             assert abs(y[0, t, 0, i].item() - math.cos(a)) < 1e-14
             assert abs(y[0, t, 0, 4 + i].item() - math.sin(a)) < 1e-14
+
+
+def test_more_threads_than_a_launch_has():
+    """One element an access, 512 tasks a workgroup of 256 threads: 2^33 tasks are 2^32 threads.
+    Interleaved or not, and as many with whole vectors."""
+    odd = dict(Hq=33, Hkv=31, D=128, n=64, qs=(128, 128 * 33, 128, 1), ks=(129, 128 * 31, 128, 1))
+    assert _call(B=1 << 21, T=1, **odd) == UNSUP  # 2^21 * 64 * 64 tasks
+    assert _call(B=1 << 20, T=2, **odd) == UNSUP
+    even = dict(odd, Hq=512, Hkv=512, qs=(128, 1 << 16, 128, 1), ks=(128, 1 << 16, 128, 1))
+    assert _call(B=1 << 20, T=1, **even) == UNSUP  # 2^20 * 1024 * 8

@@ -846,8 +846,7 @@ ttcd_status ttcd_rope_fwd(const void* q, const void* k, void* q_out, void* k_out
   if ((unsigned)dtype > TTCD_DTYPE_F32) return fail(TTCD_ERR_INVALID_ARGUMENT, "unknown dtype");
   if (!isfinite(scale)) return fail(TTCD_ERR_INVALID_ARGUMENT, "scale must be finite");
   const int64_t heads = (int64_t)Hq + Hkv;
-  if ((int64_t)B * T > 0x7fffffffLL || heads * D > (1 << 28) ||
-      (int64_t)B * T > 0x7fffffffLL * 512 / (heads * D))
+  if ((int64_t)B * T > 0x7fffffffLL || heads * D > (1 << 28))
     return fail(TTCD_ERR_UNSUPPORTED, "grid too large");
   const int64_t* all[4] = {q_stride, q_out_stride, Hkv > 0 ? k_stride : q_stride,
                            Hkv > 0 ? k_out_stride : q_out_stride};
@@ -889,9 +888,10 @@ ttcd_status ttcd_rope_fwd(const void* q, const void* k, void* q_out, void* k_out
     a.ko_st = k_out_stride[1];
     a.ko_sh = k_out_stride[2];
   }
-  return from_hip(ttcd::launch_rope(a, interleaved != 0, elem(dtype),
-                                    static_cast<hipStream_t>(stream)),
-                  "rope launch");
+  const hipError_t e = ttcd::launch_rope(a, interleaved != 0, elem(dtype),
+                                         static_cast<hipStream_t>(stream));
+  if (e == hipErrorInvalidConfiguration) return fail(TTCD_ERR_UNSUPPORTED, "grid too large");
+  return from_hip(e, "rope launch");
 }
 
 ttcd_status ttcd_qk_norm_rope_fwd(const void* q, const void* k, void* q_out, void* k_out,

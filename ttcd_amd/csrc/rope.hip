@@ -200,7 +200,8 @@ hipError_t launch_layout(const RopeArgs& args, bool pairs, hipStream_t st) {
   a.per_token = make_fast_div(per_token);
   a.div_n = make_fast_div(a.n);
   const int64_t blocks = (a.tokens * per_token + kRopeTasks - 1) / kRopeTasks;
-  if (blocks > 0x7fffffffLL) return hipErrorInvalidConfiguration;
+  // a launch has fewer than 2^32 threads
+  if (blocks >= (int64_t(1) << 32) / kRopeThreads) return hipErrorInvalidConfiguration;
   // tokens that 512 tasks in a row can touch
   const int64_t span = std::min((int64_t)(kRopeTasks - 1 + per_token - 1) / per_token + 1, a.tokens);
   const size_t lds = (size_t)span * a.n * sizeof(float2);
