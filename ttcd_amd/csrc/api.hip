@@ -1544,7 +1544,9 @@ struct Kv4TreePlan {
 // 16000 keys, 16/8 heads of 128, with 256, 512 and 768: 16 of 8 30, 31, 36; 8 of 32 94, 59,
 // 60; 64 of 8 76, 64, 70; 256 of 1 59, 54, 66). As many parts to every sequence took 50 for
 // the first of these. No split up to 40 tiles of 32 keys, or 8 of 64: the sum of the parts
-// costs more than it saves.
+// costs more than it saves. None for so many rows that their sum, of 64 threads a row, passes
+// the 2^32 threads that a launch stays below, nor above 64 sequences, which the dealing has no
+// lanes for.
 Kv4TreePlan kv4_tree_plan(const ttcd_kv4_cache* c, int N, int Hq, int window) {
   const int64_t rows = (int64_t)N * (Hq / c->kv_heads);
   Kv4TreePlan p = {};
@@ -1555,7 +1557,8 @@ Kv4TreePlan kv4_tree_plan(const ttcd_kv4_cache* c, int N, int Hq, int window) {
   int64_t keys = c->capacity;
   if (window > 0 && window < keys) keys = window;
   const int64_t tiles = (keys + N) / (block ? 64 : 32) + 2;  // of a sequence, at most
-  if (tiles <= (block ? 8 : 40) || c->batch > 64) return p;
+  if (tiles <= (block ? 8 : 40) || c->batch > 64 || c->batch * rows * c->kv_heads >= 1 << 26)
+    return p;
   p.least = 4;
   const int64_t groups = (int64_t)c->kv_heads * p.nrb, all = (tiles + p.least - 1) / p.least;
   const int64_t units = std::min((512 + groups - 1) / groups, c->batch * all);
