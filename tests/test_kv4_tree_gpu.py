@@ -391,3 +391,36 @@ def test_the_package_offers_them():
     for name in ("kv4_tree_attn", "kv4_commit", "rope", "rope_frequencies", "sample",
                  "tree_accept"):
         assert name in ttcd_amd.__all__ and hasattr(ttcd_amd, name)
+
+
+def _mixed(B, lengths, counts):
+    return ([lengths[b] if b < len(lengths) else (b * 37) % 300 for b in range(B)],
+            None if counts is None else [counts[b] if b < len(counts) else counts[-1]
+                                         for b in range(B)])
+
+
+@pytest.mark.parametrize("B,N,Hq,H,D,C,lengths,window,counts", [
+    # 64 parts for a head: some 56 of one sequence, more than 16 in the sum over the parts of
+    # many rows; others of one part (written at once), of none (counts 0), and of nothing held
+    (8, 16, 16, 8, 128, 16384, (16000, 0, 33, 200, 0, 5000, 64, 1), None,
+     (16, 16, 3, 0, 0, 16, 16, 1)),
+    (8, 16, 16, 8, 128, 16384, (16000, 0, 33, 200, 0, 5000, 64, 1), 9000, None),
+    # the same in blocks of 128 rows, and 64 parts of one sequence
+    (4, 64, 4, 2, 64, 8192, (20, 8000, 0, 300), None, (64, 40, 0, 33)),
+    (1, 20, 4, 2, 64, 65536, (65000,), None, None),
+    # as many sequences as lanes deal, and one more
+    (64, 8, 4, 2, 64, 2048, (2048, 0, 2000, 1), None, (8, 8, 0, 5)),
+    (65, 8, 4, 2, 64, 2048, (2048, 0, 2000, 1), None, (8, 8, 0, 5)),
+    (64, 40, 2, 2, 64, 2048, (2048, 0, 3000, 1), 1500, (40, 8, 0, 33)),
+])
+def test_parts_dealt_by_the_lengths(gpu, B, N, Hq, H, D, C, lengths, window, counts):
+    lengths, counts = _mixed(B, lengths, counts)
+    c, r = _pair(B, H, D, C, BF, lengths, seed=B)
+    d, rd = _drafted(c, N, N + 1, counts)
+    q, parents = _rand(N + 9, B, N, Hq, D, scale=1.5), _trees(N, B, N)
+    n = None if counts is None else torch.tensor(counts, dtype=torch.int32).cuda()
+    o, lse = kv4_tree_attn(q.cuda(), c, d, parents.cuda(), window, counts=n, return_lse=True)
+    _check(r, rd, q, parents, o, lse, window, counts)
+    for b in range(B):  # rows behind the last node
+        k = N if counts is None else counts[b]
+        assert (o[b, k:] == 0).all() and (lse[b, :, k:] == -math.inf).all()
