@@ -628,8 +628,8 @@ ttcd_status ttcd_kv4_commit(ttcd_kv4_cache* cache, ttcd_kv4_cache* draft, const 
  * (B, T, Hkv, D), Hkv = 0: none; outputs of the same shapes, which may be the inputs (same
  * strides). Strides of any sign and size but d-stride 1; 16-byte accesses are made where
  * all allow it. positions: int32, or int64 with positions_64 != 0, at b *
- * position_stride[0] + t * position_stride[1]; NULL: offset + t. D <= 1024. dtype BF16, F16
- * or F32.
+ * position_stride[0] + t * position_stride[1]; NULL: offset + t, within 2^53 in size.
+ * D <= 1024. dtype BF16, F16 or F32.
  */
 ttcd_status ttcd_rope_fwd(const void* q, const void* k, void* q_out, void* k_out,
                           const float* inv_freq, int num_freq, const void* positions,

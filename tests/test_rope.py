@@ -127,3 +127,11 @@ def test_more_threads_than_a_launch_has():
     assert _call(B=1 << 20, T=2, **odd) == UNSUP
     even = dict(odd, Hq=512, Hkv=512, qs=(128, 1 << 16, 128, 1), ks=(128, 1 << 16, 128, 1))
     assert _call(B=1 << 20, T=1, **even) == UNSUP  # 2^20 * 1024 * 8
+
+
+def test_offsets_that_are_no_position():
+    for offset, n in ((2 ** 53 + 1, 1), (-2 ** 53 - 1, 1), (2 ** 53 - 3, 5)):
+        s = _lib.strides4
+        assert _lib.lib().ttcd_rope_fwd(P, None, P, None, P, 32, None, 0, None, offset, 1, n, 2, 0, 64,
+                                        s((256, 128, 64, 1)), None, s((256, 128, 64, 1)), None, 0, 0,
+                                        1.0, 0, None) == INV

@@ -204,3 +204,11 @@ def test_the_farthest_positions(gpu, interleaved):
     start = 2 ** 53 - 9
     _check(x, rope(x, None, inv, offset=start, interleaved=interleaved), inv,
            start + torch.arange(9)[None], interleaved=interleaved)
+
+
+def test_offsets_that_are_no_position(gpu):
+    q, inv = _rand(1, 1, 4, 2, 64).cuda(), torch.ones(32, device="cuda")
+    for offset in (2 ** 53 - 2, 2 ** 53 + 1, 2 ** 64 + 5, -2 ** 53 - 1, -2 ** 70):
+        with pytest.raises(ValueError, match="position"):
+            rope(q, None, inv, offset=offset)
+    rope(q, None, inv, offset=2 ** 53 - 3), rope(q, None, inv, offset=-2 ** 53)

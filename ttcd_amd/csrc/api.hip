@@ -845,6 +845,10 @@ ttcd_status ttcd_rope_fwd(const void* q, const void* k, void* q_out, void* k_out
                 num_freq, D);
   if ((unsigned)dtype > TTCD_DTYPE_F32) return fail(TTCD_ERR_INVALID_ARGUMENT, "unknown dtype");
   if (!isfinite(scale)) return fail(TTCD_ERR_INVALID_ARGUMENT, "scale must be finite");
+  constexpr int64_t kFar = int64_t(1) << 53;
+  if (!positions && (offset < -kFar || offset > kFar - (T - 1)))
+    return fail(TTCD_ERR_INVALID_ARGUMENT, "offset %lld: positions must be within 2^53",
+                (long long)offset);
   const int64_t heads = (int64_t)Hq + Hkv;
   if ((int64_t)B * T > 0x7fffffffLL || heads * D > (1 << 28))
     return fail(TTCD_ERR_UNSUPPORTED, "grid too large");

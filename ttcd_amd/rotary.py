@@ -108,7 +108,7 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor,
     """q (B, T, Hq, D) and k (B, T, Hkv, D) (or None) with the first 2 * len(inv_freq) channels
     of every head turned in pairs, (i, n + i) or ``interleaved`` (2i, 2i + 1), by
     position * inv_freq[i], times scale; the other channels as they are. positions: int32 or
-    int64, (B, T) or (T,), on q's device; None: offset .. offset + T - 1. bf16, f16 or f32;
+    int64, (B, T) or (T,), on q's device; None: offset .. offset + T - 1 (within 2^53). bf16, f16 or f32;
     inv_freq fp32. ``inverse`` turns back. Returns new contiguous (q, k), or q alone."""
     if (not isinstance(q, torch.Tensor) or not q.is_cuda or q.dim() != 4
             or not isinstance(inv_freq, torch.Tensor) or not inv_freq.is_cuda):
@@ -145,6 +145,8 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor,
         steps = positions.stride()
         steps = _strides2(steps if len(steps) == 2 else (0,) + steps)
         at, wide = positions.data_ptr(), int(positions.dtype == torch.int64)
+    elif not -2 ** 53 <= offset <= 2 ** 53 - max(T - 1, 0):
+        raise ValueError(f"rope: offset {offset}: positions must be within 2^53")
     if Hkv and not Hq:
         raise ValueError("rope: q has no heads")
     if q.stride(3) != 1:
