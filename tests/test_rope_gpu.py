@@ -212,3 +212,18 @@ def test_offsets_that_are_no_position(gpu):
         with pytest.raises(ValueError, match="position"):
             rope(q, None, inv, offset=offset)
     rope(q, None, inv, offset=2 ** 53 - 3), rope(q, None, inv, offset=-2 ** 53)
+
+
+def test_a_scaled_key_is_turned_back(gpu):
+    """With a scale (yarn's) inverse=True alone is the gradient, scale times the inverse; a key's
+    position comes off with the scale's reciprocal. Two passes, each off by 2^-21 scale
+    (|x0| + |x1|) and its rounding, and the reciprocal by 2^-24."""
+    inv, s = rope_frequencies(64, 1e4, {"rope_type": "yarn", "factor": 4.0,
+                                        "original_max_position_embeddings": 2048}, device="cuda")
+    assert s > 1.1
+    k = _rand(1, 2, 40, 3, 64, dtype=SF).cuda()
+    turned = rope(k, None, inv, offset=70000, scale=s)
+    limit = 8 * 2.0 ** -21 * k.abs().max()
+    assert (rope(turned, None, inv, offset=70000, inverse=True, scale=1 / s) - k).abs().max() < limit
+    grad = rope(turned, None, inv, offset=70000, inverse=True, scale=s)
+    assert (grad - s * s * k).abs().max() < 2 * limit

@@ -9,8 +9,9 @@ rotates: halves of the whole head, by tables of the tensors' type, at consecutiv
 positions. This is the rotary embedding of other models and of other positions: halves or
 interleaved pairs, the first channels of a head, every token at a position of its own (a
 padded batch, packed sequences, the nodes of a tree of drafted tokens), without tables: the
-angle position * inv_freq is exact (up to 2^53 of either), so positions may be far. ``inverse`` turns back: it takes
-a cached key's position from it, and a gradient through the embedding.
+angle position * inv_freq is exact (up to 2^53 of either), so positions may be far. ``inverse`` turns back, and
+multiplies by scale as well: so it takes a gradient through the embedding. A cached key's
+position comes off with inverse=True and scale = 1 / the scale that it was turned with.
 """
 from __future__ import annotations
 
@@ -108,8 +109,9 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, inv_freq: torch.Tensor,
     """q (B, T, Hq, D) and k (B, T, Hkv, D) (or None) with the first 2 * len(inv_freq) channels
     of every head turned in pairs, (i, n + i) or ``interleaved`` (2i, 2i + 1), by
     position * inv_freq[i], times scale; the other channels as they are. positions: int32 or
-    int64, (B, T) or (T,), on q's device; None: offset .. offset + T - 1 (within 2^53). bf16, f16 or f32;
-    inv_freq fp32. ``inverse`` turns back. Returns new contiguous (q, k), or q alone."""
+    int64, (B, T) or (T,), on q's device; None: offset .. offset + T - 1 (within 2^53). bf16,
+    f16 or f32; inv_freq fp32. ``inverse`` turns back, times scale too: the gradient (with
+    1 / scale the inverse). Returns new contiguous (q, k), or q alone."""
     if (not isinstance(q, torch.Tensor) or not q.is_cuda or q.dim() != 4
             or not isinstance(inv_freq, torch.Tensor) or not inv_freq.is_cuda):
         raise ValueError("rope: q (B, T, H, D) and inv_freq must be tensors on a GPU (HIP) device")
