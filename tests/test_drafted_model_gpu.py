@@ -261,3 +261,91 @@ def test_logits_that_are_no_numbers_end_a_text():
     for draft in (None, lambda t, n: ([-1], [1])):
         with pytest.raises(RuntimeError, match="no logit"):
             m.generate(ids, 3, u, draft=draft)
+
+
+def _bush(vocab, nodes):
+    """As many drafted tokens after every text, whatever is of use: a chain and leaves."""
+    def draft(text, most):
+        parents = [-1] + [max(0, i - 1 - i % 3) for i in range(1, nodes)]
+        return parents, [(text[-1] + 7 * i) % vocab for i in range(nodes)]
+    return draft
+
+
+@pytest.mark.parametrize("cfg", CFGS[1:])
+@pytest.mark.parametrize("prompt,count,capacity,nodes", [
+    (40, 25, 64, 16), (40, 24, 64, 60), (4, 29, 32, 60), (30, 3, 32, 31)])
+def test_a_text_that_fills_its_cache(monkeypatch, cfg, prompt, count, capacity, nodes):
+    """Room for the prompt and all but the last token is enough, whatever is drafted: nodes lie in
+    drafts, and only the accepted ones take positions."""
+    m = _model(cfg, seed=2)
+    ids = _ids(1, prompt, 7).to(DEV)
+    monkeypatch.setitem(globals(), "_cache",
+                        lambda: IPTTCDv9Cache(bits=4, capacity=capacity))
+    kw = dict(temperature=0.7, top_k=8)
+    u = torch.rand(count, generator=torch.Generator().manual_seed(3))
+    plain, want, _ = _recorded(m, ids, count, u, kw)
+    assert plain == want
+    known = ids[0].tolist() + plain
+
+    def right(text, most):  # the plain text to its end, then leaves
+        tokens = known[len(text):][:nodes]
+        n = nodes - len(tokens)
+        return (list(range(-1, len(tokens) - 1)) + [-1] * n,
+                tokens + [(text[-1] + 5 * i) % 1024 for i in range(n)])
+    for draft in (_bush(1024, nodes), right):
+        text, want, calls = _recorded(m, ids, count, u, kw, draft)
+        assert text == want
+        assert max(calls) == min(nodes + 1, capacity)
+
+
+def test_accepted_nodes_need_room():
+    """A tree goes through a full cache; more of its nodes than there is room for are refused
+    before any is written, and fewer are taken."""
+    m = _model({"window_size": None})
+    cache = _cache(32)
+    m.forward(_ids(1, 30, 1).to(DEV), cache=cache)
+    tree = [-1] + list(range(7))
+    m.forward(_ids(1, 8, 2).to(DEV), cache=cache, tree=tree)
+    path = torch.arange(8, dtype=torch.int32, device=DEV)[None]
+    n = torch.full((1,), 3, dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError, match="positions"):
+        cache.accept(path, n)
+    assert cache.seen == 30 and all(c.lengths.item() == 30 for c in cache.kv4.values())
+    assert cache.accept(path, n, most=2) == 2
+    assert all(c.lengths.item() == 32 for c in cache.kv4.values())
+    m.forward(_ids(1, 8, 3).to(DEV), cache=cache, tree=tree)
+    with pytest.raises(ValueError, match="positions"):
+        cache.accept(path, n, most=1)
+    assert cache.accept(path, n, most=0) == 0 and cache.seen == 32
+    with pytest.raises(ValueError, match="positions"):
+        m.forward(_ids(1, 1, 4).to(DEV), cache=cache)
+
+
+def test_trees_over_a_window_that_its_cache_just_holds():
+    """The ring wraps: trees, accepted and not, over the last window less one positions."""
+    m = _model({"ttt_layers": [], "window_size": 64, "num_heads": 6}, seed=4)
+    four = Drafted(capacity=64)
+    held = HeldCache(four)
+    ids = _ids(1, 60, 1).to(DEV)
+    m.forward(ids, cache=four)
+    m.forward(ids, cache=held)
+    for step in range(4):
+        tokens = _ids(1, len(TREE), 10 + step).to(DEV)
+        got = m.forward(tokens, cache=four, tree=TREE)
+        lines = ref.lineage(TREE)
+        for line in lines:
+            want = m.forward(tokens[:, line], logits_to_keep=1, cache=_along(held, four, line))
+            _logits_close(got[:, line[-1]], want[:, 0])
+        line = lines[(6, 9, 4, 8)[step]]
+        path = torch.full((1, len(TREE)), -1, dtype=torch.int32, device=DEV)
+        path[0, :len(line)] = torch.tensor(line)
+        n = torch.tensor([len(line)], dtype=torch.int32, device=DEV)
+        held = _along(held, four, line)
+        m.forward(tokens[:, line], cache=held)
+        assert four.accept(path, n) == len(line)
+    assert four.seen > 70
+    small = IPTTCDv9Cache(bits=4, capacity=32)  # less than the window: wrong as soon as it wraps
+    m.forward(ids[:, :31], cache=small)
+    m.forward(tokens, cache=small, tree=TREE)
+    with pytest.raises(ValueError, match="positions"):
+        small.accept(path, n)

@@ -471,7 +471,8 @@ class IPTTCDv9Prefill:
             cache.check(B, self.Hkv, self.D, self.dtype, self.dev)
             # a TTT layer's student attends in calls of a chunk and more
             student = self.window_s if self.ttt and T >= self.cfg["ttt_chunk"] else None
-            cache.reserve(T, None if self.window_t < 0 else self.window_t, student)
+            cache.reserve(T, None if self.window_t < 0 else self.window_t, student,
+                          tree=tree is not None)
             ctx.cache, ctx.offset = cache, cache.seen
             attention_mask = None
             if tree is not None:
@@ -530,7 +531,7 @@ class IPTTCDv9Prefill:
         pos = torch.tensor(depth, device=self.dev) + ctx.offset
         cos, sin = self.tables(ctx.offset + T)
         ctx.tables, ctx.offset = (cos[pos], sin[pos]), 0
-        ctx.cache.begin_draft(T)
+        ctx.cache.begin_draft(T, None if self.window_t < 0 else self.window_t)
 
     @torch.inference_mode()
     def forward(self, input_ids: torch.Tensor, logits_to_keep: int = 1,
@@ -579,9 +580,10 @@ class IPTTCDv9Prefill:
         draft: a callable that gets the tokens so far (a list of ints, input_ids first) and the
         most that are of use, and returns (parents, tokens) of drafted ones after them, lists
         (parents: -1 the last token, or a drafted one before). They go through the model at
-        once, up to 255 of them, and those stay that are what is sampled at their place: the
-        text is the one of a token a call, as far as the roundings of the two agree. Logits none
-        of which is a number end it with a RuntimeError (as the last token they are a -1)."""
+        once, the first 255 of them (fewer than the cache's capacity, and of a model with TTT
+        layers ttt_chunk - 2), and those stay that are what is sampled at their place: the text
+        is the one of a token a call, as far as the roundings of the two agree. Logits none of
+        which is a number end it with a RuntimeError (as the last token they are a -1)."""
         if input_ids.dim() != 2 or input_ids.shape[0] != 1 or input_ids.shape[1] < 1:
             raise ValueError("generate: input_ids must be (1, T), T >= 1")
         if count < 1:
@@ -600,6 +602,8 @@ class IPTTCDv9Prefill:
             if self.window_t >= 0:
                 room = min(room, max(self.window_t, self.window_s if self.ttt else 0) + max(T, most))
             cache = IPTTCDv9Cache(bits=4, capacity=room)
+        elif cache.bits == 4:
+            most = min(most, cache.capacity)
         kw = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
         logits = self.forward(input_ids, cache=cache)[:, -1]
         done = _sampling.sample(logits, uniform[:1], **kw).tolist()
@@ -670,6 +674,8 @@ class IPTTCDv9Cache:
     allocated once: a window needs window_size + T - 1 of them for calls of T
     tokens (or as many as the prompt has; a TTT layer's student window takes the place
     of a smaller window_size), full-causal attention room for every token that is kept.
+    A tree of drafted tokens takes no positions, those that accept() keeps do; it may have
+    as many nodes as there are positions.
     keep: after a call that leaves more, each layer's kv heads keep that many keys, the
     newest `recent` and those with the largest sum of attention weights so far
     (full-causal models only; the student window of a TTT layer counts positions, so a
@@ -702,6 +708,7 @@ class IPTTCDv9Cache:
         self.drafts: dict[int, _kv4.KV4Cache] = {}  # the nodes' keys and values
         self._begun = self._nodes = 0  # nodes of the last tree; 0 until it ends, and accepted
         self._drafted = False  # a layer's draft may hold some
+        self._window: int | None = None  # of the model that it went through
 
     def check(self, B: int, Hkv: int, D: int, dtype, device) -> None:
         shape = (B, Hkv, D, dtype, torch.device(device))
@@ -710,9 +717,11 @@ class IPTTCDv9Cache:
                              f"this prefill needs {shape}")
         self._shape = shape
 
-    def reserve(self, T: int, window: int | None, student: int | None = None) -> None:
+    def reserve(self, T: int, window: int | None, student: int | None = None,
+                tree: bool = False) -> None:
         """Refuse T more tokens that a 4-bit cache has no room for, or whose student
-        window (of a TTT layer, None if none runs) reaches over dropped keys."""
+        window (of a TTT layer, None if none runs) reaches over dropped keys. A tree's
+        nodes lie in the drafts: they need what their windows see of the held ones."""
         if self.bits != 4:
             return
         if self._open:
@@ -726,9 +735,10 @@ class IPTTCDv9Cache:
                 f"a TTT layer's student window of {student} over a cache that dropped keys: "
                 f"only the newest {self.run} held positions are in a row (recent={self.recent} "
                 f"of keep={self.keep}; it takes {student - 1})")
-        need = self.held + T
+        new = 0 if tree else T
+        need = self.held + new
         if window is not None:
-            need = min(need, max(window, student or 0) + T - 1)
+            need = min(need, max(window, student or 0) + new - 1)
         if max(need, T) > self.capacity:
             raise ValueError(f"IPTTCDv9Cache: {T} more tokens need {max(need, T)} positions of "
                              f"{self.capacity}")
@@ -742,13 +752,13 @@ class IPTTCDv9Cache:
         _kv4.kv4_append(held, k, v)
         return held
 
-    def begin_draft(self, T: int) -> None:
+    def begin_draft(self, T: int, window: int | None) -> None:
         """A tree of T nodes is about to go through the layers: their drafts are emptied of
         one that was not accepted."""
         if self._drafted:
             for d in self.drafts.values():
                 d.reset()
-        self._nodes, self._begun, self._drafted = 0, T, True
+        self._nodes, self._begun, self._drafted, self._window = 0, T, True, window
 
     def draft(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> "_kv4.KV4Cache":
         """The layer's 4-bit cache, with the nodes' keys and values in its draft."""
@@ -769,7 +779,8 @@ class IPTTCDv9Cache:
     def accept(self, path: torch.Tensor, accepted: torch.Tensor, most: int | None = None) -> int:
         """The nodes path[0, :accepted[0]] of the last tree (as tree_accept gives them, `most`
         of them at the most) become the sequence's next tokens in every layer. Returns how
-        many (a host synchronisation)."""
+        many (a host synchronisation). More than the cache has room for are refused, and none
+        is taken then."""
         if not self._nodes:
             raise RuntimeError("IPTTCDv9Cache: no tree of drafted tokens to accept from")
         dev = self._shape[-1]
@@ -780,6 +791,13 @@ class IPTTCDv9Cache:
         if most is not None:
             accepted = accepted.clamp(max=most)
         n = min(max(int(accepted[0]), 0), self._nodes)
+        # of a window, what the next token sees has to stay
+        need = self.held + n
+        if self._window is not None:
+            need = min(need, self._window - 1)
+        if need > self.capacity:
+            raise ValueError(f"IPTTCDv9Cache: {n} accepted tokens need {need} positions of "
+                             f"{self.capacity}")
         self._open = True
         for i, held in self.kv4.items():
             _kv4.kv4_commit(held, self.drafts[i], path, accepted, reset=True)
