@@ -9,9 +9,10 @@ rotates: halves of the whole head, by tables of the tensors' type, at consecutiv
 positions. This is the rotary embedding of other models and of other positions: halves or
 interleaved pairs, the first channels of a head, every token at a position of its own (a
 padded batch, packed sequences, the nodes of a tree of drafted tokens), without tables: the
-angle position * inv_freq is exact (up to 2^53 of either), so positions may be far. ``inverse`` turns back, and
-multiplies by scale as well: so it takes a gradient through the embedding. A cached key's
-position comes off with inverse=True and scale = 1 / the scale that it was turned with.
+angle position * inv_freq is exact (up to 2^53 of either), so positions may be far.
+``inverse`` turns back, and multiplies by scale as well: so it takes a gradient through the
+embedding. A cached key's position comes off with inverse=True and scale = 1 / the scale that
+it was turned with.
 """
 from __future__ import annotations
 
