@@ -349,3 +349,21 @@ def test_trees_over_a_window_that_its_cache_just_holds():
     m.forward(tokens, cache=small, tree=TREE)
     with pytest.raises(ValueError, match="positions"):
         small.accept(path, n)
+
+
+def test_a_refused_accept_changes_nothing():
+    """A path on another device than the layers' caches."""
+    m = _model({"window_size": None})
+    cache, ids = _cache(), _ids(1, 4, 0).to(DEV)
+    m.forward(ids, cache=cache, tree=[-1, 0, 1, 2])
+    path, n = torch.zeros(1, 4, dtype=torch.int32, device=DEV), torch.ones(1, dtype=torch.int32,
+                                                                           device=DEV)
+    at = {i: c.device for i, c in cache.kv4.items()}
+    for c in cache.kv4.values():
+        c.device = torch.device("cuda", 1)
+    with pytest.raises(ValueError):
+        cache.accept(path, n)
+    for i, c in cache.kv4.items():
+        c.device = at[i]
+    m.forward(ids, cache=cache, tree=[-1, 0, 1, 2])
+    assert cache.accept(path, n) == 1 and cache.seen == 1

@@ -783,11 +783,11 @@ class IPTTCDv9Cache:
         is taken then."""
         if not self._nodes:
             raise RuntimeError("IPTTCDv9Cache: no tree of drafted tokens to accept from")
-        dev = self._shape[-1]
+        dev = next(iter(self.kv4.values())).device
         for name, t, shape in (("path", path, (1, self._nodes)), ("accepted", accepted, (1,))):
-            if t.shape != shape or t.dtype != torch.int32 or t.device.type != dev.type:
-                raise ValueError(f"IPTTCDv9Cache: {name} must be int32 {shape} on the GPU, got "
-                                 f"{t.dtype} {tuple(t.shape)}")
+            if t.shape != shape or t.dtype != torch.int32 or t.device != dev:
+                raise ValueError(f"IPTTCDv9Cache: {name} must be int32 {shape} on the cache's "
+                                 f"device, got {t.dtype} {tuple(t.shape)} on {t.device}")
         if most is not None:
             accepted = accepted.clamp(max=most)
         n = min(max(int(accepted[0]), 0), self._nodes)
