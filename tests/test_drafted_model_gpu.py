@@ -367,3 +367,13 @@ def test_a_refused_accept_changes_nothing():
         c.device = at[i]
     m.forward(ids, cache=cache, tree=[-1, 0, 1, 2])
     assert cache.accept(path, n) == 1 and cache.seen == 1
+
+
+def test_chunks_of_one_and_two_tokens_take_no_tree():
+    """A TTT layer whose update chunk leaves no room for a tree: a token a call."""
+    for chunk in (1, 2):
+        m = _model({"ttt_chunk": chunk, "ttt_visible_chunks": 64})
+        ids = _ids(1, 6, 1).to(DEV)
+        plain = m.generate(ids, 5, temperature=0)
+        assert torch.equal(plain, m.generate(ids, 5, temperature=0,
+                                             draft=lambda t, n: ([-1, 0], [1, 2])))

@@ -596,7 +596,7 @@ class IPTTCDv9Prefill:
             raise ValueError(f"generate: uniform must be ({count},), got {tuple(uniform.shape)}")
         T, most = input_ids.shape[1], _kv4.TREE_NODES
         if self.ttt:
-            most = min(most, self.cfg["ttt_chunk"] - 1)
+            most = min(most, max(1, self.cfg["ttt_chunk"] - 1))
         if cache is None:
             room = T + count + most
             if self.window_t >= 0:
