@@ -377,3 +377,14 @@ def test_chunks_of_one_and_two_tokens_take_no_tree():
         plain = m.generate(ids, 5, temperature=0)
         assert torch.equal(plain, m.generate(ids, 5, temperature=0,
                                              draft=lambda t, n: ([-1, 0], [1, 2])))
+
+
+def test_a_refused_call_sets_no_shape():
+    """A batch of two, refused before its first layer, and then the one sequence that goes."""
+    m = _model({"window_size": None})
+    cache, ids = _cache(), _ids(1, 4, 0).to(DEV)
+    with pytest.raises(NotImplementedError, match="one sequence"):
+        m.forward(ids.expand(2, 4), cache=cache, tree=[-1, 0, 1, 2])
+    m.forward(ids, cache=cache, tree=[-1, 0, 1, 2])
+    with pytest.raises(ValueError, match="cache holds"):
+        m.forward(ids.expand(2, 4), cache=cache)

@@ -712,7 +712,8 @@ class IPTTCDv9Cache:
 
     def check(self, B: int, Hkv: int, D: int, dtype, device) -> None:
         shape = (B, Hkv, D, dtype, torch.device(device))
-        if self._shape is not None and self._shape != shape:
+        # a call that was refused before its first layer left a shape and nothing of it
+        if self._shape is not None and self._shape != shape and (self.kv or self.kv4):
             raise ValueError(f"cache holds (B, Hkv, D, dtype, device) = {self._shape}, "
                              f"this prefill needs {shape}")
         self._shape = shape
