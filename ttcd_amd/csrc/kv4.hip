@@ -354,7 +354,7 @@ hipError_t launch_read(const Kv4ReadArgs& a, hipStream_t st) {
 // and 9.8; 10.2 and 9.7). By the capacity: the lengths are on the GPU.
 //
 // Over a tree (kv4_tree_attn) the rows are its nodes, and the draft's tiles come behind the
-// cache's. 16 nodes of 8 sequences of up to 16000 keys, 77 MB: 25 us and 5.2 for the sum of
+// cache's. 16 nodes of 8 sequences of up to 16000 keys, 77 MB: 24.5 us and 5.2 for the sum of
 // the parts; 8 nodes of 32, 294 MB: 59 in all (5.0 TB/s). Workgroups of 4 wavefronts, two of
 // them on a CU, parts dealt by the lengths and two tiles on their way brought the first from
 // 50.6 in all to 30.4.
@@ -952,7 +952,7 @@ __device__ __forceinline__ f32x16 mfma32<_Float16>(u32x4 a, u32x4 b, f32x16 c) {
 }
 
 // A tree's nodes in more than 32 rows a kv head take this kernel too: 64 nodes of 4 sequences
-// over a window of 8192 keys, 128 rows a head, 33 us (520 TFLOP/s: parts of 8 or 9 tiles,
+// over a window of 8192 keys, 128 rows a head, 32 us (530 TFLOP/s: parts of 8 or 9 tiles,
 // whose start and end take as long) and 8.4 for the sum of the parts.
 constexpr int kBlockKeys = 64;
 

@@ -7,17 +7,18 @@
 // first whose running sum exceeds uniform times the sum of all kept.
 //
 // A 16-bit logit has one of 65536 values, and everything above depends on a row only
-// through how often each value comes: no sort, and no exponential of a token, but one of
-// every value that occurs, in 64 bits, as are all sums. Counting is exact in any order, so
-// a row's token does not depend on how its sums are laid out. A workgroup takes a row: it
-// counts the values in LDS (16 bits a count, 128 KiB), finds the last kept value and the
-// drawn one with how many of its tokens come before the drawn token, and looks for that
-// one in the row, most of which is still in registers.
+// through how often each value comes: no sort, and no exponential of a token, but one for 8
+// values in a row, which are a step apart, with a product for each of the others, in 64 bits,
+// as are all sums. Counting is exact in any order, so a row's token does not depend on how
+// its sums are laid out. A workgroup takes a row: it counts the values in LDS (16 bits a
+// count, 128 KiB), finds the last kept value and the drawn one with how many of its tokens
+// come before the drawn token, and looks for that one in the row, most of which is still in
+// registers.
 //
-// Of a row of 151936 bf16 logits alone (24 us on a CU): zeroing 0.8 us, counting 12.2 (LDS
+// Of a row of 151936 bf16 logits alone (25.7 us on a CU): zeroing 0.8 us, counting 12.2 (LDS
 // atomics: 11 cycles for 64 tokens), sums of the values' weights 3.5 (f16, whose rows have
 // 8 times the values, 7; 64 lanes a block with an exponential for every two values 4.9 and
-// 14.7), cuts and draw 3.7 (one wavefront's latencies), the token 2.6. 256 rows, 78 MB: 34
+// 14.7), cuts and draw 3.7 (one wavefront's latencies), the token 2.6. 256 rows, 78 MB: 35
 // us, of which counting, at the rate of the memory (4.4 TB/s), is 17.6. Reading the row again
 // for the token took 9.3 of 256 rows and 3.5 of one; the order of a value taken while
 // counting, instead of its bits, 4 more. Not counting what a bound under the first top_k

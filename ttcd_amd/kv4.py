@@ -436,7 +436,8 @@ def kv4_tree_attn(q: torch.Tensor, cache: KV4Cache, draft: KV4Cache, parents: to
     all) positions up to its own and, within those, itself and its ancestors, which `draft`
     holds: kv4_append all nodes to an empty second cache first, node i is in its slot i
     (counts[b] of them: the first). So a chain of nodes sees what the same tokens would
-    that kv4_append adds to the cache itself, and the cache stays as it is until kv4_commit.
+    that kv4_append adds to the cache itself, where its capacity holds them beside what their
+    windows reach (nodes drop no key), and the cache stays as it is until kv4_commit.
     Returns o like q, and with ``return_lse`` lse, fp32 natural-log (B, H, N); rows behind
     the last node get o = 0 and lse = -inf. ``split_keys`` as in kv4_attn."""
     fn = "kv4_tree_attn"
