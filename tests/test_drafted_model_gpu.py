@@ -388,3 +388,9 @@ def test_a_refused_call_sets_no_shape():
     m.forward(ids, cache=cache, tree=[-1, 0, 1, 2])
     with pytest.raises(ValueError, match="cache holds"):
         m.forward(ids.expand(2, 4), cache=cache)
+
+
+def test_generate_refuses_what_is_no_cache():
+    m = _model({"window_size": None})
+    with pytest.raises(ValueError, match="IPTTCDv9Cache"):
+        m.generate(_ids(1, 4, 0).to(DEV), 3, temperature=0, cache={})

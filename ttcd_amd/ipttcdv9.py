@@ -602,6 +602,8 @@ class IPTTCDv9Prefill:
             if self.window_t >= 0:
                 room = min(room, max(self.window_t, self.window_s if self.ttt else 0) + max(T, most))
             cache = IPTTCDv9Cache(bits=4, capacity=room)
+        elif not isinstance(cache, IPTTCDv9Cache):
+            raise ValueError("generate: cache must be an IPTTCDv9Cache")
         elif cache.bits == 4:
             most = min(most, cache.capacity)
         kw = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
